@@ -290,6 +290,74 @@ int ijb_weight_status(ijb_weight *weight);
 /* Packed argmax keys -> token indices (n keys, device memory). */
 int ijb_keys_to_tokens(const unsigned long long *keys_dev, int n, int *tokens_dev, void *stream);
 
+/* ---- the paged K/V cache outside an engine ----
+ * For callers that own the cache's memory (one layer's pool, or several): the
+ * write of new rows and their read-back.
+ * No counterpart in the reference, whose cache is one fp32 array per layer
+ * written by cache_cuda (inferencer.cu:906-926) and read by attention_cuda
+ * (:981-1041).
+ *
+ * All calls are asynchronous on `stream` (a cudaStream_t of the current
+ * device; NULL is that device's default stream), allocate nothing and may be
+ * captured into a graph; what is *_dev is read when the kernels run.  A
+ * non-NULL status_dev word receives (by OR) a non-zero code when an index
+ * found on the device names nothing: such an entry is skipped. */
+#define IJB_KV_F16 0   /* fp16 rows */
+#define IJB_KV_E4M3 2  /* e4m3 rows, each with a power-of-two scale 2^(s - 127) kept as the byte s (0..254) */
+
+typedef struct {
+    int type;                   /* IJB_KV_F16 or IJB_KV_E4M3 */
+    int kv_heads;
+    int head_dim;               /* 64 or 128 */
+    int page_size;              /* positions per page: 8, 16, 32, 64, 128 or 256 */
+    long num_pages;
+    void *data_dev;             /* [num_pages][K, V][kv_heads][page_size][head_dim], 16-byte aligned */
+    uint8_t *scale_dev;         /* e4m3: [num_pages][K, V][kv_heads][page_size]; else ignored */
+    const int *page_table_dev;  /* [n_seqs][max_pages] page ids; only those of a call's positions are read */
+    int n_seqs;
+    int max_pages;
+} ijb_kv_view;
+
+/* Writes the K and V rows of n tokens ([n] tokens of [kv_heads][head_dim],
+ * src_type IJB_TYPE_F32 or IJB_TYPE_F16, `stride` elements from token to
+ * token) at position tok_pos_dev[i] of sequence tok_seq_dev[i].  fp16 rows are
+ * rounded to nearest; an e4m3 row gets the least scale 2^e with max|row| <=
+ * 448 * 2^e over its finite values (2^-126 at least), its values are rounded
+ * to nearest, infinities to the largest finite value, NaN stays NaN.  Entries
+ * with a negative position are padding and are skipped.  A (sequence,
+ * position) must not be named by two of the call's tokens. */
+int ijb_kv_append(const ijb_kv_view *kv, int src_type, const void *k_dev, const void *v_dev, long stride, int n,
+                  const int *tok_seq_dev, const int *tok_pos_dev, uint32_t *status_dev, void *stream);
+
+/* The other way: the rows of n (sequence, position) pairs, in dst_type
+ * (IJB_TYPE_F32: the stored values exactly; IJB_TYPE_F16: rounded to nearest).
+ * Rows of skipped entries are left as they were. */
+int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev, long stride, int n,
+                  const int *tok_seq_dev, const int *tok_pos_dev, uint32_t *status_dev, void *stream);
+
+/* Draws one token from each of n rows of fp32 logits ([n] rows of vocab <=
+ * 131072 values, `stride` floats apart): temperature, then top-k, top-p and
+ * min-p, then the uniform number u_dev[i] in [0, 1).  The settings are one
+ * value per row in device memory, or NULL:
+ *   temperature  > 0 (NULL: 1); anything else is greedy: the token ijb_argmax
+ *                takes (NaN counts as -infinity), with probability 1
+ *   top_k        keeps the k largest logits, equal ones by the lower index; 0, a
+ *                negative value or vocab and more keep all
+ *   top_p        keeps the shortest prefix of those, in falling order, whose
+ *                probability reaches top_p of theirs; 1 and more keep all, 0
+ *                and less the largest
+ *   min_p        drops tokens less than min_p times as likely as the largest
+ * The answer is the first token, in falling order, whose running share of what
+ * is kept exceeds u: u = 0 gives the largest.  prob_dev (may be NULL) receives
+ * its share.  A row without any value above -infinity gives token -1 and 0.
+ * The sums are whole numbers (exp in fp32, in units of 2^-44 of the largest
+ * token's weight), so the same row gives the same token in any batch.
+ * Asynchronous on `stream`, allocates nothing, may be captured.  No
+ * counterpart in the reference, whose loop is greedy (inferencer.cu:1870-1883). */
+int ijb_sample(const float *logits_dev, long stride, int n, int vocab, const float *u_dev,
+               const float *temperature_dev, const int *top_k_dev, const float *top_p_dev, const float *min_p_dev,
+               int *token_dev, float *prob_dev, void *stream);
+
 /* Number of kernels the library launched since load (for launch accounting). */
 uint64_t ijb_kernel_launches(void);
 

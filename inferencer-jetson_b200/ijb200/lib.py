@@ -38,6 +38,13 @@ class TensorView(ctypes.Structure):
                 ("dims", ctypes.c_int64 * 4), ("data_dev", ctypes.c_void_p)]
 
 
+class KvView(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("num_pages", ctypes.c_long), ("data_dev", ctypes.c_void_p),
+                ("scale_dev", ctypes.c_void_p), ("page_table_dev", ctypes.c_void_p), ("n_seqs", ctypes.c_int),
+                ("max_pages", ctypes.c_int)]
+
+
 def build() -> str:
     """Compile libijb200.so for sm_100a with the package Makefile."""
     subprocess.run(["make", "-s", "-C", PKG_ROOT], check=True)
@@ -89,6 +96,9 @@ def load():
         "ijb_weight_matmul": ([P, P, I, P, ctypes.c_float, I, P, L64, I, P, P], I),
         "ijb_weight_status": ([P], I),
         "ijb_keys_to_tokens": ([P, I, P, P], I),
+        "ijb_kv_append": ([P, I, P, P, L64, I, P, P, P, P], I),
+        "ijb_kv_gather": ([P, I, P, P, L64, I, P, P, P, P], I),
+        "ijb_sample": ([P, L64, I, I, P, P, P, P, P, P, P, P], I),
         "ijb_kernel_launches": ([], ctypes.c_uint64),
         "ijb_tokenizer_create": ([ctypes.POINTER(ctypes.c_char_p), I, ctypes.POINTER(ctypes.c_char_p), I,
                                   ctypes.POINTER(P)], I),
