@@ -23,6 +23,7 @@
 #ifndef IJB200_H
 #define IJB200_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -292,7 +293,7 @@ int ijb_keys_to_tokens(const unsigned long long *keys_dev, int n, int *tokens_de
 
 /* ---- the paged K/V cache outside an engine ----
  * For callers that own the cache's memory (one layer's pool, or several): the
- * write of new rows and their read-back.
+ * write of new rows, their read-back, and attention of new tokens over them.
  * No counterpart in the reference, whose cache is one fp32 array per layer
  * written by cache_cuda (inferencer.cu:906-926) and read by attention_cuda
  * (:981-1041).
@@ -334,6 +335,34 @@ int ijb_kv_append(const ijb_kv_view *kv, int src_type, const void *k_dev, const 
  * Rows of skipped entries are left as they were. */
 int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev, long stride, int n,
                   const int *tok_seq_dev, const int *tok_pos_dev, uint32_t *status_dev, void *stream);
+
+/* Attention of new tokens over the cache, causal, with heads / kv_heads (1..16)
+ * query heads to a KV head.  Entry e (of n_entries <= 4096) is the rows
+ * q_start_dev[e] .. q_start_dev[e + 1] of q_dev and out_dev ([n_tokens] rows of
+ * [heads][head_dim], type IJB_TYPE_F32 or IJB_TYPE_F16, strides in elements):
+ * the last of the kv_len_dev[e] positions of sequence seq_dev[e] (NULL: e),
+ * whose K and V, the new tokens' included, the cache already holds.  A token
+ * sees the positions up to its own, with softmax(scale * q . k); one before
+ * position 0 (kv_len shorter than the entry) sees none and gets zeros.  Entries
+ * may be empty; rows that belong to no entry are left as they were.  max_q > 0
+ * promises that no entry has more new tokens (0: unknown): a longer one may be
+ * left unwritten and is reported.
+ *
+ * fp32 queries and probabilities enter the products as two fp16 parts each
+ * (22 bits); fp16 queries as they are, their probabilities rounded to fp16.
+ * e4m3 rows enter as fp16, exactly while the largest value of a row is within
+ * 2^-7 .. 2^15.  Sums, maxima and the softmax are fp32.  The result is the same
+ * every time for the same call, but how an entry's positions are cut into
+ * partial sums depends on the whole call.
+ *
+ * workspace_dev: ijb_paged_attention_workspace bytes of 16-byte aligned device
+ * memory on the current device, of no meaning before and after; calls that may
+ * overlap, captured graphs among them, need one each. */
+size_t ijb_paged_attention_workspace(const ijb_kv_view *kv, int heads, int n_tokens, int n_entries);
+int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *q_dev, long q_stride, void *out_dev,
+                        long out_stride, int n_tokens, int n_entries, const int *q_start_dev, const int *seq_dev,
+                        const int *kv_len_dev, int max_q, float scale, void *workspace_dev, size_t workspace_bytes,
+                        uint32_t *status_dev, void *stream);
 
 /* Draws one token from each of n rows of fp32 logits ([n] rows of vocab <=
  * 131072 values, `stride` floats apart): temperature, then top-k, top-p and

@@ -1,14 +1,15 @@
 """The stand-alone serving operators on torch tensors: the paged K/V cache
-(write, read-back) and sampling from logits.
+(write, read-back, attention of new tokens) and sampling from logits.
 
 Thin calls of the C ABI (include/ijb200.h has each operator's definition):
 tensors are passed by address, on the current stream of their device, and
-nothing is allocated but outputs.  Arguments that
+nothing is allocated but outputs and the attention's workspace.  Arguments that
 do not fit raise ValueError or IjbError; there is no fallback.
 """
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -105,6 +106,28 @@ class PagedKV:
         _call(self.device, self._lib.ijb_kv_gather, self._ref, _TYPE[dtype], k.data_ptr(), v.data_ptr(), self.row, n,
               _ptr(seq, torch.int32, n, self.device, "seq"), _ptr(pos, torch.int32, n, self.device, "pos"), self._status)
         return k, v
+
+    def attention(self, q, q_start, kv_len, seq=None, max_q: int = 0, scale: float | None = None, out=None):
+        """Attention of new tokens: q [tokens, heads, head_dim] fp32 or fp16, entry e's tokens being rows
+        q_start[e]..q_start[e + 1] and the last of the kv_len[e] positions of sequence seq[e] (default: e), which
+        the cache already holds.  Each token sees the positions up to its own; a token before position 0 sees none and
+        gets zeros.  ``max_q``: the most new tokens of any entry, if known.  Returns out (like q)."""
+        _need(q.dim() == 3 and q.shape[2] == self.head_dim, "q: expected [tokens, heads, head_dim]")
+        n, heads = q.shape[0], q.shape[1]
+        qp, qs = _rows(q, heads * self.head_dim, self.device, "q")
+        if out is None:
+            out = torch.empty((n, heads, self.head_dim), dtype=q.dtype, device=q.device)
+        _need(out.shape == q.shape and out.dtype == q.dtype, "out: expected the shape and type of q")
+        op, os = _rows(out, heads * self.head_dim, self.device, "out")
+        e = kv_len.numel()
+        _need(e >= 1 and (seq is not None or e <= self.page_table.shape[0]), "kv_len: one length for each entry")
+        size = self._lib.ijb_paged_attention_workspace(self._ref, heads, n, e)
+        work = torch.empty((max(size, 16),), dtype=torch.uint8, device=q.device)
+        _call(self.device, self._lib.ijb_paged_attention, self._ref, heads, _TYPE[q.dtype], qp, qs, op, os, n, e,
+              _ptr(q_start, torch.int32, e + 1, self.device, "q_start"), _ptr(seq, torch.int32, e, self.device, "seq"),
+              _ptr(kv_len, torch.int32, e, self.device, "kv_len"), max_q,
+              1.0 / math.sqrt(self.head_dim) if scale is None else scale, work.data_ptr(), work.numel(), self._status)
+        return out
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):

@@ -57,3 +57,35 @@ def test_sample_arguments_are_checked(args):
     x, stride, n, vocab, u, token = args
     assert L.ijb_sample(x, stride, n, vocab, u, None, None, None, None, token, None, None) == lib.ERR_INVALID
     assert "ijb_sample" in L.ijb_last_error(None).decode()
+
+
+def attention(v, heads=4, type_=0, q=4096, qs=256, out=4096, os=256, n=2, e=1, start=256, kv_len=256, work=4096,
+              size=1 << 40):
+    return lib.load().ijb_paged_attention(ctypes.byref(v), heads, type_, q, qs, out, os, n, e, start, None, kv_len, 1,
+                                          0.125, work, size, None, None)
+
+
+@pytest.mark.parametrize("bad", BAD_VIEWS + [dict(scale_dev=8194)])
+def test_attention_views_are_checked(bad):
+    assert attention(view(**bad)) == lib.ERR_INVALID
+    assert "ijb_paged_attention" in lib.load().ijb_last_error(None).decode()
+
+
+@pytest.mark.parametrize("bad", [dict(heads=3), dict(heads=0), dict(heads=34), dict(type_=12), dict(q=None),
+                                 dict(out=None), dict(start=None), dict(kv_len=None), dict(work=None), dict(qs=255),
+                                 dict(os=255), dict(n=-1), dict(e=0), dict(e=4097), dict(q=4097), dict(type_=1, out=4097),
+                                 dict(work=4100), dict(n=1 << 30)])
+def test_attention_arguments_are_checked(bad):
+    assert attention(view(), **bad) == lib.ERR_INVALID
+
+
+def test_attention_without_tokens_is_no_launch():
+    L = lib.load()
+    before = L.ijb_kernel_launches()
+    assert attention(view(), n=0, q=None, out=None) == lib.OK
+    assert L.ijb_kernel_launches() == before
+
+
+def test_attention_workspace_of_a_bad_view_is_nothing():
+    assert lib.load().ijb_paged_attention_workspace(ctypes.byref(view(head_dim=80)), 4, 1, 1) == 0
+    assert lib.load().ijb_paged_attention_workspace(None, 4, 1, 1) == 0
