@@ -342,7 +342,7 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * [heads][head_dim], type IJB_TYPE_F32 or IJB_TYPE_F16, strides in elements):
  * the last of the kv_len_dev[e] positions of sequence seq_dev[e] (NULL: e),
  * whose K and V, the new tokens' included, the cache already holds.  A token
- * sees the positions up to its own, with softmax(scale * q . k); one before
+ * sees the positions up to its own, with softmax(scale * q . k), scale > 0; one before
  * position 0 (kv_len shorter than the entry) sees none and gets zeros.  Entries
  * may be empty; rows that belong to no entry are left as they were.  max_q > 0
  * promises that no entry has more new tokens (0: unknown): a longer one may be

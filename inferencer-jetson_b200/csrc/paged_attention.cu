@@ -47,6 +47,7 @@ struct AttnArgs {
     int n_tokens, n_entries;
     const int *q_start, *seq, *kv_len;
     int min_rows, max_rows;  // entries with rows of a KV head in this range are this kernel's
+    bool report_long;        // no other kernel takes longer ones: they are beyond the caller's max_q
     int tile_rows, unit;     // rows per tile, positions per unit
     int workers, min_units;
     float scale_log2;        // scale * log2(e)
@@ -72,8 +73,7 @@ __device__ __forceinline__ Entry entry_load(const AttnArgs &a, int e, bool repor
     if (!ok && report && a.status) atomicOr(a.status, kDevErrBadIndex);
     const long rows = ok ? static_cast<long>(x.len) * a.group : 0;
     x.rows = rows >= a.min_rows && rows <= a.max_rows ? static_cast<int>(rows) : 0;
-    if (rows > 0 && x.rows == 0 && report && a.min_rows <= 1 && a.status)
-        atomicOr(a.status, kDevErrBadIndex);  // longer than the caller's max_q
+    if (rows > a.max_rows && report && a.report_long && a.status) atomicOr(a.status, kDevErrBadIndex);
     x.tiles = (x.rows + a.tile_rows - 1) / a.tile_rows;
     return x;
 }
@@ -658,6 +658,472 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
     cp_async_wait<0>();
 }
 
+// ------------------------------------------------------------------ tile --
+//
+// 256 rows (two tiles of 128, one softmax warpgroup each) against blocks of
+// 128 positions, one CTA per SM:
+//   * warps 9..12 bring K and V blocks into a ring of shared-memory buffers, in
+//     the tensor cores' 128-byte-swizzled layout, as fp16 (e4m3 rows are
+//     converted on the way; rows behind the last position are zeros);
+//   * warp 8, one lane: S = Q K^T (K-major, from shared memory) and O += P V
+//     (P from TMEM, V as it lies: MN-major) with tcgen05.mma, M = 128, sums in
+//     TMEM; while one tile's softmax runs, the other's products do;
+//   * warps 0..3 and 4..7: one thread a row: maximum, exponentials and sum of
+//     its 128 scores, P written over S as fp16 (fp32 queries: hi and lo parts
+//     side by side); at the end of a run the output or its state.
+// The maximum is raised, and O rescaled, only when a row's scores pass it by
+// more than 2^8: until then the weights are relative to an older maximum, at
+// most 256, which fp16 and the fp32 sums hold as exactly.  TMEM: S of both
+// tiles in columns 0..255, O in 256..511.
+//
+// What bounds it: the exponentials (16 a clock and SM: 1024 clocks a tile and
+// block) beside the products (256 clocks at head_dim 64, 512 at 128, for each
+// of S and O; twice that for fp32 queries).
+
+constexpr int kTileRows = 256, kBlock = 128;
+constexpr int kTileThreads = 13 * 32, kMmaWarpId = 8, kLoadWarp0 = 9;
+
+template <int HD, typename T>
+struct Tile {
+    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr int kHalf = kBlock * 128;                 // 128 rows x 64 fp16
+    static constexpr int kPart = kHalf * (HD / 64);            // a 128-row operand tile
+    static constexpr int kQ = 2 * kPart * (kSplit ? 2 : 1);    // both tiles, hi (and lo)
+    static constexpr int kFit = (227 * 1024 - 2048 - kQ) / kPart;
+    static constexpr int kBufs = kFit > 8 ? 8 : kFit;
+    static constexpr int kSmem = kQ + kBufs * kPart + 1024 + 512;
+    static_assert(kBufs >= 3, "a V block and the next K block are in use while another loads");
+    static_assert(kBufs * kPart >= (kMaxEntries + kMaxTiles + 2) * 4, "the plan lies over the buffers");
+};
+
+struct TileCtl {
+    uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2];
+    uint32_t tmem;
+    uint32_t abort;
+};
+
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Shared-memory operand, 128-byte swizzle: 8-row groups 1024 bytes apart;
+// `lbo`: bytes between 64-element column blocks of an MN-major operand.
+__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lbo) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16 |
+           static_cast<uint64_t>(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// 32 columns of this warp's TMEM lanes, one row a thread; tm_wait completes it.
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tm_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// Byte offset of 16-byte piece c (8 fp16) of row r in a 128-row operand tile.
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+    return static_cast<uint32_t>((c >> 3) * (kBlock * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// Loads the K and V blocks of a worker's runs (128 threads, p of them).
+template <int HD, bool E4M3, int BUFS>
+__device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, TileCtl *ctl, int p) {
+    constexpr int P = E4M3 ? HD / 16 : HD / 8;    // 16-byte pieces of a cached row
+    constexpr int RS = 128 / P, STEPS = 128 / RS;  // rows a step, steps a block
+    constexpr int RB = HD * (E4M3 ? 1 : 2);
+    const int pc = p % P, pr = p / P;
+    const long v_off = static_cast<long>(a.kv.kv_heads) << a.kv.page_shift;
+    Segment s;
+    int i = 0;  // buffers filled so far
+    while (cursor_next(a, c, s)) {
+        for (int b = s.b0; b < s.b1; ++b) {
+            int row_ok = 0;
+            long row[STEPS];  // cache rows (K) of this thread's positions
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                const int pos = b * kBlock + k * RS + pr;
+                const bool live = pos < s.x.kv;
+                row[k] = live ? kv_row(a.kv, page_of(a, s.x.seq, pos), 0, s.head, pos & ((1 << a.kv.page_shift) - 1)) : 0;
+                row_ok |= live ? 1 << k : 0;
+            }
+#pragma unroll 1
+            for (int which = 0; which < 2; ++which, ++i) {
+                const int slot = i % BUFS;
+                const uint32_t dst = bufs + slot * part;
+                if constexpr (E4M3) {
+                    uint4 w[STEPS];
+                    uint32_t sc[STEPS];
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        const long r = row[k] + (which ? v_off : 0);
+                        const bool live = (row_ok >> k) & 1;
+                        w[k] = live ? *reinterpret_cast<const uint4 *>(a.kv.data + r * RB + pc * 16) : make_uint4(0, 0, 0, 0);
+                        sc[k] = live ? a.kv.scale[r] : 0u;
+                    }
+                    if (i >= BUFS) mbar_wait_bounded(&ctl->empty[slot], (i / BUFS - 1) & 1, a.status, &ctl->abort);
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        const __half2 s2 = __half2half2(scale_half(sc[k]));
+                        const uint32_t sb = *reinterpret_cast<const uint32_t *>(&s2);
+                        const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+                        uint32_t h[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            h[2 * j] = hmul2(e4m3x2_half2(u[j] & 0xffffu), sb);
+                            h[2 * j + 1] = hmul2(e4m3x2_half2(u[j] >> 16), sb);
+                        }
+                        const int r = k * RS + pr;
+                        const int flip = (pc >> 2) & 1;  // the halves of a 128-wide row start on the same banks
+                        const uint32_t at0 = dst + tile_off(r, 2 * pc), at1 = dst + tile_off(r, 2 * pc + 1);
+                        if (flip) {
+                            sts128(at1, h[4], h[5], h[6], h[7]);
+                            sts128(at0, h[0], h[1], h[2], h[3]);
+                        } else {
+                            sts128(at0, h[0], h[1], h[2], h[3]);
+                            sts128(at1, h[4], h[5], h[6], h[7]);
+                        }
+                    }
+                    proxy_fence();
+                    mbar_arrive(&ctl->full[slot]);
+                } else {
+                    if (i >= BUFS) mbar_wait_bounded(&ctl->empty[slot], (i / BUFS - 1) & 1, a.status, &ctl->abort);
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        const long r = row[k] + (which ? v_off : 0);
+                        const bool live = (row_ok >> k) & 1;
+                        cp_async16(dst + tile_off(k * RS + pr, pc), a.kv.data + (live ? r * RB : 0) + pc * 16, live);
+                    }
+                    cp_async_commit();
+                    if (i > 0) {  // the buffer before this one has arrived
+                        cp_async_wait<1>();
+                        proxy_fence();
+                        mbar_arrive(&ctl->full[(i - 1) % BUFS]);
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (!E4M3) {
+        cp_async_wait<0>();
+        proxy_fence();
+        if (i > 0) mbar_arrive(&ctl->full[(i - 1) % BUFS]);
+    }
+}
+
+// Issues the matrix products of a worker's runs (one thread).
+template <int HD, bool SPLIT, int BUFS>
+__device__ void tile_mma(const AttnArgs &a, Cursor c, uint32_t q, uint32_t bufs, int part, TileCtl *ctl, uint32_t tmem) {
+    constexpr uint32_t kIdS = (1u << 4) | (kBlock / 8) << 17 | (128u / 16) << 24;
+    constexpr uint32_t kIdO = (1u << 4) | 1u << 16 | (HD / 8) << 17 | (128u / 16) << 24;  // B is MN-major
+    constexpr int kHalf = kBlock * 128;
+    Segment s;
+    int i = 0, runs[2] = {0, 0}, blocks[2] = {0, 0};
+    auto wait_full = [&](int n) { mbar_wait_bounded(&ctl->full[n % BUFS], (n / BUFS) & 1, a.status, &ctl->abort); };
+    auto score = [&](int t, int n) {
+        const uint32_t k = bufs + (n % BUFS) * part;
+#pragma unroll
+        for (int h = 0; h < (SPLIT ? 2 : 1); ++h)
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) {
+                const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
+                mma_ss(tmem + t * 128, desc128(q + (t * (SPLIT ? 2 : 1) + h) * part + off, 16), desc128(k + off, 16), kIdS,
+                       h > 0 || ks > 0);
+            }
+        mma_commit(&ctl->s_full[t]);
+    };
+    while (cursor_next(a, c, s)) {
+        const int tiles = s.x.rows - s.ti * kTileRows > 128 ? 2 : 1, n = s.b1 - s.b0;
+        wait_full(i);
+        for (int t = 0; t < tiles; ++t) {
+            mbar_wait_bounded(&ctl->q_full[t], runs[t]++ & 1, a.status, &ctl->abort);
+            tc_after();
+            score(t, i);
+        }
+        mma_commit(&ctl->empty[i % BUFS]);
+        for (int b = 0; b < n; ++b) {
+            const int vi = i + 2 * b + 1, ki = vi + 1;
+            wait_full(vi);
+            for (int t = 0; t < tiles; ++t) {
+                mbar_wait_bounded(&ctl->p_full[t], blocks[t]++ & 1, a.status, &ctl->abort);
+                tc_after();
+                const uint32_t v = bufs + (vi % BUFS) * part;
+#pragma unroll
+                for (int ks = 0; ks < kBlock / 16; ++ks) {
+                    const uint64_t vd = desc128(v + ks * 2048, kHalf);
+                    const uint32_t pa = tmem + t * 128 + ks * (SPLIT ? 16 : 8);
+                    mma_ts(tmem + 256 + t * 128, pa, vd, kIdO, b > 0 || ks > 0);
+                    if constexpr (SPLIT) mma_ts(tmem + 256 + t * 128, pa + 8, vd, kIdO, 1);
+                }
+                if (b + 1 < n) {
+                    if (t == 0) {
+                        wait_full(ki);
+                        tc_after();
+                    }
+                    score(t, ki);
+                } else {
+                    mma_commit(&ctl->o_full[t]);
+                }
+            }
+            mma_commit(&ctl->empty[vi % BUFS]);
+            if (b + 1 < n) mma_commit(&ctl->empty[ki % BUFS]);
+        }
+        i += 2 * n;
+    }
+}
+
+// Softmax and output of tile t of a worker's runs (128 threads, row r of them).
+template <int HD, typename T>
+__device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q, int part, TileCtl *ctl, uint32_t tmem, int t,
+                             int r) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr float kRaise = 8.f;
+    const int warp = r >> 5, lane = r & 31;
+    const uint32_t ts = tmem + t * 128 + (static_cast<uint32_t>(warp * 32) << 16), to = ts + 256;
+    const T *qp = static_cast<const T *>(a.q);
+    T *op = static_cast<T *>(a.out);
+    const bool qvec = aligned4<T>(a.q, a.q_stride), ovec = aligned4<T>(a.out, a.out_stride);
+    q += t * (SPLIT ? 2 : 1) * part;
+    Segment s;
+    int runs = 0, blocks = 0;
+    while (cursor_next(a, c, s)) {
+        const int row0 = s.ti * kTileRows + t * 128;  // of the entry's rows
+        if (row0 >= s.x.rows) continue;
+        // ---- queries: a warp its own 32 rows, 8 dims a lane
+        constexpr int P = HD / 8;
+        for (int k = 0; k < P; ++k) {
+            const int qr = warp * 32 + k * (32 / P) + lane / P, pc = lane % P, row = row0 + qr;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (row < s.x.rows) {
+                const T *src = qp + static_cast<long>(s.x.q0 + row / a.group) * a.q_stride +
+                               (s.head * a.group + row % a.group) * HD + pc * 8;
+                x = load4(src, qvec);
+                y = load4(src + 4, qvec);
+            }
+            const uint32_t h[4] = {half2_bits(x.x, x.y), half2_bits(x.z, x.w), half2_bits(y.x, y.y), half2_bits(y.z, y.w)};
+            sts128(q + tile_off(qr, pc), h[0], h[1], h[2], h[3]);
+            if constexpr (SPLIT) {
+                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h[0])),
+                             f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h[1])),
+                             f2 = __half22float2(*reinterpret_cast<const __half2 *>(&h[2])),
+                             f3 = __half22float2(*reinterpret_cast<const __half2 *>(&h[3]));
+                sts128(q + part + tile_off(qr, pc), half2_bits(x.x - f0.x, x.y - f0.y), half2_bits(x.z - f1.x, x.w - f1.y),
+                       half2_bits(y.x - f2.x, y.y - f2.y), half2_bits(y.z - f3.x, y.w - f3.y));
+            }
+        }
+        proxy_fence();
+        mbar_arrive(&ctl->q_full[t]);
+
+        const int row = row0 + r;
+        const bool live = row < s.x.rows;
+        const int limit = live ? s.x.kv - s.x.len + row / a.group : -1;  // last position this row sees
+        const int all_see = s.x.kv - s.x.len + row0 / a.group;
+        float m = -INFINITY, l = 0.f;  // maximum in units of the raw scores
+        const float sc = a.scale_log2;
+        for (int b = s.b0; b < s.b1; ++b) {
+            mbar_wait_bounded(&ctl->s_full[t], blocks++ & 1, a.status, &ctl->abort);
+            tc_after();
+            const int p0 = b * kBlock;
+            const bool masked = p0 + kBlock - 1 > all_see;
+            const int seen = limit - p0;  // columns 0..seen count
+            float mx = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t x[32];
+                tm_ld32(ts + 32 * k, x);
+                tm_wait(x);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const float v = __uint_as_float(x[j]);
+                    mx = fmaxf(mx, !masked || 32 * k + j <= seen ? v : -INFINITY);
+                }
+            }
+            const bool raise = m != -INFINITY && mx * sc > m * sc + kRaise;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float alpha = raise ? ex2((m - mx) * sc) : 1.f;
+                l *= alpha;
+#pragma unroll 1
+                for (int k = 0; k < HD / 32; ++k) {
+                    uint32_t x[32];
+                    tm_ld32(to + 32 * k, x);
+                    tm_wait(x);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
+                    tm_st32(to + 32 * k, x);
+                }
+            }
+            if (raise || m == -INFINITY) m = mx;
+            const float mu = m == -INFINITY ? 0.f : m * sc;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t x[32];
+                tm_ld32(ts + 32 * k, x);
+                tm_wait(x);
+                float p[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const float v = __uint_as_float(x[j]);
+                    p[j] = ex2(fmaf(!masked || 32 * k + j <= seen ? v : -INFINITY, sc, -mu));
+                    sum += p[j];
+                }
+                if constexpr (SPLIT) {
+                    uint32_t w[32];  // two k16 steps of hi (8 columns), lo (8)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const __half2 h = __floats2half2_rn(p[2 * j], p[2 * j + 1]);
+                        const float2 f = __half22float2(h);
+                        const int at = (j >> 3) * 16 + (j & 7);
+                        w[at] = *reinterpret_cast<const uint32_t *>(&h);
+                        w[at + 8] = half2_bits(p[2 * j] - f.x, p[2 * j + 1] - f.y);
+                    }
+                    tm_st32(ts + 32 * k, w);
+                } else {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) w[j] = half2_bits(p[2 * j], p[2 * j + 1]);
+                    tm_st16(ts + 16 * k, w);
+                }
+            }
+            l += sum;
+            tm_wait_st();
+            tc_before();
+            mbar_arrive(&ctl->p_full[t]);
+        }
+        // ---- the run's end
+        mbar_wait_bounded(&ctl->o_full[t], runs++ & 1, a.status, &ctl->abort);
+        tc_after();
+        const bool whole = s.b0 == 0 && s.b1 == s.units;
+        const float inv = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
+        float *state = a.part + part_slot(s, worker) * part_floats<kTileRows, HD>();
+        const int pr = t * 128 + r;  // row within the 256
+        T *dst = op + static_cast<long>(s.x.q0 + (live ? row / a.group : 0)) * a.out_stride +
+                 (s.head * a.group + (live ? row % a.group : 0)) * HD;
+#pragma unroll 1
+        for (int k = 0; k < HD / 32; ++k) {
+            uint32_t x[32];
+            tm_ld32(to + 32 * k, x);
+            tm_wait(x);
+            if (!live) continue;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const float f0 = __uint_as_float(x[j]), f1 = __uint_as_float(x[j + 1]), f2 = __uint_as_float(x[j + 2]),
+                            f3 = __uint_as_float(x[j + 3]);
+                if (whole) store4(dst + 32 * k + j, ovec, f0 * inv, f1 * inv, f2 * inv, f3 * inv);
+                else store4(state + pr * HD + 32 * k + j, f0, f1, f2, f3);
+            }
+        }
+        if (!whole && live) {
+            state[kTileRows * HD + pr] = m == -INFINITY ? m : m * sc;
+            state[kTileRows * HD + kTileRows + pr] = l;
+        }
+        tc_before();  // O has been read before the next run's first product
+    }
+}
+
+template <int HD, bool E4M3, typename T>
+__global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const __grid_constant__ AttnArgs a) {
+    using L = Tile<HD, T>;
+    extern __shared__ uint8_t raw[];
+    __shared__ PlanOut po;
+    __shared__ TileCtl ctl;
+    const uint32_t pad = (1024u - (smem_u32(raw) & 1023u)) & 1023u;  // swizzled tiles start on 1024 bytes
+    uint8_t *smem = raw + pad;
+    const uint32_t q = smem_u32(smem), bufs = q + L::kQ;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *first = reinterpret_cast<int *>(smem + L::kQ), *sums = first + a.n_entries + 1;
+    plan_build<kTileThreads>(a, first, sums, &po);
+    const Cursor c = cursor_start(a, first, sums, po, blockIdx.x);
+    if (po.units == 0 || static_cast<long>(blockIdx.x) * po.per >= static_cast<long>(po.units) * a.kv.kv_heads) return;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 8; ++i) {
+            mbar_init(&ctl.full[i], 128);
+            mbar_init(&ctl.empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&ctl.q_full[t], 128);
+            mbar_init(&ctl.s_full[t], 1);
+            mbar_init(&ctl.p_full[t], 128);
+            mbar_init(&ctl.o_full[t], 1);
+        }
+        ctl.abort = 0u;
+        fence_barrier_init();
+    }
+    if (warp == kMmaWarpId) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();  // barriers, TMEM; the plan's shared memory becomes the buffers
+    tc_after();
+    const uint32_t tmem = ctl.tmem;
+    if (warp >= kLoadWarp0) {
+        tile_load<HD, E4M3, L::kBufs>(a, c, bufs, L::kPart, &ctl, threadIdx.x - kLoadWarp0 * 32);
+    } else if (warp == kMmaWarpId) {
+        if (lane == 0) tile_mma<HD, L::kSplit, L::kBufs>(a, c, q, bufs, L::kPart, &ctl, tmem);
+        __syncwarp();
+    } else {
+        tile_softmax<HD, T>(a, c, blockIdx.x, q, L::kPart, &ctl, tmem, warp >> 2, threadIdx.x & 127);
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == kMmaWarpId)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
 // ----------------------------------------------------------------- merge --
 
 // Joins the states of one (tile, KV head): 16 of its rows a block.
@@ -749,33 +1215,68 @@ int sm_count() {
 }
 
 template <int HD, bool E4M3, typename T>
-cudaError_t decode_launch(AttnArgs a, int sms, cudaStream_t s) {
+cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     using D = Dec<HD, E4M3>;
     const int smem = D::kSmem > kDecPlanBytes ? D::kSmem : kDecPlanBytes;
     auto kernel = ijb_paged_decode_kernel<HD, E4M3, T>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     a.min_rows = 1;
-    a.max_rows = 0x7fffffff;
+    a.max_rows = kDecRows;
+    a.report_long = all;
     a.tile_rows = kDecRows;
     a.unit = kChunk;
     a.workers = sms * D::kWarps;
     a.min_units = 1;
     kernel<<<sms, D::kWarps * 32, smem, s>>>(a);
-    ijb_paged_merge_kernel<kDecRows, HD, T><<<dim3(a.n_tokens * a.group / kDecRows + a.n_entries, a.kv.kv_heads, 1), 256, 0, s>>>(a);
+    ijb_paged_merge_kernel<kDecRows, HD, T><<<dim3(a.n_entries, a.kv.kv_heads, 1), 256, 0, s>>>(a);
+    count_launches(2);
     return cudaGetLastError();
 }
 
+template <int HD, bool E4M3, typename T>
+cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
+    using L = Tile<HD, T>;
+    auto kernel = ijb_paged_tile_kernel<HD, E4M3, T>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    if (e != cudaSuccess) return e;
+    a.min_rows = min_rows;
+    a.max_rows = 0x7fffffff;
+    a.report_long = false;
+    a.tile_rows = kTileRows;
+    a.unit = kBlock;
+    a.workers = sms;
+    a.min_units = 2;
+    kernel<<<sms, kTileThreads, L::kSmem, s>>>(a);
+    const int tiles = static_cast<int>(static_cast<long>(a.n_tokens) * a.group / kTileRows) + a.n_entries;
+    ijb_paged_merge_kernel<kTileRows, HD, T><<<dim3(tiles, a.kv.kv_heads, kTileRows / 16), 256, 0, s>>>(a);
+    count_launches(2);
+    return cudaGetLastError();
+}
+
+// Which kernels serve a call.  Entries of up to 16 rows go to the decode kernel,
+// longer ones to the tile kernel; a call that may hold longer ones and has few
+// entries leaves them all to the tile kernel, for the launches.
+template <int HD, bool E4M3, typename T>
+cudaError_t attention_call(const AttnArgs &a, int max_q, int sms, cudaStream_t s) {
+    const long most = static_cast<long>(max_q > 0 ? min(max_q, a.n_tokens) : a.n_tokens) * a.group;
+    if (most <= kDecRows) return decode_launch<HD, E4M3, T>(a, sms, true, s);
+    if (a.n_entries < 8) return tile_launch<HD, E4M3, T>(a, sms, 1, s);
+    const cudaError_t e = decode_launch<HD, E4M3, T>(a, sms, false, s);
+    return e != cudaSuccess ? e : tile_launch<HD, E4M3, T>(a, sms, kDecRows + 1, s);
+}
 template <typename T>
-cudaError_t attention_call(const AttnArgs &a, bool e4m3, int sms, cudaStream_t s) {
-    if (a.kv.head_dim == 64) return e4m3 ? decode_launch<64, true, T>(a, sms, s) : decode_launch<64, false, T>(a, sms, s);
-    return e4m3 ? decode_launch<128, true, T>(a, sms, s) : decode_launch<128, false, T>(a, sms, s);
+cudaError_t attention_call(const AttnArgs &a, bool e4m3, int max_q, int sms, cudaStream_t s) {
+    if (a.kv.head_dim == 64)
+        return e4m3 ? attention_call<64, true, T>(a, max_q, sms, s) : attention_call<64, false, T>(a, max_q, sms, s);
+    return e4m3 ? attention_call<128, true, T>(a, max_q, sms, s) : attention_call<128, false, T>(a, max_q, sms, s);
 }
 
 constexpr size_t kPlanBytes = (kPlanHead + 3 * kMaxTiles + 8) * sizeof(int);
 
 size_t workspace_bytes(int sms, int head_dim) {
-    return kPlanBytes + static_cast<size_t>(sms) * 8 * 2 * kDecRows * (head_dim + 2) * sizeof(float);
+    const int rows = kTileRows > 8 * kDecRows ? kTileRows : 8 * kDecRows;  // an SM's workers, two states each
+    return kPlanBytes + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -813,6 +1314,7 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         if (n_entries < 1 || n_entries > kMaxEntries) return kv_fail(IJB_ERR_INVALID, fn, "n_entries must be 1..4096");
         if (n_tokens < 0) return kv_fail(IJB_ERR_INVALID, fn, "negative token count");
         if (n_tokens == 0) return IJB_OK;
+        if (!(scale > 0.f && scale <= 3.402823466e38f)) return kv_fail(IJB_ERR_INVALID, fn, "scale must be positive and finite");
         if (!q_dev || !out_dev || !q_start_dev || !kv_len_dev || !workspace_dev)
             return kv_fail(IJB_ERR_INVALID, fn, "null argument");
         const int elem = type == IJB_TYPE_F32 ? 4 : 2;
@@ -822,7 +1324,7 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
             return kv_fail(IJB_ERR_INVALID, fn, "rows must be aligned to their elements");
         if (reinterpret_cast<uintptr_t>(workspace_dev) % 16)
             return kv_fail(IJB_ERR_INVALID, fn, "the workspace must be 16-byte aligned");
-        if (static_cast<long>(n_tokens) * (heads / kv->kv_heads) / kDecRows + n_entries > kMaxTiles)
+        if (static_cast<long>(n_tokens) * (heads / kv->kv_heads) / kTileRows + n_entries > kMaxTiles)
             return kv_fail(IJB_ERR_INVALID, fn, "too many rows for one call");
         const int sms = sm_count();
         if (sms < 1) return kv_fail(IJB_ERR_CUDA, fn, "no CUDA device");
@@ -845,11 +1347,9 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         a.status = status_dev;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const bool e4m3 = kv->type == IJB_KV_E4M3;
-        const cudaError_t e = type == IJB_TYPE_F32 ? attention_call<float>(a, e4m3, sms, s)
-                                                   : attention_call<__half>(a, e4m3, sms, s);
+        const cudaError_t e = type == IJB_TYPE_F32 ? attention_call<float>(a, e4m3, max_q, sms, s)
+                                                   : attention_call<__half>(a, e4m3, max_q, sms, s);
         if (e != cudaSuccess) return kv_fail(IJB_ERR_CUDA, fn, cudaGetErrorString(e));
-        count_launches(2);
-        (void)max_q;
         return IJB_OK;
     } catch (...) {
         return IJB_ERR_NOMEM;
