@@ -51,11 +51,10 @@ struct AttnArgs {
     int tile_rows, unit;     // rows per tile, positions per unit
     int workers, min_units;
     float scale_log2;        // scale * log2(e)
-    int *plan;               // workspace: kPlanHead ints, tile -> entry, tile -> first unit
+    int4 *left;              // workspace: per worker, the tile it leaves to be gone on with
     float *part;             // workspace: two states per worker
     uint32_t *status;
 };
-constexpr int kPlanHead = 8;  // tiles, units per KV head, units per worker
 
 struct Entry {
     int q0, len, kv, seq, rows, tiles;
@@ -134,8 +133,8 @@ struct PlanOut {
 };
 
 // Cuts the call's work: `first` [n_entries + 1] receives each entry's first
-// tile, `sums` [tiles + 1] each tile's first unit (of one KV head).  Block 0
-// keeps them in the workspace for the merge.  All NT threads call it.
+// tile, `sums` [tiles + 1] each tile's first unit (of one KV head).  All NT
+// threads call it.
 template <int NT>
 __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po) {
     const bool lead = blockIdx.x == 0;
@@ -154,21 +153,14 @@ __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po
     base = 0;
     for (int t0 = 0; t0 < tiles; t0 += NT) {
         const int t = t0 + static_cast<int>(threadIdx.x);
-        int n = 0, e = 0;
+        int n = 0;
         if (t < tiles) {
-            e = find_le(first, a.n_entries, t);
+            const int e = find_le(first, a.n_entries, t);
             n = tile_units(a, entry_load(a, e, false), t - first[e]);
         }
         int total;
         const int inc = block_scan_int<NT>(n, po->warp_sums, &total);
-        if (t < tiles) {
-            sums[t] = base + inc - n;
-            if (lead) {
-                a.plan[kPlanHead + t] = e;
-                a.plan[kPlanHead + kMaxTiles + t] = t - first[e];
-                a.plan[kPlanHead + 2 * kMaxTiles + t] = base + inc - n;
-            }
-        }
+        if (t < tiles) sums[t] = base + inc - n;
         base += total;
     }
     const long all = static_cast<long>(base) * a.kv.kv_heads;
@@ -178,12 +170,6 @@ __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po
         po->tiles = tiles;
         po->units = base;
         po->per = per;
-        if (lead) {
-            a.plan[kPlanHead + 2 * kMaxTiles + tiles] = base;
-            a.plan[0] = tiles;
-            a.plan[1] = base;
-            a.plan[2] = per;
-        }
     }
     __syncthreads();
 }
@@ -247,6 +233,14 @@ __device__ __forceinline__ long part_slot(const Segment &s, int worker) { return
 template <int ROWS, int HD>
 __host__ __device__ constexpr long part_floats() { return static_cast<long>(ROWS) * (HD + 2); }
 
+// What the merge has to join for a worker: entry, tile, head and states of the
+// tile that its last run begins and does not end; no states if there is none.
+__device__ __forceinline__ int4 left_none() { return make_int4(0, 0, 0, 0); }
+__device__ __forceinline__ int4 left_of(const Segment &s, int per) {
+    if (s.b0 > 0 || s.b1 == s.units) return left_none();
+    return make_int4(s.e, s.ti, s.head, 1 + (s.units - s.b1 + per - 1) / per);
+}
+
 __device__ __forceinline__ void store4(float *p, float a, float b, float c, float d) {
     *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
 }
@@ -278,6 +272,17 @@ __device__ __forceinline__ float4 load4(const __half *p, bool vec) {
     const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)),
                  y = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
     return make_float4(x.x, x.y, y.x, y.y);
+}
+// Eight fp16 values as they are.
+__device__ __forceinline__ float4 load8_raw(const __half *p, bool vec) {
+    if (vec) return *reinterpret_cast<const float4 *>(p);
+    __half h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = p[i];
+    return *reinterpret_cast<const float4 *>(h);
+}
+__device__ __forceinline__ bool aligned16(const void *p, long stride_bytes) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride_bytes % 16 == 0;
 }
 template <typename T>
 __device__ __forceinline__ bool aligned4(const void *p, long stride) {
@@ -446,6 +451,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
 
     // ---- the computing side
     int stage = 0;
+    int4 left = left_none();
     Segment s;
     while (cursor_next(a, use_c, s)) {
         const int row0 = s.ti * kDecRows, rows = min(kDecRows, s.x.rows - row0);
@@ -624,6 +630,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
         }
 
         // ---- the run's end: the output, or its state
+        left = left_of(s, po.per);
         const bool whole = s.b0 == 0 && s.b1 == s.units;
         float *part = a.part + part_slot(s, worker) * part_floats<kDecRows, HD>();
 #pragma unroll
@@ -656,16 +663,17 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
         }
     }
     cp_async_wait<0>();
+    if (lane == 0) a.left[worker] = left;
 }
 
 // ------------------------------------------------------------------ tile --
 //
 // 256 rows (two tiles of 128, one softmax warpgroup each) against blocks of
 // 128 positions, one CTA per SM:
-//   * warps 9..12 bring K and V blocks into a ring of shared-memory buffers, in
+//   * warps 8..11 bring K and V blocks into a ring of shared-memory buffers, in
 //     the tensor cores' 128-byte-swizzled layout, as fp16 (e4m3 rows are
 //     converted on the way; rows behind the last position are zeros);
-//   * warp 8, one lane: S = Q K^T (K-major, from shared memory) and O += P V
+//   * warps 12 and 13, one a tile: S = Q K^T (K-major, from shared memory) and O += P V
 //     (P from TMEM, V as it lies: MN-major) with tcgen05.mma, M = 128, sums in
 //     TMEM; while one tile's softmax runs, the other's products do;
 //   * warps 0..3 and 4..7: one thread a row: maximum, exponentials and sum of
@@ -681,7 +689,11 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
 // of S and O; twice that for fp32 queries).
 
 constexpr int kTileRows = 256, kBlock = 128;
-constexpr int kTileThreads = 13 * 32, kMmaWarpId = 8, kLoadWarp0 = 9;
+constexpr int kTileThreads = 16 * 32, kMmaWarpId = 12, kLoadWarp0 = 8;
+// Registers a thread of each warpgroup; the sum is what the launch gives them:
+// 2 * 168 + 112 + 64 = 4 * 128.
+constexpr int kSoftmaxRegs = 168, kLoadRegs = 112, kMmaRegs = 64;
+static_assert(2 * kSoftmaxRegs + kLoadRegs + kMmaRegs <= 4 * 128, "register shares");
 
 template <int HD, typename T>
 struct Tile {
@@ -697,11 +709,40 @@ struct Tile {
 };
 
 struct TileCtl {
-    uint64_t full[8], empty[8], q_full[2], s_full[2], p_full[2], o_full[2];
+    uint64_t full[8], empty[8], q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
     uint32_t tmem;
     uint32_t abort;
 };
 
+__device__ __forceinline__ bool try_bar(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// mbar_wait_bounded without its call: a call does not go with warps of
+// different register shares.
+__device__ __forceinline__ void wait_bar(const AttnArgs &a, TileCtl *ctl, uint64_t *bar, uint32_t parity) {
+    if (try_bar(bar, parity)) return;
+    volatile uint32_t *abort = &ctl->abort;
+    uint64_t start = 0;
+#pragma unroll 1
+    for (uint32_t n = 1; !try_bar(bar, parity); ++n) {
+        if ((n & 255u) != 0) continue;
+        if (*abort) return;
+        const uint64_t now = global_timer_ns();
+        if (start == 0) {
+            start = now;
+        } else if (now - start > kWaitLimitNs) {
+            *abort = 1u;
+            if (a.status) atomicOr(a.status, kDevErrWaitTimeout);
+            return;
+        }
+    }
+}
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -710,6 +751,11 @@ __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lbo) {
     return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16 |
            static_cast<uint64_t>(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(ok));
+    return ok != 0;
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -777,149 +823,379 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c) {
     return static_cast<uint32_t>((c >> 3) * (kBlock * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// The positions of a 128-position block that one of the 128 loading threads
+// copies: LANES 16-byte pieces of a row side by side (an e4m3 row's four then
+// fall on different banks than the next row's once they are fp16), HALVES times.
+// Page ids are read a block ahead, for their latency.
+template <int HD, bool E4M3>
+struct Rows {
+    static constexpr int LANES = E4M3 ? 4 : 8, HALVES = HD / 64;
+    static constexpr int RS = 128 / LANES, N = 128 / RS;  // rows a step, rows of a thread
+    static constexpr int RB = HD * (E4M3 ? 1 : 2);
+    int next[N];   // page ids of the block after this one
+    long row[N];   // cache rows (K)
+    int live;      // bit k: row k's position exists
+    Segment s;
+    int b;
+    bool more;
+    __device__ __forceinline__ void peek(const AttnArgs &a, int pr) {
+        if (!more) return;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int pos = b * kBlock + k * RS + pr;
+            next[k] = pos < s.x.kv ? a.kv.page_table[static_cast<long>(s.x.seq) * a.kv.max_pages + (pos >> a.kv.page_shift)] : -1;
+        }
+    }
+    __device__ __forceinline__ void start(const AttnArgs &a, Cursor &c, int pr) {
+        more = cursor_next(a, c, s);
+        b = s.b0;
+        peek(a, pr);
+    }
+    // Makes the peeked block the current one and peeks the next; false at the end.
+    __device__ __forceinline__ bool step(const AttnArgs &a, Cursor &c, int pr) {
+        if (!more) return false;
+        live = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int pos = b * kBlock + k * RS + pr;
+            const bool in = pos < s.x.kv, ok = next[k] >= 0 && next[k] < a.kv.num_pages;
+            if (in && !ok && a.status) atomicOr(a.status, kDevErrBadIndex);
+            live |= in ? 1 << k : 0;
+            row[k] = in ? kv_row(a.kv, ok ? next[k] : 0, 0, s.head, pos & ((1 << a.kv.page_shift) - 1)) : 0;
+        }
+        if (++b == s.b1) {
+            more = cursor_next(a, c, s);
+            b = s.b0;
+        }
+        peek(a, pr);
+        return true;
+    }
+};
+
 // Loads the K and V blocks of a worker's runs (128 threads, p of them).
 template <int HD, bool E4M3, int BUFS>
 __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, TileCtl *ctl, int p) {
-    constexpr int P = E4M3 ? HD / 16 : HD / 8;    // 16-byte pieces of a cached row
-    constexpr int RS = 128 / P, STEPS = 128 / RS;  // rows a step, steps a block
-    constexpr int RB = HD * (E4M3 ? 1 : 2);
-    const int pc = p % P, pr = p / P;
+    using R = Rows<HD, E4M3>;
+    constexpr int STEPS = R::N * R::HALVES, RB = R::RB;
+    const int pc = p % R::LANES, pr = p / R::LANES;
     const long v_off = static_cast<long>(a.kv.kv_heads) << a.kv.page_shift;
-    Segment s;
+    R rows;
+    rows.start(a, c, pr);
+    auto wait_empty = [&](int i) {
+        if (i >= BUFS) wait_bar(a, ctl, &ctl->empty[i % BUFS], (i / BUFS - 1) & 1);
+    };
     int i = 0;  // buffers filled so far
-    while (cursor_next(a, c, s)) {
-        for (int b = s.b0; b < s.b1; ++b) {
-            int row_ok = 0;
-            long row[STEPS];  // cache rows (K) of this thread's positions
+    if constexpr (E4M3) {
+        uint4 wk[STEPS], wv[STEPS];
+        uint32_t sk[R::N], sv[R::N];
+        auto load = [&](uint4(&w)[STEPS], uint32_t(&sc)[R::N], long off) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k) {
-                const int pos = b * kBlock + k * RS + pr;
-                const bool live = pos < s.x.kv;
-                row[k] = live ? kv_row(a.kv, page_of(a, s.x.seq, pos), 0, s.head, pos & ((1 << a.kv.page_shift) - 1)) : 0;
-                row_ok |= live ? 1 << k : 0;
+                const int j = k / R::HALVES, h = k % R::HALVES;
+                const bool in = (rows.live >> j) & 1;
+                const long r = rows.row[j] + off;
+                w[k] = in ? *reinterpret_cast<const uint4 *>(a.kv.data + r * RB + (pc + h * R::LANES) * 16)
+                          : make_uint4(0, 0, 0, 0);
+                if (h == 0) sc[j] = in ? a.kv.scale[r] : 0u;
             }
+        };
+        auto store = [&](const uint4(&w)[STEPS], const uint32_t(&sc)[R::N]) {
+            wait_empty(i);
+            const uint32_t dst = bufs + (i % BUFS) * part;
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                const int j = k / R::HALVES, c2 = 2 * (pc + (k % R::HALVES) * R::LANES);
+                const __half2 s2 = __half2half2(scale_half(sc[j]));
+                const uint32_t sb = *reinterpret_cast<const uint32_t *>(&s2);
+                const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+                uint32_t h[8];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    h[2 * n] = hmul2(e4m3x2_half2(u[n] & 0xffffu), sb);
+                    h[2 * n + 1] = hmul2(e4m3x2_half2(u[n] >> 16), sb);
+                }
+                const int r = j * R::RS + pr;
+                sts128(dst + tile_off(r, c2), h[0], h[1], h[2], h[3]);
+                sts128(dst + tile_off(r, c2 + 1), h[4], h[5], h[6], h[7]);
+            }
+            proxy_fence();
+            mbar_arrive(&ctl->full[i % BUFS]);
+            ++i;
+        };
+        bool more = rows.step(a, c, pr);
+        if (more) load(wk, sk, 0);
+        while (more) {
+            load(wv, sv, v_off);
+            store(wk, sk);
+            more = rows.step(a, c, pr);
+            if (more) load(wk, sk, 0);
+            store(wv, sv);
+        }
+    } else {
+        // a buffer is handed over once LAG later ones are on their way.  The MMA
+        // warp frees a V buffer only when the K buffer behind it is full too, so
+        // at most BUFS - 2 may be unannounced.
+        constexpr int LAG = BUFS >= 6 ? 3 : (BUFS >= 4 ? 2 : 1);
+        while (rows.step(a, c, pr)) {
 #pragma unroll 1
             for (int which = 0; which < 2; ++which, ++i) {
-                const int slot = i % BUFS;
-                const uint32_t dst = bufs + slot * part;
-                if constexpr (E4M3) {
-                    uint4 w[STEPS];
-                    uint32_t sc[STEPS];
+                wait_empty(i);
+                const uint32_t dst = bufs + (i % BUFS) * part;
 #pragma unroll
-                    for (int k = 0; k < STEPS; ++k) {
-                        const long r = row[k] + (which ? v_off : 0);
-                        const bool live = (row_ok >> k) & 1;
-                        w[k] = live ? *reinterpret_cast<const uint4 *>(a.kv.data + r * RB + pc * 16) : make_uint4(0, 0, 0, 0);
-                        sc[k] = live ? a.kv.scale[r] : 0u;
-                    }
-                    if (i >= BUFS) mbar_wait_bounded(&ctl->empty[slot], (i / BUFS - 1) & 1, a.status, &ctl->abort);
-#pragma unroll
-                    for (int k = 0; k < STEPS; ++k) {
-                        const __half2 s2 = __half2half2(scale_half(sc[k]));
-                        const uint32_t sb = *reinterpret_cast<const uint32_t *>(&s2);
-                        const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-                        uint32_t h[8];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            h[2 * j] = hmul2(e4m3x2_half2(u[j] & 0xffffu), sb);
-                            h[2 * j + 1] = hmul2(e4m3x2_half2(u[j] >> 16), sb);
-                        }
-                        const int r = k * RS + pr;
-                        const int flip = (pc >> 2) & 1;  // the halves of a 128-wide row start on the same banks
-                        const uint32_t at0 = dst + tile_off(r, 2 * pc), at1 = dst + tile_off(r, 2 * pc + 1);
-                        if (flip) {
-                            sts128(at1, h[4], h[5], h[6], h[7]);
-                            sts128(at0, h[0], h[1], h[2], h[3]);
-                        } else {
-                            sts128(at0, h[0], h[1], h[2], h[3]);
-                            sts128(at1, h[4], h[5], h[6], h[7]);
-                        }
-                    }
+                for (int k = 0; k < STEPS; ++k) {
+                    const int j = k / R::HALVES, c = pc + (k % R::HALVES) * R::LANES;
+                    const bool in = (rows.live >> j) & 1;
+                    const long r = in ? rows.row[j] + (which ? v_off : 0) : 0;
+                    cp_async16(dst + tile_off(j * R::RS + pr, c), a.kv.data + r * RB + c * 16, in);
+                }
+                cp_async_commit();
+                if (i >= LAG) {
+                    cp_async_wait<LAG>();
                     proxy_fence();
-                    mbar_arrive(&ctl->full[slot]);
-                } else {
-                    if (i >= BUFS) mbar_wait_bounded(&ctl->empty[slot], (i / BUFS - 1) & 1, a.status, &ctl->abort);
-#pragma unroll
-                    for (int k = 0; k < STEPS; ++k) {
-                        const long r = row[k] + (which ? v_off : 0);
-                        const bool live = (row_ok >> k) & 1;
-                        cp_async16(dst + tile_off(k * RS + pr, pc), a.kv.data + (live ? r * RB : 0) + pc * 16, live);
-                    }
-                    cp_async_commit();
-                    if (i > 0) {  // the buffer before this one has arrived
-                        cp_async_wait<1>();
-                        proxy_fence();
-                        mbar_arrive(&ctl->full[(i - 1) % BUFS]);
-                    }
+                    mbar_arrive(&ctl->full[(i - LAG) % BUFS]);
                 }
             }
         }
-    }
-    if constexpr (!E4M3) {
         cp_async_wait<0>();
         proxy_fence();
-        if (i > 0) mbar_arrive(&ctl->full[(i - 1) % BUFS]);
+        for (int k = max(0, i - LAG); k < i; ++k) mbar_arrive(&ctl->full[k % BUFS]);
     }
 }
 
-// Issues the matrix products of a worker's runs (one thread).
+// Issues tile t's matrix products of a worker's runs (one warp).  A thread gets
+// one product in about 130 clocks, whatever its width, and two warps twice as
+// many: with one warp for both tiles the products of 128 columns (64 clocks)
+// waited for their issue.
 template <int HD, bool SPLIT, int BUFS>
-__device__ void tile_mma(const AttnArgs &a, Cursor c, uint32_t q, uint32_t bufs, int part, TileCtl *ctl, uint32_t tmem) {
+__device__ void tile_mma(const AttnArgs &a, Cursor c, uint32_t q, uint32_t bufs, int part, TileCtl *ctl, uint32_t tmem, int t) {
     constexpr uint32_t kIdS = (1u << 4) | (kBlock / 8) << 17 | (128u / 16) << 24;
     constexpr uint32_t kIdO = (1u << 4) | 1u << 16 | (HD / 8) << 17 | (128u / 16) << 24;  // B is MN-major
     constexpr int kHalf = kBlock * 128;
+    q += t * (SPLIT ? 2 : 1) * part;
+    const uint32_t ts = tmem + t * 128, to = ts + 256;
     Segment s;
-    int i = 0, runs[2] = {0, 0}, blocks[2] = {0, 0};
-    auto wait_full = [&](int n) { mbar_wait_bounded(&ctl->full[n % BUFS], (n / BUFS) & 1, a.status, &ctl->abort); };
-    auto score = [&](int t, int n) {
-        const uint32_t k = bufs + (n % BUFS) * part;
+    int i = 0;
+    uint32_t runs = 0, blocks = 0;
+    auto wait_full = [&](int n) { wait_bar(a, ctl, &ctl->full[n % BUFS], (n / BUFS) & 1); };
+    auto score = [&](int n) {  // S = Q K^T, by the elected lane
+        const uint64_t qd = desc128(q, 16), kd = desc128(bufs + (n % BUFS) * part, 16);
 #pragma unroll
         for (int h = 0; h < (SPLIT ? 2 : 1); ++h)
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks) {
-                const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
-                mma_ss(tmem + t * 128, desc128(q + (t * (SPLIT ? 2 : 1) + h) * part + off, 16), desc128(k + off, 16), kIdS,
-                       h > 0 || ks > 0);
+                const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
+                mma_ss(ts, qd + off + h * (part >> 4), kd + off, kIdS, h > 0 || ks > 0);
             }
         mma_commit(&ctl->s_full[t]);
     };
     while (cursor_next(a, c, s)) {
-        const int tiles = s.x.rows - s.ti * kTileRows > 128 ? 2 : 1, n = s.b1 - s.b0;
-        wait_full(i);
-        for (int t = 0; t < tiles; ++t) {
-            mbar_wait_bounded(&ctl->q_full[t], runs[t]++ & 1, a.status, &ctl->abort);
-            tc_after();
-            score(t, i);
+        const int n = s.b1 - s.b0;
+        if (t == 1 && s.x.rows - s.ti * kTileRows <= 128) {  // no rows here: pass the buffers on
+            for (int k = 0; k < 2 * n; ++k, ++i) {
+                wait_full(i);
+                if (elect_one()) mbar_arrive(&ctl->empty[i % BUFS]);
+            }
+            continue;
         }
-        mma_commit(&ctl->empty[i % BUFS]);
+        wait_full(i);
+        wait_bar(a, ctl, &ctl->q_full[t], runs++ & 1);
+        tc_after();
+        if (elect_one()) {
+            score(i);
+            mma_commit(&ctl->empty[i % BUFS]);
+        }
         for (int b = 0; b < n; ++b) {
             const int vi = i + 2 * b + 1, ki = vi + 1;
             wait_full(vi);
-            for (int t = 0; t < tiles; ++t) {
-                mbar_wait_bounded(&ctl->p_full[t], blocks[t]++ & 1, a.status, &ctl->abort);
-                tc_after();
-                const uint32_t v = bufs + (vi % BUFS) * part;
+            const uint64_t vd = desc128(bufs + (vi % BUFS) * part, kHalf);
+            auto value = [&](int k0) {  // O += P V over 64 positions
 #pragma unroll
-                for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    const uint64_t vd = desc128(v + ks * 2048, kHalf);
-                    const uint32_t pa = tmem + t * 128 + ks * (SPLIT ? 16 : 8);
-                    mma_ts(tmem + 256 + t * 128, pa, vd, kIdO, b > 0 || ks > 0);
-                    if constexpr (SPLIT) mma_ts(tmem + 256 + t * 128, pa + 8, vd, kIdO, 1);
+                for (int ks = k0; ks < k0 + 4; ++ks) {
+                    mma_ts(to, ts + ks * (SPLIT ? 16 : 8), vd + ks * (2048 >> 4), kIdO, b > 0 || ks > 0);
+                    if constexpr (SPLIT) mma_ts(to, ts + ks * 16 + 8, vd + ks * (2048 >> 4), kIdO, 1);
                 }
-                if (b + 1 < n) {
-                    if (t == 0) {
-                        wait_full(ki);
-                        tc_after();
-                    }
-                    score(t, ki);
-                } else {
-                    mma_commit(&ctl->o_full[t]);
-                }
+            };
+            wait_bar(a, ctl, &ctl->p_half[t], blocks & 1);
+            tc_after();
+            if (elect_one()) value(0);
+            __syncwarp();
+            if (b + 1 < n) wait_full(ki);
+            wait_bar(a, ctl, &ctl->p_full[t], blocks++ & 1);
+            tc_after();
+            if (elect_one()) {
+                value(4);
+                if (b + 1 < n) score(ki);
+                else mma_commit(&ctl->o_full[t]);
+                mma_commit(&ctl->empty[vi % BUFS]);
+                if (b + 1 < n) mma_commit(&ctl->empty[ki % BUFS]);
             }
-            mma_commit(&ctl->empty[vi % BUFS]);
-            if (b + 1 < n) mma_commit(&ctl->empty[ki % BUFS]);
         }
         i += 2 * n;
+    }
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return d;
+}
+
+// 2^x of a pair on the FMA pipes, for x <= 2^8 (below -126: 2^-126 or so): with
+// n = round(x) and f = x - n in [-1/2, 1/2], 2^f by a polynomial of degree 4, fitted by least
+// squares of the relative error over Chebyshev nodes (off by 1e-5 at most), n added to the
+// exponent.  Adding 1.5 * 2^23 rounds x and leaves n in the low bits.
+constexpr float kE1 = 0.693121995f, kE2 = 0.240237185f, kE3 = 0.055916894f, kE4 = 0.009600396f;
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 magic = make_float2(12582912.f, 12582912.f), one = make_float2(1.f, 1.f);
+    const float2 k = add2(x, magic);
+    const float2 n = add2(k, make_float2(-12582912.f, -12582912.f));
+    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 p = make_float2(kE4, kE4);
+    p = fma2(p, f, make_float2(kE3, kE3));
+    p = fma2(p, f, make_float2(kE2, kE2));
+    p = fma2(p, f, make_float2(kE1, kE1));
+    p = fma2(p, f, one);
+    p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(k.x) << 23));
+    p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(k.y) << 23));
+    return p;
+}
+
+// One row's 128 scores (TMEM columns of ts) become its weights there; m and l
+// are the row's maximum and sum.  MASK: only columns 0..seen count.
+constexpr int kMufuPairs = 6;  // of 8 pairs, on the exponential unit
+template <int HD, bool SPLIT, bool MASK>
+__device__ __forceinline__ void softmax_block(uint32_t ts, float sc, int seen, uint64_t *half, float &m, float &l) {
+    constexpr float kRaise = 8.f;
+    uint32_t x[2][32];
+    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    tm_ld32(ts, x[0]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        tm_wait(x[k & 1]);
+        tm_ld32(ts + 32 * ((k + 1) & 3), x[(k + 1) & 1]);  // at the end the first columns again
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            float v = __uint_as_float(x[k & 1][j]);
+            if (MASK) v = 32 * k + j <= seen ? v : -INFINITY;
+            mx4[j & 3] = fmaxf(mx4[j & 3], v);
+        }
+    }
+    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+    const bool raise = m != -INFINITY && mx * sc > m * sc + kRaise;
+    if (__any_sync(0xffffffffu, raise)) {
+        const float alpha = raise ? ex2((m - mx) * sc) : 1.f;
+        l *= alpha;
+        const uint32_t to = ts + 256;
+#pragma unroll 1
+        for (int k = 0; k < HD / 32; ++k) {
+            uint32_t o[32];
+            tm_ld32(to + 32 * k, o);
+            tm_wait(o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tm_st32(to + 32 * k, o);
+        }
+    }
+    if (raise || m == -INFINITY) m = mx;
+    const float mu = m == -INFINITY ? 0.f : m * sc;
+    const float2 sc2 = make_float2(sc, sc), mu2 = make_float2(-mu, -mu);
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // two k16 steps of the second product
+        tm_wait(x[k & 1]);
+        if (k < 3) tm_ld32(ts + 32 * (k + 1), x[(k + 1) & 1]);
+        uint32_t w[SPLIT ? 32 : 16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            float2 v = make_float2(__uint_as_float(x[k & 1][2 * j]), __uint_as_float(x[k & 1][2 * j + 1]));
+            v = fma2(v, sc2, mu2);
+            if (MASK) {
+                v.x = 32 * k + 2 * j <= seen ? v.x : -INFINITY;
+                v.y = 32 * k + 2 * j + 1 <= seen ? v.y : -INFINITY;
+            }
+            // some pairs on the FMA pipes, the exponential unit being the busier one
+            if (!SPLIT && (j & 7) >= kMufuPairs) {
+                v = ex2_poly(v);
+            } else {
+                v.x = ex2(v.x);
+                v.y = ex2(v.y);
+            }
+            sum[j & 1] = add2(sum[j & 1], v);
+            if constexpr (SPLIT) {
+                // hi: the weight's first 11 bits, lo: the rest (8 columns each a step)
+                const float2 hi = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xffffe000u),
+                                              __uint_as_float(__float_as_uint(v.y) & 0xffffe000u));
+                const int at = (j >> 3) * 16 + (j & 7);
+                w[at] = half2_bits(hi.x, hi.y);
+                w[at + 8] = half2_bits(v.x - hi.x, v.y - hi.y);
+            } else {
+                w[j] = half2_bits(v.x, v.y);
+            }
+        }
+        if constexpr (SPLIT) tm_st32(ts + 32 * k, w);
+        else tm_st16(ts + 16 * k, w);
+        if (k == 1) {  // the second product may start on the first 64 positions
+            tm_wait_st();
+            tc_before();
+            mbar_arrive(half);
+        }
+    }
+    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+}
+
+// Writes a warp's 32 rows of O (TMEM columns of `to`, one row a lane), times
+// inv, at dst + to_row (each lane its own row's), the first `rows` of them.
+template <int HD, typename O>
+__device__ __forceinline__ void write_rows(uint32_t to, uint32_t st, O *dst, bool vec, long to_row, int rows, float inv,
+                                           int lane) {
+    constexpr int E = 16 / sizeof(O), D = 8 * E;  // elements of a 16-byte piece, of a pass
+#pragma unroll 1
+    for (int d0 = 0; d0 < HD; d0 += D) {
+#pragma unroll
+        for (int h = 0; h < D / 32; ++h) {
+            uint32_t x[32];
+            tm_ld32(to + d0 + 32 * h, x);
+            tm_wait(x);
+#pragma unroll
+            for (int c = 0; c < 32 / E; ++c) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (sizeof(O) == 4)
+                        w[i] = __float_as_uint(__uint_as_float(x[4 * c + i]) * inv);
+                    else
+                        w[i] = half2_bits(__uint_as_float(x[8 * c + 2 * i]) * inv, __uint_as_float(x[8 * c + 2 * i + 1]) * inv);
+                }
+                sts128(st + lane * 128 + (((h * (32 / E) + c) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int r = 4 * k + (lane >> 3), c = lane & 7;
+            O *p = dst + __shfl_sync(0xffffffffu, to_row, r) + d0 + c * E;
+            const uint4 v = lds128(st + r * 128 + ((c ^ (r & 7)) << 4));
+            if (r >= rows) continue;
+            if (vec) {
+                *reinterpret_cast<uint4 *>(p) = v;
+            } else {
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < E; ++i) p[i] = reinterpret_cast<const O *>(u)[i];
+            }
+        }
+        __syncwarp();
     }
 }
 
@@ -928,38 +1204,56 @@ template <int HD, typename T>
 __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q, int part, TileCtl *ctl, uint32_t tmem, int t,
                              int r) {
     constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr float kRaise = 8.f;
     const int warp = r >> 5, lane = r & 31;
     const uint32_t ts = tmem + t * 128 + (static_cast<uint32_t>(warp * 32) << 16), to = ts + 256;
     const T *qp = static_cast<const T *>(a.q);
     T *op = static_cast<T *>(a.out);
-    const bool qvec = aligned4<T>(a.q, a.q_stride), ovec = aligned4<T>(a.out, a.out_stride);
+    [[maybe_unused]] const bool qvec = aligned4<T>(a.q, a.q_stride);
+    [[maybe_unused]] const bool qvec8 = aligned16(a.q, a.q_stride * sizeof(T));
+    const bool ovec = aligned16(a.out, a.out_stride * sizeof(T));
     q += t * (SPLIT ? 2 : 1) * part;
     Segment s;
     int runs = 0, blocks = 0;
     while (cursor_next(a, c, s)) {
         const int row0 = s.ti * kTileRows + t * 128;  // of the entry's rows
         if (row0 >= s.x.rows) continue;
-        // ---- queries: a warp its own 32 rows, 8 dims a lane
-        constexpr int P = HD / 8;
-        for (int k = 0; k < P; ++k) {
-            const int qr = warp * 32 + k * (32 / P) + lane / P, pc = lane % P, row = row0 + qr;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-            if (row < s.x.rows) {
-                const T *src = qp + static_cast<long>(s.x.q0 + row / a.group) * a.q_stride +
-                               (s.head * a.group + row % a.group) * HD + pc * 8;
-                x = load4(src, qvec);
-                y = load4(src + 4, qvec);
+        // ---- queries: a warp its own 32 rows, 8 dims a lane; eight rows' loads in flight
+        constexpr int P = HD / 8, RQ = 32 / P, B = SPLIT ? 4 : 8;  // lanes a row, rows a step, steps a batch
+#pragma unroll 1
+        for (int k0 = 0; k0 < P; k0 += B) {
+            float4 x[B], y[B];
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const int row = row0 + warp * 32 + (k0 + k) * RQ + lane / P;
+                x[k] = y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (row < s.x.rows) {
+                    const T *src = qp + static_cast<long>(s.x.q0 + row / a.group) * a.q_stride +
+                                   (s.head * a.group + row % a.group) * HD + (lane % P) * 8;
+                    if constexpr (SPLIT) {
+                        x[k] = load4(src, qvec);
+                        y[k] = load4(src + 4, qvec);
+                    } else {
+                        x[k] = load8_raw(src, qvec8);
+                    }
+                }
             }
-            const uint32_t h[4] = {half2_bits(x.x, x.y), half2_bits(x.z, x.w), half2_bits(y.x, y.y), half2_bits(y.z, y.w)};
-            sts128(q + tile_off(qr, pc), h[0], h[1], h[2], h[3]);
-            if constexpr (SPLIT) {
-                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h[0])),
-                             f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h[1])),
-                             f2 = __half22float2(*reinterpret_cast<const __half2 *>(&h[2])),
-                             f3 = __half22float2(*reinterpret_cast<const __half2 *>(&h[3]));
-                sts128(q + part + tile_off(qr, pc), half2_bits(x.x - f0.x, x.y - f0.y), half2_bits(x.z - f1.x, x.w - f1.y),
-                       half2_bits(y.x - f2.x, y.y - f2.y), half2_bits(y.z - f3.x, y.w - f3.y));
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const uint32_t at = q + tile_off(warp * 32 + (k0 + k) * RQ + lane / P, lane % P);
+                if constexpr (SPLIT) {
+                    const uint32_t h[4] = {half2_bits(x[k].x, x[k].y), half2_bits(x[k].z, x[k].w),
+                                           half2_bits(y[k].x, y[k].y), half2_bits(y[k].z, y[k].w)};
+                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h[0])),
+                                 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h[1])),
+                                 f2 = __half22float2(*reinterpret_cast<const __half2 *>(&h[2])),
+                                 f3 = __half22float2(*reinterpret_cast<const __half2 *>(&h[3]));
+                    sts128(at, h[0], h[1], h[2], h[3]);
+                    sts128(at + part, half2_bits(x[k].x - f0.x, x[k].y - f0.y), half2_bits(x[k].z - f1.x, x[k].w - f1.y),
+                           half2_bits(y[k].x - f2.x, y[k].y - f2.y), half2_bits(y[k].z - f3.x, y[k].w - f3.y));
+                } else {
+                    sts128(at, __float_as_uint(x[k].x), __float_as_uint(x[k].y), __float_as_uint(x[k].z),
+                           __float_as_uint(x[k].w));
+                }
             }
         }
         proxy_fence();
@@ -970,103 +1264,35 @@ __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q
         const int limit = live ? s.x.kv - s.x.len + row / a.group : -1;  // last position this row sees
         const int all_see = s.x.kv - s.x.len + row0 / a.group;
         float m = -INFINITY, l = 0.f;  // maximum in units of the raw scores
-        const float sc = a.scale_log2;
         for (int b = s.b0; b < s.b1; ++b) {
-            mbar_wait_bounded(&ctl->s_full[t], blocks++ & 1, a.status, &ctl->abort);
+            wait_bar(a, ctl, &ctl->s_full[t], blocks++ & 1);
             tc_after();
             const int p0 = b * kBlock;
-            const bool masked = p0 + kBlock - 1 > all_see;
-            const int seen = limit - p0;  // columns 0..seen count
-            float mx = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                uint32_t x[32];
-                tm_ld32(ts + 32 * k, x);
-                tm_wait(x);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float v = __uint_as_float(x[j]);
-                    mx = fmaxf(mx, !masked || 32 * k + j <= seen ? v : -INFINITY);
-                }
-            }
-            const bool raise = m != -INFINITY && mx * sc > m * sc + kRaise;
-            if (__any_sync(0xffffffffu, raise)) {
-                const float alpha = raise ? ex2((m - mx) * sc) : 1.f;
-                l *= alpha;
-#pragma unroll 1
-                for (int k = 0; k < HD / 32; ++k) {
-                    uint32_t x[32];
-                    tm_ld32(to + 32 * k, x);
-                    tm_wait(x);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
-                    tm_st32(to + 32 * k, x);
-                }
-            }
-            if (raise || m == -INFINITY) m = mx;
-            const float mu = m == -INFINITY ? 0.f : m * sc;
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                uint32_t x[32];
-                tm_ld32(ts + 32 * k, x);
-                tm_wait(x);
-                float p[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float v = __uint_as_float(x[j]);
-                    p[j] = ex2(fmaf(!masked || 32 * k + j <= seen ? v : -INFINITY, sc, -mu));
-                    sum += p[j];
-                }
-                if constexpr (SPLIT) {
-                    uint32_t w[32];  // two k16 steps of hi (8 columns), lo (8)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const __half2 h = __floats2half2_rn(p[2 * j], p[2 * j + 1]);
-                        const float2 f = __half22float2(h);
-                        const int at = (j >> 3) * 16 + (j & 7);
-                        w[at] = *reinterpret_cast<const uint32_t *>(&h);
-                        w[at + 8] = half2_bits(p[2 * j] - f.x, p[2 * j + 1] - f.y);
-                    }
-                    tm_st32(ts + 32 * k, w);
-                } else {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) w[j] = half2_bits(p[2 * j], p[2 * j + 1]);
-                    tm_st16(ts + 16 * k, w);
-                }
-            }
-            l += sum;
+            if (p0 + kBlock - 1 > all_see) softmax_block<HD, SPLIT, true>(ts, a.scale_log2, limit - p0, &ctl->p_half[t], m, l);
+            else softmax_block<HD, SPLIT, false>(ts, a.scale_log2, 0, &ctl->p_half[t], m, l);
             tm_wait_st();
             tc_before();
             mbar_arrive(&ctl->p_full[t]);
         }
+        const float sc = a.scale_log2;
         // ---- the run's end
-        mbar_wait_bounded(&ctl->o_full[t], runs++ & 1, a.status, &ctl->abort);
+        wait_bar(a, ctl, &ctl->o_full[t], runs++ & 1);
         tc_after();
+        // O goes out by way of the queries' shared memory, idle now (128 bytes a row
+        // and pass, 4 KB a warp), so that whole rows are written side by side
         const bool whole = s.b0 == 0 && s.b1 == s.units;
         const float inv = whole ? (l > 0.f || l != l ? 1.f / l : 0.f) : 1.f;
         float *state = a.part + part_slot(s, worker) * part_floats<kTileRows, HD>();
-        const int pr = t * 128 + r;  // row within the 256
-        T *dst = op + static_cast<long>(s.x.q0 + (live ? row / a.group : 0)) * a.out_stride +
-                 (s.head * a.group + (live ? row % a.group : 0)) * HD;
-#pragma unroll 1
-        for (int k = 0; k < HD / 32; ++k) {
-            uint32_t x[32];
-            tm_ld32(to + 32 * k, x);
-            tm_wait(x);
-            if (!live) continue;
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-                const float f0 = __uint_as_float(x[j]), f1 = __uint_as_float(x[j + 1]), f2 = __uint_as_float(x[j + 2]),
-                            f3 = __uint_as_float(x[j + 3]);
-                if (whole) store4(dst + 32 * k + j, ovec, f0 * inv, f1 * inv, f2 * inv, f3 * inv);
-                else store4(state + pr * HD + 32 * k + j, f0, f1, f2, f3);
-            }
-        }
+        const long to_row = whole ? static_cast<long>(s.x.q0 + (live ? row / a.group : 0)) * a.out_stride +
+                                        (s.head * a.group + (live ? row % a.group : 0)) * HD
+                                  : static_cast<long>(t * 128 + r) * HD;
+        const int rows = min(32, s.x.rows - (row0 + warp * 32));
+        const uint32_t st = q + warp * 4096;
+        if (whole) write_rows<HD, T>(to, st, op, ovec, to_row, rows, inv, lane);
+        else write_rows<HD, float>(to, st, state, true, to_row, rows, 1.f, lane);
         if (!whole && live) {
-            state[kTileRows * HD + pr] = m == -INFINITY ? m : m * sc;
-            state[kTileRows * HD + kTileRows + pr] = l;
+            state[kTileRows * HD + t * 128 + r] = m == -INFINITY ? m : m * sc;
+            state[kTileRows * HD + kTileRows + t * 128 + r] = l;
         }
         tc_before();  // O has been read before the next run's first product
     }
@@ -1081,19 +1307,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
     const uint32_t pad = (1024u - (smem_u32(raw) & 1023u)) & 1023u;  // swizzled tiles start on 1024 bytes
     uint8_t *smem = raw + pad;
     const uint32_t q = smem_u32(smem), bufs = q + L::kQ;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
     int *first = reinterpret_cast<int *>(smem + L::kQ), *sums = first + a.n_entries + 1;
     plan_build<kTileThreads>(a, first, sums, &po);
     const Cursor c = cursor_start(a, first, sums, po, blockIdx.x);
-    if (po.units == 0 || static_cast<long>(blockIdx.x) * po.per >= static_cast<long>(po.units) * a.kv.kv_heads) return;
+    if (threadIdx.x == 0) {  // the last run of this worker
+        int4 left = left_none();
+        Cursor w = c;
+        Segment s;
+        while (cursor_next(a, w, s)) left = left_of(s, po.per);
+        a.left[blockIdx.x] = left;
+    }
+    if (c.at >= c.end) return;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; ++i) {
             mbar_init(&ctl.full[i], 128);
-            mbar_init(&ctl.empty[i], 1);
+            mbar_init(&ctl.empty[i], 2);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&ctl.q_full[t], 128);
             mbar_init(&ctl.s_full[t], 1);
+            mbar_init(&ctl.p_half[t], 128);
             mbar_init(&ctl.p_full[t], 128);
             mbar_init(&ctl.o_full[t], 1);
         }
@@ -1109,12 +1343,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
     __syncthreads();  // barriers, TMEM; the plan's shared memory becomes the buffers
     tc_after();
     const uint32_t tmem = ctl.tmem;
-    if (warp >= kLoadWarp0) {
+    if (warp >= kMmaWarpId) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+        if (warp < kMmaWarpId + 2)
+            tile_mma<HD, L::kSplit, L::kBufs>(a, c, q, bufs, L::kPart, &ctl, tmem, warp - kMmaWarpId);
+    } else if (warp >= kLoadWarp0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         tile_load<HD, E4M3, L::kBufs>(a, c, bufs, L::kPart, &ctl, threadIdx.x - kLoadWarp0 * 32);
-    } else if (warp == kMmaWarpId) {
-        if (lane == 0) tile_mma<HD, L::kSplit, L::kBufs>(a, c, q, bufs, L::kPart, &ctl, tmem);
-        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         tile_softmax<HD, T>(a, c, blockIdx.x, q, L::kPart, &ctl, tmem, warp >> 2, threadIdx.x & 127);
     }
     tc_before();
@@ -1126,19 +1363,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
 
 // ----------------------------------------------------------------- merge --
 
-// Joins the states of one (tile, KV head): 16 of its rows a block.
+// Joins the states of the tile that a worker left: 16 of its rows a block.
 template <int ROWS, int HD, typename T>
 __global__ void __launch_bounds__(256) ijb_paged_merge_kernel(const __grid_constant__ AttnArgs a) {
     __shared__ float top[16], total[16];
     __shared__ float4 sum[256];
-    const int tile = blockIdx.x, head = blockIdx.y, row0 = blockIdx.z * 16;
-    if (tile >= a.plan[0]) return;
-    const int e = a.plan[kPlanHead + tile], ti = a.plan[kPlanHead + kMaxTiles + tile];
-    const int *sums = a.plan + kPlanHead + 2 * kMaxTiles;
-    const long per = a.plan[2], head_base = static_cast<long>(head) * a.plan[1];
-    const long u0 = head_base + sums[tile], u1 = head_base + sums[tile + 1];
-    const int w0 = static_cast<int>(u0 / per), n = static_cast<int>((u1 - 1) / per) - w0 + 1;
-    if (n == 1) return;  // written by its only worker
+    const int w0 = blockIdx.x, row0 = blockIdx.y * 16;
+    const int4 left = a.left[w0];
+    const int e = left.x, ti = left.y, head = left.z, n = left.w;
+    if (n == 0) return;
     const Entry x = entry_load(a, e, false);
     const int live = min(ROWS, x.rows - ti * ROWS), rows = min(16, live - row0);
     if (rows <= 0) return;
@@ -1229,7 +1462,7 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.workers = sms * D::kWarps;
     a.min_units = 1;
     kernel<<<sms, D::kWarps * 32, smem, s>>>(a);
-    ijb_paged_merge_kernel<kDecRows, HD, T><<<dim3(a.n_entries, a.kv.kv_heads, 1), 256, 0, s>>>(a);
+    ijb_paged_merge_kernel<kDecRows, HD, T><<<a.workers, 256, 0, s>>>(a);
     count_launches(2);
     return cudaGetLastError();
 }
@@ -1248,8 +1481,7 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     a.workers = sms;
     a.min_units = 2;
     kernel<<<sms, kTileThreads, L::kSmem, s>>>(a);
-    const int tiles = static_cast<int>(static_cast<long>(a.n_tokens) * a.group / kTileRows) + a.n_entries;
-    ijb_paged_merge_kernel<kTileRows, HD, T><<<dim3(tiles, a.kv.kv_heads, kTileRows / 16), 256, 0, s>>>(a);
+    ijb_paged_merge_kernel<kTileRows, HD, T><<<dim3(a.workers, kTileRows / 16), 256, 0, s>>>(a);
     count_launches(2);
     return cudaGetLastError();
 }
@@ -1272,11 +1504,12 @@ cudaError_t attention_call(const AttnArgs &a, bool e4m3, int max_q, int sms, cud
     return e4m3 ? attention_call<128, true, T>(a, max_q, sms, s) : attention_call<128, false, T>(a, max_q, sms, s);
 }
 
-constexpr size_t kPlanBytes = (kPlanHead + 3 * kMaxTiles + 8) * sizeof(int);
+constexpr int kMaxWorkers = 8;  // per SM: the decode kernel's warps
 
 size_t workspace_bytes(int sms, int head_dim) {
-    const int rows = kTileRows > 8 * kDecRows ? kTileRows : 8 * kDecRows;  // an SM's workers, two states each
-    return kPlanBytes + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
+    constexpr int rows = kTileRows > kMaxWorkers * kDecRows ? kTileRows : kMaxWorkers * kDecRows;
+    // a word per worker, and two states each
+    return static_cast<size_t>(sms) * kMaxWorkers * sizeof(int4) + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -1342,8 +1575,8 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         a.seq = seq_dev;
         a.kv_len = kv_len_dev;
         a.scale_log2 = scale * 1.4426950408889634f;
-        a.plan = static_cast<int *>(workspace_dev);
-        a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace_dev) + kPlanBytes);
+        a.left = static_cast<int4 *>(workspace_dev);
+        a.part = reinterpret_cast<float *>(a.left + sms * kMaxWorkers);
         a.status = status_dev;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const bool e4m3 = kv->type == IJB_KV_E4M3;
