@@ -355,10 +355,11 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * every time for the same call, but how an entry's positions are cut into
  * partial sums depends on the whole call.
  *
- * workspace_dev: ijb_paged_attention_workspace bytes of 16-byte aligned device
+ * workspace_dev: ijb_paged_attention_workspace(kv) bytes (the same for every call
+ * on caches of that head_dim; 0 for a bad view) of 16-byte aligned device
  * memory on the current device, of no meaning before and after; calls that may
  * overlap, captured graphs among them, need one each. */
-size_t ijb_paged_attention_workspace(const ijb_kv_view *kv, int heads, int n_tokens, int n_entries);
+size_t ijb_paged_attention_workspace(const ijb_kv_view *kv);
 int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *q_dev, long q_stride, void *out_dev,
                         long out_stride, int n_tokens, int n_entries, const int *q_start_dev, const int *seq_dev,
                         const int *kv_len_dev, int max_q, float scale, void *workspace_dev, size_t workspace_bytes,

@@ -27,6 +27,7 @@
 // output is fp16 too).  Cached rows enter as fp16: fp16 rows exactly, e4m3 rows as
 // code * 2^e, exact while a row's largest value is in [2^-7, 2^15].
 #include <mutex>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -1447,12 +1448,28 @@ int sm_count() {
     return sms[dev];
 }
 
+// Raises a kernel's shared-memory limit, once per device (A, B: tell apart kernels
+// of one signature).
+template <class K, class A, class B>
+cudaError_t allow_smem(K kernel, int bytes) {
+    static bool ready[kMaxDevices];
+    static std::mutex mu;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    if (ready[dev]) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    ready[dev] = e == cudaSuccess;
+    return e;
+}
+
 template <int HD, bool E4M3, typename T>
 cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     using D = Dec<HD, E4M3>;
     const int smem = D::kSmem > kDecPlanBytes ? D::kSmem : kDecPlanBytes;
     auto kernel = ijb_paged_decode_kernel<HD, E4M3, T>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = allow_smem<decltype(kernel), Dec<HD, E4M3>, T>(kernel, smem);
     if (e != cudaSuccess) return e;
     a.min_rows = 1;
     a.max_rows = kDecRows;
@@ -1471,7 +1488,7 @@ template <int HD, bool E4M3, typename T>
 cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     using L = Tile<HD, T>;
     auto kernel = ijb_paged_tile_kernel<HD, E4M3, T>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    const cudaError_t e = allow_smem<decltype(kernel), Tile<HD, T>, std::bool_constant<E4M3>>(kernel, L::kSmem);
     if (e != cudaSuccess) return e;
     a.min_rows = min_rows;
     a.max_rows = 0x7fffffff;
@@ -1517,15 +1534,14 @@ size_t workspace_bytes(int sms, int head_dim) {
 
 extern "C" {
 
-size_t ijb_paged_attention_workspace(const ijb_kv_view *kv, int heads, int n_tokens, int n_entries) {
+size_t ijb_paged_attention_workspace(const ijb_kv_view *kv) {
     using namespace ijb;
     KvDev d;
     try {
-        if (!kv_view_check(kv, &d).empty() || heads < 1 || n_tokens < 0 || n_entries < 1) return 0;
+        return kv_view_check(kv, &d).empty() ? workspace_bytes(sm_count(), kv->head_dim) : 0;
     } catch (...) {
         return 0;
     }
-    return workspace_bytes(sm_count(), kv->head_dim);
 }
 
 int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *q_dev, long q_stride, void *out_dev,

@@ -98,7 +98,7 @@ def load():
         "ijb_keys_to_tokens": ([P, I, P, P], I),
         "ijb_kv_append": ([P, I, P, P, L64, I, P, P, P, P], I),
         "ijb_kv_gather": ([P, I, P, P, L64, I, P, P, P, P], I),
-        "ijb_paged_attention_workspace": ([P, I, I, I], ctypes.c_size_t),
+        "ijb_paged_attention_workspace": ([P], ctypes.c_size_t),
         "ijb_paged_attention": ([P, I, I, P, L64, P, L64, I, I, P, P, P, I, ctypes.c_float, P, ctypes.c_size_t, P, P], I),
         "ijb_sample": ([P, L64, I, I, P, P, P, P, P, P, P, P], I),
         "ijb_kernel_launches": ([], ctypes.c_uint64),

@@ -20,6 +20,8 @@ F32, F16 = 0, 1  # IJB_TYPE_F32, IJB_TYPE_F16
 KV_F16, KV_E4M3 = 0, 2
 _TYPE = {torch.float32: F32, torch.float16: F16}
 _stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
+_empty = torch.empty
 
 
 def _need(ok: bool, what: str) -> None:
@@ -29,7 +31,7 @@ def _need(ok: bool, what: str) -> None:
 
 def _call(device: int, fn, *args) -> None:
     """One library call with `device` current, on its current stream."""
-    if torch.cuda.current_device() == device:
+    if _current() == device:
         rc = fn(*args, _stream(device))
     else:
         with torch.cuda.device(device):
@@ -47,12 +49,14 @@ def _ptr(t, dtype, n: int, device: int, what: str):
     return t.data_ptr()
 
 
-def _rows(t, inner: int, device: int, what: str):
-    """(address, stride in elements) of a [n, ..] tensor whose tokens are `inner` contiguous elements."""
+def _rows(t, n: int, inner: int, device: int, what: str):
+    """(address, stride in elements) of [n, ..] rows, each of `inner` contiguous elements."""
+    if t.is_contiguous() and t.numel() == n * inner and t.get_device() == device:
+        return t.data_ptr(), inner
     flat = t.dim() == 2 and t.stride(1) == 1 or t.dim() == 3 and t.stride(2) == 1 and t.stride(1) == t.shape[2]
-    if t.get_device() != device or t.dtype not in _TYPE or not flat or t[0:1].numel() not in (0, inner):
-        raise ValueError(f"{what}: expected [n, {inner}] fp32 or fp16 values on cuda:{device}, each token's contiguous")
-    return t.data_ptr(), max(t.stride(0), inner) if t.shape[0] <= 1 else t.stride(0)
+    if t.get_device() != device or not flat or t.numel() != n * inner or t.stride(0) < inner and n > 1:
+        raise ValueError(f"{what}: expected [{n}, {inner}] values on cuda:{device}, each row's contiguous")
+    return t.data_ptr(), max(t.stride(0), inner)
 
 
 class PagedKV:
@@ -85,24 +89,26 @@ class PagedKV:
                                n_seqs=page_table.shape[0], max_pages=page_table.shape[1])
         self._ref = ctypes.byref(self._view)
         self._status = status.data_ptr() if status is not None else None
+        self._scale, self._seqs = 1.0 / math.sqrt(self.head_dim), page_table.shape[0]
+        with torch.cuda.device(dev):
+            self._work = self._lib.ijb_paged_attention_workspace(self._ref)
 
     def append(self, k, v, seq, pos) -> None:
         """Writes rows k, v [n, kv_heads, head_dim] (fp32 or fp16) at positions pos [n] of sequences seq [n]."""
-        n = k.shape[0]
-        kp, stride = _rows(k, self.row, self.device, "k")
-        vp, vstride = _rows(v, self.row, self.device, "v")
-        _need(k.dtype == v.dtype and v.shape[0] == n and (vstride == stride or n <= 1),
-              "k and v differ in type, length or stride")
-        _call(self.device, self._lib.ijb_kv_append, self._ref, _TYPE[k.dtype], kp, vp, stride, n,
-              _ptr(seq, torch.int32, n, self.device, "seq"), _ptr(pos, torch.int32, n, self.device, "pos"), self._status)
+        n, dev = k.shape[0], self.device
+        kp, stride = _rows(k, n, self.row, dev, "k")
+        vp, vstride = _rows(v, n, self.row, dev, "v")
+        if k.dtype not in _TYPE or v.dtype != k.dtype or vstride != stride:
+            raise ValueError("k and v: expected fp32 or fp16 rows of one type and stride")
+        _call(dev, self._lib.ijb_kv_append, self._ref, _TYPE[k.dtype], kp, vp, stride, n,
+              _ptr(seq, torch.int32, n, dev, "seq"), _ptr(pos, torch.int32, n, dev, "pos"), self._status)
 
     def gather(self, seq, pos, dtype=torch.float32):
         """The rows at positions pos [n] of sequences seq [n]: (k, v), each [n, kv_heads, head_dim].
         Rows of entries that are skipped (a negative position) hold no meaning."""
         _need(dtype in _TYPE, "dtype must be float32 or float16")
         n = seq.numel()
-        out = torch.empty((2, n, self.kv_heads, self.head_dim), dtype=dtype, device=self.data.device)
-        k, v = out[0], out[1]
+        k, v = _empty((2, n, self.kv_heads, self.head_dim), dtype=dtype, device=self.data.device).unbind(0)
         _call(self.device, self._lib.ijb_kv_gather, self._ref, _TYPE[dtype], k.data_ptr(), v.data_ptr(), self.row, n,
               _ptr(seq, torch.int32, n, self.device, "seq"), _ptr(pos, torch.int32, n, self.device, "pos"), self._status)
         return k, v
@@ -112,21 +118,24 @@ class PagedKV:
         q_start[e]..q_start[e + 1] and the last of the kv_len[e] positions of sequence seq[e] (default: e), which
         the cache already holds.  Each token sees the positions up to its own; a token before position 0 sees none and
         gets zeros.  ``max_q``: the most new tokens of any entry, if known.  Returns out (like q)."""
-        _need(q.dim() == 3 and q.shape[2] == self.head_dim, "q: expected [tokens, heads, head_dim]")
-        n, heads = q.shape[0], q.shape[1]
-        qp, qs = _rows(q, heads * self.head_dim, self.device, "q")
+        if q.dim() != 3 or q.shape[2] != self.head_dim or q.dtype not in _TYPE:
+            raise ValueError("q: expected [tokens, heads, head_dim], fp32 or fp16")
+        n, heads, _ = q.shape
+        dev, row = self.device, heads * self.head_dim
+        qp, qs = _rows(q, n, row, dev, "q")
         if out is None:
-            out = torch.empty((n, heads, self.head_dim), dtype=q.dtype, device=q.device)
-        _need(out.shape == q.shape and out.dtype == q.dtype, "out: expected the shape and type of q")
-        op, os = _rows(out, heads * self.head_dim, self.device, "out")
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            op, os = out.data_ptr(), row
+        else:
+            _need(out.shape == q.shape and out.dtype == q.dtype, "out: expected the shape and type of q")
+            op, os = _rows(out, n, row, dev, "out")
         e = kv_len.numel()
-        _need(e >= 1 and (seq is not None or e <= self.page_table.shape[0]), "kv_len: one length for each entry")
-        size = self._lib.ijb_paged_attention_workspace(self._ref, heads, n, e)
-        work = torch.empty((max(size, 16),), dtype=torch.uint8, device=q.device)
-        _call(self.device, self._lib.ijb_paged_attention, self._ref, heads, _TYPE[q.dtype], qp, qs, op, os, n, e,
-              _ptr(q_start, torch.int32, e + 1, self.device, "q_start"), _ptr(seq, torch.int32, e, self.device, "seq"),
-              _ptr(kv_len, torch.int32, e, self.device, "kv_len"), max_q,
-              1.0 / math.sqrt(self.head_dim) if scale is None else scale, work.data_ptr(), work.numel(), self._status)
+        _need(e >= 1 and (seq is not None or e <= self._seqs), "kv_len: one length for each entry")
+        work = _empty(self._work, dtype=torch.uint8, device=q.device)
+        _call(dev, self._lib.ijb_paged_attention, self._ref, heads, _TYPE[q.dtype], qp, qs, op, os, n, e,
+              _ptr(q_start, torch.int32, e + 1, dev, "q_start"), _ptr(seq, torch.int32, e, dev, "seq"),
+              _ptr(kv_len, torch.int32, e, dev, "kv_len"), max_q, self._scale if scale is None else scale,
+              work.data_ptr(), self._work, self._status)
         return out
 
 

@@ -87,5 +87,5 @@ def test_attention_without_tokens_is_no_launch():
 
 
 def test_attention_workspace_of_a_bad_view_is_nothing():
-    assert lib.load().ijb_paged_attention_workspace(ctypes.byref(view(head_dim=80)), 4, 1, 1) == 0
-    assert lib.load().ijb_paged_attention_workspace(None, 4, 1, 1) == 0
+    assert lib.load().ijb_paged_attention_workspace(ctypes.byref(view(head_dim=80))) == 0
+    assert lib.load().ijb_paged_attention_workspace(None) == 0
