@@ -133,46 +133,66 @@ struct PlanOut {
     int tiles, units, per;
 };
 
+__device__ __forceinline__ void plan_end(const AttnArgs &a, int *sums, PlanOut *po, int tiles, int units) {
+    const long all = static_cast<long>(units) * a.kv.kv_heads;
+    if (threadIdx.x == 0) {
+        sums[tiles] = units;
+        po->tiles = tiles;
+        po->units = units;
+        po->per = static_cast<int>(max(static_cast<long>(a.min_units), (all + a.workers - 1) / a.workers));
+    }
+    __syncthreads();
+}
+
 // Cuts the call's work: `first` [n_entries + 1] receives each entry's first
-// tile, `sums` [tiles + 1] each tile's first unit (of one KV head).  All NT
-// threads call it.
-template <int NT>
+// tile, `sums` [tiles + 1] each tile's first unit (of one KV head).  ONE: no entry
+// has two tiles, and tiles are entries.  All NT threads call it.
+template <int NT, bool ONE>
 __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po) {
     const bool lead = blockIdx.x == 0;
     int base = 0;
-    for (int e0 = 0; e0 < a.n_entries; e0 += NT) {
-        const int e = e0 + static_cast<int>(threadIdx.x);
-        const int n = e < a.n_entries ? entry_load(a, e, lead).tiles : 0;
-        int total;
-        const int inc = block_scan_int<NT>(n, po->warp_sums, &total);
-        if (e < a.n_entries) first[e] = base + inc - n;
-        base += total;
-    }
-    if (threadIdx.x == 0) first[a.n_entries] = base;
-    __syncthreads();
-    const int tiles = min(base, kMaxTiles);
-    base = 0;
-    for (int t0 = 0; t0 < tiles; t0 += NT) {
-        const int t = t0 + static_cast<int>(threadIdx.x);
-        int n = 0;
-        if (t < tiles) {
-            const int e = find_le(first, a.n_entries, t);
-            n = tile_units(a, entry_load(a, e, false), t - first[e]);
+    if constexpr (ONE) {
+        // one tile an entry at most: tiles are entries, some of no units
+        for (int e0 = 0; e0 < a.n_entries; e0 += NT) {
+            const int e = e0 + static_cast<int>(threadIdx.x);
+            int n = 0;
+            if (e < a.n_entries) {
+                const Entry x = entry_load(a, e, lead);
+                n = x.tiles ? tile_units(a, x, 0) : 0;
+            }
+            int total;
+            const int inc = block_scan_int<NT>(n, po->warp_sums, &total);
+            if (e < a.n_entries) sums[e] = base + inc - n;
+            base += total;
         }
-        int total;
-        const int inc = block_scan_int<NT>(n, po->warp_sums, &total);
-        if (t < tiles) sums[t] = base + inc - n;
-        base += total;
+        plan_end(a, sums, po, a.n_entries, base);
+    } else {
+        for (int e0 = 0; e0 < a.n_entries; e0 += NT) {
+            const int e = e0 + static_cast<int>(threadIdx.x);
+            const int n = e < a.n_entries ? entry_load(a, e, lead).tiles : 0;
+            int total;
+            const int inc = block_scan_int<NT>(n, po->warp_sums, &total);
+            if (e < a.n_entries) first[e] = base + inc - n;
+            base += total;
+        }
+        if (threadIdx.x == 0) first[a.n_entries] = base;
+        __syncthreads();
+        const int tiles = min(base, kMaxTiles);
+        base = 0;
+        for (int t0 = 0; t0 < tiles; t0 += NT) {
+            const int t = t0 + static_cast<int>(threadIdx.x);
+            int n = 0;
+            if (t < tiles) {
+                const int e = find_le(first, a.n_entries, t);
+                n = tile_units(a, entry_load(a, e, false), t - first[e]);
+            }
+            int total;
+            const int inc = block_scan_int<NT>(n, po->warp_sums, &total);
+            if (t < tiles) sums[t] = base + inc - n;
+            base += total;
+        }
+        plan_end(a, sums, po, tiles, base);
     }
-    const long all = static_cast<long>(base) * a.kv.kv_heads;
-    const int per = static_cast<int>(max(static_cast<long>(a.min_units), (all + a.workers - 1) / a.workers));
-    if (threadIdx.x == 0) {
-        sums[tiles] = base;
-        po->tiles = tiles;
-        po->units = base;
-        po->per = per;
-    }
-    __syncthreads();
 }
 
 // A worker's position in the line of work.
@@ -181,6 +201,7 @@ struct Cursor {
     int e, ti, head, b0;
 };
 
+template <bool ONE>
 __device__ __forceinline__ Cursor cursor_start(const AttnArgs &a, const int *first, const int *sums, const PlanOut &po,
                                                int worker) {
     Cursor c;
@@ -189,11 +210,12 @@ __device__ __forceinline__ Cursor cursor_start(const AttnArgs &a, const int *fir
     c.end = min(all, c.at + po.per);
     c.e = c.ti = c.head = c.b0 = 0;
     if (c.at < c.end) {
-        c.head = static_cast<int>(c.at / po.units);
+        c.head = (c.at >> 32) ? static_cast<int>(c.at / po.units)
+                              : static_cast<int>(static_cast<uint32_t>(c.at) / static_cast<uint32_t>(po.units));
         const int u = static_cast<int>(c.at - static_cast<long>(c.head) * po.units);
         const int t = find_le(sums, po.tiles, u);
-        c.e = find_le(first, a.n_entries, t);
-        c.ti = t - first[c.e];
+        c.e = ONE ? t : find_le(first, a.n_entries, t);
+        c.ti = ONE ? 0 : t - first[c.e];
         c.b0 = u - sums[t];
     }
     return c;
@@ -340,16 +362,20 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 constexpr int kChunk = 32;  // positions
 constexpr int kDecRows = 16;
 
-template <int HD, bool E4M3>
+// WIDE: more than 8 rows.  Up to 8 leave the upper half of the products' 16 rows
+// unused, and with half the registers an SM holds more warps: 64 ragged
+// sequences of 4 rows took 25 us with the wide kernel's 8 warps.
+template <int HD, bool E4M3, bool WIDE>
 struct Dec {
     static constexpr int kRowBytes = HD * (E4M3 ? 1 : 2);
     static constexpr int kTile = kChunk * kRowBytes;
-    static constexpr int kStage = 2 * kTile + (E4M3 ? 64 : 0);  // K, V, their scale bytes
-    static constexpr int kWarps = kRowBytes == 256 ? 6 : 8;
-    static constexpr int kStages = kRowBytes == 256 ? 2 : (kRowBytes == 128 ? 3 : 4);
+    static constexpr int kStage = 2 * kTile + (E4M3 ? 256 : 0);  // K, V, their scale bytes and what they stand for
+    static constexpr int kWarps = kRowBytes == 256 ? 6 : (WIDE || HD == 128 ? 8 : (E4M3 ? 16 : 12));
+    static constexpr int kStages = kRowBytes == 256 ? 2 : (kRowBytes == 128 ? (kWarps == 8 ? 3 : 2) : (WIDE ? 4 : 3));
     static constexpr int kSmem = kWarps * kStages * kStage;
+    static_assert(kSmem <= 226 * 1024, "stages");
 };
-constexpr int kDecPlanBytes = (kMaxEntries + kMaxTiles + 2) * 4;  // entries' first tiles and tiles' first units
+constexpr int kDecPlanBytes = (kMaxEntries + 1) * 4;  // entries' first units
 
 // Byte offset of 16-byte piece c of row r in a chunk tile.
 template <int RB>
@@ -383,19 +409,35 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Rows 0..7 alone (the others are zeros): a = {row gid, first and second k pair}.
+__device__ __forceinline__ void mma(float (&d)[2], const uint32_t (&a)[2], uint32_t b0, uint32_t b1) {
+    [[maybe_unused]] float x, y;
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %8, %5, %8}, {%6, %7}, "
+        "{%0, %1, %9, %9};"
+        : "+f"(d[0]), "+f"(d[1]), "=f"(x), "=f"(y)
+        : "r"(a[0]), "r"(a[1]), "r"(b0), "r"(b1), "r"(0u), "f"(0.f));
+}
 
-template <int HD, bool E4M3, typename T>
-__global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_kernel(const __grid_constant__ AttnArgs a) {
-    using D = Dec<HD, E4M3>;
+template <int HD, bool E4M3, bool WIDE, typename T>
+__global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
+    ijb_paged_decode_kernel(const __grid_constant__ AttnArgs a) {
+    using D = Dec<HD, E4M3, WIDE>;
+    constexpr int H = WIDE ? 2 : 1;  // halves of the 16 rows in use
+    // up to 8 fp32 rows: their hi parts are rows 0..7 of the products, their lo
+    // parts rows 8..15, for the products of one
+    constexpr bool PAIR = sizeof(T) == 4 && !WIDE;
+    constexpr int C = WIDE || PAIR ? 4 : 2;  // accumulators a lane
     constexpr bool SPLIT = sizeof(T) == 4;  // fp32 queries: hi + lo
     constexpr int NT = D::kWarps * 32, RB = D::kRowBytes, KS = HD / 16, NTILE = HD / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PlanOut po;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t4 = lane & 3;
-    int *first = reinterpret_cast<int *>(smem), *sums = first + a.n_entries + 1;
-    plan_build<NT>(a, first, sums, &po);
+    pdl_trigger();
+    int *sums = reinterpret_cast<int *>(smem);
+    plan_build<NT, true>(a, nullptr, sums, &po);
     const int worker = blockIdx.x * D::kWarps + warp;
-    Cursor load_c = cursor_start(a, first, sums, po, worker), use_c = load_c;
+    Cursor load_c = cursor_start<true>(a, nullptr, sums, po, worker), use_c = load_c;
     __syncthreads();  // the plan's shared memory becomes the stages
 
     const uint32_t base = smem_u32(smem) + warp * D::kStages * D::kStage;
@@ -456,10 +498,10 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
     Segment s;
     while (cursor_next(a, use_c, s)) {
         const int row0 = s.ti * kDecRows, rows = min(kDecRows, s.x.rows - row0);
-        uint32_t qf[KS][4], ql[SPLIT ? KS : 1][4];
-        int limit[2];  // last position that rows gid and gid + 8 see
+        uint32_t qf[KS][C], ql[SPLIT && WIDE ? KS : 1][4];
+        int limit[H];  // last position that rows gid and gid + 8 see
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int hf = 0; hf < H; ++hf) {
             const int r = gid + 8 * hf;
             const int tok = r < rows ? (row0 + r) / a.group : 0, in = r < rows ? (row0 + r) % a.group : 0;
             limit[hf] = r < rows ? s.x.kv - s.x.len + tok : -1;
@@ -470,17 +512,25 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
                 const float4 v = r < rows ? load4(src + d, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
                 const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
                 qf[ks][hf] = *reinterpret_cast<const uint32_t *>(&h0);
-                qf[ks][2 + hf] = *reinterpret_cast<const uint32_t *>(&h1);
+                qf[ks][C / 2 + hf] = *reinterpret_cast<const uint32_t *>(&h1);
                 if constexpr (SPLIT) {
                     const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                    ql[ks][hf] = half2_bits(v.x - f0.x, v.y - f0.y);
-                    ql[ks][2 + hf] = half2_bits(v.z - f1.x, v.w - f1.y);
+                    uint32_t(&lo)[4] = PAIR ? reinterpret_cast<uint32_t(&)[4]>(qf[ks]) : ql[WIDE ? ks : 0];
+                    lo[PAIR ? 1 : hf] = half2_bits(v.x - f0.x, v.y - f0.y);
+                    lo[PAIR ? 3 : 2 + hf] = half2_bits(v.z - f1.x, v.w - f1.y);
                 }
             }
         }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[NTILE][4];
+        float m[H], l[H], o[NTILE][C];
 #pragma unroll
-        for (int i = 0; i < NTILE; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        for (int hf = 0; hf < H; ++hf) {
+            m[hf] = -INFINITY;
+            l[hf] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NTILE; ++i)
+#pragma unroll
+            for (int k = 0; k < C; ++k) o[i][k] = 0.f;
         const int all_see = s.x.kv - s.x.len + row0 / a.group;  // positions up to here are seen by every row
 
         for (int b = s.b0; b < s.b1; ++b) {
@@ -489,11 +539,31 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
             __syncwarp();
             const uint32_t kt = base + stage * D::kStage, vt = kt + D::kTile, sc = kt + 2 * D::kTile;
             const int p0 = b * kChunk;
+            float kscale[8];         // of positions t4 + 4 i
+            uint32_t vscale[4];      // fp16, of positions t4 + 8 i and t4 + 8 i + 4
+            if constexpr (E4M3) {
+                // lane r turns position r's scale bytes into numbers, kept so that a lane reads
+                // its eight positions' side by side; those behind the last mean nothing
+                const bool in = p0 + lane < s.x.kv;
+                const int at = (lane & 3) * 8 + (lane >> 2);
+                const float ks = in ? kv_scale(lds8(sc + lane)) : 0.f;
+                const __half vs = in ? scale_half(lds8(sc + 32 + lane)) : __half(0.f);
+                const uint32_t nums = kt + 2 * D::kTile + 64;
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(nums + at * 4), "f"(ks * a.scale_log2) : "memory");
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(nums + 128 + at * 2), "h"(__half_as_ushort(vs)) : "memory");
+                __syncwarp();
+                const uint4 k0 = lds128(nums + t4 * 32), k1 = lds128(nums + t4 * 32 + 16), vv = lds128(nums + 128 + t4 * 16);
+                const uint32_t ku[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) kscale[i] = __uint_as_float(ku[i]);
+                vscale[0] = vv.x; vscale[1] = vv.y; vscale[2] = vv.z; vscale[3] = vv.w;
+            }
             // ---- scores: tile nt, column n is position 16 (nt / 2) + 8 (nt % 2) + n / 2 + 4 (n % 2)
-            float p[4][4];
+            float p[4][C];
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt) {
-                p[nt][0] = p[nt][1] = p[nt][2] = p[nt][3] = 0.f;
+#pragma unroll
+                for (int k = 0; k < C; ++k) p[nt][k] = 0.f;
                 const int r = 8 * nt + (gid >> 1) + 4 * (gid & 1);
 #pragma unroll
                 for (int j = 0; j < RB / 64; ++j) {
@@ -504,34 +574,37 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
                         for (int e = 0; e < 4; ++e) {
                             const uint32_t b0 = e4m3x2_half2(u[e] & 0xffffu), b1 = e4m3x2_half2(u[e] >> 16);
                             mma(p[nt], qf[4 * j + e], b0, b1);
-                            if constexpr (SPLIT) mma(p[nt], ql[4 * j + e], b0, b1);
+                            if constexpr (SPLIT && WIDE) mma(p[nt], ql[4 * j + e], b0, b1);
                         }
                     } else {
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             mma(p[nt], qf[2 * j + e], u[2 * e], u[2 * e + 1]);
-                            if constexpr (SPLIT) mma(p[nt], ql[2 * j + e], u[2 * e], u[2 * e + 1]);
+                            if constexpr (SPLIT && WIDE) mma(p[nt], ql[2 * j + e], u[2 * e], u[2 * e + 1]);
                         }
                     }
                 }
             }
             // ---- online softmax (base 2) of rows gid and gid + 8
             const bool masked = p0 + kChunk - 1 > all_see;
-            float mx[2] = {-INFINITY, -INFINITY};
+            float mx[H];
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
+            for (int hf = 0; hf < H; ++hf) mx[hf] = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 8 * nt + t4 + 4 * (i & 1);
-                    float v = p[nt][i] * a.scale_log2;
-                    if constexpr (E4M3) v *= kv_scale(lds8(sc + r));
-                    if (masked && p0 + r > limit[i >> 1]) v = -INFINITY;
+            for (int nt = 0; nt < 4; ++nt) {
+#pragma unroll
+                for (int i = 0; i < 2 * H; ++i) {
+                    float v = PAIR ? p[nt][i] + p[nt][C - 2 + i] : p[nt][i];
+                    v *= E4M3 ? kscale[2 * nt + (i & 1)] : a.scale_log2;
+                    if (masked && p0 + 8 * nt + t4 + 4 * (i & 1) > limit[i >> 1]) v = -INFINITY;
                     p[nt][i] = v;
                     mx[i >> 1] = fmaxf(mx[i >> 1], v);
                 }
-            float alpha[2], mu[2];
+            }
+            float alpha[H], mu[H];
+            bool same = true;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
+            for (int hf = 0; hf < H; ++hf) {
                 mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
                 mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
                 const float mn = fmaxf(m[hf], mx[hf]);
@@ -539,46 +612,40 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
                 alpha[hf] = ex2(m[hf] - mu[hf]);
                 m[hf] = mn;
                 l[hf] *= alpha[hf];
+                same = same && alpha[hf] == 1.f;
             }
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 2 * H; ++i) {
                     p[nt][i] = ex2(p[nt][i] - mu[i >> 1]);
                     l[i >> 1] += p[nt][i];
                 }
-            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+            if (!__all_sync(0xffffffffu, same)) {
 #pragma unroll
-                for (int i = 0; i < NTILE; ++i) {
-                    o[i][0] *= alpha[0];
-                    o[i][1] *= alpha[0];
-                    o[i][2] *= alpha[1];
-                    o[i][3] *= alpha[1];
-                }
+                for (int i = 0; i < NTILE; ++i)
+#pragma unroll
+                    for (int k = 0; k < C; ++k) o[i][k] *= alpha[PAIR ? 0 : k >> 1];
             }
             // ---- values: k slots 2t, 2t+1, 2t+8, 2t+9 are positions 16 st + t, + 4, + 8, + 12
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                uint32_t ph[4], pl[4];
+                uint32_t ph[C], pl[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = p[2 * st + (i >> 1)][2 * (i & 1)], y = p[2 * st + (i >> 1)][2 * (i & 1) + 1];
+                for (int i = 0; i < 2 * H; ++i) {
+                    const float x = p[2 * st + i / H][2 * (i % H)], y = p[2 * st + i / H][2 * (i % H) + 1];
                     const __half2 h = __floats2half2_rn(x, y);
-                    ph[i] = *reinterpret_cast<const uint32_t *>(&h);
+                    ph[PAIR ? 2 * i : i] = *reinterpret_cast<const uint32_t *>(&h);
                     if constexpr (SPLIT) {
                         const float2 f = __half22float2(h);
-                        pl[i] = half2_bits(x - f.x, y - f.y);
+                        const uint32_t lo = half2_bits(x - f.x, y - f.y);
+                        if constexpr (PAIR) ph[2 * i + 1] = lo;
+                        else pl[i] = lo;
                     }
                 }
                 const int r0 = 16 * st + t4;
                 if constexpr (E4M3) {
-                    __half vs[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)  // scale bytes behind the last position mean nothing
-                        vs[i] = p0 + r0 + 4 * i < s.x.kv ? scale_half(lds8(sc + 32 + r0 + 4 * i)) : __half(0.f);
-                    const __half2 s01 = __halves2half2(vs[0], vs[1]), s23 = __halves2half2(vs[2], vs[3]);
-                    const uint32_t sa = *reinterpret_cast<const uint32_t *>(&s01),
-                                   sb = *reinterpret_cast<const uint32_t *>(&s23);
+                    const uint32_t sa = vscale[2 * st], sb = vscale[2 * st + 1];
                     uint32_t w[4][HD / 32];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -602,7 +669,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
                                 const uint32_t b0 = hmul2(e4m3x2_half2(e ? y0 >> 16 : y0 & 0xffffu), sa);
                                 const uint32_t b1 = hmul2(e4m3x2_half2(e ? y1 >> 16 : y1 & 0xffffu), sb);
                                 mma(o[4 * k + 2 * d + e], ph, b0, b1);
-                                if constexpr (SPLIT) mma(o[4 * k + 2 * d + e], pl, b0, b1);
+                                if constexpr (SPLIT && WIDE) mma(o[4 * k + 2 * d + e], pl, b0, b1);
                             }
                         }
                 } else {
@@ -621,7 +688,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
                                 const uint32_t sel = e ? 0x7632 : 0x5410;
                                 const uint32_t b0 = prmt(w[0][k], w[1][k], sel), b1 = prmt(w[2][k], w[3][k], sel);
                                 mma(o[8 * h + 2 * k + e], ph, b0, b1);
-                                if constexpr (SPLIT) mma(o[8 * h + 2 * k + e], pl, b0, b1);
+                                if constexpr (SPLIT && WIDE) mma(o[8 * h + 2 * k + e], pl, b0, b1);
                             }
                     }
                 }
@@ -630,12 +697,19 @@ __global__ void __launch_bounds__(Dec<HD, E4M3>::kWarps * 32) ijb_paged_decode_k
             stage = stage + 1 == D::kStages ? 0 : stage + 1;
         }
 
+        if constexpr (PAIR) {
+#pragma unroll
+            for (int i = 0; i < NTILE; ++i) {
+                o[i][0] += o[i][C - 2];
+                o[i][1] += o[i][C - 1];
+            }
+        }
         // ---- the run's end: the output, or its state
         left = left_of(s, po.per);
         const bool whole = s.b0 == 0 && s.b1 == s.units;
         float *part = a.part + part_slot(s, worker) * part_floats<kDecRows, HD>();
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int hf = 0; hf < H; ++hf) {
             l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
             l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
             const int r = gid + 8 * hf;
@@ -1310,8 +1384,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
     const uint32_t q = smem_u32(smem), bufs = q + L::kQ;
     const int warp = threadIdx.x >> 5;
     int *first = reinterpret_cast<int *>(smem + L::kQ), *sums = first + a.n_entries + 1;
-    plan_build<kTileThreads>(a, first, sums, &po);
-    const Cursor c = cursor_start(a, first, sums, po, blockIdx.x);
+    pdl_trigger();
+    plan_build<kTileThreads, false>(a, first, sums, &po);
+    const Cursor c = cursor_start<false>(a, first, sums, po, blockIdx.x);
     if (threadIdx.x == 0) {  // the last run of this worker
         int4 left = left_none();
         Cursor w = c;
@@ -1370,6 +1445,7 @@ __global__ void __launch_bounds__(256) ijb_paged_merge_kernel(const __grid_const
     __shared__ float top[16], total[16];
     __shared__ float4 sum[256];
     const int w0 = blockIdx.x, row0 = blockIdx.y * 16;
+    pdl_wait();
     const int4 left = a.left[w0];
     const int e = left.x, ti = left.y, head = left.z, n = left.w;
     if (n == 0) return;
@@ -1464,24 +1540,42 @@ cudaError_t allow_smem(K kernel, int bytes) {
     return e;
 }
 
-template <int HD, bool E4M3, typename T>
+// The merge behind the kernel just launched, on the GPU early (programmatic
+// dependent launch): it waits there for the states.
+template <int ROWS, int HD, typename T>
+cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.workers, ROWS / 16);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, ijb_paged_merge_kernel<ROWS, HD, T>, a);
+    count_launches(2);
+    return e;
+}
+
+template <int HD, bool E4M3, bool WIDE, typename T>
 cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
-    using D = Dec<HD, E4M3>;
-    const int smem = D::kSmem > kDecPlanBytes ? D::kSmem : kDecPlanBytes;
-    auto kernel = ijb_paged_decode_kernel<HD, E4M3, T>;
-    const cudaError_t e = allow_smem<decltype(kernel), Dec<HD, E4M3>, T>(kernel, smem);
+    using D = Dec<HD, E4M3, WIDE>;
+    constexpr int smem = D::kSmem > kDecPlanBytes ? D::kSmem : kDecPlanBytes;
+    auto kernel = ijb_paged_decode_kernel<HD, E4M3, WIDE, T>;
+    const cudaError_t e = allow_smem<decltype(kernel), D, T>(kernel, smem);
     if (e != cudaSuccess) return e;
     a.min_rows = 1;
-    a.max_rows = kDecRows;
+    a.max_rows = WIDE ? kDecRows : 8;
     a.report_long = all;
     a.tile_rows = kDecRows;
     a.unit = kChunk;
     a.workers = sms * D::kWarps;
-    a.min_units = 1;
+    a.min_units = 2;
     kernel<<<sms, D::kWarps * 32, smem, s>>>(a);
-    ijb_paged_merge_kernel<kDecRows, HD, T><<<a.workers, 256, 0, s>>>(a);
-    count_launches(2);
-    return cudaGetLastError();
+    return merge_launch<kDecRows, HD, T>(a, s);
 }
 
 template <int HD, bool E4M3, typename T>
@@ -1498,9 +1592,7 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     a.workers = sms;
     a.min_units = 2;
     kernel<<<sms, kTileThreads, L::kSmem, s>>>(a);
-    ijb_paged_merge_kernel<kTileRows, HD, T><<<dim3(a.workers, kTileRows / 16), 256, 0, s>>>(a);
-    count_launches(2);
-    return cudaGetLastError();
+    return merge_launch<kTileRows, HD, T>(a, s);
 }
 
 // Which kernels serve a call.  Entries of up to 16 rows go to the decode kernel,
@@ -1509,9 +1601,10 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
 template <int HD, bool E4M3, typename T>
 cudaError_t attention_call(const AttnArgs &a, int max_q, int sms, cudaStream_t s) {
     const long most = static_cast<long>(max_q > 0 ? min(max_q, a.n_tokens) : a.n_tokens) * a.group;
-    if (most <= kDecRows) return decode_launch<HD, E4M3, T>(a, sms, true, s);
+    if (most <= 8) return decode_launch<HD, E4M3, false, T>(a, sms, true, s);
+    if (most <= kDecRows) return decode_launch<HD, E4M3, true, T>(a, sms, true, s);
     if (a.n_entries < 8) return tile_launch<HD, E4M3, T>(a, sms, 1, s);
-    const cudaError_t e = decode_launch<HD, E4M3, T>(a, sms, false, s);
+    const cudaError_t e = decode_launch<HD, E4M3, true, T>(a, sms, false, s);
     return e != cudaSuccess ? e : tile_launch<HD, E4M3, T>(a, sms, kDecRows + 1, s);
 }
 template <typename T>
@@ -1521,7 +1614,7 @@ cudaError_t attention_call(const AttnArgs &a, bool e4m3, int max_q, int sms, cud
     return e4m3 ? attention_call<128, true, T>(a, max_q, sms, s) : attention_call<128, false, T>(a, max_q, sms, s);
 }
 
-constexpr int kMaxWorkers = 8;  // per SM: the decode kernel's warps
+constexpr int kMaxWorkers = 16;  // per SM: the decode kernel's warps
 
 size_t workspace_bytes(int sms, int head_dim) {
     constexpr int rows = kTileRows > kMaxWorkers * kDecRows ? kTileRows : kMaxWorkers * kDecRows;
