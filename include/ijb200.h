@@ -85,6 +85,15 @@ typedef struct {
  * inferencer.cu:1218-1230).  Replaces FastGPU::FastGPU + FastRunner::FastRunner. */
 int ijb_create(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, ijb_engine **out);
 
+/* The same engine with its K/V pool of cache type kv_type (IJB_KV_F16 or
+ * IJB_KV_E4M3, below; desc->kv_f32 is ignored) and ijb_paged_attention in every
+ * step: prompts run their chunks' attention on the tensor cores a tile at a time
+ * where an engine of ijb_create reads the cache once for each new token, and an
+ * e4m3 pool holds twice the positions.  max_batch <= 4096.  The rounding of a
+ * token's attention depends on the step it runs in (ijb_paged_attention). */
+int ijb_create_kv(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, int kv_type,
+                  ijb_engine **out);
+
 /* Frees everything the engine owns (FastGPU::~FastGPU, inferencer.cu:1141-1150). */
 void ijb_destroy(ijb_engine *engine);
 
@@ -158,6 +167,14 @@ int ijb_seq_length(const ijb_engine *engine, int seq_id);
  * sequences (decode).  With next_tokens non-NULL, each entry's greedy argmax is
  * copied to the host; the call returns after the step completed. */
 int ijb_decode_step(ijb_engine *engine, int n, const int *seq_ids, const int *tokens, int *next_tokens);
+
+/* ijb_decode_step with each entry's next token drawn by ijb_sample from its
+ * logits: u[i] and the settings (host arrays of n values; temperature, top_k,
+ * top_p and min_p may be NULL) are entry i's.  next_tokens receives the tokens,
+ * probs (may be NULL) the probability each was drawn with. */
+int ijb_decode_sample(ijb_engine *engine, int n, const int *seq_ids, const int *tokens, const float *u,
+                      const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+                      int *next_tokens, float *probs);
 
 /* Greedy generation of one sequence with the token feedback on the device:
  * the reference's decode loop (main, inferencer.cu:1870-1883) from `next`

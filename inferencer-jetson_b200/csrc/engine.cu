@@ -21,6 +21,7 @@
 #include <unordered_map>
 #include <vector>
 #include <atomic>
+#include <functional>
 
 #include "../../include/ijb200.h"
 #include "attention.cuh"
@@ -28,6 +29,7 @@
 #include "gemv.cuh"
 #include "misc.cuh"
 #include "mma_gemm.cuh"
+#include "paged.cuh"
 
 namespace ijb {
 
@@ -95,6 +97,20 @@ struct ijb_engine {
     int kv_f32 = 0;
     int kv_elem = 2;
     long page_stride = 0;
+    // engines made by ijb_create_kv: attention is ijb_paged_attention over the pool
+    // (IJB_KV_F16 / IJB_KV_E4M3; -1: the engine's own attention).  An e4m3 pool is
+    // written by ijb_kv_append from the fp32 rows that the QKV projection leaves,
+    // [max_batch][K, V][kv_dim]: to the projection a cache of one-token pages,
+    // entry i in slot i.
+    int paged = -1;
+    int pool_elem = 2;            // bytes of a pool element
+    uint8_t *kv_scale = nullptr;  // e4m3: a scale byte per row, like the pool
+    float *kv_rows = nullptr;
+    int *row_slot = nullptr;      // 0, 1, 2, ...
+    int out_page_size = 0;        // the pages the projection writes
+    long out_page_stride = 0;
+    void *paged_work = nullptr;
+    size_t paged_work_bytes = 0;
     long num_pages = 0;
     std::vector<int> free_pages;
     int max_pages_per_seq = 0;
@@ -112,7 +128,10 @@ struct ijb_engine {
     float *x = nullptr, *q = nullptr, *attn = nullptr, *h = nullptr, *logits = nullptr;
     unsigned long long *keys = nullptr;
     int *next_dev = nullptr;
-    int *meta_dev = nullptr;   // [4][max_batch]: token, seq, pos, slot
+    // [4][max_batch]: token, seq, pos, slot; with paged attention behind them the
+    // step's entries: q_start [max_batch + 1], seq and kv_len [max_batch]
+    int *meta_dev = nullptr;
+    int meta_ints = 0;
     int *meta_host = nullptr;  // pinned
     int *next_host = nullptr;  // pinned
     float *attn_partial = nullptr;
@@ -133,8 +152,12 @@ struct ijb_engine {
     int attn_stream_min = 1;  // smallest step that uses the streaming attention
     uint32_t *status = nullptr;
     unsigned long long *scratch_key = nullptr;
+    // ijb_decode_sample (allocated on first use): u, temperature, top_p, min_p,
+    // top_k, then the tokens and their probabilities, [max_batch] words each
+    uint32_t *sample_dev = nullptr;
+    uint32_t *sample_host = nullptr;  // pinned
 
-    std::unordered_map<int, StepGraph> graphs;  // key: (n * 2 + need_logits) * 2 + traced
+    std::unordered_map<int, StepGraph> graphs;  // key: ((n * 2 + need_logits) * 2 + traced) * 3 + shape (StepShape)
     // device-side greedy loop (ijb_generate): its step graph, state, outputs, stop ids
     StepGraph gen_graph;
     GenState *gen_state = nullptr;
@@ -225,8 +248,8 @@ GemvParams base_params(ijb_engine *e, int cols, int batch, const float *x, long 
     p.half_head = e->head_dim / 2;
     p.kv_heads = e->d.kv_heads;
     p.head_dim = e->head_dim;
-    p.page_size = e->d.page_size;
-    p.page_stride = e->page_stride;
+    p.page_size = e->out_page_size;
+    p.page_stride = e->out_page_stride;
     p.kv_f32 = e->kv_f32;
     p.argmax_keys = e->keys;
     p.status = e->status;
@@ -271,7 +294,7 @@ void launch_projection(ijb_engine *e, cudaStream_t s, int g0, int gn, const floa
                        bool x16_ready = false, bool gemv_pdl = false) {
     const ijb_model_desc &d = e->d;
     const int *tpos = e->meta_dev + 2 * d.max_batch;
-    const int *tslot = e->meta_dev + 3 * d.max_batch;
+    const int *tslot = e->row_slot ? e->row_slot : e->meta_dev + 3 * d.max_batch;
     int dp = -1;
     const bool mma_ok = proj_uses_mma(e, gn, segs, nsegs, &dp);
     require(!x16_ready || (mma_ok && gn <= kMmaMaxN), "prepared activation without a single tensor-core chunk");
@@ -347,8 +370,8 @@ void launch_projection(ijb_engine *e, cudaStream_t s, int g0, int gn, const floa
             m.kv_f32 = e->kv_f32;
             m.kv_heads = d.kv_heads;
             m.head_dim = e->head_dim;
-            m.page_size = d.page_size;
-            m.page_stride = e->page_stride;
+            m.page_size = e->out_page_size;
+            m.page_stride = e->out_page_stride;
             m.argmax_keys = e->keys + g0 + t0;
             m.status = e->status;
             require(m.total_tiles == tiles, "projection tile count");
@@ -389,18 +412,68 @@ void enqueue_trace_quant(ijb_engine *e, int n, const float *x, long x_stride, co
     ++g_launches;
 }
 
+// Layer l's pool as the paged operators see it.
+ijb_kv_view layer_view(const ijb_engine *e, int l) {
+    const long pool = e->num_pages * e->page_stride;  // elements of a layer
+    ijb_kv_view v;
+    std::memset(&v, 0, sizeof(v));
+    v.type = e->paged;
+    v.kv_heads = e->d.kv_heads;
+    v.head_dim = e->head_dim;
+    v.page_size = e->d.page_size;
+    v.num_pages = e->num_pages;
+    v.data_dev = static_cast<char *>(e->kv) + l * pool * e->pool_elem;
+    v.scale_dev = e->kv_scale ? e->kv_scale + l * (pool / e->head_dim) : nullptr;
+    v.page_table_dev = e->page_table_dev;
+    v.n_seqs = e->d.max_seqs;
+    v.max_pages = e->max_pages_per_seq;
+    return v;
+}
+
+// The entries of a packed step for the paged attention: runs of consecutive
+// positions of one sequence.  A step of single tokens, or of one run, is
+// launched for what it is.
+enum StepShape { kStepSingles = 0, kStepOneRun = 1, kStepMixed = 2 };
+
+// Fills the entries behind the step block in meta_host from its n (seq, pos) pairs.
+StepShape fill_entries(ijb_engine *e, int n) {
+    if (e->paged < 0) return kStepSingles;
+    const int B = e->d.max_batch;
+    int *mt = e->meta_host, *start = mt + 4 * B, *seq = start + B + 1, *len = seq + B;
+    const int *sq = mt + B, *pos = mt + 2 * B;
+    int runs = 0;
+    for (int i = 0; i < n; ++i) {
+        if (i == 0 || sq[i] != sq[i - 1] || pos[i] != pos[i - 1] + 1) {
+            start[runs] = i;
+            seq[runs] = sq[i];
+            ++runs;
+        }
+        len[runs - 1] = pos[i] + 1;
+    }
+    for (int r = runs; r < B; ++r) seq[r] = len[r] = 0;  // empty
+    for (int r = runs; r <= B; ++r) start[r] = n;
+    return runs == n ? kStepSingles : (runs == 1 ? kStepOneRun : kStepMixed);
+}
+
 // The four projection launches of layer l for a packed step of n tokens (the
 // step's meta already on the device).
 void enqueue_qkv(ijb_engine *e, int l, int n, cudaStream_t s) {
     const ijb_model_desc &d = e->d;
     const auto &L = e->layers[l];
-    char *kbase = static_cast<char *>(e->kv) + l * e->num_pages * e->page_stride * e->kv_elem;
-    const long v_off = static_cast<long>(d.kv_heads) * d.page_size * e->head_dim;
+    char *kbase = e->kv_rows ? reinterpret_cast<char *>(e->kv_rows)
+                             : static_cast<char *>(e->kv) + l * e->num_pages * e->page_stride * e->kv_elem;
+    const long v_off = static_cast<long>(d.kv_heads) * e->out_page_size * e->head_dim;
     const ProjSeg segs[3] = {{L.q, -1, kEpiRopeQ, e->q, d.dim},
                              {L.k, -1, kEpiRopeKCache, nullptr, 0},
                              {L.v, -1, kEpiVCache, nullptr, 0}};
     launch_projection(e, s, 0, n, e->x, d.dim, reinterpret_cast<const float *>(e->w[L.attn_norm].data), segs, 3,
                       kbase, v_off, false, n < e->mma_min_batch && e->small_attn_pdl);
+    if (e->kv_rows) {
+        const ijb_kv_view v = layer_view(e, l);
+        if (ijb_kv_append(&v, IJB_TYPE_F32, e->kv_rows, e->kv_rows + e->kv_dim, 2L * e->kv_dim, n,
+                          e->meta_dev + d.max_batch, e->meta_dev + 2 * d.max_batch, e->status, s) != IJB_OK)
+            throw Error(IJB_ERR_CUDA, t_create_err);
+    }
 }
 void enqueue_o(ijb_engine *e, int l, int n, cudaStream_t s, bool x16_ready = false) {
     const ProjSeg o_segs[1] = {{e->layers[l].o, -1, kEpiAdd, e->x, e->d.dim}};
@@ -463,7 +536,20 @@ AttnParams attn_params(ijb_engine *e, int l, int n) {
     return a;
 }
 
-void enqueue_step(ijb_engine *e, int n, bool need_logits, cudaStream_t s, bool traced = false) {
+// Layer l's attention of the step by ijb_paged_attention.
+void enqueue_paged_attention(ijb_engine *e, int l, int n, StepShape shape, cudaStream_t s) {
+    const ijb_model_desc &d = e->d;
+    const int B = d.max_batch;
+    const int *start = e->meta_dev + 4 * B, *seq = start + B + 1, *len = seq + B;
+    const ijb_kv_view v = layer_view(e, l);
+    if (ijb_paged_attention(&v, d.heads, IJB_TYPE_F32, e->q, d.dim, e->attn, d.dim, n, shape == kStepOneRun ? 1 : n, start,
+                            seq, len, shape == kStepSingles ? 1 : 0, 1.0f / std::sqrt(static_cast<float>(e->head_dim)),
+                            e->paged_work, e->paged_work_bytes, e->status, s) != IJB_OK)
+        throw Error(IJB_ERR_CUDA, t_create_err);
+}
+
+void enqueue_step(ijb_engine *e, int n, bool need_logits, cudaStream_t s, bool traced = false,
+                  StepShape shape = kStepSingles) {
     const ijb_model_desc &d = e->d;
     const int *tok = e->meta_dev;
     const Weight &emb = e->w[e->token_embd];
@@ -475,23 +561,27 @@ void enqueue_step(ijb_engine *e, int n, bool need_logits, cudaStream_t s, bool t
             enqueue_trace_quant(e, n, e->x, d.dim, reinterpret_cast<const float *>(e->w[L.attn_norm].data), d.dim, l, 0,
                                 s);
         enqueue_qkv(e, l, n, s);
-        AttnParams a = attn_params(e, l, n);
-        // the streaming attention's finish kernel also builds the O projection's
-        // activation tile when that projection is one tensor-core chunk
-        const ProjSeg o_segs[1] = {{L.o, -1, kEpiAdd, e->x, d.dim}};
-        int o_dp = 0;
-        const bool o_fused =
-            e->attn_prep && attention_kernels(a) == 2 && n <= kMmaMaxN && proj_uses_mma(e, n, o_segs, 1, &o_dp);
-        if (o_fused) {
-            a.x16 = e->x16;
-            a.x_inv = e->x_inv;
-            a.n_pad = (n + 15) / 16 * 16;
-            a.use_dp4a = o_dp;
+        bool o_fused = false;
+        if (e->paged >= 0) {
+            enqueue_paged_attention(e, l, n, shape, s);
+        } else {
+            AttnParams a = attn_params(e, l, n);
+            // the streaming attention's finish kernel also builds the O projection's
+            // activation tile when that projection is one tensor-core chunk
+            const ProjSeg o_segs[1] = {{L.o, -1, kEpiAdd, e->x, d.dim}};
+            int o_dp = 0;
+            o_fused = e->attn_prep && attention_kernels(a) == 2 && n <= kMmaMaxN && proj_uses_mma(e, n, o_segs, 1, &o_dp);
+            if (o_fused) {
+                a.x16 = e->x16;
+                a.x_inv = e->x_inv;
+                a.n_pad = (n + 15) / 16 * 16;
+                a.use_dp4a = o_dp;
+            }
+            // tensor-core steps chain their launches with programmatic dependent launch
+            ck(attention_launch(a, s, e->pdl || (n >= e->mma_min_batch ? e->attn_pdl : e->small_attn_pdl)),
+               "attention launch");
+            g_launches += attention_kernels(a);
         }
-        // tensor-core steps chain their launches with programmatic dependent launch
-        ck(attention_launch(a, s, e->pdl || (n >= e->mma_min_batch ? e->attn_pdl : e->small_attn_pdl)),
-           "attention launch");
-        g_launches += attention_kernels(a);
         if (traced) enqueue_trace_quant(e, n, e->attn, d.dim, nullptr, d.dim, l, d.dim, s);
         enqueue_o(e, l, n, s, o_fused && !traced);
         if (traced)
@@ -538,19 +628,20 @@ void check_device_status(ijb_engine *e) {
 }
 
 // Captures (once per n / need_logits) and replays the whole step: H2D of the
-// step's metadata, every kernel, D2H of the next tokens.
-void run_step(ijb_engine *e, int n, bool need_logits, bool traced = false) {
-    const int key = (n * 2 + (need_logits ? 1 : 0)) * 2 + (traced ? 1 : 0);
+// step's metadata, every kernel, D2H of the next tokens.  `then` is queued behind
+// the step, before the host waits for both.
+void run_step(ijb_engine *e, int n, bool need_logits, bool traced = false, StepShape shape = kStepSingles,
+              const std::function<void(cudaStream_t)> &then = nullptr) {
+    const int key = ((n * 2 + (need_logits ? 1 : 0)) * 2 + (traced ? 1 : 0)) * 3 + shape;
     auto it = e->graphs.find(key);
     if (it == e->graphs.end()) {
         cudaGraph_t graph;
         const uint64_t before = g_launches.load();
         ck(cudaStreamBeginCapture(e->stream, cudaStreamCaptureModeThreadLocal), "begin capture");
         try {
-            ck(cudaMemcpyAsync(e->meta_dev, e->meta_host, 4 * e->d.max_batch * sizeof(int), cudaMemcpyHostToDevice,
-                               e->stream),
+            ck(cudaMemcpyAsync(e->meta_dev, e->meta_host, e->meta_ints * sizeof(int), cudaMemcpyHostToDevice, e->stream),
                "meta H2D");
-            enqueue_step(e, n, need_logits, e->stream, traced);
+            enqueue_step(e, n, need_logits, e->stream, traced, shape);
             // the next tokens with the status word behind them, or the status word alone
             const int B = e->d.max_batch;
             if (need_logits)
@@ -578,6 +669,7 @@ void run_step(ijb_engine *e, int n, bool need_logits, bool traced = false) {
     ck(cudaEventRecord(e->ev_start, e->stream), "step timer start");
     ck(cudaGraphLaunch(it->second.exec, e->stream), "graph launch");
     ck(cudaEventRecord(e->ev_end, e->stream), "step timer end");
+    if (then) then(e->stream);
     ck(cudaStreamSynchronize(e->stream), "step synchronize");
     ck(cudaEventElapsedTime(&e->last_step_ms, e->ev_start, e->ev_end), "step timer");
     check_status_word(e, static_cast<uint32_t>(e->next_host[e->d.max_batch]));
@@ -607,7 +699,7 @@ int slot_for(ijb_engine *e, int seq, int pos) {
 
 // Fills meta for entries (seq, token) at explicit positions and runs a step.
 void packed_step(ijb_engine *e, int n, const int *seqs, const int *tokens, const int *positions, bool need_logits,
-                 bool traced = false) {
+                 bool traced = false, const std::function<void(cudaStream_t)> &then = nullptr) {
     const ijb_model_desc &d = e->d;
     require(n >= 1 && n <= d.max_batch, "step size must be 1..max_batch", IJB_ERR_CAPACITY);
     int *mt = e->meta_host;
@@ -622,7 +714,19 @@ void packed_step(ijb_engine *e, int n, const int *seqs, const int *tokens, const
         mt[3 * d.max_batch + i] = slot_for(e, sq, pos);
     }
     for (int i = n; i < d.max_batch; ++i) mt[i] = mt[d.max_batch + i] = mt[2 * d.max_batch + i] = mt[3 * d.max_batch + i] = 0;
-    run_step(e, n, need_logits, traced);
+    run_step(e, n, need_logits, traced, fill_entries(e, n), then);
+}
+
+// The position of each entry of a decode step, and every sequence's length after it.
+void step_positions(const ijb_engine *e, int n, const int *seq_ids, std::vector<int> &pos,
+                    std::unordered_map<int, int> &next_pos) {
+    for (int i = 0; i < n; ++i) {
+        const int s = seq_ids[i];
+        require(s >= 0 && s < e->d.max_seqs && e->seq_used[s], "unknown sequence id");
+        auto it = next_pos.find(s);
+        pos[i] = it == next_pos.end() ? e->seq_len[s] : it->second;
+        next_pos[s] = pos[i] + 1;
+    }
 }
 
 void ensure_trace_buffers(ijb_engine *e) {
@@ -660,10 +764,14 @@ void validate_weight(const Weight &w, int type_a, int type_b, int rows, int cols
 
 extern "C" {
 
-int ijb_create(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, ijb_engine **out) {
+static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, int kv_type,
+                         ijb_engine **out) {
     std::unique_ptr<ijb_engine> e(new ijb_engine());
     try {
         require(desc && out && tensors, "null argument");
+        require(kv_type == -1 || kv_type == IJB_KV_F16 || kv_type == IJB_KV_E4M3,
+                "cache type must be IJB_KV_F16 or IJB_KV_E4M3");
+        e->paged = kv_type;
         e->d = *desc;
         ijb_model_desc &d = e->d;
         if (d.page_size <= 0) d.page_size = 16;
@@ -870,12 +978,28 @@ int ijb_create(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n
         e->max_pages_per_seq = (d.context + d.page_size - 1) / d.page_size;
         e->num_pages = d.num_pages > 0 ? d.num_pages : static_cast<long>(d.max_seqs) * e->max_pages_per_seq;
         e->page_stride = 2L * d.kv_heads * d.page_size * e->head_dim;
+        if (e->paged >= 0) d.kv_f32 = e->paged == IJB_KV_E4M3;  // what the projection writes
         e->kv_f32 = d.kv_f32 ? 1 : 0;
         e->kv_elem = e->kv_f32 ? 4 : 2;
-        const size_t kv_bytes = static_cast<size_t>(d.layers) * e->num_pages * e->page_stride * e->kv_elem;
+        e->pool_elem = e->paged == IJB_KV_E4M3 ? 1 : e->kv_elem;
+        e->out_page_size = d.page_size;
+        e->out_page_stride = e->page_stride;
+        if (e->paged == IJB_KV_E4M3) {
+            e->out_page_size = 1;
+            e->out_page_stride = 2L * e->kv_dim;
+            e->kv_rows = dev_alloc<float>(static_cast<size_t>(d.max_batch) * 2 * e->kv_dim, "K/V rows");
+            std::vector<int> slot(d.max_batch);
+            for (int i = 0; i < d.max_batch; ++i) slot[i] = i;
+            e->row_slot = dev_alloc<int>(d.max_batch, "K/V row slots");
+            ck(cudaMemcpy(e->row_slot, slot.data(), d.max_batch * sizeof(int), cudaMemcpyHostToDevice), "K/V row slots");
+            const size_t scales = static_cast<size_t>(d.layers) * e->num_pages * (e->page_stride / e->head_dim);
+            e->kv_scale = dev_alloc<uint8_t>(scales, "KV scales");
+            ck(cudaMemset(e->kv_scale, 0, scales), "KV scales clear");
+        }
+        const size_t kv_bytes = static_cast<size_t>(d.layers) * e->num_pages * e->page_stride * e->pool_elem;
         e->kv = dev_alloc<char>(kv_bytes, "KV pool");
         ck(cudaMemset(e->kv, 0, kv_bytes), "KV clear");
-        if (!e->kv_f32 && (e->head_dim == 64 || e->head_dim == 128)) {
+        if (!e->kv_f32 && e->paged < 0 && (e->head_dim == 64 || e->head_dim == 128)) {
             const long layer_pool = e->num_pages * e->page_stride;
             e->kv_maps.resize(d.layers);
             for (int l = 0; l < d.layers && !e->kv_maps.empty(); ++l)
@@ -904,11 +1028,20 @@ int ijb_create(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n
         e->keys = dev_alloc<unsigned long long>(B, "argmax keys");
         // the next tokens, then the device status word: one copy brings both back
         e->next_dev = dev_alloc<int>(B + 1, "next tokens");
-        e->meta_dev = dev_alloc<int>(4 * B, "step meta");
-        ck(cudaMemset(e->meta_dev, 0, 4 * B * sizeof(int)), "meta clear");
-        ck(cudaMallocHost(&e->meta_host, 4 * B * sizeof(int)), "meta staging");
+        e->meta_ints = static_cast<int>(e->paged >= 0 ? 7 * B + 1 : 4 * B);
+        e->meta_dev = dev_alloc<int>(e->meta_ints, "step meta");
+        ck(cudaMemset(e->meta_dev, 0, e->meta_ints * sizeof(int)), "meta clear");
+        ck(cudaMallocHost(&e->meta_host, e->meta_ints * sizeof(int)), "meta staging");
         ck(cudaMallocHost(&e->next_host, (B + 1) * sizeof(int)), "next staging");
-        std::memset(e->meta_host, 0, 4 * B * sizeof(int));
+        std::memset(e->meta_host, 0, e->meta_ints * sizeof(int));
+        if (e->paged >= 0) {
+            const ijb_kv_view v = layer_view(e.get(), 0);
+            e->paged_work_bytes = ijb_paged_attention_workspace(&v);
+            require(e->paged_work_bytes > 0, "paged attention: " + t_create_err);
+            require(d.max_batch <= 4096, "max_batch must be <= 4096 with a paged attention cache type");
+            e->paged_work = dev_alloc<uint8_t>(e->paged_work_bytes, "paged attention workspace");
+            ck(paged_attention_prepare(e->head_dim, e->paged == IJB_KV_E4M3), "paged attention attributes");
+        }
         // attention: partial softmax records per (token, head) at work-item granularity
         e->attn_split_len = attention_split_len();
         e->attn_max_splits = (d.context + attention_item_len() - 1) / attention_item_len();
@@ -928,6 +1061,19 @@ int ijb_create(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n
     }
 }
 
+int ijb_create(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, ijb_engine **out) {
+    return create_engine(desc, tensors, n_tensors, -1, out);
+}
+
+int ijb_create_kv(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, int kv_type,
+                  ijb_engine **out) {
+    if (kv_type < 0) {
+        set_thread_error("ijb_create_kv: cache type must be IJB_KV_F16 or IJB_KV_E4M3");
+        return IJB_ERR_INVALID;
+    }
+    return create_engine(desc, tensors, n_tensors, kv_type, out);
+}
+
 void ijb_destroy(ijb_engine *e) {
     if (!e) return;
     if (e->d.device >= 0) cudaSetDevice(e->d.device);
@@ -943,6 +1089,12 @@ void ijb_destroy(ijb_engine *e) {
         if (w.mma_owned) cudaFree(w.mma_owned);
     }
     cudaFree(e->kv);
+    cudaFree(e->kv_scale);
+    cudaFree(e->kv_rows);
+    cudaFree(e->row_slot);
+    cudaFree(e->paged_work);
+    cudaFree(e->sample_dev);
+    if (e->sample_host) cudaFreeHost(e->sample_host);
     cudaFree(e->page_table_dev);
     if (e->page_table_host) cudaFreeHost(e->page_table_host);
     cudaFree(e->rope_cos);
@@ -1151,13 +1303,31 @@ int ijb_time_layer_attention(ijb_engine *e, int n, const int *seq_ids, int reps,
         }
         ck(cudaMemcpyAsync(e->meta_dev, e->meta_host, 4 * d.max_batch * sizeof(int), cudaMemcpyHostToDevice, e->stream),
            "meta H2D");
+        const StepShape shape = fill_entries(e, n);
+        if (e->paged >= 0)
+            ck(cudaMemcpyAsync(e->meta_dev, e->meta_host, e->meta_ints * sizeof(int), cudaMemcpyHostToDevice, e->stream),
+               "meta H2D");
         const AttnParams a = attn_params(e, 0, n);
+        const uint64_t before = g_launches.load();
         const bool pdl = e->pdl || (n >= e->mma_min_batch ? e->attn_pdl : e->small_attn_pdl);
         cudaGraph_t graph;
         cudaGraphExec_t exec = nullptr;
         ck(cudaStreamBeginCapture(e->stream, cudaStreamCaptureModeThreadLocal), "begin capture");
         cudaError_t ce = cudaSuccess;
-        for (int r = 0; r < reps && ce == cudaSuccess; ++r) ce = attention_launch(a, e->stream, pdl);
+        try {
+            for (int r = 0; r < reps && ce == cudaSuccess; ++r) {
+                if (e->paged >= 0) {
+                    enqueue_paged_attention(e, 0, n, shape, e->stream);
+                } else {
+                    ce = attention_launch(a, e->stream, pdl);
+                    g_launches += attention_kernels(a);
+                }
+            }
+        } catch (...) {
+            cudaStreamEndCapture(e->stream, &graph);
+            throw;
+        }
+        const uint64_t launches = g_launches.load() - before;
         const cudaError_t ee = cudaStreamEndCapture(e->stream, &graph);
         if (ee == cudaSuccess && ce != cudaSuccess) cudaGraphDestroy(graph);
         ck(ce, "attention launch");
@@ -1174,10 +1344,10 @@ int ijb_time_layer_attention(ijb_engine *e, int n, const int *seq_ids, int reps,
         if (le == cudaSuccess) le = cudaEventElapsedTime(&ms, e->ev_start, e->ev_end);
         cudaGraphExecDestroy(exec);
         ck(le, "attention timing");
-        g_launches += 2ull * reps * attention_kernels(a);
+        g_launches += launches;  // the second replay (the capture counted the first)
         check_device_status(e);
         *ms_per_layer = ms / reps;
-        *kv_bytes = positions * d.kv_heads * 2LL * e->head_dim * e->kv_elem;
+        *kv_bytes = positions * d.kv_heads * 2LL * (e->head_dim * e->pool_elem + (e->kv_scale ? 1 : 0));
         return IJB_OK;
     } catch (const std::exception &ex) {
         return fail(e, ex);
@@ -1275,12 +1445,14 @@ int ijb_generate(ijb_engine *e, int seq, int first_token, int max_tokens, const 
         // at most this many steps feed a new position; their pages are allocated now
         const int steps = std::min(max_tokens - 1, d.context - pos0);
         int *mt = e->meta_host;
-        std::memset(mt, 0, 4 * d.max_batch * sizeof(int));
+        std::memset(mt, 0, e->meta_ints * sizeof(int));
         for (int k = steps - 1; k >= 0; --k) slot_for(e, seq, pos0 + k);
         mt[0] = first_token;
         mt[d.max_batch] = seq;
         mt[2 * d.max_batch] = pos0;
         mt[3 * d.max_batch] = slot_for(e, seq, pos0);
+        fill_entries(e, 1);
+        int *gen_len = e->paged >= 0 ? e->meta_dev + 6 * d.max_batch + 1 : nullptr;  // the entry's kv_len
         if (!e->gen_state) {
             e->gen_state = dev_alloc<GenState>(1, "generate state");
             e->gen_out = dev_alloc<int>(d.context + 1, "generate output");
@@ -1295,7 +1467,7 @@ int ijb_generate(ijb_engine *e, int seq, int first_token, int max_tokens, const 
         g.page_size = d.page_size;
         g.max_pages_per_seq = e->max_pages_per_seq;
         cudaStream_t s = e->stream;
-        ck(cudaMemcpyAsync(e->meta_dev, mt, 4 * d.max_batch * sizeof(int), cudaMemcpyHostToDevice, s), "meta H2D");
+        ck(cudaMemcpyAsync(e->meta_dev, mt, e->meta_ints * sizeof(int), cudaMemcpyHostToDevice, s), "meta H2D");
         ck(cudaMemcpyAsync(e->gen_state, &g, sizeof(g), cudaMemcpyHostToDevice, s), "generate state H2D");
         if (n_stop) ck(cudaMemcpyAsync(e->gen_stop, stop_ids, n_stop * sizeof(int), cudaMemcpyHostToDevice, s), "stop H2D");
         ck(cudaStreamSynchronize(s), "generate setup");  // the host buffers above are stack / staging memory
@@ -1307,7 +1479,7 @@ int ijb_generate(ijb_engine *e, int seq, int first_token, int max_tokens, const 
             try {
                 enqueue_step(e, 1, true, s, false);
                 ck(gen_advance_launch(e->gen_state, e->next_dev, e->meta_dev, d.max_batch, e->page_table_dev,
-                                      e->gen_stop, e->gen_out, s),
+                                      e->gen_stop, e->gen_out, gen_len, s),
                    "generate advance launch");
                 ++g_launches;
             } catch (...) {
@@ -1365,16 +1537,51 @@ int ijb_decode_step(ijb_engine *e, int n, const int *seq_ids, const int *tokens,
         require(n >= 1 && n <= e->d.max_batch, "step size must be 1..max_batch", IJB_ERR_CAPACITY);
         std::vector<int> pos(n);
         std::unordered_map<int, int> next_pos;
-        for (int i = 0; i < n; ++i) {
-            const int s = seq_ids[i];
-            require(s >= 0 && s < e->d.max_seqs && e->seq_used[s], "unknown sequence id");
-            auto it = next_pos.find(s);
-            pos[i] = it == next_pos.end() ? e->seq_len[s] : it->second;
-            next_pos[s] = pos[i] + 1;
-        }
+        step_positions(e, n, seq_ids, pos, next_pos);
         packed_step(e, n, seq_ids, tokens, pos.data(), true);
         for (auto &kv : next_pos) e->seq_len[kv.first] = kv.second;
         if (next_tokens) std::memcpy(next_tokens, e->next_host, n * sizeof(int));
+        return IJB_OK;
+    } catch (const std::exception &ex) {
+        return fail(e, ex);
+    }
+}
+
+int ijb_decode_sample(ijb_engine *e, int n, const int *seq_ids, const int *tokens, const float *u,
+                      const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+                      int *next_tokens, float *probs) {
+    try {
+        require(e != nullptr && seq_ids != nullptr && tokens != nullptr && u != nullptr && next_tokens != nullptr,
+                "bad arguments");
+        const int B = e->d.max_batch;
+        require(n >= 1 && n <= B, "step size must be 1..max_batch", IJB_ERR_CAPACITY);
+        if (!e->sample_host) {
+            if (!e->sample_dev) e->sample_dev = dev_alloc<uint32_t>(7 * static_cast<size_t>(B), "sampling settings");
+            ck(cudaMallocHost(&e->sample_host, 7 * static_cast<size_t>(B) * 4), "sampling staging");
+        }
+        uint32_t *h = e->sample_host, *dv = e->sample_dev;
+        const void *given[5] = {u, temperature, top_p, min_p, top_k};
+        std::memset(h, 0, 5 * static_cast<size_t>(B) * 4);
+        for (int i = 0; i < 5; ++i)
+            if (given[i]) std::memcpy(h + static_cast<size_t>(i) * B, given[i], static_cast<size_t>(n) * 4);
+        std::vector<int> pos(n);
+        std::unordered_map<int, int> next_pos;
+        step_positions(e, n, seq_ids, pos, next_pos);
+        auto f32 = [&](int i) { return given[i] ? reinterpret_cast<const float *>(dv + static_cast<size_t>(i) * B) : nullptr; };
+        packed_step(e, n, seq_ids, tokens, pos.data(), true, false, [&](cudaStream_t s) {
+            ck(cudaMemcpyAsync(dv, h, 5 * static_cast<size_t>(B) * 4, cudaMemcpyHostToDevice, s), "sampling settings H2D");
+            if (ijb_sample(e->logits, e->d.vocab, n, e->d.vocab, f32(0), f32(1),
+                           top_k ? reinterpret_cast<const int *>(dv + 4 * static_cast<size_t>(B)) : nullptr, f32(2), f32(3),
+                           reinterpret_cast<int *>(dv + 5 * static_cast<size_t>(B)),
+                           reinterpret_cast<float *>(dv + 6 * static_cast<size_t>(B)), s) != IJB_OK)
+                throw Error(IJB_ERR_CUDA, t_create_err);
+            ck(cudaMemcpyAsync(h + 5 * static_cast<size_t>(B), dv + 5 * static_cast<size_t>(B),
+                               2 * static_cast<size_t>(B) * 4, cudaMemcpyDeviceToHost, s),
+               "sampled tokens D2H");
+        });
+        for (auto &kv : next_pos) e->seq_len[kv.first] = kv.second;
+        std::memcpy(next_tokens, h + 5 * static_cast<size_t>(B), static_cast<size_t>(n) * 4);
+        if (probs) std::memcpy(probs, h + 6 * static_cast<size_t>(B), static_cast<size_t>(n) * 4);
         return IJB_OK;
     } catch (const std::exception &ex) {
         return fail(e, ex);

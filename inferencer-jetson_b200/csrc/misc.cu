@@ -259,7 +259,7 @@ cudaError_t wait_probe_launch(uint32_t *status, uint64_t limit_ns, cudaStream_t 
 // step already queued recomputes the last position: the same K/V, written to
 // the same slot.
 __global__ void ijb_gen_advance_kernel(GenState *g, const int *next, int *meta, int max_batch, const int *page_table,
-                                       const int *stop_ids, int *out) {
+                                       const int *stop_ids, int *out, int *kv_len) {
     if (threadIdx.x != 0 || g->done) return;
     const int t = next[0];
     ++g->processed;  // the token in meta was fed at its position
@@ -278,11 +278,12 @@ __global__ void ijb_gen_advance_kernel(GenState *g, const int *next, int *meta, 
     meta[0] = t;
     meta[2 * max_batch] = pos;
     meta[3 * max_batch] = page_table[static_cast<long>(g->seq) * g->max_pages_per_seq + pos / ps] * ps + pos % ps;
+    if (kv_len) *kv_len = pos + 1;  // the paged attention's entry
 }
 
 cudaError_t gen_advance_launch(GenState *g, const int *next, int *meta, int max_batch, const int *page_table,
-                               const int *stop_ids, int *out, cudaStream_t stream) {
-    ijb_gen_advance_kernel<<<1, 32, 0, stream>>>(g, next, meta, max_batch, page_table, stop_ids, out);
+                               const int *stop_ids, int *out, int *kv_len, cudaStream_t stream) {
+    ijb_gen_advance_kernel<<<1, 32, 0, stream>>>(g, next, meta, max_batch, page_table, stop_ids, out, kv_len);
     return cudaGetLastError();
 }
 

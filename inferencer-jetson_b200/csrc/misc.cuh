@@ -37,8 +37,9 @@ struct GenState {
     int max_tokens, context, n_stop, seq, page_size, max_pages_per_seq;
 };
 // One thread: consumes the step's next token and sets up the next step's meta
-// (token, position, KV slot) in place, or ends the loop.
+// (token, position, KV slot; kv_len, unless NULL, the positions cached with it) in
+// place, or ends the loop.
 cudaError_t gen_advance_launch(GenState *g, const int *next, int *meta, int max_batch, const int *page_table,
-                               const int *stop_ids, int *out, cudaStream_t stream);
+                               const int *stop_ids, int *out, int *kv_len, cudaStream_t stream);
 
 }  // namespace ijb

@@ -45,5 +45,8 @@ inline int kv_fail(int code, const char *fn, const std::string &msg) {
 }
 // Checks a caller's view and fills the device view; returns an empty string, or what is wrong.
 std::string kv_view_check(const ijb_kv_view *v, KvDev *out);
+// Sets the attributes of ijb_paged_attention's fp32 kernels on the current device
+// (done by the first call otherwise; an engine does it before it captures one).
+cudaError_t paged_attention_prepare(int head_dim, bool e4m3);
 
 }  // namespace ijb

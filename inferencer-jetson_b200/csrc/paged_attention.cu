@@ -1560,12 +1560,25 @@ cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     return e;
 }
 
+template <int HD, bool E4M3, bool WIDE>
+constexpr int decode_smem() {
+    return Dec<HD, E4M3, WIDE>::kSmem > kDecPlanBytes ? Dec<HD, E4M3, WIDE>::kSmem : kDecPlanBytes;
+}
+template <int HD, bool E4M3, bool WIDE, typename T>
+cudaError_t decode_allow() {
+    auto kernel = ijb_paged_decode_kernel<HD, E4M3, WIDE, T>;
+    return allow_smem<decltype(kernel), Dec<HD, E4M3, WIDE>, T>(kernel, decode_smem<HD, E4M3, WIDE>());
+}
+template <int HD, bool E4M3, typename T>
+cudaError_t tile_allow() {
+    auto kernel = ijb_paged_tile_kernel<HD, E4M3, T>;
+    return allow_smem<decltype(kernel), Tile<HD, T>, std::bool_constant<E4M3>>(kernel, Tile<HD, T>::kSmem);
+}
+
 template <int HD, bool E4M3, bool WIDE, typename T>
 cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     using D = Dec<HD, E4M3, WIDE>;
-    constexpr int smem = D::kSmem > kDecPlanBytes ? D::kSmem : kDecPlanBytes;
-    auto kernel = ijb_paged_decode_kernel<HD, E4M3, WIDE, T>;
-    const cudaError_t e = allow_smem<decltype(kernel), D, T>(kernel, smem);
+    const cudaError_t e = decode_allow<HD, E4M3, WIDE, T>();
     if (e != cudaSuccess) return e;
     a.min_rows = 1;
     a.max_rows = WIDE ? kDecRows : 8;
@@ -1574,15 +1587,14 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.unit = kChunk;
     a.workers = sms * D::kWarps;
     a.min_units = 2;
-    kernel<<<sms, D::kWarps * 32, smem, s>>>(a);
+    ijb_paged_decode_kernel<HD, E4M3, WIDE, T><<<sms, D::kWarps * 32, decode_smem<HD, E4M3, WIDE>(), s>>>(a);
     return merge_launch<kDecRows, HD, T>(a, s);
 }
 
 template <int HD, bool E4M3, typename T>
 cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     using L = Tile<HD, T>;
-    auto kernel = ijb_paged_tile_kernel<HD, E4M3, T>;
-    const cudaError_t e = allow_smem<decltype(kernel), Tile<HD, T>, std::bool_constant<E4M3>>(kernel, L::kSmem);
+    const cudaError_t e = tile_allow<HD, E4M3, T>();
     if (e != cudaSuccess) return e;
     a.min_rows = min_rows;
     a.max_rows = 0x7fffffff;
@@ -1591,7 +1603,7 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     a.unit = kBlock;
     a.workers = sms;
     a.min_units = 2;
-    kernel<<<sms, kTileThreads, L::kSmem, s>>>(a);
+    ijb_paged_tile_kernel<HD, E4M3, T><<<sms, kTileThreads, L::kSmem, s>>>(a);
     return merge_launch<kTileRows, HD, T>(a, s);
 }
 
@@ -1622,7 +1634,21 @@ size_t workspace_bytes(int sms, int head_dim) {
     return static_cast<size_t>(sms) * kMaxWorkers * sizeof(int4) + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
 }
 
+template <int HD, bool E4M3>
+cudaError_t prepare() {
+    cudaError_t e = decode_allow<HD, E4M3, false, float>();
+    if (e == cudaSuccess) e = decode_allow<HD, E4M3, true, float>();
+    if (e == cudaSuccess) e = tile_allow<HD, E4M3, float>();
+    return e;
+}
+
 }  // namespace
+
+cudaError_t paged_attention_prepare(int head_dim, bool e4m3) {
+    if (head_dim == 64) return e4m3 ? prepare<64, true>() : prepare<64, false>();
+    return e4m3 ? prepare<128, true>() : prepare<128, false>();
+}
+
 }  // namespace ijb
 
 extern "C" {

@@ -33,7 +33,7 @@ def copy_d2h(dst: np.ndarray, src_ptr: int) -> np.ndarray:
 class Engine:
     def __init__(self, cfg: ModelConfig, weights: dict, context: int = 1024, max_batch: int = 1,
                  max_seqs: int = 2, use_dp4a: bool = True, use_q6_dp4a: bool = True, device: int = 0,
-                 num_pages: int = 0, page_size: int = 16, kv_f32: bool = False):
+                 num_pages: int = 0, page_size: int = 16, kv_f32: bool = False, kv_type: str | None = None):
         import torch
         self.lib = _L.load()
         self.cfg = cfg
@@ -65,7 +65,11 @@ class Engine:
                          num_pages=num_pages, use_dp4a=int(use_dp4a), use_q6_dp4a=int(use_q6_dp4a),
                          kv_f32=int(kv_f32), device=device)
         h = ctypes.c_void_p()
-        rc = self.lib.ijb_create(ctypes.byref(d), views, len(weights), ctypes.byref(h))
+        if kv_type is None:
+            rc = self.lib.ijb_create(ctypes.byref(d), views, len(weights), ctypes.byref(h))
+        else:  # "f16" or "e4m3": a pool of that type, read by the paged attention
+            rc = self.lib.ijb_create_kv(ctypes.byref(d), views, len(weights), {"f16": 0, "e4m3": 2}[kv_type],
+                                        ctypes.byref(h))
         _L.check(rc, None)
         self.h = h
         self.context = context
@@ -163,6 +167,23 @@ class Engine:
         _L.check(self.lib.ijb_decode_step(self.h, n, s.ctypes.data_as(ip), t.ctypes.data_as(ip),
                                           out.ctypes.data_as(ip)), self.h)
         return out
+
+    def decode_sample(self, seq_ids, tokens, u, temperature=None, top_k=None, top_p=None, min_p=None):
+        """ijb_decode_sample: one packed step whose next tokens are drawn with ijb_sample;
+        settings are one value per entry, or None.  Returns (tokens, probabilities)."""
+        s = np.ascontiguousarray(seq_ids, dtype=np.int32)
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        n = len(s)
+        given = [None if v is None else np.ascontiguousarray(v, dtype=dt) for v, dt in (
+            (u, np.float32), (temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        if len(t) != n or any(v is not None and v.shape != (n,) for v in given):
+            raise ValueError("tokens and settings: one value for each of seq_ids")
+        out, prob = np.empty(n, dtype=np.int32), np.empty(n, dtype=np.float32)
+        ip = ctypes.POINTER(ctypes.c_int)
+        _L.check(self.lib.ijb_decode_sample(self.h, n, s.ctypes.data_as(ip), t.ctypes.data_as(ip),
+                                            *[None if v is None else v.ctypes.data for v in given],
+                                            out.ctypes.data_as(ip), prob.ctypes.data), self.h)
+        return out, prob
 
     def generate(self, seq_id: int, first_token: int, max_tokens: int, stop_ids=()) -> list:
         """ijb_generate: greedy tokens from first_token on, fed back on the device

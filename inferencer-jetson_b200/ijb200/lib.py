@@ -64,6 +64,7 @@ def load():
     IP = ctypes.POINTER(ctypes.c_int)
     sig = {
         "ijb_create": ([ctypes.POINTER(ModelDesc), ctypes.POINTER(TensorView), I, ctypes.POINTER(P)], I),
+        "ijb_create_kv": ([ctypes.POINTER(ModelDesc), ctypes.POINTER(TensorView), I, I, ctypes.POINTER(P)], I),
         "ijb_destroy": ([P], None),
         "ijb_last_error": ([P], ctypes.c_char_p),
         "ijb_tensor_index": ([P, ctypes.c_char_p], I),
@@ -77,6 +78,7 @@ def load():
         "ijb_seq_close": ([P, I], I),
         "ijb_seq_length": ([P, I], I),
         "ijb_decode_step": ([P, I, IP, IP, IP], I),
+        "ijb_decode_sample": ([P, I, IP, IP, P, P, P, P, P, IP, P], I),
         "ijb_generate": ([P, I, I, I, IP, I, IP, IP], I),
         "ijb_seq_prefill": ([P, I, IP, I, IP], I),
         "ijb_argmax": ([P, I, P, P], I),
