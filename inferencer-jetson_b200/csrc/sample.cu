@@ -18,14 +18,17 @@
 //
 // One cluster per row: each CTA keeps its part of the row in shared memory, so
 // the logits are read from HBM once.  The order is never built.  The tokens are
-// counted in 2048 bins of -t (64 a nat, the last open); a bin's tokens weigh
-// between exp(-(b + 1) / 64) and exp(-b / 64) each, so the counts alone say, to
-// 1.6 %, in which few bins a mass falls.  Those bins' tokens (and all before
-// them where they fit) are gathered in the leader CTA, sorted and summed; the
-// mass before them is summed in registers.  (Counting masses in the bins too
-// took 15 us a row: a 64-bit shared-memory addition a token.)  A range of more
-// than kCap tokens is split first, by finer bins of t, then by the bits of the
-// logits, down to equal ones, which the order by index decides.
+// counted and weighed in 1024 bins of -t (64 a nat, the last open), which says in
+// which bin a cut falls.  That bin's tokens (and all before them where they fit)
+// are gathered in the leader CTA, which narrows them by finer bins to at most
+// kFew and finds each one's place by looking at all.  A bin of too many tokens is
+// split over the cluster first, by finer bins of t, then by the bits of the
+// logits, down to equal ones, which the order by index decides.  A row with a
+// small top-k weighs only what its list holds: then the first pass only counts.
+//
+// What bounds it: for many rows the instructions of the first pass (about 60 a
+// logit with exp, its conversion and two shared-memory additions); for one row
+// the chain of cluster-wide steps.
 #include <mutex>
 #include <string>
 
@@ -38,11 +41,11 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kSplit = 1024;          // bins of a split
-constexpr int kCap = 1024;            // tokens the leader sorts: two a thread
-constexpr int kMaxChunk = 16384;      // logits per CTA
-constexpr int kMaxCluster = 8;
+constexpr int kBins = 1024;
+constexpr int kCap = 1024;            // tokens of the leader's list
+constexpr int kFew = 128;             // tokens that are put in order
+constexpr int kMaxVocab = 131072;
+constexpr int kMaxCluster = 16;
 constexpr float kBinsPerNat = 64.f;
 constexpr float kFixed = 17592186044416.f;  // 2^44
 typedef unsigned long long u64;
@@ -58,10 +61,10 @@ struct SampleParams {
     float *prob;
 };
 
-enum Cmd { kDone, kSums, kHist, kGather, kEqual };
+enum Cmd { kDone, kMass, kHist, kGather, kEqual };
 
 // Which tokens an order is about: bins lo..hi of -t; with sub >= 0 the sub-th of
-// kSplit equal parts of those; with sh < 32 the logits whose key starts with pref.
+// kBins equal parts of those; with sh < 32 the logits whose key starts with pref.
 struct Range {
     int lo, hi, sub, sh;
     uint32_t pref;
@@ -70,28 +73,29 @@ struct Range {
 struct Ctl {
     // this CTA's part of a reduction
     float max;
-    u64 key, total, above, before;
+    u64 key, above;
     int equal, found, place;
     // the leader's orders and results
-    int cmd, next_sh, list_n, equal_index;
+    int cmd, next_sh, list_n, index;
     Range range;
-    u64 equal_j;
+    u64 equal_j, cut_mass, cut_w;
     // within the CTA
     u64 warp_mass[kWarps];
-    float warp_f[kWarps];
     int warp_cnt[kWarps];
 };
 
 struct Smem {
     Ctl ctl;
-    uint32_t hcnt[kBins];  // this CTA's counts
-    uint32_t mcnt[kBins];  // leader: the row's counts up to each bin
-    float mlow[kBins];     // leader: the least mass up to each bin
-    u64 list[kCap];        // leader: gathered tokens; a split's masses of this CTA
-    u64 mass[kCap];        // leader: running masses of the sorted list; a split's masses of the row
-    uint32_t scnt[kSplit]; // leader: a split's counts of the row
+    uint32_t hcnt[kBins];  // this CTA's counts and masses
+    u64 hmass[kBins];
+    uint32_t mcnt[kBins];  // leader: the row's, up to each bin
+    u64 mmass[kBins];
+    uint32_t scnt[kBins];  // leader: a split's, up to each part
+    u64 smass[kBins];      // (also where a CTA collects what it gathers)
+    u64 few[kFew], few_w[kFew];
+    // the leader's list lies over its hmass
 };
-static_assert(kSplit == kCap, "a split's masses lie over the list's");
+static_assert(kCap <= kBins, "the list lies over a histogram");
 
 __device__ __forceinline__ uint32_t ctarank() {
     uint32_t r;
@@ -108,15 +112,18 @@ __device__ __forceinline__ T *peer(T *p, uint32_t rank) {
     asm("mapa.u64 %0, %1, %2;" : "=l"(out) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
     return reinterpret_cast<T *>(out);
 }
-
-// Sum over the cluster of f(q), the reads of all CTAs in flight together.
+// Sum over the cluster of f(q), the reads of eight CTAs in flight together.
 template <class T, class F>
 __device__ __forceinline__ T over_peers(int C, F f) {
-    T v[kMaxCluster], sum = 0;
+    T sum = 0;
+#pragma unroll 1
+    for (int q0 = 0; q0 < C; q0 += 8) {
+        T v[8];
 #pragma unroll
-    for (int q = 0; q < kMaxCluster; ++q) v[q] = q < C ? f(q) : T(0);
+        for (int q = 0; q < 8; ++q) v[q] = q0 + q < C ? f(q0 + q) : T(0);
 #pragma unroll
-    for (int q = 0; q < kMaxCluster; ++q) sum += v[q];
+        for (int q = 0; q < 8; ++q) sum += v[q];
+    }
     return sum;
 }
 
@@ -147,9 +154,10 @@ struct Row {
     __device__ __forceinline__ static int bin(float t) {
         return static_cast<int>(fminf(-t * kBinsPerNat, static_cast<float>(kBins - 1)));
     }
-    __device__ __forceinline__ static int sub_bin(float t, int lo, int hi) {
-        const float f = (-t * kBinsPerNat - static_cast<float>(lo)) * (static_cast<float>(kSplit) / static_cast<float>(hi + 1 - lo));
-        return static_cast<int>(fminf(fmaxf(f, 0.f), static_cast<float>(kSplit - 1)));
+    // Which of kBins equal parts of bins lo..hi.
+    __device__ __forceinline__ static int part(float t, int lo, int hi) {
+        const float f = (-t * kBinsPerNat - static_cast<float>(lo)) * (static_cast<float>(kBins) / static_cast<float>(hi + 1 - lo));
+        return static_cast<int>(fminf(fmaxf(f, 0.f), static_cast<float>(kBins - 1)));
     }
     // 0 for a NaN (a logit of -infinity at an infinite temperature)
     __device__ __forceinline__ static u64 fixed(float w) {
@@ -158,8 +166,19 @@ struct Row {
     __device__ __forceinline__ bool in(float x, const Range &r) const {
         const float tt = t(x);
         const int b = bin(tt);
-        return b >= r.lo && b <= r.hi && (r.sub < 0 || sub_bin(tt, r.lo, r.hi) == r.sub) &&
+        return b >= r.lo && b <= r.hi && (r.sub < 0 || part(tt, r.lo, r.hi) == r.sub) &&
                (r.sh == 32 || (desc_key(x) >> r.sh) == r.pref);
+    }
+    // Bounds on the logits of bins lo..hi, with room for t's rounding.
+    __device__ __forceinline__ float least(int hi) const {
+        return hi == kBins - 1 || !(max < INFINITY)
+                   ? -INFINITY
+                   : max - (static_cast<float>(hi + 2) / kBinsPerNat) * temp * 1.0001f - fabsf(max) * 1e-5f;
+    }
+    __device__ __forceinline__ float most(int lo) const {
+        return lo == 0 || !(max < INFINITY)
+                   ? INFINITY
+                   : max - (static_cast<float>(lo - 1) / kBinsPerNat) * temp * 0.9999f + fabsf(max) * 1e-5f;
     }
 };
 
@@ -168,38 +187,6 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-
-// Inclusive sums over N (kThreads times 1, 2 or 4) values in place.
-template <int N, class T>
-__device__ __forceinline__ void block_scan(T *v, T *warp_sums) {
-    constexpr int PER = N / kThreads;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, base = threadIdx.x * PER;
-    T x[PER], m = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        x[i] = v[base + i];
-        m += x[i];
-    }
-    const T own = m;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const T p = __shfl_up_sync(0xffffffffu, m, o);
-        if (lane >= o) m += p;
-    }
-    if (lane == 31) warp_sums[warp] = m;
-    __syncthreads();
-    T w = lane < warp ? warp_sums[lane] : T(0);  // kWarps <= 32
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    m += w - own;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        m += x[i];
-        v[base + i] = m;
-    }
-    __syncthreads();
-}
-
 // Sum over the CTA, the same in every thread.
 __device__ __forceinline__ u64 block_sum(Smem &s, u64 v) {
     v = warp_sum64(v);
@@ -209,7 +196,51 @@ __device__ __forceinline__ u64 block_sum(Smem &s, u64 v) {
     const int lane = threadIdx.x & 31;
     return warp_sum64(lane < kWarps ? s.ctl.warp_mass[lane] : 0ull);
 }
-
+// Inclusive sums over N (a multiple of kThreads) pairs in place.
+template <int N>
+__device__ __forceinline__ void block_scan(Smem &s, u64 *mass, uint32_t *cnt) {
+    constexpr int PER = N / kThreads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, base = threadIdx.x * PER;
+    u64 x[PER], m = 0;
+    uint32_t y[PER], c = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        x[i] = mass ? mass[base + i] : 0ull;
+        y[i] = cnt[base + i];
+        m += x[i];
+        c += y[i];
+    }
+    const u64 own_m = m;
+    const uint32_t own_c = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 pm = __shfl_up_sync(0xffffffffu, m, o);
+        const uint32_t pc = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) {
+            m += pm;
+            c += pc;
+        }
+    }
+    if (lane == 31) {
+        s.ctl.warp_mass[warp] = m;
+        s.ctl.warp_cnt[warp] = static_cast<int>(c);
+    }
+    __syncthreads();
+    u64 wm = lane < warp ? s.ctl.warp_mass[lane] : 0ull;  // kWarps <= 32
+    uint32_t wc = lane < warp ? static_cast<uint32_t>(s.ctl.warp_cnt[lane]) : 0u;
+    wm = warp_sum64(wm);
+    wc = __reduce_add_sync(0xffffffffu, wc);
+    m += wm - own_m;
+    c += wc - own_c;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        m += x[i];
+        c += y[i];
+        if (mass) mass[base + i] = m;
+        cnt[base + i] = c;
+    }
+    __syncthreads();
+}
 // First i of n (a multiple of kThreads) at which the rising predicate f holds,
 // n - 1 if none; every thread calls it.
 template <class F>
@@ -219,237 +250,138 @@ __device__ __forceinline__ int first_of(int n, F f) {
     return min(at, n - 1);
 }
 
-// Counts the CTA's tokens by bin; with SUMS also its mass, and the mass of what
-// min_p keeps.
-template <bool SUMS>
-__device__ __forceinline__ void count_bins(Smem &s, const float *xs, int len, const Row &row, float min_p) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.hcnt[i] = 0;
-    __syncthreads();
-    u64 total = 0, above = 0;
-#pragma unroll 4
-    for (int i0 = 0; i0 < len; i0 += kThreads) {
-        const int i = i0 + threadIdx.x;
-        const bool live = i < len;
-        const float x = live ? xs[i] : -INFINITY;
-        const float t = row.t(x);
-        const int b = Row::bin(t);
-        if (SUMS) {
-            const float w = expf(t);
-            const u64 m = live ? Row::fixed(w) : 0ull;
-            total += m;
-            if (w >= min_p || x == row.max) above += m;
-        }
-        if (live) atomicAdd(&s.hcnt[b], 1u);
+__device__ __forceinline__ void clear_hist(uint32_t *cnt, u64 *mass) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        cnt[i] = 0;
+        mass[i] = 0;
     }
-    if (SUMS) {
-        total = block_sum(s, total);
-        above = block_sum(s, above);
-        if (threadIdx.x == 0) {
-            s.ctl.total = total;
-            s.ctl.above = above;
+    __syncthreads();
+}
+
+// 64-bit addition in shared memory by its two words (shared memory has no 64-bit
+// addition of its own; a loop of compare-and-swap took four times as long).
+__device__ __forceinline__ void add64(u64 *p, u64 m) {
+    uint32_t *w = reinterpret_cast<uint32_t *>(p);
+    const uint32_t lo = static_cast<uint32_t>(m), old = atomicAdd(w, lo);
+    const uint32_t hi = static_cast<uint32_t>(m >> 32) + (old + lo < old ? 1u : 0u);
+    if (hi) atomicAdd(w + 1, hi);
+}
+
+// Counts (and weighs) the CTA's tokens by bin; with MASS also what min_p keeps.
+template <bool MASS>
+__device__ __forceinline__ void local_hist(Smem &s, const float *xs, int len, const Row &row, float min_p) {
+    clear_hist(s.hcnt, s.hmass);
+    u64 above = 0, last = 0;
+    uint32_t last_n = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < len; i += kThreads) {
+        const float x = xs[i], t = row.t(x);
+        const int b = Row::bin(t);
+        u64 m = 0;
+        if (MASS) {
+            const float w = expf(t);
+            m = Row::fixed(w);
+            if (min_p > 0.f && (w >= min_p || x == row.max)) above += m;
         }
+        if (b == kBins - 1) {  // the open bin may hold most of the row
+            ++last_n;
+            last += m;
+        } else {
+            atomicAdd(&s.hcnt[b], 1u);
+            if (MASS) add64(&s.hmass[b], m);
+        }
+    }
+    last_n = __reduce_add_sync(0xffffffffu, last_n);
+    if (MASS) last = warp_sum64(last);
+    if ((threadIdx.x & 31) == 0 && last_n) {
+        atomicAdd(&s.hcnt[kBins - 1], last_n);
+        if (MASS) add64(&s.hmass[kBins - 1], last);
+    }
+    if (MASS && min_p > 0.f) {
+        above = block_sum(s, above);
+        if (threadIdx.x == 0) s.ctl.above = above;
     }
 }
 
+// Adds the cluster's histograms into the leader's (cnt, mass): CTA r a slice.
+__device__ __forceinline__ void merge_hist(Smem &s, uint32_t *cnt, u64 *mass, int C, int rank) {
+    cluster_sync();  // every CTA's is there
+    const int per = kBins / C;
+    for (int i = rank * per + threadIdx.x; i < (rank + 1) * per; i += kThreads) {
+        *peer(&cnt[i], 0) = over_peers<uint32_t>(C, [&](int q) { return *peer(&s.hcnt[i], q); });
+        *peer(&mass[i], 0) = over_peers<u64>(C, [&](int q) { return *peer(&s.hmass[i], q); });
+    }
+    cluster_sync();
+}
+
 // What every CTA of the cluster does for one order of the leader.
-__device__ __forceinline__ void execute(Smem &s, const float *xs, int len, int begin, const Row &row, float min_p, int C, int rank) {
+__device__ __forceinline__ void execute(Smem &s, const float *xs, int len, int begin, const Row &row, float min_p, int C,
+                                        int rank) {
     const Ctl *lead = peer(&s.ctl, 0);
     const int cmd = lead->cmd;
     const Range range = lead->range;
-    if (cmd == kSums) {  // the mass, and the mass of what min_p keeps
-        u64 total = 0, above = 0;
-        for (int i = threadIdx.x; i < len; i += kThreads) {
-            const float x = xs[i], w = expf(row.t(x));
-            const u64 m = Row::fixed(w);
-            total += m;
-            if (w >= min_p || x == row.max) above += m;
-        }
-        total = block_sum(s, total);
-        above = block_sum(s, above);
-        if (threadIdx.x == 0) {
-            s.ctl.total = total;
-            s.ctl.above = above;
-        }
-        cluster_sync();
-    } else if (cmd == kHist) {  // counts and masses of a split: by finer bins (next_sh 32) or by key bits
+    if (cmd == kMass) {
+        local_hist<true>(s, xs, len, row, min_p);
+        merge_hist(s, s.mcnt, s.mmass, C, rank);
+    } else if (cmd == kHist) {  // counts and masses of a split: by parts (next_sh 32) or by key bits
         const int sh = lead->next_sh;
-        for (int i = threadIdx.x; i < kSplit; i += kThreads) {
-            s.list[i] = 0;
-            s.hcnt[i] = 0;
-        }
-        __syncthreads();
+        const float least = row.least(range.hi), most = row.most(range.lo);
+        clear_hist(s.hcnt, s.hmass);
         for (int i = threadIdx.x; i < len; i += kThreads) {
             const float x = xs[i];
-            if (!row.in(x, range)) continue;
+            if (x < least || x > most || !row.in(x, range)) continue;
             const float t = row.t(x);
-            const int d = sh == 32 ? Row::sub_bin(t, range.lo, range.hi)
+            const int d = sh == 32 ? Row::part(t, range.lo, range.hi)
                                    : static_cast<int>((desc_key(x) >> sh) & ((1u << (range.sh - sh)) - 1u));
             const u64 m = Row::fixed(expf(t));
             atomicAdd(&s.hcnt[d], 1u);
-            if (m) atomicAdd(&s.list[d], m);
+            if (m) add64(&s.hmass[d], m);
         }
-        cluster_sync();
-        const int per = kSplit / C;
-        for (int i = rank * per + threadIdx.x; i < (rank + 1) * per; i += kThreads) {
-            *peer(&s.mass[i], 0) = over_peers<u64>(C, [&](int q) { return *peer(&s.list[i], q); });
-            *peer(&s.scnt[i], 0) = over_peers<uint32_t>(C, [&](int q) { return *peer(&s.hcnt[i], q); });
-        }
-        cluster_sync();
-    } else if (cmd == kGather) {  // the range's tokens to the leader; the mass of the bins before it
-        // first into this CTA's own memory (s.mass, idle now), then in one piece to the leader's list
-        u64 before = 0;
-        const int lane = threadIdx.x & 31;
+        merge_hist(s, s.scnt, s.smass, C, rank);
+    } else if (cmd == kGather) {  // the range's tokens, first together here, then in one piece to the leader's list
+        const float least = row.least(range.hi), most = row.most(range.lo);
         if (threadIdx.x == 0) s.ctl.found = 0;
         __syncthreads();
-        // below this no token is in the range (with room for t's rounding)
-        const float least = range.hi == kBins - 1 || !(row.max < INFINITY)
-                                ? -INFINITY
-                                : row.max - (static_cast<float>(range.hi + 2) / kBinsPerNat) * row.temp * 1.0001f -
-                                      fabsf(row.max) * 1e-5f;
 #pragma unroll 4
-        for (int i0 = 0; i0 < len; i0 += kThreads) {
-            const int i = i0 + threadIdx.x;
-            const float x = i < len ? xs[i] : -INFINITY;
-            bool take = i < len && x >= least;
-            if (!__any_sync(0xffffffffu, take)) continue;
-            if (take) {
-                const float t = row.t(x);
-                if (range.lo > 0 && Row::bin(t) < range.lo) before += Row::fixed(expf(t));
-                take = row.in(x, range);
+        for (int i = threadIdx.x; i < len; i += kThreads) {
+            const float x = xs[i];
+            if (x >= least && x <= most && row.in(x, range)) {
+                const int at = atomicAdd(&s.ctl.found, 1);
+                if (at < kCap) s.smass[at] = (static_cast<u64>(desc_key(x)) << 32) | static_cast<uint32_t>(begin + i);
             }
-            const uint32_t all = __ballot_sync(0xffffffffu, take);
-            if (all == 0) continue;
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&s.ctl.found, __popc(all));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1u));
-            if (take && at < kCap) s.mass[at] = (static_cast<u64>(desc_key(x)) << 32) | static_cast<uint32_t>(begin + i);
         }
         __syncthreads();
         const int found = min(s.ctl.found, kCap);
         if (threadIdx.x == 0 && found) s.ctl.place = atomicAdd(peer(&s.ctl.list_n, 0), found);
         __syncthreads();
-        u64 *list = peer(s.list, 0);
+        u64 *list = peer(s.hmass, 0);
         for (int i = threadIdx.x; i < found; i += kThreads)
-            if (s.ctl.place + i < kCap) list[s.ctl.place + i] = s.mass[i];
-        if (range.lo > 0) {
-            before = block_sum(s, before);
-            if (threadIdx.x == 0) s.ctl.before = before;
-        }
+            if (s.ctl.place + i < kCap) list[s.ctl.place + i] = s.smass[i];
         cluster_sync();
     } else if (cmd == kEqual) {
         // the range's tokens (one logit) in index order: a run of the part per thread
         const int per = (len + kThreads - 1) / kThreads, i0 = min(len, static_cast<int>(threadIdx.x) * per),
                   i1 = min(len, i0 + per);
-        int c = 0;
-        for (int i = i0; i < i1; ++i) c += desc_key(xs[i]) == range.pref ? 1 : 0;
-        int *runs = reinterpret_cast<int *>(s.hcnt);
+        uint32_t c = 0;
+        for (int i = i0; i < i1; ++i) c += desc_key(xs[i]) == range.pref ? 1u : 0u;
         __syncthreads();
-        runs[threadIdx.x] = c;
+        s.hcnt[threadIdx.x] = c;
         __syncthreads();
-        block_scan<kThreads>(runs, s.ctl.warp_cnt);
-        if (threadIdx.x == kThreads - 1) s.ctl.equal = runs[kThreads - 1];
+        block_scan<kThreads>(s, nullptr, s.hcnt);
+        if (threadIdx.x == kThreads - 1) s.ctl.equal = static_cast<int>(s.hcnt[kThreads - 1]);
         cluster_sync();
         long j = static_cast<long>(lead->equal_j);
         for (int q = 0; q < rank; ++q) j -= *peer(&s.ctl.equal, q);
-        const long before = runs[threadIdx.x] - c;
-        if (j >= before && j < before + c) {
+        const long before = static_cast<long>(s.hcnt[threadIdx.x]) - c;
+        if (j >= before && j < before + static_cast<long>(c)) {
             for (int i = i0; i < i1; ++i)
                 if (desc_key(xs[i]) == range.pref && j-- == before) {
-                    *peer(&s.ctl.equal_index, 0) = begin + i;
+                    *peer(&s.ctl.index, 0) = begin + i;
                     break;
                 }
         }
         cluster_sync();
     }
-}
-
-// ------------------------------------------------------------- the leader --
-
-struct List {  // tokens of bins [lo, hi] in order, with what comes before them
-    int lo, hi, n;
-    u64 base_mass;
-    int base_cnt;
-};
-
-// Sorts the n gathered tokens and leaves their running masses in s.mass.  Up to
-// kFew tokens: each thread finds its token's place, and the mass before it, by
-// looking at all; more: bitonic, elements t and t + kThreads in thread t, strides
-// below 32 by shuffle.
-constexpr int kFew = 128;
-__device__ __forceinline__ void sort_list(Smem &s, int n, const Row &row) {
-    const int t = threadIdx.x;
-    auto weight = [&](u64 v) { return Row::fixed(expf(row.t(desc_value(static_cast<uint32_t>(v >> 32))))); };
-    if (n <= kFew) {
-        u64 *w = reinterpret_cast<u64 *>(s.scnt);
-        static_assert(kFew * 8 <= sizeof(s.scnt), "weights of a short list");
-        u64 mine = 0, m = 0;
-        if (t < n) {
-            mine = s.list[t];
-            w[t] = m = weight(mine);
-        }
-        __syncthreads();
-        int place = 0;
-        if (t < n) {
-#pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-                const bool before = s.list[i] < mine;
-                place += before ? 1 : 0;
-                m += before ? w[i] : 0ull;
-            }
-        }
-        __syncthreads();
-        if (t < n) {
-            s.list[place] = mine;
-            s.mass[place] = m;
-        }
-        __syncthreads();
-        return;
-    }
-    int p2 = kFew;
-    while (p2 < n) p2 <<= 1;
-    const bool two = p2 > kThreads;
-    u64 v[2];
-    v[0] = t < n ? s.list[t] : ~0ull;
-    v[1] = t + kThreads < n ? s.list[t + kThreads] : ~0ull;
-    __syncthreads();
-#pragma unroll 1
-    for (int k = 2; k <= p2; k <<= 1) {
-#pragma unroll 1
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            if (j == kThreads) {  // k = 2 * kThreads: ascending
-                if (v[0] > v[1]) {
-                    const u64 w = v[0];
-                    v[0] = v[1];
-                    v[1] = w;
-                }
-                continue;
-            }
-            if (j >= 32) {
-                if (t < p2) s.list[t] = v[0];
-                if (two) s.list[t + kThreads] = v[1];
-                __syncthreads();
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (e == 1 && !two) break;
-                const int i = t + e * kThreads;
-                u64 o;
-                if (j >= 32) o = i < p2 ? s.list[i ^ j] : ~0ull;
-                else o = __shfl_xor_sync(0xffffffffu, v[e], j);
-                const bool low = ((i & j) == 0) == ((i & k) == 0);  // keeps the smaller
-                v[e] = low ? (o < v[e] ? o : v[e]) : (o > v[e] ? o : v[e]);
-            }
-            if (j >= 32) __syncthreads();
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int i = t + e * kThreads;
-        s.list[i] = v[e];
-        s.mass[i] = i < n ? weight(v[e]) : 0ull;
-    }
-    __syncthreads();
-    block_scan<kCap>(s.mass, s.ctl.warp_mass);
 }
 
 // The leader's cuts, one after another (top-k, top-p, the draw), as steps
@@ -460,84 +392,67 @@ __device__ __forceinline__ void sort_list(Smem &s, int n, const Row &row) {
 // running it.
 struct Leader {
     enum Step { kTopK, kTopP, kDraw };
-    enum Phase { kBegin, kSummed, kLook, kGathered, kBefore, kSplitNext, kSplitDone, kOnly, kEqualDone, kCut };
+    enum Phase { kBegin, kWeighed, kLook, kGathered, kInList, kSplitDone, kOrder, kEqualDone, kCut };
     Row row;
     float min_p, top_p, u;
     int k, vocab, C;
-    bool few;  // the row's sums are not there yet
+    bool weighed;  // the bins' masses are there
     int step = kTopK, phase = kBegin;
-    // the list: tokens of bins [lo, hi] in order, with what comes before them
-    int list_lo = 0, list_hi = -1, list_n = 0, list_cnt = 0;
-    u64 list_mass = 0;
-    u64 total = 0, above = 0, kept = 0;  // the row's mass and what min_p keeps (0: unknown); the mass kept so far
-    int limit = kBins - 1;               // no cut falls behind this bin
+    int list_lo = 0, list_hi = -1, list_n = 0;  // the list: tokens of bins [lo, hi]
+    u64 kept = 0, above = 0;
     // the cut at work: where the running count reaches `target`, or the running mass first exceeds it
     bool by_count = false;
     u64 target = 0;
-    Range r{0, kBins - 1, -1, 32, 0u};
-    bool split = false;
-    u64 base_m = 0;
+    Range r{0, 0, -1, 32, 0u};
+    u64 base_m = 0;  // what comes before the tokens looked at
     int base_c = 0;
-    // its token
-    u64 cut_mass = 0, cut_w = 0;
-    int cut_index = -1;
 
-    __device__ __forceinline__ void order(Smem &s, int cmd, int then, Range range, int next_sh = 32, u64 j = 0) {
+    __device__ __forceinline__ void order(Smem &s, int cmd, int then, int next_sh = 32, u64 j = 0) {
         __syncthreads();  // what the last order left has been read
         if (threadIdx.x == 0) {
             Ctl &c = s.ctl;
             c.cmd = cmd;
-            c.range = range;
+            c.range = r;
             c.next_sh = next_sh;
             c.list_n = 0;
             c.equal_j = j;
         }
         phase = then;
     }
-    __device__ __forceinline__ void read_sums(Smem &s) {
-        total = over_peers<u64>(C, [&](int q) { return peer(&s.ctl, q)->total; });
-        above = over_peers<u64>(C, [&](int q) { return peer(&s.ctl, q)->above; });
-        few = false;
+    __device__ __forceinline__ u64 weight(u64 v) const {
+        return Row::fixed(expf(row.t(desc_value(static_cast<uint32_t>(v >> 32)))));
     }
-    // The bins that a mass falls in.  A bin's true running mass lies between low - count and
-    // low * e^(1/64) + count (in units of 2^-44, where a weight is rounded by half), give or take
-    // fp32 sums; with the row's mass known, what follows the bin is bounded the same way.
-    __device__ __forceinline__ void mass_range(Smem &s) {
-        const float want = static_cast<float>(target), all_low = s.mlow[kBins - 1], slack = 4e-6f * all_low;
-        const float rest = total ? static_cast<float>(total - target) : INFINITY;
-        const float all_cnt = static_cast<float>(s.mcnt[kBins - 1]);
-        r.lo = first_of(kBins, [&](int i) {
-            const float c = static_cast<float>(s.mcnt[i]), low = s.mlow[i];
-            return low * 1.0161f + c + slack > want && (all_low - low) * 0.9997f - (all_cnt - c) - slack < rest;
-        });
-        r.hi = first_of(kBins, [&](int i) {
-            const float c = static_cast<float>(s.mcnt[i]), low = s.mlow[i];
-            return i >= r.lo && (low * 0.9997f - c - slack > want || (all_low - low) * 1.0161f + (all_cnt - c) + slack < rest);
-        });
-        r.lo = min(r.lo, limit);
-        r.hi = min(r.hi, limit);
+    // Part d (of a scanned split) holds the cut: moves the base there; its tokens.
+    __device__ __forceinline__ int enter(Smem &s, int &d) {
+        d = by_count ? first_of(kBins, [&](int i) { return s.scnt[i] >= static_cast<uint32_t>(target - base_c); })
+                     : first_of(kBins, [&](int i) { return s.smass[i] > target - base_m; });
+        const int before = d ? static_cast<int>(s.scnt[d - 1]) : 0, n = static_cast<int>(s.scnt[d]) - before;
+        base_m += d ? s.smass[d - 1] : 0ull;
+        base_c += before;
+        return n;
     }
-    // True with an order, false with the answer.
+    // True with an order, false with the answer (s.ctl.index, cut_w; kept).
     __device__ __forceinline__ bool next(Smem &s) {
+        u64 *list = s.hmass;
         while (true) {
             if (phase == kBegin) {
-                if (few && (k <= 0 || k >= vocab)) {  // all are kept: the mass is needed
-                    order(s, kSums, kSummed, r);
+                by_count = step == kTopK;
+                if (!by_count && !weighed && list_hi < 0) {  // no list that holds all that is kept
+                    order(s, kMass, kWeighed);
                     return true;
                 }
                 if (step == kTopK) {
-                    if (!few && total == 0) {
-                        read_sums(s);
-                        kept = total;
-                    }
-                    by_count = true;
-                    target = k;
+                    if (weighed) kept = s.mmass[kBins - 1];
                     if (k <= 0 || k >= vocab) {
+                        if (!weighed) {
+                            order(s, kMass, kWeighed);
+                            return true;
+                        }
                         step = kTopP;
                         continue;
                     }
+                    target = k;
                 } else if (step == kTopP) {
-                    by_count = false;
                     if (!(top_p < 1.f)) {
                         step = kDraw;
                         continue;
@@ -545,18 +460,16 @@ struct Leader {
                     const double want = ceil(static_cast<double>(top_p) * static_cast<double>(kept));
                     target = want < 1.0 ? 0ull : min(kept, static_cast<u64>(want)) - 1;
                 } else {
-                    by_count = false;
                     if (min_p > 0.f) {
-                        if (few && list_hi >= 0 && list_lo == 0) {  // the list holds all that is kept
+                        if (weighed) {
+                            above = over_peers<u64>(C, [&](int q) { return peer(&s.ctl, q)->above; });
+                        } else {  // the list holds all that is kept
                             u64 m = 0;
                             for (int i = threadIdx.x; i < list_n; i += kThreads) {
-                                const float x = desc_value(static_cast<uint32_t>(s.list[i] >> 32)), w = expf(row.t(x));
+                                const float x = desc_value(static_cast<uint32_t>(list[i] >> 32)), w = expf(row.t(x));
                                 if (w >= min_p || x == row.max) m += Row::fixed(w);
                             }
                             above = block_sum(s, m);
-                        } else if (few) {
-                            order(s, kSums, kSummed, r);
-                            return true;
                         }
                         kept = min(kept, above);
                     }
@@ -564,89 +477,140 @@ struct Leader {
                     target = at > 0.0 ? min(kept - 1, static_cast<u64>(at)) : 0ull;
                 }
                 phase = kLook;
-            } else if (phase == kSummed) {
-                read_sums(s);
-                if (step == kTopK) kept = total;
+            } else if (phase == kWeighed) {
+                block_scan<kBins>(s, s.mmass, s.mcnt);
+                weighed = true;
+                list_hi = -1;  // the histogram lay over it
                 phase = kBegin;
             } else if (phase == kLook) {
-                r = Range{0, 0, -1, 32, 0u};
-                if (by_count) r.lo = r.hi = first_of(kBins, [&](int i) { return s.mcnt[i] >= static_cast<uint32_t>(target); });
-                else mass_range(s);
-                limit = r.hi;
-                if (r.lo >= list_lo && r.hi <= list_hi) {
-                    phase = kCut;
+                r = Range{list_lo, list_hi, -1, 32, 0u};
+                base_m = 0;
+                base_c = 0;
+                if (!weighed && !by_count) {  // a list from bin 0 on holds all that is kept
+                    phase = kInList;
                     continue;
                 }
-                const int upto = static_cast<int>(s.mcnt[r.hi]);
-                if (upto <= kCap) r.lo = 0;  // everything up to here fits: later cuts need no gather
+                const int b = by_count ? first_of(kBins, [&](int i) { return s.mcnt[i] >= static_cast<uint32_t>(target); })
+                                       : first_of(kBins, [&](int i) { return s.mmass[i] > target; });
+                if (list_hi >= 0 && b >= list_lo && b <= list_hi) {
+                    base_m = list_lo ? s.mmass[list_lo - 1] : 0ull;
+                    base_c = list_lo ? static_cast<int>(s.mcnt[list_lo - 1]) : 0;
+                    phase = kInList;
+                    continue;
+                }
+                const int upto = static_cast<int>(s.mcnt[b]);
+                r.hi = b;
+                r.lo = upto <= kCap ? 0 : b;  // everything up to here fits: later cuts need no gather
+                if (r.lo && !weighed) {
+                    order(s, kMass, kWeighed);
+                    return true;
+                }
                 base_c = r.lo ? static_cast<int>(s.mcnt[r.lo - 1]) : 0;
-                base_m = 0;
+                base_m = r.lo ? s.mmass[r.lo - 1] : 0ull;
+                list_lo = r.lo;
                 list_hi = -1;
-                split = upto - base_c > kCap;
-                Range get = r;
-                if (split) get.hi = get.lo;  // for the mass before the range alone
-                order(s, kGather, split ? kBefore : kGathered, get);
+                list_n = upto - base_c;
+                if (list_n <= kCap) {
+                    order(s, kGather, kGathered);
+                } else {
+                    order(s, kHist, kSplitDone);
+                }
                 return true;
             } else if (phase == kGathered) {
-                list_lo = r.lo;
                 list_hi = r.hi;
-                list_n = static_cast<int>(s.mcnt[r.hi]) - base_c;
-                list_cnt = base_c;
-                list_mass = r.lo ? over_peers<u64>(C, [&](int q) { return peer(&s.ctl, q)->before; }) : 0;
-                sort_list(s, list_n, row);
-                phase = kCut;
-            } else if (phase == kBefore) {
-                if (r.lo) base_m = over_peers<u64>(C, [&](int q) { return peer(&s.ctl, q)->before; });
-                order(s, kHist, kSplitDone, r, 32);
-                return true;
+                phase = kInList;
+            } else if (phase == kInList) {
+                if (list_n <= kFew) {
+                    for (int i = threadIdx.x; i < list_n; i += kThreads) s.few[i] = list[i];
+                    if (threadIdx.x == 0) s.ctl.list_n = list_n;
+                    __syncthreads();
+                    phase = kOrder;
+                    continue;
+                }
+                clear_hist(s.scnt, s.smass);
+                for (int i = threadIdx.x; i < list_n; i += kThreads) {
+                    const u64 v = list[i];
+                    const int d = Row::part(row.t(desc_value(static_cast<uint32_t>(v >> 32))), r.lo, r.hi);
+                    atomicAdd(&s.scnt[d], 1u);
+                    add64(&s.smass[d], weight(v));
+                }
+                __syncthreads();
+                block_scan<kBins>(s, s.smass, s.scnt);
+                int d;
+                const int n = enter(s, d);
+                r.sub = d;
+                if (n > kFew) {
+                    order(s, kHist, kSplitDone, 22);
+                    list_hi = -1;
+                    return true;
+                }
+                if (threadIdx.x == 0) s.ctl.list_n = 0;
+                __syncthreads();
+                for (int i = threadIdx.x; i < list_n; i += kThreads) {
+                    const u64 v = list[i];
+                    if (Row::part(row.t(desc_value(static_cast<uint32_t>(v >> 32))), r.lo, r.hi) == d)
+                        s.few[atomicAdd(&s.ctl.list_n, 1)] = v;
+                }
+                __syncthreads();
+                phase = kOrder;
             } else if (phase == kSplitDone) {
                 const int sh = s.ctl.next_sh;
-                block_scan<kSplit>(s.mass, s.ctl.warp_mass);
-                block_scan<kSplit>(s.scnt, reinterpret_cast<uint32_t *>(s.ctl.warp_cnt));
-                const int d = by_count ? first_of(kSplit, [&](int i) { return s.scnt[i] >= static_cast<uint32_t>(target - base_c); })
-                                       : first_of(kSplit, [&](int i) { return s.mass[i] > target - base_m; });
-                const u64 dm = d ? s.mass[d - 1] : 0, in_m = s.mass[d] - dm;
-                const int dc = d ? static_cast<int>(s.scnt[d - 1]) : 0, in_c = static_cast<int>(s.scnt[d]) - dc;
-                base_m += dm;
-                base_c += dc;
+                block_scan<kBins>(s, s.smass, s.scnt);
+                const u64 m0 = base_m;
+                int d;
+                const int n = enter(s, d);
                 if (sh == 32) {
                     r.sub = d;
                 } else {
                     r.pref = r.sh == 32 ? static_cast<uint32_t>(d) : (r.pref << (r.sh - sh)) | static_cast<uint32_t>(d);
                     r.sh = sh;
                 }
-                if (in_c <= kCap) {
-                    list_n = in_c;
-                    list_cnt = base_c;
-                    list_mass = base_m;
-                    order(s, kGather, kOnly, r);
+                if (n <= kFew) {
+                    list_n = n;
+                    order(s, kGather, kInList);  // a list of use to this cut only
                     return true;
                 }
                 if (r.sh == 0) {  // equal logits
-                    const u64 w = in_m / static_cast<u64>(in_c);
+                    const u64 w = (m0 + s.smass[d] - base_m) / static_cast<u64>(n);
                     const u64 j = by_count ? target - 1 - base_c : (w ? (target - base_m) / w : 0);
-                    cut_mass = base_m + (j + 1) * w;
-                    cut_w = w;
-                    order(s, kEqual, kEqualDone, r, 32, j);
+                    order(s, kEqual, kEqualDone, 32, j);
+                    if (threadIdx.x == 0) {
+                        s.ctl.cut_mass = base_m + (j + 1) * w;
+                        s.ctl.cut_w = w;
+                    }
                     return true;
                 }
-                order(s, kHist, kSplitDone, r, r.sh == 2 ? 0 : r.sh - 10);
+                order(s, kHist, kSplitDone, r.sh == 32 ? 22 : (r.sh == 2 ? 0 : r.sh - 10));
                 return true;
-            } else if (phase == kOnly) {  // a list of use to this cut only
-                sort_list(s, list_n, row);
-                phase = kCut;
-            } else {
-                if (phase == kEqualDone) {
-                    cut_index = s.ctl.equal_index;
-                } else {
-                    const int i = by_count ? static_cast<int>(target) - 1 - list_cnt
-                                           : min(list_n - 1, first_of(kCap, [&](int i) { return i >= list_n || s.mass[i] > target - list_mass; }));
-                    cut_mass = list_mass + s.mass[i];
-                    cut_w = s.mass[i] - (i ? s.mass[i - 1] : 0);
-                    cut_index = static_cast<int>(s.list[i] & 0xffffffffull);
+            } else if (phase == kOrder) {
+                // each of a few tokens finds its place, and the mass before it
+                const int n = s.ctl.list_n, t = threadIdx.x;
+                u64 mine = 0, w = 0, m = 0;
+                int place = 0;
+                if (t < n) {
+                    mine = s.few[t];
+                    s.few_w[t] = w = weight(mine);
                 }
+                __syncthreads();
+                if (t < n) {
+#pragma unroll 4
+                    for (int i = 0; i < n; ++i) {
+                        const bool before = s.few[i] < mine;
+                        place += before ? 1 : 0;
+                        m += before ? s.few_w[i] : 0ull;
+                    }
+                    if (by_count ? place == static_cast<int>(target) - 1 - base_c
+                                 : m <= target - base_m && target - base_m < m + w) {
+                        s.ctl.cut_mass = base_m + m + w;
+                        s.ctl.cut_w = w;
+                        s.ctl.index = static_cast<int>(mine & 0xffffffffull);
+                    }
+                }
+                __syncthreads();
+                phase = kCut;
+            } else {  // kEqualDone, kCut
                 if (step == kDraw) return false;
-                kept = cut_mass;
+                kept = s.ctl.cut_mass;
                 ++step;
                 phase = kBegin;
             }
@@ -693,32 +657,41 @@ __global__ void __launch_bounds__(kThreads, 2) ijb_sample_kernel(const __grid_co
         for (int i = threadIdx.x; i < len; i += kThreads) take(i, x[i]);
     }
     m = warp_max(m);
+    if (greedy) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 other = __shfl_xor_sync(0xffffffffu, key, o);
-        key = other > key ? other : key;
+        for (int o = 16; o > 0; o >>= 1) {
+            const u64 other = __shfl_xor_sync(0xffffffffu, key, o);
+            key = other > key ? other : key;
+        }
     }
-    if (threadIdx.x == 0) {
-        s.ctl.max = -INFINITY;
-        s.ctl.key = 0;
-    }
-    __syncthreads();
     if ((threadIdx.x & 31) == 0) {
         s.ctl.warp_mass[threadIdx.x >> 5] = key;
         s.ctl.warp_cnt[threadIdx.x >> 5] = __float_as_int(m);
     }
     __syncthreads();
-    if (threadIdx.x == 0)
-        for (int w = 0; w < kWarps; ++w) {
-            s.ctl.max = fmaxf(s.ctl.max, __int_as_float(s.ctl.warp_cnt[w]));
-            s.ctl.key = s.ctl.warp_mass[w] > s.ctl.key ? s.ctl.warp_mass[w] : s.ctl.key;
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        float v = lane < kWarps ? __int_as_float(s.ctl.warp_cnt[lane]) : -INFINITY;
+        u64 k = lane < kWarps ? s.ctl.warp_mass[lane] : 0ull;
+        v = warp_max(v);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const u64 other = __shfl_xor_sync(0xffffffffu, k, o);
+            k = other > k ? other : k;
         }
+        if (lane == 0) {
+            s.ctl.max = v;
+            s.ctl.key = k;
+            s.ctl.above = 0;
+        }
+    }
     cluster_sync();
     Row row;
-    row.max = -INFINITY;
+    {
+        const int lane = threadIdx.x & 31;
+        row.max = warp_max(lane < C ? peer(&s.ctl, lane)->max : -INFINITY);
+    }
     row.temp = temp;
-#pragma unroll
-    for (int q = 0; q < kMaxCluster; ++q) row.max = fmaxf(row.max, peer(&s.ctl, q < C ? q : 0)->max);
     if (row.max == -INFINITY || greedy) {  // nothing to choose from, or the largest
         if (rank == 0 && threadIdx.x == 0) {
             u64 best = 0;
@@ -733,23 +706,13 @@ __global__ void __launch_bounds__(kThreads, 2) ijb_sample_kernel(const __grid_co
     row.plain_div = !(temp >= 1e-6f && temp <= 1e6f);
     const float min_p = p.min_p ? p.min_p[r] : 0.f;
     const int k = p.top_k ? p.top_k[r] : 0;
-    const bool few = k > 0 && k <= kCap / 2;  // usually the list holds all that is kept: no sums over the row
-    if (few) count_bins<false>(s, xs, len, row, min_p);
-    else count_bins<true>(s, xs, len, row, min_p);
-    cluster_sync();
-    {  // CTA r adds a slice of the counts
-        const int per = kBins / C;
-        for (int i = rank * per + threadIdx.x; i < (rank + 1) * per; i += kThreads) {
-            const uint32_t c = over_peers<uint32_t>(C, [&](int q) { return *peer(&s.hcnt[i], q); });
-            *peer(&s.mcnt[i], 0) = c;
-            *peer(&s.mlow[i], 0) = i == kBins - 1 ? 0.f : static_cast<float>(c) * exp2f(static_cast<float>(i + 1) * (-1.4426950408889634f / kBinsPerNat) + 44.f);
-        }
-    }
-    cluster_sync();
+    const bool few = k > 0 && k <= kCap / 2 && k < p.vocab;  // most likely the list holds all that is kept
+    if (few) local_hist<false>(s, xs, len, row, 0.f);
+    else local_hist<true>(s, xs, len, row, min_p);
+    merge_hist(s, s.mcnt, s.mmass, C, rank);
     Leader lead;
     if (rank == 0) {
-        block_scan<kBins>(s.mcnt, reinterpret_cast<uint32_t *>(s.ctl.warp_cnt));
-        block_scan<kBins>(s.mlow, s.ctl.warp_f);
+        block_scan<kBins>(s, s.mmass, s.mcnt);
         lead.row = row;
         lead.min_p = min_p;
         lead.top_p = p.top_p ? p.top_p[r] : 1.f;
@@ -757,14 +720,14 @@ __global__ void __launch_bounds__(kThreads, 2) ijb_sample_kernel(const __grid_co
         lead.k = k;
         lead.vocab = p.vocab;
         lead.C = C;
-        lead.few = few;
+        lead.weighed = !few;
     }
     while (true) {
         if (rank == 0 && !lead.next(s)) {
             if (threadIdx.x == 0) {
                 s.ctl.cmd = kDone;
-                p.token[r] = lead.cut_index;
-                if (p.prob) p.prob[r] = static_cast<float>(static_cast<double>(lead.cut_w) / static_cast<double>(lead.kept));
+                p.token[r] = s.ctl.index;
+                if (p.prob) p.prob[r] = static_cast<float>(static_cast<double>(s.ctl.cut_w) / static_cast<double>(lead.kept));
             }
         }
         cluster_sync();  // the order is there
@@ -780,8 +743,11 @@ cudaError_t sample_launch(const float *x, long stride, int n, int vocab, const f
                           const int *top_k, const float *top_p, const float *min_p, int *token, float *prob,
                           cudaStream_t stream) {
     SampleParams p{x, stride, vocab, 0, u, temperature, top_k, top_p, min_p, token, prob};
-    int c = 1;  // parts of at most 2048 logits where the cluster may be that large
-    while (c < kMaxCluster && (vocab + c - 1) / c > 2048) c *= 2;
+    // parts of at most 2048 logits, in clusters of up to 8 CTAs; 16 for few rows, where the row's
+    // time counts (a size that the device has to allow: all of a B200's GPCs hold one)
+    const int most = n <= 8 ? kMaxCluster : 8;
+    int c = 1;
+    while (c < most && (vocab + c - 1) / c > 2048) c *= 2;
     p.chunk = ((vocab + c - 1) / c + 3) / 4 * 4;
     const int smem = static_cast<int>(sizeof(Smem)) + p.chunk * 4;
     static bool ready[64];
@@ -794,10 +760,12 @@ cudaError_t sample_launch(const float *x, long stride, int n, int vocab, const f
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[dev]) {
             e = cudaFuncSetAttribute(ijb_sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(sizeof(Smem)) + kMaxChunk * 4);
+                                     static_cast<int>(sizeof(Smem)) + kMaxVocab / 8 * 4);
             if (e == cudaSuccess)
                 e = cudaFuncSetAttribute(ijb_sample_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                                          cudaSharedmemCarveoutMaxShared);
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(ijb_sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return e;
             ready[dev] = true;
         }
@@ -826,7 +794,7 @@ extern "C" int ijb_sample(const float *logits_dev, long stride, int n, int vocab
     try {
         const char *bad = nullptr;
         if (n < 0 || n > (1 << 24)) bad = "ijb_sample: n must be 0..2^24";
-        else if (vocab < 1 || vocab > kMaxCluster * kMaxChunk) bad = "ijb_sample: vocab must be 1..131072";
+        else if (vocab < 1 || vocab > kMaxVocab) bad = "ijb_sample: vocab must be 1..131072";
         else if (stride < vocab) bad = "ijb_sample: the stride is shorter than a row";
         else if (n > 0 && (!logits_dev || !u_dev || !token_dev)) bad = "ijb_sample: null pointer";
         if (bad) {
