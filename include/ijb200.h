@@ -386,8 +386,9 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
  * 131072 values, `stride` floats apart): temperature, then top-k, top-p and
  * min-p, then the uniform number u_dev[i] in [0, 1).  The settings are one
  * value per row in device memory, or NULL:
- *   temperature  > 0 (NULL: 1); anything else is greedy: the token ijb_argmax
- *                takes (NaN counts as -infinity), with probability 1
+ *   temperature  > 0 (NULL: 1), taken as 1e-15 at least and 1e15 at most; anything
+ *                else is greedy: the token ijb_argmax takes (NaN counts as
+ *                -infinity), with probability 1
  *   top_k        keeps the k largest logits, equal ones by the lower index; 0, a
  *                negative value or vocab and more keep all
  *   top_p        keeps the shortest prefix of those, in falling order, whose

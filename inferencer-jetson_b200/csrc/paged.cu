@@ -10,8 +10,11 @@
 // and not per page: a page is filled a token at a time, and a later, larger
 // token must not change the rows already there.
 //
-// Both kernels move bytes: 8 elements a thread, 16-byte loads and stores, a
-// row per 8 (head_dim 64) or 16 threads.
+// Both kernels move bytes: 16-byte loads and stores, 8 elements of a row a
+// thread, a row per 8 (head_dim 64) or 16 threads.  A thread's loads wait for two
+// others (the slot, its page), so with many rows each takes four heads of its
+// token at once: 32768 rows of 8 heads x 128 read back as fp16 took 75 us a head
+// at a time (2.7 TB/s).
 #include "paged.cuh"
 
 namespace ijb {
@@ -55,9 +58,9 @@ struct RowsParams {
     uint32_t *status;
 };
 
-// The cache row of token t (which, head); -1 when the entry is padding (a
+// The cache row of token t (which, head 0); -1 when the entry is padding (a
 // negative position) or names no slot, which is reported.
-__device__ __forceinline__ long slot_row(const RowsParams &p, int t, int which, int head) {
+__device__ __forceinline__ long slot_row(const RowsParams &p, int t, int which) {
     const int seq = p.tok_seq[t], pos = p.tok_pos[t];
     if (pos < 0) return -1;
     const int pg = pos >> p.kv.page_shift;
@@ -68,7 +71,7 @@ __device__ __forceinline__ long slot_row(const RowsParams &p, int t, int which, 
         if (p.status) atomicOr(p.status, kDevErrBadIndex);
         return -1;
     }
-    return kv_row(p.kv, page, which, head, pos & ((1 << p.kv.page_shift) - 1));
+    return kv_row(p.kv, page, which, 0, pos & ((1 << p.kv.page_shift) - 1));
 }
 
 template <bool VEC>
@@ -117,102 +120,148 @@ __device__ __forceinline__ void store_row8(__half *p, const float (&f)[8]) {
     }
 }
 
-// Thread -> (token, K or V, head, 8 elements): rows of one token are
-// consecutive, so a block reads whole tokens.
-template <typename T, bool E4M3, bool VEC, int HD>
-__global__ void __launch_bounds__(kRowThreads) ijb_kv_append_kernel(const __grid_constant__ RowsParams p) {
-    constexpr int L = HD / 8;  // threads a row
-    const long idx = blockIdx.x * static_cast<long>(kRowThreads) + threadIdx.x;
-    const int c = static_cast<int>(idx % L);
-    const long row = idx / L;
-    const int per = 2 * p.kv.kv_heads;
-    const bool live = row < static_cast<long>(p.n) * per;  // whole rows: uniform over a row's threads
-    const int t = live ? static_cast<int>(row / per) : 0, r = static_cast<int>(row % per);
-    const int which = r / p.kv.kv_heads, head = r % p.kv.kv_heads;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    long to = -1;
-    if (live) {
-        const T *src = static_cast<const T *>(which ? p.v : p.k);
-        load_row8<VEC>(src + t * p.stride + static_cast<long>(head) * HD + c * 8, f);
-        to = slot_row(p, t, which, head);
+// Thread -> (token, K or V, U heads, 8 elements of each): rows of one token are
+// consecutive, so a block moves whole tokens.  All L threads of a row are of one
+// warp and agree on everything but their elements.
+template <int HD, int U>
+struct Place {
+    static constexpr int L = HD / 8;  // threads a row
+    int c, t, which, head, n;         // n: heads of this thread, 0 past the end
+    __device__ __forceinline__ explicit Place(const RowsParams &p) {
+        const long idx = blockIdx.x * static_cast<long>(kRowThreads) + threadIdx.x;
+        c = static_cast<int>(idx % L);
+        const long row = idx / L;
+        const int groups = (p.kv.kv_heads + U - 1) / U, per = 2 * groups;
+        t = static_cast<int>(row / per);
+        const int r = static_cast<int>(row % per);
+        which = r / groups;
+        head = (r % groups) * U;
+        n = t < p.n ? min(U, p.kv.kv_heads - head) : 0;
     }
-    if constexpr (E4M3) {
-        float a = 0.f;  // over the finite values: an infinity saturates, a NaN stays one
+};
+
+template <typename T, bool E4M3, bool VEC, int HD, int U>
+__global__ void __launch_bounds__(kRowThreads) ijb_kv_append_kernel(const __grid_constant__ RowsParams p) {
+    const Place<HD, U> w(p);
+    const long src = w.n ? w.t * p.stride + static_cast<long>(w.head) * HD + w.c * 8 : 0;
+    const T *from = static_cast<const T *>(w.which ? p.v : p.k) + src;
+    float f[U][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[i]) <= 3.402823466e38f ? fabsf(f[i]) : 0.f);
+    for (int j = 0; j < U; ++j) {
+        if (j < w.n) {
+            load_row8<VEC>(from + j * HD, f[j]);
+        } else {
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        if (to < 0) return;
-        // a = m 2^x with m in [1, 2): 448 = 1.75 * 2^8, so e = x - 8, one more when m > 1.75
-        // (a below 2^-126 has x = -127 here and e ends at the floor)
-        const uint32_t bits = __float_as_uint(a);
-        int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-        e = max(e, -126);
-        const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        uint32_t w[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * j] * inv, f[4 * j + 1] * inv),
-                                                         __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * j + 2] * inv, f[4 * j + 3] * inv),
-                                                         __NV_SATFINITE, __NV_E4M3);
-            w[j] = lo | (hi << 16);
+            for (int i = 0; i < 8; ++i) f[j][i] = 0.f;
         }
-        *reinterpret_cast<uint2 *>(p.kv.data + to * HD + c * 8) = make_uint2(w[0], w[1]);
-        if (c == 0) p.kv.scale[to] = static_cast<uint8_t>(e + 127);
-    } else {
-        if (to < 0) return;
-        store_row8<true>(reinterpret_cast<__half *>(p.kv.data) + to * HD + c * 8, f);
+    }
+    const long slot = w.n ? slot_row(p, w.t, w.which) : -1;
+    const long to0 = slot + (static_cast<long>(w.head) << p.kv.page_shift);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const long to = to0 + (static_cast<long>(j) << p.kv.page_shift);
+        const bool live = slot >= 0 && j < w.n;
+        if constexpr (E4M3) {
+            float a = 0.f;  // over the finite values: an infinity saturates, a NaN stays one
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[j][i]) <= 3.402823466e38f ? fabsf(f[j][i]) : 0.f);
+#pragma unroll
+            for (int o = HD / 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            // a = m 2^x with m in [1, 2): 448 = 1.75 * 2^8, so e = x - 8, one more when m > 1.75
+            // (a below 2^-126 has x = -127 here and e ends at the floor)
+            const uint32_t bits = __float_as_uint(a);
+            int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+            e = max(e, -126);
+            const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            uint32_t q[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[j][4 * h] * inv, f[j][4 * h + 1] * inv),
+                                                             __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[j][4 * h + 2] * inv, f[j][4 * h + 3] * inv),
+                                                             __NV_SATFINITE, __NV_E4M3);
+                q[h] = lo | (hi << 16);
+            }
+            if (live) {
+                *reinterpret_cast<uint2 *>(p.kv.data + to * HD + w.c * 8) = make_uint2(q[0], q[1]);
+                if (w.c == 0) p.kv.scale[to] = static_cast<uint8_t>(e + 127);
+            }
+        } else {
+            if (live) store_row8<true>(reinterpret_cast<__half *>(p.kv.data) + to * HD + w.c * 8, f[j]);
+        }
     }
 }
 
 // Reads back: code * 2^e (exact in fp32), or the fp16 row; rows of padding
 // entries and of entries that name no slot are left as they were.
-template <typename T, bool E4M3, bool VEC, int HD>
+template <typename T, bool E4M3, bool VEC, int HD, int U>
 __global__ void __launch_bounds__(kRowThreads) ijb_kv_gather_kernel(const __grid_constant__ RowsParams p) {
-    constexpr int L = HD / 8;
-    const long idx = blockIdx.x * static_cast<long>(kRowThreads) + threadIdx.x;
-    const int c = static_cast<int>(idx % L);
-    const long row = idx / L;
-    const int per = 2 * p.kv.kv_heads;
-    if (row >= static_cast<long>(p.n) * per) return;
-    const int t = static_cast<int>(row / per), r = static_cast<int>(row % per);
-    const int which = r / p.kv.kv_heads, head = r % p.kv.kv_heads;
-    const long from = slot_row(p, t, which, head);
-    if (from < 0) return;
-    float f[8];
-    if constexpr (E4M3) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p.kv.data + from * HD + c * 8);
-        const float s = kv_scale(p.kv.scale[from]);
+    const Place<HD, U> w(p);
+    if (w.n == 0) return;
+    const long slot = slot_row(p, w.t, w.which);
+    if (slot < 0) return;
+    const long from0 = slot + (static_cast<long>(w.head) << p.kv.page_shift);
+    T *dst = static_cast<T *>(w.which ? p.v : p.k) + w.t * p.stride + static_cast<long>(w.head) * HD + w.c * 8;
+    uint4 raw[U];
+    uint32_t sc[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t u = j < 2 ? w.x : w.y;
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(u >> (16 * (j & 1))),
-                                                             __NV_E4M3);
-            const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-            f[2 * j] = v.x * s;
-            f[2 * j + 1] = v.y * s;
+    for (int j = 0; j < U; ++j) {
+        if (j >= w.n) continue;
+        const long from = from0 + (static_cast<long>(j) << p.kv.page_shift);
+        if constexpr (E4M3) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p.kv.data + from * HD + w.c * 8);
+            raw[j].x = u.x;
+            raw[j].y = u.y;
+            sc[j] = p.kv.scale[from];
+        } else {
+            raw[j] = *reinterpret_cast<const uint4 *>(p.kv.data + (from * HD + w.c * 8) * 2);
         }
-    } else {
-        load_row8<true>(reinterpret_cast<const __half *>(p.kv.data) + from * HD + c * 8, f);
     }
-    T *dst = static_cast<T *>(which ? p.v : p.k);
-    store_row8<VEC>(dst + t * p.stride + static_cast<long>(head) * HD + c * 8, f);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        if (j >= w.n) continue;
+        float f[8];
+        if constexpr (E4M3) {
+            const float s = kv_scale(sc[j]);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const uint32_t u = h < 2 ? raw[j].x : raw[j].y;
+                const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(u >> (16 * (h & 1))),
+                                                                 __NV_E4M3);
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&x));
+                f[2 * h] = v.x * s;
+                f[2 * h + 1] = v.y * s;
+            }
+        } else {
+            const __half *h = reinterpret_cast<const __half *>(&raw[j]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __half2float(h[i]);
+        }
+        store_row8<VEC>(dst + j * HD, f);
+    }
 }
 
-template <bool APPEND, typename T, bool E4M3, bool VEC, int HD>
+constexpr int kHeads = 4;              // heads a thread takes of many rows
+constexpr long kManyThreads = 1 << 18; // a head each from here on fills the GPU about once
+
+template <bool APPEND, typename T, bool E4M3, bool VEC, int HD, int U>
 void rows_launch(const RowsParams &p, cudaStream_t s) {
-    const long threads = static_cast<long>(p.n) * 2 * p.kv.kv_heads * (HD / 8);
+    const long threads = static_cast<long>(p.n) * 2 * ((p.kv.kv_heads + U - 1) / U) * (HD / 8);
     const unsigned blocks = static_cast<unsigned>((threads + kRowThreads - 1) / kRowThreads);
-    if constexpr (APPEND) ijb_kv_append_kernel<T, E4M3, VEC, HD><<<blocks, kRowThreads, 0, s>>>(p);
-    else ijb_kv_gather_kernel<T, E4M3, VEC, HD><<<blocks, kRowThreads, 0, s>>>(p);
+    if constexpr (APPEND) ijb_kv_append_kernel<T, E4M3, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
+    else ijb_kv_gather_kernel<T, E4M3, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
+}
+template <bool APPEND, typename T, bool E4M3, int HD>
+void rows_launch(const RowsParams &p, bool vec, cudaStream_t s) {
+    const bool many = static_cast<long>(p.n) * 2 * p.kv.kv_heads * (HD / 8) > kManyThreads && p.kv.kv_heads >= kHeads;
+    if (!vec) rows_launch<APPEND, T, E4M3, false, HD, 1>(p, s);
+    else if (many) rows_launch<APPEND, T, E4M3, true, HD, kHeads>(p, s);
+    else rows_launch<APPEND, T, E4M3, true, HD, 1>(p, s);
 }
 template <bool APPEND, typename T, bool E4M3>
 void rows_launch(const RowsParams &p, bool vec, cudaStream_t s) {
-    if (p.kv.head_dim == 64)
-        vec ? rows_launch<APPEND, T, E4M3, true, 64>(p, s) : rows_launch<APPEND, T, E4M3, false, 64>(p, s);
-    else
-        vec ? rows_launch<APPEND, T, E4M3, true, 128>(p, s) : rows_launch<APPEND, T, E4M3, false, 128>(p, s);
+    if (p.kv.head_dim == 64) rows_launch<APPEND, T, E4M3, 64>(p, vec, s);
+    else rows_launch<APPEND, T, E4M3, 128>(p, vec, s);
 }
 
 template <bool APPEND>

@@ -16,7 +16,9 @@
 //    products and the exponentials.  256 rows at a time on tcgen05.
 // Both cut all the call's work (tiles of rows x units of positions, over all
 // entries and KV heads, in one line) into equal runs, one per worker, so ragged
-// lengths and long contexts fill the GPU alike.  A tile's run that another
+// lengths and long contexts fill the GPU alike.  A tile counts for `over` units
+// more than it has (its queries come in, its output goes out), and a cut that
+// would leave less than `least` units of a tile on one side moves to its end.  A tile's run that another
 // worker began or goes on with leaves its softmax state in the workspace, and
 // ijb_paged_merge_kernel joins the states in order: no atomics, the same result
 // every time for the same call.
@@ -51,6 +53,7 @@ struct AttnArgs {
     bool report_long;        // no other kernel takes longer ones: they are beyond the caller's max_q
     int tile_rows, unit;     // rows per tile, positions per unit
     int workers, min_units;
+    int over, least;
     float scale_log2;        // scale * log2(e)
     int4 *left;              // workspace: per worker, the tile it leaves to be gone on with
     float *part;             // workspace: two states per worker
@@ -92,6 +95,7 @@ __device__ __forceinline__ int tile_units(const AttnArgs &a, const Entry &x, int
 struct Segment {
     Entry x;
     int e, ti, head, b0, b1, units;
+    long start;  // the tile's place in the line
 };
 
 // Inclusive sum over the block's threads of v; *total receives the sum.
@@ -139,7 +143,7 @@ __device__ __forceinline__ void plan_end(const AttnArgs &a, int *sums, PlanOut *
         sums[tiles] = units;
         po->tiles = tiles;
         po->units = units;
-        po->per = static_cast<int>(max(static_cast<long>(a.min_units), (all + a.workers - 1) / a.workers));
+        po->per = static_cast<int>(max(static_cast<long>(a.min_units + a.over), (all + a.workers - 1) / a.workers));
     }
     __syncthreads();
 }
@@ -158,7 +162,7 @@ __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po
             int n = 0;
             if (e < a.n_entries) {
                 const Entry x = entry_load(a, e, lead);
-                n = x.tiles ? tile_units(a, x, 0) : 0;
+                n = x.tiles ? tile_units(a, x, 0) + a.over : 0;
             }
             int total;
             const int inc = block_scan_int<NT>(n, po->warp_sums, &total);
@@ -184,7 +188,7 @@ __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po
             int n = 0;
             if (t < tiles) {
                 const int e = find_le(first, a.n_entries, t);
-                n = tile_units(a, entry_load(a, e, false), t - first[e]);
+                n = tile_units(a, entry_load(a, e, false), t - first[e]) + a.over;
             }
             int total;
             const int inc = block_scan_int<NT>(n, po->warp_sums, &total);
@@ -195,29 +199,46 @@ __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po
     }
 }
 
-// A worker's position in the line of work.
+// A place in the line of work: `at` counts units and tiles' `over`; a tile is
+// entered past its `over`.
 struct Cursor {
     long at, end;
     int e, ti, head, b0;
 };
 
+// Where a worker begins: w runs along, or the start or end of the tile there.
+template <bool ONE>
+__device__ __forceinline__ Cursor cursor_at(const AttnArgs &a, const int *first, const int *sums, const PlanOut &po, int w) {
+    Cursor c;
+    const long all = static_cast<long>(po.units) * a.kv.kv_heads;
+    c.at = c.end = min(all, static_cast<long>(w) * po.per);
+    c.e = c.ti = c.head = c.b0 = 0;
+    if (c.at >= all) return c;
+    c.head = (c.at >> 32) ? static_cast<int>(c.at / po.units)
+                          : static_cast<int>(static_cast<uint32_t>(c.at) / static_cast<uint32_t>(po.units));
+    const int u = static_cast<int>(c.at - static_cast<long>(c.head) * po.units);
+    int t = find_le(sums, po.tiles, u);
+    const int in = u - sums[t] - a.over, units = sums[t + 1] - sums[t] - a.over;  // units of the tile before the place
+    if (in < a.least) {
+        c.at -= u - sums[t];
+    } else if (units - in < a.least) {
+        c.at += sums[t + 1] - u;
+        if (++t == po.tiles) {
+            t = 0;
+            ++c.head;
+        }
+    } else {
+        c.b0 = in;
+    }
+    c.e = ONE ? t : find_le(first, a.n_entries, t);
+    c.ti = ONE ? 0 : t - first[c.e];
+    return c;
+}
 template <bool ONE>
 __device__ __forceinline__ Cursor cursor_start(const AttnArgs &a, const int *first, const int *sums, const PlanOut &po,
                                                int worker) {
-    Cursor c;
-    const long all = static_cast<long>(po.units) * a.kv.kv_heads;
-    c.at = min(all, static_cast<long>(worker) * po.per);
-    c.end = min(all, c.at + po.per);
-    c.e = c.ti = c.head = c.b0 = 0;
-    if (c.at < c.end) {
-        c.head = (c.at >> 32) ? static_cast<int>(c.at / po.units)
-                              : static_cast<int>(static_cast<uint32_t>(c.at) / static_cast<uint32_t>(po.units));
-        const int u = static_cast<int>(c.at - static_cast<long>(c.head) * po.units);
-        const int t = find_le(sums, po.tiles, u);
-        c.e = ONE ? t : find_le(first, a.n_entries, t);
-        c.ti = ONE ? 0 : t - first[c.e];
-        c.b0 = u - sums[t];
-    }
+    Cursor c = cursor_at<ONE>(a, first, sums, po, worker);
+    c.end = cursor_at<ONE>(a, first, sums, po, worker + 1).at;
     return c;
 }
 
@@ -237,8 +258,10 @@ __device__ __forceinline__ bool cursor_next(const AttnArgs &a, Cursor &c, Segmen
     s.head = c.head;
     s.b0 = c.b0;
     s.units = tile_units(a, s.x, c.ti);
-    s.b1 = static_cast<int>(min(static_cast<long>(s.units), c.b0 + (c.end - c.at)));
-    c.at += s.b1 - s.b0;
+    s.start = c.at - (c.b0 > 0 ? a.over + c.b0 : 0);
+    const long stop = c.end - s.start - a.over;  // units of the tile before the worker's end
+    s.b1 = static_cast<int>(min(static_cast<long>(s.units), stop));
+    c.at = s.start + a.over + s.b1;
     c.b0 = 0;
     if (++c.ti >= s.x.tiles) {
         c.ti = 0;
@@ -259,9 +282,11 @@ __host__ __device__ constexpr long part_floats() { return static_cast<long>(ROWS
 // What the merge has to join for a worker: entry, tile, head and states of the
 // tile that its last run begins and does not end; no states if there is none.
 __device__ __forceinline__ int4 left_none() { return make_int4(0, 0, 0, 0); }
-__device__ __forceinline__ int4 left_of(const Segment &s, int per) {
+__device__ __forceinline__ int4 left_of(const AttnArgs &a, const Segment &s, int worker, int per) {
     if (s.b0 > 0 || s.b1 == s.units) return left_none();
-    return make_int4(s.e, s.ti, s.head, 1 + (s.units - s.b1 + per - 1) / per);
+    // workers w' > worker begin in the tile up to the last w' * per that leaves `least` units of it
+    const long last = s.start + a.over + s.units - a.least;
+    return make_int4(s.e, s.ti, s.head, 1 + static_cast<int>(last / per) - worker);
 }
 
 __device__ __forceinline__ void store4(float *p, float a, float b, float c, float d) {
@@ -705,7 +730,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
             }
         }
         // ---- the run's end: the output, or its state
-        left = left_of(s, po.per);
+        left = left_of(a, s, worker, po.per);
         const bool whole = s.b0 == 0 && s.b1 == s.units;
         float *part = a.part + part_slot(s, worker) * part_floats<kDecRows, HD>();
 #pragma unroll
@@ -1391,7 +1416,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
         int4 left = left_none();
         Cursor w = c;
         Segment s;
-        while (cursor_next(a, w, s)) left = left_of(s, po.per);
+        while (cursor_next(a, w, s)) left = left_of(a, s, blockIdx.x, po.per);
         a.left[blockIdx.x] = left;
     }
     if (c.at >= c.end) return;
@@ -1587,6 +1612,8 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.unit = kChunk;
     a.workers = sms * D::kWarps;
     a.min_units = 2;
+    a.over = 1;
+    a.least = 1;
     ijb_paged_decode_kernel<HD, E4M3, WIDE, T><<<sms, D::kWarps * 32, decode_smem<HD, E4M3, WIDE>(), s>>>(a);
     return merge_launch<kDecRows, HD, T>(a, s);
 }
@@ -1603,6 +1630,8 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     a.unit = kBlock;
     a.workers = sms;
     a.min_units = 2;
+    a.over = 4;
+    a.least = 2;
     ijb_paged_tile_kernel<HD, E4M3, T><<<sms, kTileThreads, L::kSmem, s>>>(a);
     return merge_launch<kTileRows, HD, T>(a, s);
 }

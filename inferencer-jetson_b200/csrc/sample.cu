@@ -139,30 +139,30 @@ __device__ __forceinline__ float desc_value(uint32_t key) {
 }
 
 struct Row {
-    float max, temp, inv;
-    bool plain_div;
-    // (x - m) / T, rounded to nearest.  With inv = 1 / T rounded to nearest, one
+    float max, temp, inv;  // max finite, temp within 1e-15 .. 1e15
+    // (x - m) / T, rounded to nearest: with inv = 1 / T rounded to nearest, one
     // residual correction of d * inv gives the quotient rounded to nearest
-    // (Markstein), as long as nothing leaves the normal range; else the division.
+    // (Markstein).  Differences below -1e20, -infinity included, count as that:
+    // exp makes 0 of all of them.
     __device__ __forceinline__ float t(float x) const {
-        const float d = x == max ? 0.f : x - max;
-        if (plain_div) return d / temp;
+        const float d = fmaxf(x - max, -1e20f);
         const float q = d * inv;
-        const float r = fmaf(fmaf(-q, temp, d), inv, q);
-        return d >= -1e30f ? r : d;  // -infinity, and what exp makes 0 either way
+        return fmaf(fmaf(-q, temp, d), inv, q);
     }
+    // Nearest whole number of -64 t, kBins - 1 at most (adding 2^23 leaves it in the low bits).
     __device__ __forceinline__ static int bin(float t) {
-        return static_cast<int>(fminf(-t * kBinsPerNat, static_cast<float>(kBins - 1)));
+        const float c = fmaxf(t, -static_cast<float>(kBins - 1) / kBinsPerNat);
+        return __float_as_int(fmaf(c, -kBinsPerNat, 8388608.f)) & (2 * kBins - 1);
     }
-    // Which of kBins equal parts of bins lo..hi.
+    // Which of kBins equal parts of bins lo..hi, the open bin taken to end at -t = 32 (where
+    // weights end), its rest in the last part.
     __device__ __forceinline__ static int part(float t, int lo, int hi) {
-        const float f = (-t * kBinsPerNat - static_cast<float>(lo)) * (static_cast<float>(kBins) / static_cast<float>(hi + 1 - lo));
+        const float end = hi == kBins - 1 ? 32.f * kBinsPerNat : static_cast<float>(hi) + 0.5f;
+        const float begin = static_cast<float>(lo) - 0.5f;
+        const float f = (-t * kBinsPerNat - begin) * (static_cast<float>(kBins) / (end - begin));
         return static_cast<int>(fminf(fmaxf(f, 0.f), static_cast<float>(kBins - 1)));
     }
-    // 0 for a NaN (a logit of -infinity at an infinite temperature)
-    __device__ __forceinline__ static u64 fixed(float w) {
-        return w > 0.f ? static_cast<u64>(__float2ll_rn(w * kFixed)) : 0ull;
-    }
+    __device__ __forceinline__ static u64 fixed(float w) { return __float2ull_rn(w * kFixed); }
     __device__ __forceinline__ bool in(float x, const Range &r) const {
         const float tt = t(x);
         const int b = bin(tt);
@@ -171,12 +171,12 @@ struct Row {
     }
     // Bounds on the logits of bins lo..hi, with room for t's rounding.
     __device__ __forceinline__ float least(int hi) const {
-        return hi == kBins - 1 || !(max < INFINITY)
+        return hi == kBins - 1
                    ? -INFINITY
                    : max - (static_cast<float>(hi + 2) / kBinsPerNat) * temp * 1.0001f - fabsf(max) * 1e-5f;
     }
     __device__ __forceinline__ float most(int lo) const {
-        return lo == 0 || !(max < INFINITY)
+        return lo == 0
                    ? INFINITY
                    : max - (static_cast<float>(lo - 1) / kBinsPerNat) * temp * 0.9999f + fabsf(max) * 1e-5f;
     }
@@ -304,12 +304,12 @@ __device__ __forceinline__ void local_hist(Smem &s, const float *xs, int len, co
 }
 
 // Adds the cluster's histograms into the leader's (cnt, mass): CTA r a slice.
-__device__ __forceinline__ void merge_hist(Smem &s, uint32_t *cnt, u64 *mass, int C, int rank) {
+__device__ __forceinline__ void merge_hist(Smem &s, uint32_t *cnt, u64 *mass, int C, int rank, bool masses = true) {
     cluster_sync();  // every CTA's is there
     const int per = kBins / C;
     for (int i = rank * per + threadIdx.x; i < (rank + 1) * per; i += kThreads) {
         *peer(&cnt[i], 0) = over_peers<uint32_t>(C, [&](int q) { return *peer(&s.hcnt[i], q); });
-        *peer(&mass[i], 0) = over_peers<u64>(C, [&](int q) { return *peer(&s.hmass[i], q); });
+        if (masses) *peer(&mass[i], 0) = over_peers<u64>(C, [&](int q) { return *peer(&s.hmass[i], q); });
     }
     cluster_sync();
 }
@@ -399,6 +399,7 @@ struct Leader {
     bool weighed;  // the bins' masses are there
     int step = kTopK, phase = kBegin;
     int list_lo = 0, list_hi = -1, list_n = 0;  // the list: tokens of bins [lo, hi]
+    bool sorted = false;                        // the whole list is in s.few, in order, with its running masses
     u64 kept = 0, above = 0;
     // the cut at work: where the running count reaches `target`, or the running mass first exceeds it
     bool by_count = false;
@@ -481,6 +482,7 @@ struct Leader {
                 block_scan<kBins>(s, s.mmass, s.mcnt);
                 weighed = true;
                 list_hi = -1;  // the histogram lay over it
+                sorted = false;
                 phase = kBegin;
             } else if (phase == kLook) {
                 r = Range{list_lo, list_hi, -1, 32, 0u};
@@ -509,6 +511,7 @@ struct Leader {
                 base_m = r.lo ? s.mmass[r.lo - 1] : 0ull;
                 list_lo = r.lo;
                 list_hi = -1;
+                sorted = false;
                 list_n = upto - base_c;
                 if (list_n <= kCap) {
                     order(s, kGather, kGathered);
@@ -521,9 +524,11 @@ struct Leader {
                 phase = kInList;
             } else if (phase == kInList) {
                 if (list_n <= kFew) {
-                    for (int i = threadIdx.x; i < list_n; i += kThreads) s.few[i] = list[i];
-                    if (threadIdx.x == 0) s.ctl.list_n = list_n;
-                    __syncthreads();
+                    if (!sorted) {
+                        for (int i = threadIdx.x; i < list_n; i += kThreads) s.few[i] = list[i];
+                        if (threadIdx.x == 0) s.ctl.list_n = list_n;
+                        __syncthreads();
+                    }
                     phase = kOrder;
                     continue;
                 }
@@ -583,27 +588,38 @@ struct Leader {
                 order(s, kHist, kSplitDone, r.sh == 32 ? 22 : (r.sh == 2 ? 0 : r.sh - 10));
                 return true;
             } else if (phase == kOrder) {
-                // each of a few tokens finds its place, and the mass before it
                 const int n = s.ctl.list_n, t = threadIdx.x;
-                u64 mine = 0, w = 0, m = 0;
-                int place = 0;
-                if (t < n) {
-                    mine = s.few[t];
-                    s.few_w[t] = w = weight(mine);
-                }
-                __syncthreads();
-                if (t < n) {
-#pragma unroll 4
-                    for (int i = 0; i < n; ++i) {
-                        const bool before = s.few[i] < mine;
-                        place += before ? 1 : 0;
-                        m += before ? s.few_w[i] : 0ull;
+                if (!sorted) {  // each of a few tokens finds its place, and the mass before it
+                    u64 mine = 0, m = 0;
+                    int place = 0;
+                    if (t < n) {
+                        mine = s.few[t];
+                        s.few_w[t] = m = weight(mine);
                     }
-                    if (by_count ? place == static_cast<int>(target) - 1 - base_c
-                                 : m <= target - base_m && target - base_m < m + w) {
-                        s.ctl.cut_mass = base_m + m + w;
-                        s.ctl.cut_w = w;
-                        s.ctl.index = static_cast<int>(mine & 0xffffffffull);
+                    __syncthreads();
+                    if (t < n) {
+#pragma unroll 4
+                        for (int i = 0; i < n; ++i) {
+                            const bool before = s.few[i] < mine;
+                            place += before ? 1 : 0;
+                            m += before ? s.few_w[i] : 0ull;
+                        }
+                    }
+                    __syncthreads();
+                    if (t < n) {
+                        s.few[place] = mine;
+                        s.few_w[place] = m;
+                    }
+                    __syncthreads();
+                    sorted = list_hi >= 0 && list_n <= kFew;
+                }
+                if (t < n) {
+                    const u64 m = s.few_w[t], before = t ? s.few_w[t - 1] : 0ull;
+                    if (by_count ? t == static_cast<int>(target) - 1 - base_c
+                                 : before <= target - base_m && target - base_m < m) {
+                        s.ctl.cut_mass = base_m + m;
+                        s.ctl.cut_w = m - before;
+                        s.ctl.index = static_cast<int>(s.few[t] & 0xffffffffull);
                     }
                 }
                 __syncthreads();
@@ -691,7 +707,6 @@ __global__ void __launch_bounds__(kThreads, 2) ijb_sample_kernel(const __grid_co
         const int lane = threadIdx.x & 31;
         row.max = warp_max(lane < C ? peer(&s.ctl, lane)->max : -INFINITY);
     }
-    row.temp = temp;
     if (row.max == -INFINITY || greedy) {  // nothing to choose from, or the largest
         if (rank == 0 && threadIdx.x == 0) {
             u64 best = 0;
@@ -702,17 +717,22 @@ __global__ void __launch_bounds__(kThreads, 2) ijb_sample_kernel(const __grid_co
         cluster_sync();  // no CTA leaves while the leader reads it
         return;
     }
-    row.inv = 1.f / temp;
-    row.plain_div = !(temp >= 1e-6f && temp <= 1e6f);
+    if (row.max == INFINITY) {  // the infinite ones share everything: as logits 0 beside -infinity
+        for (int i = threadIdx.x; i < len; i += kThreads) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
+        row.max = 0.f;
+        __syncthreads();
+    }
+    row.temp = fminf(fmaxf(temp, 1e-15f), 1e15f);
+    row.inv = 1.f / row.temp;
     const float min_p = p.min_p ? p.min_p[r] : 0.f;
     const int k = p.top_k ? p.top_k[r] : 0;
     const bool few = k > 0 && k <= kCap / 2 && k < p.vocab;  // most likely the list holds all that is kept
     if (few) local_hist<false>(s, xs, len, row, 0.f);
     else local_hist<true>(s, xs, len, row, min_p);
-    merge_hist(s, s.mcnt, s.mmass, C, rank);
+    merge_hist(s, s.mcnt, s.mmass, C, rank, !few);
     Leader lead;
     if (rank == 0) {
-        block_scan<kBins>(s, s.mmass, s.mcnt);
+        block_scan<kBins>(s, few ? nullptr : s.mmass, s.mcnt);
         lead.row = row;
         lead.min_p = min_p;
         lead.top_p = p.top_p ? p.top_p[r] : 1.f;

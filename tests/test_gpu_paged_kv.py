@@ -56,7 +56,7 @@ def rows(cuda, n, kvh, hd, dtype, seed):
 
 
 @pytest.mark.parametrize("kvh,hd,page,n", [(1, 64, 8, 1), (2, 64, 16, 37), (8, 64, 16, 64), (3, 128, 32, 33),
-                                           (8, 128, 256, 29), (5, 128, 8, 50)])
+                                           (8, 128, 256, 29), (5, 128, 8, 50), (8, 128, 256, 1100), (5, 128, 256, 1700), (7, 64, 256, 2400)])
 @pytest.mark.parametrize("src", ["float32", "float16"])
 @pytest.mark.parametrize("e4m3", [True, False])
 def test_append_and_gather(cuda, kvh, hd, page, n, src, e4m3):
