@@ -40,6 +40,22 @@ namespace {
 
 constexpr int kMaxEntries = 4096, kMaxTiles = 8192;
 
+// A place in the line of work: `at` counts units and tiles' `over`; a tile is
+// entered past its `over`.
+struct Cursor {
+    long at, end;
+    int e, ti, head, b0;
+};
+
+// What a worker leaves to the merge: the tile that its last run begins and does
+// not end, as rows row0 .. row0 + rows of the entry whose tokens start at q0, and
+// the number of its states (0: there is none); whether any value it computed is
+// not finite; where its runs began.
+struct __align__(16) Left {
+    int states, q0, row0, rows, head, bad, pad[2];
+    Cursor runs;
+};
+
 struct AttnArgs {
     KvDev kv;
     const void *q;
@@ -55,7 +71,7 @@ struct AttnArgs {
     int workers, min_units;
     int over, least;
     float scale_log2;        // scale * log2(e)
-    int4 *left;              // workspace: per worker, the tile it leaves to be gone on with
+    Left *left;              // workspace: per worker, the tile it leaves to be gone on with
     float *part;             // workspace: two states per worker
     uint32_t *status;
 };
@@ -199,12 +215,30 @@ __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po
     }
 }
 
-// A place in the line of work: `at` counts units and tiles' `over`; a tile is
-// entered past its `over`.
-struct Cursor {
-    long at, end;
-    int e, ti, head, b0;
-};
+// plan_build<NT, true> for up to 32 entries by each warp on its own, without the
+// block's barriers: sums in the warp's memory, the rest in *po.
+__device__ __forceinline__ void plan_warp(const AttnArgs &a, int *sums, PlanOut *po, bool report) {
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    if (lane < a.n_entries) {
+        const Entry x = entry_load(a, lane, report);
+        n = x.tiles ? tile_units(a, x, 0) + a.over : 0;
+    }
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int p = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += p;
+    }
+    sums[lane] = inc - n;
+    const int units = __shfl_sync(0xffffffffu, inc, 31);
+    if (lane == 0) sums[a.n_entries] = units;
+    const long all = static_cast<long>(units) * a.kv.kv_heads;
+    po->tiles = a.n_entries;
+    po->units = units;
+    po->per = static_cast<int>(max(static_cast<long>(a.min_units + a.over), (all + a.workers - 1) / a.workers));
+    __syncwarp();
+}
 
 // Where a worker begins: w runs along, or the start or end of the tile there.
 template <bool ONE>
@@ -279,14 +313,17 @@ __device__ __forceinline__ long part_slot(const Segment &s, int worker) { return
 template <int ROWS, int HD>
 __host__ __device__ constexpr long part_floats() { return static_cast<long>(ROWS) * (HD + 2); }
 
-// What the merge has to join for a worker: entry, tile, head and states of the
-// tile that its last run begins and does not end; no states if there is none.
-__device__ __forceinline__ int4 left_none() { return make_int4(0, 0, 0, 0); }
-__device__ __forceinline__ int4 left_of(const AttnArgs &a, const Segment &s, int worker, int per) {
-    if (s.b0 > 0 || s.b1 == s.units) return left_none();
+__device__ __forceinline__ Left left_of(const AttnArgs &a, const Segment &s, int worker, int per) {
+    Left x = {};
+    if (s.b0 > 0 || s.b1 == s.units) return x;
     // workers w' > worker begin in the tile up to the last w' * per that leaves `least` units of it
     const long last = s.start + a.over + s.units - a.least;
-    return make_int4(s.e, s.ti, s.head, 1 + static_cast<int>(last / per) - worker);
+    x.states = 1 + static_cast<int>(last / per) - worker;
+    x.q0 = s.x.q0;
+    x.row0 = s.ti * a.tile_rows;
+    x.rows = min(a.tile_rows, s.x.rows - x.row0);
+    x.head = s.head;
+    return x;
 }
 
 __device__ __forceinline__ void store4(float *p, float a, float b, float c, float d) {
@@ -456,14 +493,27 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
     constexpr bool SPLIT = sizeof(T) == 4;  // fp32 queries: hi + lo
     constexpr int NT = D::kWarps * 32, RB = D::kRowBytes, KS = HD / 16, NTILE = HD / 8;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ PlanOut po;
+    __shared__ PlanOut block_po;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t4 = lane & 3;
     pdl_trigger();
-    int *sums = reinterpret_cast<int *>(smem);
-    plan_build<NT, true>(a, nullptr, sums, &po);
     const int worker = blockIdx.x * D::kWarps + warp;
-    Cursor load_c = cursor_start<true>(a, nullptr, sums, po, worker), use_c = load_c;
-    __syncthreads();  // the plan's shared memory becomes the stages
+    Cursor load_c;
+    int per;
+    if (a.n_entries < 32) {
+        int *sums = reinterpret_cast<int *>(smem + warp * D::kStages * D::kStage);
+        PlanOut po;
+        plan_warp(a, sums, &po, worker == 0);
+        load_c = cursor_start<true>(a, nullptr, sums, po, worker);
+        per = po.per;
+        __syncwarp();  // the plan's shared memory becomes the stages
+    } else {
+        int *sums = reinterpret_cast<int *>(smem);
+        plan_build<NT, true>(a, nullptr, sums, &block_po);
+        load_c = cursor_start<true>(a, nullptr, sums, block_po, worker);
+        per = block_po.per;
+        __syncthreads();
+    }
+    Cursor use_c = load_c;
 
     const uint32_t base = smem_u32(smem) + warp * D::kStages * D::kStage;
     const T *qp = static_cast<const T *>(a.q);
@@ -519,7 +569,9 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
 
     // ---- the computing side
     int stage = 0;
-    int4 left = left_none();
+    Left left = {};
+    bool bad = false;
+    const Cursor runs = use_c;
     Segment s;
     while (cursor_next(a, use_c, s)) {
         const int row0 = s.ti * kDecRows, rows = min(kDecRows, s.x.rows - row0);
@@ -729,8 +781,14 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
                 o[i][1] += o[i][C - 1];
             }
         }
+        float zero = 0.f;  // NaN once a value is not finite
+#pragma unroll
+        for (int i = 0; i < NTILE; ++i)
+#pragma unroll
+            for (int k = 0; k < 2 * H; ++k) zero = fmaf(o[i][k], 0.f, zero);
+        bad |= !(zero == 0.f);
         // ---- the run's end: the output, or its state
-        left = left_of(a, s, worker, po.per);
+        left = left_of(a, s, worker, per);
         const bool whole = s.b0 == 0 && s.b1 == s.units;
         float *part = a.part + part_slot(s, worker) * part_floats<kDecRows, HD>();
 #pragma unroll
@@ -763,6 +821,9 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
         }
     }
     cp_async_wait<0>();
+    bad = __any_sync(0xffffffffu, bad);
+    left.bad = bad ? 1 : 0;
+    left.runs = runs;
     if (lane == 0) a.left[worker] = left;
 }
 
@@ -812,6 +873,7 @@ struct TileCtl {
     uint64_t full[8], empty[8], q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
     uint32_t tmem;
     uint32_t abort;
+    uint32_t bad;  // a value of the output is not finite
 };
 
 __device__ __forceinline__ bool try_bar(uint64_t *bar, uint32_t parity) {
@@ -1256,9 +1318,11 @@ __device__ __forceinline__ void softmax_block(uint32_t ts, float sc, int seen, u
 
 // Writes a warp's 32 rows of O (TMEM columns of `to`, one row a lane), times
 // inv, at dst + to_row (each lane its own row's), the first `rows` of them.
+// False if one of the lane's own row's values is not finite.
 template <int HD, typename O>
-__device__ __forceinline__ void write_rows(uint32_t to, uint32_t st, O *dst, bool vec, long to_row, int rows, float inv,
+__device__ __forceinline__ bool write_rows(uint32_t to, uint32_t st, O *dst, bool vec, long to_row, int rows, float inv,
                                            int lane) {
+    float zero = 0.f;
     constexpr int E = 16 / sizeof(O), D = 8 * E;  // elements of a 16-byte piece, of a pass
 #pragma unroll 1
     for (int d0 = 0; d0 < HD; d0 += D) {
@@ -1267,6 +1331,8 @@ __device__ __forceinline__ void write_rows(uint32_t to, uint32_t st, O *dst, boo
             uint32_t x[32];
             tm_ld32(to + d0 + 32 * h, x);
             tm_wait(x);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) zero = fmaf(__uint_as_float(x[c]), 0.f, zero);
 #pragma unroll
             for (int c = 0; c < 32 / E; ++c) {
                 uint32_t w[4];
@@ -1297,6 +1363,7 @@ __device__ __forceinline__ void write_rows(uint32_t to, uint32_t st, O *dst, boo
         }
         __syncwarp();
     }
+    return zero == 0.f;
 }
 
 // Softmax and output of tile t of a worker's runs (128 threads, row r of them).
@@ -1317,8 +1384,15 @@ __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q
     while (cursor_next(a, c, s)) {
         const int row0 = s.ti * kTileRows + t * 128;  // of the entry's rows
         if (row0 >= s.x.rows) continue;
-        // ---- queries: a warp its own 32 rows, 8 dims a lane; eight rows' loads in flight
-        constexpr int P = HD / 8, RQ = 32 / P, B = SPLIT ? 4 : 8;  // lanes a row, rows a step, steps a batch
+        // ---- queries: a warp its own 32 rows, 8 dims a lane; all loads of a batch in flight
+        constexpr int P = HD / 8, RQ = 32 / P, B = SPLIT && P > 8 ? 8 : P;  // lanes a row, rows a step, steps a batch
+        int tok, in;  // of the lane's row, going on by RQ rows a step
+        {
+            const int row = row0 + warp * 32 + lane / P;
+            tok = row / a.group;
+            in = row % a.group;
+        }
+        const int tok_step = RQ / a.group, in_step = RQ % a.group;
 #pragma unroll 1
         for (int k0 = 0; k0 < P; k0 += B) {
             float4 x[B], y[B];
@@ -1327,14 +1401,20 @@ __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q
                 const int row = row0 + warp * 32 + (k0 + k) * RQ + lane / P;
                 x[k] = y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (row < s.x.rows) {
-                    const T *src = qp + static_cast<long>(s.x.q0 + row / a.group) * a.q_stride +
-                                   (s.head * a.group + row % a.group) * HD + (lane % P) * 8;
+                    const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD +
+                                   (lane % P) * 8;
                     if constexpr (SPLIT) {
                         x[k] = load4(src, qvec);
                         y[k] = load4(src + 4, qvec);
                     } else {
                         x[k] = load8_raw(src, qvec8);
                     }
+                }
+                tok += tok_step;
+                in += in_step;
+                if (in >= a.group) {
+                    in -= a.group;
+                    ++tok;
                 }
             }
 #pragma unroll
@@ -1388,8 +1468,9 @@ __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q
                                   : static_cast<long>(t * 128 + r) * HD;
         const int rows = min(32, s.x.rows - (row0 + warp * 32));
         const uint32_t st = q + warp * 4096;
-        if (whole) write_rows<HD, T>(to, st, op, ovec, to_row, rows, inv, lane);
-        else write_rows<HD, float>(to, st, state, true, to_row, rows, 1.f, lane);
+        const bool fine = whole ? write_rows<HD, T>(to, st, op, ovec, to_row, rows, inv, lane)
+                                : write_rows<HD, float>(to, st, state, true, to_row, rows, 1.f, lane);
+        if (live && !fine) ctl->bad = 1u;
         if (!whole && live) {
             state[kTileRows * HD + t * 128 + r] = m == -INFINITY ? m : m * sc;
             state[kTileRows * HD + kTileRows + t * 128 + r] = l;
@@ -1413,11 +1494,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
     plan_build<kTileThreads, false>(a, first, sums, &po);
     const Cursor c = cursor_start<false>(a, first, sums, po, blockIdx.x);
     if (threadIdx.x == 0) {  // the last run of this worker
-        int4 left = left_none();
+        Left left = {};
         Cursor w = c;
         Segment s;
         while (cursor_next(a, w, s)) left = left_of(a, s, blockIdx.x, po.per);
+        left.runs = c;
         a.left[blockIdx.x] = left;
+        ctl.bad = 0u;
     }
     if (c.at >= c.end) return;
     if (threadIdx.x == 0) {
@@ -1458,82 +1541,187 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
     tc_before();
     __syncthreads();
     tc_after();
+    if (threadIdx.x == 0 && ctl.bad) a.left[blockIdx.x].bad = 1;
     if (warp == kMmaWarpId)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ----------------------------------------------------------------- merge --
 
-// Joins the states of the tile that a worker left: 16 of its rows a block.
-template <int ROWS, int HD, typename T>
-__global__ void __launch_bounds__(256) ijb_paged_merge_kernel(const __grid_constant__ AttnArgs a) {
+// A weight of 0 times a value that is not finite is NaN, so a NaN or an infinity in
+// a later token's V reaches the earlier tokens that share its block.  The kernels
+// say when a value came out that way, and the merge then computes the rows of those
+// tiles again that do not see all of the positions read, one position at a
+// time: 16 rows a block, for the tiles that worker w begins.
+template <int HD, bool E4M3>
+__device__ __forceinline__ float cached(const AttnArgs &a, long row, int d) {
+    if constexpr (E4M3) {
+        const uint32_t h = e4m3x2_half2(a.kv.data[row * HD + d]);
+        const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&h), __half2half2(scale_half(a.kv.scale[row])));
+        return __low2float(v);
+    } else {
+        return __half2float(reinterpret_cast<const __half *>(a.kv.data)[row * HD + d]);
+    }
+}
+template <int ROWS, int HD, int NT, bool E4M3, typename T>
+__device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float4 *shared) {
+    float *weight = reinterpret_cast<float *>(shared), *red = weight + NT;  // 4 * NT floats are there
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Cursor c = a.left[w].runs;
+    Segment s;
+    while (cursor_next(a, c, s)) {
+        if (s.b0 > 0) continue;
+        const int end = static_cast<int>(min(static_cast<long>(s.x.kv), static_cast<long>(s.units) * a.unit));  // read
+        for (int r = s.ti * ROWS + row0; r < min(s.x.rows, s.ti * ROWS + row0 + 16); ++r) {
+            const int tok = r / a.group, h = s.head * a.group + r % a.group;
+            const int n = s.x.kv - s.x.len + tok + 1;  // positions it sees
+            if (n <= 0 || n >= end) continue;
+            const T *q = static_cast<const T *>(a.q) + static_cast<long>(s.x.q0 + tok) * a.q_stride + h * HD;
+            T *out = static_cast<T *>(a.out) + static_cast<long>(s.x.q0 + tok) * a.out_stride + h * HD;
+            const float now = tid < HD ? static_cast<float>(out[tid]) : 0.f;
+            if (__syncthreads_and(now * 0.f == 0.f)) continue;
+            auto slot = [&](int t) {
+                return kv_row(a.kv, page_of(a, s.x.seq, t), 0, s.head, t & ((1 << a.kv.page_shift) - 1));
+            };
+            const long v_off = static_cast<long>(a.kv.kv_heads) << a.kv.page_shift;
+            float m = -INFINITY, l = 0.f, o = 0.f;  // o: dim tid
+            for (int t0 = 0; t0 < n; t0 += NT) {
+                float x = -INFINITY;
+                if (t0 + tid < n) {
+                    const long row = slot(t0 + tid);
+                    x = 0.f;
+                    for (int d = 0; d < HD; ++d) x = fmaf(static_cast<float>(q[d]), cached<HD, E4M3>(a, row, d), x);
+                    x *= a.scale_log2;
+                }
+                const float mx = warp_max(x);  // a NaN is left to its weight
+                __syncthreads();  // the weights of the last positions have been used
+                if (lane == 0) red[warp] = mx;
+                __syncthreads();
+                float to = m;
+                for (int i = 0; i < NT / 32; ++i) to = fmaxf(to, red[i]);
+                const float mu = to == -INFINITY ? 0.f : to, alpha = ex2(m - mu), p = ex2(x - mu);
+                m = to;
+                weight[tid] = t0 + tid < n ? p : 0.f;
+                const float add = warp_sum(weight[tid]);
+                __syncthreads();
+                if (lane == 0) red[warp] = add;
+                __syncthreads();
+                l *= alpha;
+                for (int i = 0; i < NT / 32; ++i) l += red[i];
+                o *= alpha;
+                if (tid < HD)
+                    for (int i = 0; i < min(NT, n - t0); ++i)
+                        o = fmaf(weight[i], cached<HD, E4M3>(a, slot(t0 + i) + v_off, tid), o);
+            }
+            if (tid < HD) out[tid] = static_cast<T>(o * (l > 0.f || l != l ? 1.f / l : 0.f));
+            __syncthreads();
+        }
+    }
+}
+
+// Joins the states of the tiles that EACH workers left (few leave one): 16 rows of
+// them a block of NT threads.  A thread has 4 dims of a row over some of the states, whose values it
+// loads (kMergeBatch at a time) before the row's maximum and sum are there.
+constexpr int kMergeBatch = 4;
+template <int ROWS, int HD, int NT, int EACH, bool E4M3, typename T>
+__global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_constant__ AttnArgs a) {
     __shared__ float top[16], total[16];
-    __shared__ float4 sum[256];
-    const int w0 = blockIdx.x, row0 = blockIdx.y * 16;
+    __shared__ float4 sum[NT];
+    const int row0 = blockIdx.y * 16;
     pdl_wait();
-    const int4 left = a.left[w0];
-    const int e = left.x, ti = left.y, head = left.z, n = left.w;
-    if (n == 0) return;
-    const Entry x = entry_load(a, e, false);
-    const int live = min(ROWS, x.rows - ti * ROWS), rows = min(16, live - row0);
-    if (rows <= 0) return;
-    constexpr long PF = part_floats<ROWS, HD>();
-    auto part = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0 ? 1 : 0)) * PF; };
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = warp; r < rows; r += 8) {
-        float m = -INFINITY, l = 0.f;
-        for (int i = lane; i < n; i += 32) m = fmaxf(m, part(i)[ROWS * HD + row0 + r]);
-        m = warp_max(m);
-        const float mu = m == -INFINITY ? 0.f : m;
-        for (int i = lane; i < n; i += 32) {
-            const float *p = part(i) + ROWS * HD + row0 + r;
-            l += p[ROWS] * ex2(p[0] - mu);
-        }
-        l = warp_sum(l);
-        if (lane == 0) {
-            top[r] = mu;
-            total[r] = l;
+    uint32_t some = 0, again = 0;  // bit j: worker j of this block's left a tile; has rows to look at again
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const int w = blockIdx.x * EACH + j;
+        if (w < a.workers) {
+            const int4 x = *reinterpret_cast<const int4 *>(&a.left[w].states), y = *reinterpret_cast<const int4 *>(&a.left[w].head);
+            some |= x.x > 0 ? 1u << j : 0u;
+            again |= y.y != 0 ? 1u << j : 0u;
         }
     }
-    __syncthreads();
-    constexpr int Q = HD / 4;  // float4 of a row
-    const int outs = rows * Q, groups = outs < 256 ? 256 / outs : 1;
-    T *op = static_cast<T *>(a.out);
-    const bool vec = aligned4<T>(a.out, a.out_stride);
-    for (int o0 = 0; o0 < outs; o0 += 256) {
-        const int g = outs < 256 ? threadIdx.x / outs : 0, o = outs < 256 ? threadIdx.x % outs : o0 + threadIdx.x;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int r = o / Q, c = o % Q;
-        if (g < groups && o < outs) {
-#pragma unroll 4
-            for (int i = g; i < n; i += groups) {
-                const float *p = part(i);
-                const float f = ex2(p[ROWS * HD + row0 + r] - top[r]);
-                const float4 v = *reinterpret_cast<const float4 *>(p + (row0 + r) * HD + 4 * c);
-                // a state without positions (f = 0) may hold no values
-                acc.x = f != 0.f ? fmaf(f, v.x, acc.x) : acc.x;
-                acc.y = f != 0.f ? fmaf(f, v.y, acc.y) : acc.y;
-                acc.z = f != 0.f ? fmaf(f, v.z, acc.z) : acc.z;
-                acc.w = f != 0.f ? fmaf(f, v.w, acc.w) : acc.w;
+    for (; some; some &= some - 1) {
+        const int w0 = blockIdx.x * EACH + __ffs(some) - 1;
+        const Left left = a.left[w0];
+        const int n = left.states, rows = min(16, left.rows - row0);
+        if (rows <= 0) continue;
+        constexpr long PF = part_floats<ROWS, HD>();
+        auto part = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0 ? 1 : 0)) * PF; };
+        constexpr int Q = HD / 4;  // float4 of a row
+        const int outs = rows * Q, groups = outs < NT ? NT / outs : 1;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        T *op = static_cast<T *>(a.out);
+        const bool vec = aligned4<T>(a.out, a.out_stride);
+        bool fine = true;
+        for (int o0 = 0; o0 < outs; o0 += NT) {
+            const int g = outs < NT ? threadIdx.x / outs : 0, o = outs < NT ? threadIdx.x % outs : o0 + threadIdx.x;
+            const int r = min(o / Q, rows - 1), c = o % Q;
+            const bool mine = g < groups && o < outs;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i0 = g; i0 - g < n; i0 += kMergeBatch * groups) {
+                float4 v[kMergeBatch];
+                float m[kMergeBatch];
+    #pragma unroll
+                for (int k = 0; k < kMergeBatch; ++k) {
+                    const int i = i0 + k * groups;
+                    m[k] = -INFINITY;
+                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (mine && i < n) {
+                        const float *p = part(i);
+                        m[k] = p[ROWS * HD + row0 + r];
+                        v[k] = *reinterpret_cast<const float4 *>(p + (row0 + r) * HD + 4 * c);
+                    }
+                }
+                if (o0 == 0 && i0 == g) {  // the rows' maxima and sums, a warp a row
+                    for (int q = warp; q < rows; q += NT / 32) {
+                        float mx = -INFINITY, l = 0.f;
+                        for (int i = lane; i < n; i += 32) {
+                            const float *p = part(i) + ROWS * HD + row0 + q;
+                            const float pm = p[0], pl = p[ROWS], to = fmaxf(mx, pm);
+                            if (to != -INFINITY) l = l * ex2(mx - to) + pl * ex2(pm - to);
+                            mx = to;
+                        }
+                        const float all = warp_max(mx), mu = all == -INFINITY ? 0.f : all;
+                        l = warp_sum(l * ex2(mx - mu));
+                        if (lane == 0) {
+                            top[q] = mu;
+                            total[q] = l;
+                        }
+                    }
+                    __syncthreads();
+                }
+    #pragma unroll
+                for (int k = 0; k < kMergeBatch; ++k) {
+                    const float f = ex2(m[k] - top[r]);
+                    if (f != 0.f) {  // a state without positions may hold no values
+                        acc.x = fmaf(f, v[k].x, acc.x);
+                        acc.y = fmaf(f, v[k].y, acc.y);
+                        acc.z = fmaf(f, v[k].z, acc.z);
+                        acc.w = fmaf(f, v[k].w, acc.w);
+                    }
+                }
+            }
+            __syncthreads();
+            sum[threadIdx.x] = acc;
+            __syncthreads();
+            if (g == 0 && o < outs) {
+                for (int k = 1; k < groups; ++k) {
+                    const float4 v = sum[k * outs + o];
+                    acc.x += v.x;
+                    acc.y += v.y;
+                    acc.z += v.z;
+                    acc.w += v.w;
+                }
+                const float l = total[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
+                fine = fine && (acc.x * 0.f + acc.y * 0.f + acc.z * 0.f + acc.w * 0.f) * inv == 0.f;
+                const int rr = left.row0 + row0 + r;
+                store4(op + static_cast<long>(left.q0 + rr / a.group) * a.out_stride + (left.head * a.group + rr % a.group) * HD + 4 * c,
+                       vec, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             }
         }
-        __syncthreads();
-        sum[threadIdx.x] = acc;
-        __syncthreads();
-        if (g == 0 && o < outs) {
-            for (int k = 1; k < groups; ++k) {
-                const float4 v = sum[k * outs + o];
-                acc.x += v.x;
-                acc.y += v.y;
-                acc.z += v.z;
-                acc.w += v.w;
-            }
-            const float l = total[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
-            const int rr = ti * ROWS + row0 + r;
-            store4(op + static_cast<long>(x.q0 + rr / a.group) * a.out_stride + (head * a.group + rr % a.group) * HD + 4 * c,
-                   vec, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-        }
+        // (also: the shared sums have been read)
+        if (__syncthreads_or(!fine)) again |= 1u << (w0 - blockIdx.x * EACH);
     }
+    for (; again; again &= again - 1) mend_rows<ROWS, HD, NT, E4M3, T>(a, blockIdx.x * EACH + __ffs(again) - 1, row0, sum);
 }
 
 // ---------------------------------------------------------------- launch --
@@ -1567,20 +1755,21 @@ cudaError_t allow_smem(K kernel, int bytes) {
 
 // The merge behind the kernel just launched, on the GPU early (programmatic
 // dependent launch): it waits there for the states.
-template <int ROWS, int HD, typename T>
+template <int ROWS, int HD, bool E4M3, typename T>
 cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.workers, ROWS / 16);
-    cfg.blockDim = dim3(256);
+    constexpr int NT = 256, EACH = ROWS == kDecRows ? 4 : 1;
+    cfg.gridDim = dim3((a.workers + EACH - 1) / EACH, ROWS / 16);
+    cfg.blockDim = dim3(NT);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, ijb_paged_merge_kernel<ROWS, HD, T>, a);
+    e = cudaLaunchKernelEx(&cfg, ijb_paged_merge_kernel<ROWS, HD, NT, EACH, E4M3, T>, a);
     count_launches(2);
     return e;
 }
@@ -1615,7 +1804,7 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.over = 1;
     a.least = 1;
     ijb_paged_decode_kernel<HD, E4M3, WIDE, T><<<sms, D::kWarps * 32, decode_smem<HD, E4M3, WIDE>(), s>>>(a);
-    return merge_launch<kDecRows, HD, T>(a, s);
+    return merge_launch<kDecRows, HD, E4M3, T>(a, s);
 }
 
 template <int HD, bool E4M3, typename T>
@@ -1633,7 +1822,7 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     a.over = 4;
     a.least = 2;
     ijb_paged_tile_kernel<HD, E4M3, T><<<sms, kTileThreads, L::kSmem, s>>>(a);
-    return merge_launch<kTileRows, HD, T>(a, s);
+    return merge_launch<kTileRows, HD, E4M3, T>(a, s);
 }
 
 // Which kernels serve a call.  Entries of up to 16 rows go to the decode kernel,
@@ -1660,7 +1849,7 @@ constexpr int kMaxWorkers = 16;  // per SM: the decode kernel's warps
 size_t workspace_bytes(int sms, int head_dim) {
     constexpr int rows = kTileRows > kMaxWorkers * kDecRows ? kTileRows : kMaxWorkers * kDecRows;
     // a word per worker, and two states each
-    return static_cast<size_t>(sms) * kMaxWorkers * sizeof(int4) + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
+    return static_cast<size_t>(sms) * kMaxWorkers * sizeof(Left) + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
 }
 
 template <int HD, bool E4M3>
@@ -1739,7 +1928,7 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         a.seq = seq_dev;
         a.kv_len = kv_len_dev;
         a.scale_log2 = scale * 1.4426950408889634f;
-        a.left = static_cast<int4 *>(workspace_dev);
+        a.left = static_cast<Left *>(workspace_dev);
         a.part = reinterpret_cast<float *>(a.left + sms * kMaxWorkers);
         a.status = status_dev;
         cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -158,3 +158,68 @@ def test_unknown_lengths(cuda, max_q):
                     [(1, 5)] * 12 + [(99, 99)] + [(2, 400)] * 6):
         check(cuda, entries, 2, 4, 64, 16, "f16", "float32", max_q=max_q)
         check(cuda, entries, 2, 4, 128, 16, "e4m3", "float16", max_q=max_q)
+
+
+@CACHES
+@TYPES
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_values_behind_a_token_do_not_reach_it(cuda, hd, cache, dtype, value):
+    """A K or V that is not finite at a later token's position changes no earlier token's output (an e4m3
+    cache holds no infinity); tokens that see it get no finite value where it stands."""
+    import torch
+    if cache == "e4m3" and value == float("inf"):
+        pytest.skip("e4m3 has no infinity")
+    for entries, at in (([(1, 40), (6, 50), (3, 3)], 47), ([(300, 700), (40, 40)], 560), ([(600, 600)], 1), ([(900, 5000)], 4999)):
+        e = 1 if len(entries) == 3 else 0
+        kv, q, clean = check(cuda, entries, 2, 2, hd, 16, cache, dtype, seed=11)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+        start, kv_len = np.cumsum([0] + [l for l, _ in entries]).tolist(), [t for _, t in entries]
+        page, off = int(kv.page_table[e, at // 16]), at % 16
+        first = start[e] + at - (kv_len[e] - entries[e][0])  # the token at that position
+        for which, head, dim in ((1, 0, 5), (0, 1, hd - 1)):
+            kept = kv.data[page, which, head, off].clone()
+            kv.data[page, which, head, off, dim] = value
+            got = kv.attention(q, i32(start), i32(kv_len), max_q=max(l for l, _ in entries))
+            kv.data[page, which, head, off] = kept
+            heads = slice(head * 2, head * 2 + 2)
+            sees = torch.zeros(got.shape[0], dtype=torch.bool, device=cuda)
+            sees[first:start[e + 1]] = True
+            assert torch.isfinite(got[~sees]).all()
+            tol = 4e-5 * 5 if dtype == "float32" else 2.0 ** -9 * 5  # both sums' own errors (see above)
+            assert float((got[~sees].double() - clean[~sees].double()).abs().max()) <= tol
+            if which == 1 or value != value:
+                bad = got[sees][:, heads, dim] if which == 1 else got[sees][:, heads]
+                assert not torch.isfinite(bad).any()
+            other = torch.ones(got.shape[1], dtype=torch.bool)
+            other[heads] = False
+            assert torch.equal(got[sees][:, other.to(cuda)], clean[sees][:, other.to(cuda)])
+        assert int(kv.status) == 0
+
+
+def test_entries_that_do_not_fit_are_left_and_reported(cuda):
+    """Bad starts, sequences and lengths, and an entry longer than max_q: unwritten and reported, the others computed."""
+    import torch
+    kv, q, clean = check(cuda, [(1, 30), (1, 31), (1, 32), (1, 33)], 2, 2, 64, 16, "f16", "float32")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    good = dict(start=[0, 1, 2, 3, 4], len=[30, 31, 32, 33], seq=[0, 1, 2, 3], max_q=1)
+    for name, row, value in (("len", 1, -1), ("len", 1, 16 * kv.page_table.shape[1] + 1), ("seq", 1, 4), ("seq", 1, -1)):
+        case = {k: list(v) if isinstance(v, list) else v for k, v in good.items()}
+        case[name][row] = value
+        out = torch.full_like(q, 9.0)
+        kv.status.zero_()
+        kv.attention(q, i32(case["start"]), i32(case["len"]), seq=i32(case["seq"]), max_q=1, out=out)
+        assert int(kv.status) != 0
+        # the work is cut elsewhere without the bad entry: each result is within 2e-5 max|v| of the exact one
+        assert torch.all(out[1] == 9.0) and float((out[[0, 2, 3]] - clean[[0, 2, 3]]).abs().max()) <= 4e-5 * 5
+    for start, left in (([0, 1, 2, 3, 5], [3]), ([0, 1, 2, 1, 4], [1, 2, 3]), ([-1, 1, 2, 3, 4], [0])):
+        out = torch.full_like(q, 9.0)
+        kv.status.zero_()
+        kv.attention(q, i32(start), i32(good["len"]), max_q=1, out=out)
+        assert int(kv.status) != 0
+        assert all(torch.all(out[r] == 9.0) for r in left if start != [0, 1, 2, 1, 4] or r == 2)
+    kv, q, clean = check(cuda, [(1, 30), (9, 31)], 1, 2, 64, 16, "f16", "float32")
+    out = torch.full_like(q, 9.0)
+    kv.status.zero_()
+    kv.attention(q, i32([0, 1, 10]), i32([30, 31]), max_q=2, out=out)
+    assert int(kv.status) != 0 and torch.all(out[1:] == 9.0) and float((out[:1] - clean[:1]).abs().max()) <= 4e-5 * 5
