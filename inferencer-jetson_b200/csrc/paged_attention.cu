@@ -73,6 +73,7 @@ struct AttnArgs {
     float scale_log2;        // scale * log2(e)
     Left *left;              // workspace: per worker, the tile it leaves to be gone on with
     float *part;             // workspace: two states per worker
+    float *held;             // workspace: the tile kernel's sums outside TMEM, a worker's 256 rows
     uint32_t *status;
 };
 
@@ -845,6 +846,13 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
 // most 256, which fp16 and the fp32 sums hold as exactly.  TMEM: S of both
 // tiles in columns 0..255, O in 256..511.
 //
+// The tensor cores' fp32 additions drop the bits that do not fit: each loses half
+// a unit of the last place of the sum so far, always towards zero, 4e-8 of O a
+// product step.  Over 23000 positions that was 1.5e-5 of an output, too much for
+// fp32 queries; so with those O is started anew every few blocks (kFlush) and
+// what it held is added, rounded to nearest, to sums kept in TMEM (head_dim 64,
+// where half of O's columns are free) or in the workspace (128).
+//
 // What bounds it: the exponentials (16 a clock and SM: 1024 clocks a tile and
 // block) beside the products (256 clocks at head_dim 64, 512 at 128, for each
 // of S and O; twice that for fp32 queries).
@@ -865,6 +873,8 @@ struct Tile {
     static constexpr int kFit = (227 * 1024 - 2048 - kQ) / kPart;
     static constexpr int kBufs = kFit > 8 ? 8 : kFit;
     static constexpr int kSmem = kQ + kBufs * kPart + 1024 + 512;
+    // blocks that O sums up before they are added to the sums outside
+    static constexpr int kFlush = kSplit ? 2 : 0;
     static_assert(kBufs >= 3, "a V block and the next K block are in use while another loads");
     static_assert(kBufs * kPart >= (kMaxEntries + kMaxTiles + 2) * 4, "the plan lies over the buffers");
 };
@@ -1128,7 +1138,7 @@ __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, 
 // one product in about 130 clocks, whatever its width, and two warps twice as
 // many: with one warp for both tiles the products of 128 columns (64 clocks)
 // waited for their issue.
-template <int HD, bool SPLIT, int BUFS>
+template <int HD, bool SPLIT, int BUFS, int FLUSH>
 __device__ void tile_mma(const AttnArgs &a, Cursor c, uint32_t q, uint32_t bufs, int part, TileCtl *ctl, uint32_t tmem, int t) {
     constexpr uint32_t kIdS = (1u << 4) | (kBlock / 8) << 17 | (128u / 16) << 24;
     constexpr uint32_t kIdO = (1u << 4) | 1u << 16 | (HD / 8) << 17 | (128u / 16) << 24;  // B is MN-major
@@ -1142,11 +1152,11 @@ __device__ void tile_mma(const AttnArgs &a, Cursor c, uint32_t q, uint32_t bufs,
     auto score = [&](int n) {  // S = Q K^T, by the elected lane
         const uint64_t qd = desc128(q, 16), kd = desc128(bufs + (n % BUFS) * part, 16);
 #pragma unroll
-        for (int h = 0; h < (SPLIT ? 2 : 1); ++h)
+        for (int h = SPLIT ? 1 : 0; h >= 0; --h)  // the small parts first: sums drop bits of their own size
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks) {
                 const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
-                mma_ss(ts, qd + off + h * (part >> 4), kd + off, kIdS, h > 0 || ks > 0);
+                mma_ss(ts, qd + off + h * (part >> 4), kd + off, kIdS, (SPLIT && h == 0) || ks > 0);
             }
         mma_commit(&ctl->s_full[t]);
     };
@@ -1170,10 +1180,11 @@ __device__ void tile_mma(const AttnArgs &a, Cursor c, uint32_t q, uint32_t bufs,
             const int vi = i + 2 * b + 1, ki = vi + 1;
             wait_full(vi);
             const uint64_t vd = desc128(bufs + (vi % BUFS) * part, kHalf);
+            const bool add = FLUSH ? b % (FLUSH ? FLUSH : 1) > 0 : b > 0;  // to what O holds
             auto value = [&](int k0) {  // O += P V over 64 positions
 #pragma unroll
                 for (int ks = k0; ks < k0 + 4; ++ks) {
-                    mma_ts(to, ts + ks * (SPLIT ? 16 : 8), vd + ks * (2048 >> 4), kIdO, b > 0 || ks > 0);
+                    mma_ts(to, ts + ks * (SPLIT ? 16 : 8), vd + ks * (2048 >> 4), kIdO, add || ks > 0);
                     if constexpr (SPLIT) mma_ts(to, ts + ks * 16 + 8, vd + ks * (2048 >> 4), kIdO, 1);
                 }
             };
@@ -1366,6 +1377,54 @@ __device__ __forceinline__ bool write_rows(uint32_t to, uint32_t st, O *dst, boo
     return zero == 0.f;
 }
 
+// Adds O (relative to the maximum m) to the row's sums outside it (relative to
+// held_m; with `more` they hold something), which become relative to m.  LAST: into
+// O, for the output.
+template <int HD, bool LAST>
+__device__ __forceinline__ void hold(uint32_t to, float *held, bool more, float held_m, float m, float sc) {
+    const float f = !more || held_m == -INFINITY ? 0.f : ex2((held_m - m) * sc);
+#pragma unroll 1
+    for (int k = 0; k < HD / 32; ++k) {
+        uint32_t x[32];
+        tm_ld32(to + 32 * k, x);
+        if constexpr (HD == 64) {
+            uint32_t y[32];
+            tm_ld32(to + 64 + 32 * k, y);
+            tm_wait(y);
+            tm_wait(x);
+            if (more) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    x[j] = __float_as_uint(fmaf(__uint_as_float(y[j]), f, __uint_as_float(x[j])));
+            }
+            tm_st32(to + (LAST ? 0 : 64) + 32 * k, x);
+        } else {
+            float4 y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                y[j] = more ? *reinterpret_cast<const float4 *>(held + (k * 8 + j) * 512) : make_float4(0.f, 0.f, 0.f, 0.f);
+            tm_wait(x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                y[j].x = fmaf(y[j].x, f, __uint_as_float(x[4 * j]));
+                y[j].y = fmaf(y[j].y, f, __uint_as_float(x[4 * j + 1]));
+                y[j].z = fmaf(y[j].z, f, __uint_as_float(x[4 * j + 2]));
+                y[j].w = fmaf(y[j].w, f, __uint_as_float(x[4 * j + 3]));
+                if constexpr (LAST) {
+                    x[4 * j] = __float_as_uint(y[j].x);
+                    x[4 * j + 1] = __float_as_uint(y[j].y);
+                    x[4 * j + 2] = __float_as_uint(y[j].z);
+                    x[4 * j + 3] = __float_as_uint(y[j].w);
+                } else {
+                    *reinterpret_cast<float4 *>(held + (k * 8 + j) * 512) = y[j];
+                }
+            }
+            if constexpr (LAST) tm_st32(to + 32 * k, x);
+        }
+    }
+    if constexpr (LAST || HD == 64) tm_wait_st();
+}
+
 // Softmax and output of tile t of a worker's runs (128 threads, row r of them).
 template <int HD, typename T>
 __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q, int part, TileCtl *ctl, uint32_t tmem, int t,
@@ -1444,9 +1503,19 @@ __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q
         const int limit = live ? s.x.kv - s.x.len + row / a.group : -1;  // last position this row sees
         const int all_see = s.x.kv - s.x.len + row0 / a.group;
         float m = -INFINITY, l = 0.f;  // maximum in units of the raw scores
+        constexpr int FLUSH = Tile<HD, T>::kFlush;
+        [[maybe_unused]] float held_m = -INFINITY;  // the maximum that the sums outside O go by
+        [[maybe_unused]] float *held = a.held + ((blockIdx.x * 2 + t) * static_cast<long>(HD / 4) * 128 + r) * 4;
         for (int b = s.b0; b < s.b1; ++b) {
             wait_bar(a, ctl, &ctl->s_full[t], blocks++ & 1);
             tc_after();
+            if constexpr (FLUSH > 0) {
+                const int n = b - s.b0;
+                if (n > 0 && n % FLUSH == 0) {
+                    hold<HD, false>(to, held, n > FLUSH, held_m, m, a.scale_log2);
+                    held_m = m;
+                }
+            }
             const int p0 = b * kBlock;
             if (p0 + kBlock - 1 > all_see) softmax_block<HD, SPLIT, true>(ts, a.scale_log2, limit - p0, &ctl->p_half[t], m, l);
             else softmax_block<HD, SPLIT, false>(ts, a.scale_log2, 0, &ctl->p_half[t], m, l);
@@ -1458,6 +1527,8 @@ __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q
         // ---- the run's end
         wait_bar(a, ctl, &ctl->o_full[t], runs++ & 1);
         tc_after();
+        if constexpr (FLUSH > 0)
+            if (s.b1 - s.b0 > FLUSH) hold<HD, true>(to, held, true, held_m, m, a.scale_log2);
         // O goes out by way of the queries' shared memory, idle now (128 bytes a row
         // and pass, 4 KB a warp), so that whole rows are written side by side
         const bool whole = s.b0 == 0 && s.b1 == s.units;
@@ -1530,7 +1601,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
     if (warp >= kMmaWarpId) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
         if (warp < kMmaWarpId + 2)
-            tile_mma<HD, L::kSplit, L::kBufs>(a, c, q, bufs, L::kPart, &ctl, tmem, warp - kMmaWarpId);
+            tile_mma<HD, L::kSplit, L::kBufs, L::kFlush>(a, c, q, bufs, L::kPart, &ctl, tmem, warp - kMmaWarpId);
     } else if (warp >= kLoadWarp0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
         tile_load<HD, E4M3, L::kBufs>(a, c, bufs, L::kPart, &ctl, threadIdx.x - kLoadWarp0 * 32);
@@ -1847,9 +1918,11 @@ cudaError_t attention_call(const AttnArgs &a, bool e4m3, int max_q, int sms, cud
 constexpr int kMaxWorkers = 16;  // per SM: the decode kernel's warps
 
 size_t workspace_bytes(int sms, int head_dim) {
-    constexpr int rows = kTileRows > kMaxWorkers * kDecRows ? kTileRows : kMaxWorkers * kDecRows;
+    constexpr int rows = kTileRows;
+    static_assert(kMaxWorkers * kDecRows <= kTileRows, "the decode kernel's states fit in the tile kernel's");
     // a word per worker, and two states each
-    return static_cast<size_t>(sms) * kMaxWorkers * sizeof(Left) + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
+    const size_t held = head_dim == 128 ? static_cast<size_t>(sms) * kTileRows * head_dim * sizeof(float) : 0;
+    return static_cast<size_t>(sms) * kMaxWorkers * sizeof(Left) + held + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
 }
 
 template <int HD, bool E4M3>
@@ -1930,6 +2003,7 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         a.scale_log2 = scale * 1.4426950408889634f;
         a.left = static_cast<Left *>(workspace_dev);
         a.part = reinterpret_cast<float *>(a.left + sms * kMaxWorkers);
+        a.held = a.part + static_cast<size_t>(sms) * 2 * kTileRows * (kv->head_dim + 2);
         a.status = status_dev;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const bool e4m3 = kv->type == IJB_KV_E4M3;
