@@ -1623,7 +1623,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
 // a later token's V reaches the earlier tokens that share its block.  The kernels
 // say when a value came out that way, and the merge then computes the rows of those
 // tiles again that do not see all of the positions read, one position at a
-// time: 16 rows a block, for the tiles that worker w begins.
+// time: RB rows a block, for the tiles that worker w begins.
 template <int HD, bool E4M3>
 __device__ __forceinline__ float cached(const AttnArgs &a, long row, int d) {
     if constexpr (E4M3) {
@@ -1634,7 +1634,7 @@ __device__ __forceinline__ float cached(const AttnArgs &a, long row, int d) {
         return __half2float(reinterpret_cast<const __half *>(a.kv.data)[row * HD + d]);
     }
 }
-template <int ROWS, int HD, int NT, bool E4M3, typename T>
+template <int ROWS, int HD, int NT, int RB, bool E4M3, typename T>
 __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float4 *shared) {
     float *weight = reinterpret_cast<float *>(shared), *red = weight + NT;  // 4 * NT floats are there
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1643,7 +1643,7 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float
     while (cursor_next(a, c, s)) {
         if (s.b0 > 0) continue;
         const int end = static_cast<int>(min(static_cast<long>(s.x.kv), static_cast<long>(s.units) * a.unit));  // read
-        for (int r = s.ti * ROWS + row0; r < min(s.x.rows, s.ti * ROWS + row0 + 16); ++r) {
+        for (int r = s.ti * ROWS + row0; r < min(s.x.rows, min((s.ti + 1) * ROWS, s.ti * ROWS + row0 + RB)); ++r) {
             const int tok = r / a.group, h = s.head * a.group + r % a.group;
             const int n = s.x.kv - s.x.len + tok + 1;  // positions it sees
             if (n <= 0 || n >= end) continue;
@@ -1690,30 +1690,33 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float
     }
 }
 
-// Joins the states of the tiles that EACH workers left (few leave one): 16 rows of
-// them a block of NT threads.  A thread has 4 dims of a row over some of the states, whose values it
-// loads (kMergeBatch at a time) before the row's maximum and sum are there.
+// Joins the states of the tiles that EACH workers left (few leave one): RB rows of
+// them a block of NT threads.  A thread has 4 dims of a row over some of the states,
+// whose values it loads (kMergeBatch at a time) before the row's maximum and sum are
+// there.  Bound by the latency of its few rounds of loads, so the decode kernel, which
+// may leave hundreds of states of a few rows, spreads them: two contexts of 39,000
+// positions, 12 rows of 128 each, took 25, 30, 39 and 80 us in all with 1, 2, 4 and 16
+// rows a block, and 64 ragged sequences 27, 25, 25 and 27 us.
 constexpr int kMergeBatch = 4;
-template <int ROWS, int HD, int NT, int EACH, bool E4M3, typename T>
+template <int ROWS, int HD, int NT, int EACH, int RB, bool E4M3, typename T>
 __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_constant__ AttnArgs a) {
-    __shared__ float top[16], total[16];
+    __shared__ float top[RB], total[RB];
     __shared__ float4 sum[NT];
-    const int row0 = blockIdx.y * 16;
+    const int row0 = blockIdx.y * RB;
     pdl_wait();
-    uint32_t some = 0, again = 0;  // bit j: worker j of this block's left a tile; has rows to look at again
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-        const int w = blockIdx.x * EACH + j;
-        if (w < a.workers) {
-            const int4 x = *reinterpret_cast<const int4 *>(&a.left[w].states), y = *reinterpret_cast<const int4 *>(&a.left[w].head);
-            some |= x.x > 0 ? 1u << j : 0u;
-            again |= y.y != 0 ? 1u << j : 0u;
-        }
+    uint32_t some, again;  // bit j: worker j of this block's left a tile; has rows to look at again
+    {
+        static_assert(EACH <= 32, "a lane a worker");
+        const int j = threadIdx.x & 31, w = blockIdx.x * EACH + j;
+        const bool in = j < EACH && w < a.workers;
+        const int4 x = in ? *reinterpret_cast<const int4 *>(&a.left[w].states) : make_int4(0, 0, 0, 0);
+        some = __ballot_sync(0xffffffffu, x.x > 0 && x.w > row0);
+        again = __ballot_sync(0xffffffffu, in && a.left[w].bad != 0);
     }
     for (; some; some &= some - 1) {
         const int w0 = blockIdx.x * EACH + __ffs(some) - 1;
         const Left left = a.left[w0];
-        const int n = left.states, rows = min(16, left.rows - row0);
+        const int n = left.states, rows = min(RB, left.rows - row0);
         if (rows <= 0) continue;
         constexpr long PF = part_floats<ROWS, HD>();
         auto part = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0 ? 1 : 0)) * PF; };
@@ -1792,7 +1795,7 @@ __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_consta
         // (also: the shared sums have been read)
         if (__syncthreads_or(!fine)) again |= 1u << (w0 - blockIdx.x * EACH);
     }
-    for (; again; again &= again - 1) mend_rows<ROWS, HD, NT, E4M3, T>(a, blockIdx.x * EACH + __ffs(again) - 1, row0, sum);
+    for (; again; again &= again - 1) mend_rows<ROWS, HD, NT, RB, E4M3, T>(a, blockIdx.x * EACH + __ffs(again) - 1, row0, sum);
 }
 
 // ---------------------------------------------------------------- launch --
@@ -1831,8 +1834,9 @@ cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    constexpr int NT = 256, EACH = ROWS == kDecRows ? 4 : 1;
-    cfg.gridDim = dim3((a.workers + EACH - 1) / EACH, ROWS / 16);
+    constexpr int NT = 256, EACH = ROWS == kDecRows ? 8 : 1, RB = ROWS == kDecRows ? 2 : 16;
+    const int rows = min(a.tile_rows, a.max_rows);
+    cfg.gridDim = dim3((a.workers + EACH - 1) / EACH, (rows + RB - 1) / RB);
     cfg.blockDim = dim3(NT);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -1840,7 +1844,7 @@ cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, ijb_paged_merge_kernel<ROWS, HD, NT, EACH, E4M3, T>, a);
+    e = cudaLaunchKernelEx(&cfg, ijb_paged_merge_kernel<ROWS, HD, NT, EACH, RB, E4M3, T>, a);
     count_launches(2);
     return e;
 }
