@@ -978,7 +978,18 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
         e->max_pages_per_seq = (d.context + d.page_size - 1) / d.page_size;
         e->num_pages = d.num_pages > 0 ? d.num_pages : static_cast<long>(d.max_seqs) * e->max_pages_per_seq;
         e->page_stride = 2L * d.kv_heads * d.page_size * e->head_dim;
-        if (e->paged >= 0) d.kv_f32 = e->paged == IJB_KV_E4M3;  // what the projection writes
+        if (e->paged >= 0) {  // what the paged operators would refuse at the first step
+            ijb_kv_view v = layer_view(e.get(), 0);
+            alignas(16) static uint8_t none[16];  // for the pointers: the pool is not there yet
+            v.data_dev = v.scale_dev = none;
+            v.page_table_dev = reinterpret_cast<const int *>(none);
+            KvDev kv;
+            const std::string bad = kv_view_check(&v, &kv);
+            require(bad.empty(), "paged attention: " + bad);
+            require(d.heads / d.kv_heads <= 16, "paged attention: heads must be 1 to 16 times kv_heads");
+            require(d.max_batch <= 4096, "max_batch must be <= 4096 with a paged attention cache type");
+            d.kv_f32 = e->paged == IJB_KV_E4M3;  // what the projection writes
+        }
         e->kv_f32 = d.kv_f32 ? 1 : 0;
         e->kv_elem = e->kv_f32 ? 4 : 2;
         e->pool_elem = e->paged == IJB_KV_E4M3 ? 1 : e->kv_elem;
@@ -1037,8 +1048,6 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
         if (e->paged >= 0) {
             const ijb_kv_view v = layer_view(e.get(), 0);
             e->paged_work_bytes = ijb_paged_attention_workspace(&v);
-            require(e->paged_work_bytes > 0, "paged attention: " + t_create_err);
-            require(d.max_batch <= 4096, "max_batch must be <= 4096 with a paged attention cache type");
             e->paged_work = dev_alloc<uint8_t>(e->paged_work_bytes, "paged attention workspace");
             ck(paged_attention_prepare(e->head_dim, e->paged == IJB_KV_E4M3), "paged attention attributes");
         }

@@ -5,6 +5,8 @@ With an fp16 pool both engines cache the same rows and attend over them to fp32 
 so on the FP32 activation path logits agree to the project's bar for two summation orders
 (rel-L2 1e-2; about 1e-3 is seen between paths).  An e4m3 pool rounds every cached value by up to 2^-4 of
 itself (1.8 % rms): logits are held to 2 * 2^-4."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -146,11 +148,19 @@ def test_timing_helpers_on_a_paged_engine(cuda):
         e.seq_prefill(s, synth.prompt_tokens(10 + i, seed=i, vocab_limit=cfg.vocab))
     ms, kv_bytes = e.time_layer_attention(seqs, reps=3)
     assert ms > 0 and kv_bytes == 33 * cfg.kv_heads * 2 * (cfg.head_dim + 1)
+    out = ctypes.c_float()
+    assert e.lib.ijb_time_layer_projections(e.h, 8, 3, ctypes.byref(out)) == lib.OK and out.value > 0
+    want = e.decode_step(seqs, [1, 2, 3])
+    f = Engine(cfg, synth.make_model(cfg, seed=3), context=96, max_batch=16, max_seqs=4, kv_type="e4m3")
+    again = [f.seq_open() for _ in range(3)]
+    for i, s in enumerate(again):
+        f.seq_prefill(s, synth.prompt_tokens(10 + i, seed=i, vocab_limit=cfg.vocab))
+    np.testing.assert_array_equal(f.decode_step(again, [1, 2, 3]), want)  # the timing left no trace
     e.close()
+    f.close()
 
 
 def test_create_kv_refuses_other_types(cuda):
-    import ctypes
     L = lib.load()
     h = ctypes.c_void_p()
     d = lib.ModelDesc()
@@ -158,3 +168,14 @@ def test_create_kv_refuses_other_types(cuda):
     for t in (-1, 1, 3):
         assert L.ijb_create_kv(ctypes.byref(d), views, 0, t, ctypes.byref(h)) == lib.ERR_INVALID
         assert "cache type" in L.ijb_last_error(None).decode()
+
+
+@pytest.mark.parametrize("kw,what", [(dict(page_size=12), "page_size"), (dict(max_batch=4097), "4096"),
+                                     (dict(max_batch=64, kv_heads=1), "heads")])
+def test_create_kv_refuses_what_its_attention_would(cuda, kw, what):
+    cfg = synth.TINY
+    if "kv_heads" in kw:
+        kw.pop("kv_heads")
+        cfg = synth.ModelConfig("mqa", dim=32 * 64, layers=1, heads=32, kv_heads=1, hidden=256, vocab=512)
+    with pytest.raises(lib.IjbError, match=what):
+        Engine(cfg, synth.make_model(cfg, seed=3), kv_type="f16", **dict(dict(context=96, max_batch=4, max_seqs=4), **kw))
