@@ -361,7 +361,8 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * whose K and V, the new tokens' included, the cache already holds.  A token
  * sees the positions up to its own, with softmax(scale * q . k), scale > 0; one before
  * position 0 (kv_len shorter than the entry) sees none and gets zeros.  Entries
- * may be empty; rows that belong to no entry are left as they were.  max_q > 0
+ * may be empty; rows that belong to no entry are left as they were.  The starts
+ * must not fall, and out_dev must not overlap q_dev.  max_q > 0
  * promises that no entry has more new tokens (0: unknown): a longer one may be
  * left unwritten and is reported.
  *

@@ -198,7 +198,9 @@ __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po
         }
         if (threadIdx.x == 0) first[a.n_entries] = base;
         __syncthreads();
-        const int tiles = min(base, kMaxTiles);
+        // more tiles than the call's tokens have: starts that fall, whose entries overlap
+        if (base > kMaxTiles && lead && threadIdx.x == 0 && a.status) atomicOr(a.status, kDevErrBadIndex);
+        const int tiles = base > kMaxTiles ? 0 : base;
         base = 0;
         for (int t0 = 0; t0 < tiles; t0 += NT) {
             const int t = t0 + static_cast<int>(threadIdx.x);
@@ -1980,6 +1982,7 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         if (!(scale > 0.f && scale <= 3.402823466e38f)) return kv_fail(IJB_ERR_INVALID, fn, "scale must be positive and finite");
         if (!q_dev || !out_dev || !q_start_dev || !kv_len_dev || !workspace_dev)
             return kv_fail(IJB_ERR_INVALID, fn, "null argument");
+        if (q_dev == out_dev) return kv_fail(IJB_ERR_INVALID, fn, "the output must not lie over the queries");
         const int elem = type == IJB_TYPE_F32 ? 4 : 2;
         const long row = static_cast<long>(heads) * kv->head_dim;
         if (q_stride < row || out_stride < row) return kv_fail(IJB_ERR_INVALID, fn, "a stride is shorter than a token's row");
@@ -1989,6 +1992,11 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
             return kv_fail(IJB_ERR_INVALID, fn, "the workspace must be 16-byte aligned");
         if (static_cast<long>(n_tokens) * (heads / kv->kv_heads) / kTileRows + n_entries > kMaxTiles)
             return kv_fail(IJB_ERR_INVALID, fn, "too many rows for one call");
+        // the plan counts units of one KV head, and a worker's units of all, in 32 bits
+        const long positions = static_cast<long>(kv->max_pages) * kv->page_size;
+        const long units = max(n_entries * (positions / kChunk + 2), kMaxTiles * (positions / kBlock + 5));
+        if (units > 0x7fffffffL || units * kv->kv_heads / 64 > 0x7fffffffL)
+            return kv_fail(IJB_ERR_INVALID, fn, "max_pages * page_size is too large for this many entries and heads");
         const int sms = sm_count();
         if (sms < 1) return kv_fail(IJB_ERR_CUDA, fn, "no CUDA device");
         if (workspace_size < workspace_bytes(sms, kv->head_dim))

@@ -77,7 +77,7 @@ class PagedKV:
         _need(not e4m3 or scale is not None and scale.dtype == torch.uint8 and scale.shape == data.shape[:4] and
               scale.is_contiguous() and scale.get_device() == dev,
               "scale: an e4m3 cache needs contiguous uint8 [pages, 2, kv_heads, page_size] beside data")
-        _need(status is None or status.element_size() == 4 and status.numel() == 1 and status.get_device() == dev,
+        _need(status is None or status.dtype in (torch.int32, torch.uint32) and status.numel() == 1 and status.get_device() == dev,
               "status: expected one 32-bit word beside data")
         self.data, self.page_table, self.scale, self.status = data, page_table, scale if e4m3 else None, status
         self.device, self.kv_heads, self.head_dim = dev, data.shape[2], data.shape[4]

@@ -233,6 +233,12 @@ def test_entries_that_do_not_fit_are_left_and_reported(cuda):
         kv.attention(q, i32(start), i32(good["len"]), max_q=1, out=out)
         assert int(kv.status) != 0
         assert torch.all(out[left] == 9.0) and torch.all(out[1:3] != 9.0)
+    # starts that fall again and again: more tiles than tokens, none computed
+    kv, q, clean = check(cuda, [(520, 530)] + [(1, 9)] * 9, 2, 4, 64, 16, "f16", "float32")
+    out = torch.full_like(q, 9.0)
+    kv.status.zero_()
+    kv.attention(q, i32([0, 520] * 2048 + [0]), i32([530] * 4096), seq=i32([0] * 4096), out=out)
+    assert int(kv.status) != 0 and torch.all(out == 9.0)
     kv, q, clean = check(cuda, [(1, 30), (9, 31)], 1, 2, 64, 16, "f16", "float32")
     out = torch.full_like(q, 9.0)
     kv.status.zero_()

@@ -179,3 +179,24 @@ def test_sample_same_row_in_any_batch_stream_and_graph(cuda):
     torch.cuda.synchronize()
     want_t, want_p = ops.sample(x, u, t, None, p)
     assert torch.equal(g_t, want_t) and torch.equal(g_p, want_p)
+
+
+def test_quotient_is_rounded_to_nearest(cuda):
+    """The operator forms (x - m) / T from 1 / T and one residual correction; a division gives the same.  For
+    quotients t in [-15, -8] a wrong last bit is 2^-20 and moves exp(t) by 2^-20 of itself; expf is good to two
+    units in the last place, 2^-22, and min_p's own rounding is 2^-24.  So with min_p at exp(t) (1 -+ 2^-21) the
+    token of weight exp(t) is kept and dropped."""
+    import torch
+    from ijb200 import ops
+    n = 1 << 16
+    rng = np.random.default_rng(5)
+    T = np.exp(rng.uniform(np.log(1e-3), np.log(1e3), n)).astype(np.float32)
+    d = (rng.uniform(8.01, 15.0, n) * T).astype(np.float32)
+    dT, dd = torch.from_numpy(T).to(cuda), torch.from_numpy(-d).to(cuda)
+    t = (dd / dT).double()  # CUDA's division, in fp32
+    x = torch.zeros((n, 2), dtype=torch.float32, device=cuda)
+    x[:, 1] = dd
+    u = torch.full((n,), 1 - 2.0 ** -24, dtype=torch.float32, device=cuda)  # the last token kept
+    for sign in (-1, 1):
+        token, _ = ops.sample(x, u, dT, None, None, (torch.exp(t) * (1 + sign * 2.0 ** -21)).float())
+        assert int((token != (0 if sign > 0 else 1)).sum()) == 0

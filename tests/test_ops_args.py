@@ -59,7 +59,7 @@ def test_sample_arguments_are_checked(args):
     assert "ijb_sample" in L.ijb_last_error(None).decode()
 
 
-def attention(v, heads=4, type_=0, q=4096, qs=256, out=4096, os=256, n=2, e=1, start=256, kv_len=256, work=4096,
+def attention(v, heads=4, type_=0, q=4096, qs=256, out=8192, os=256, n=2, e=1, start=256, kv_len=256, work=4096,
               size=1 << 40):
     return lib.load().ijb_paged_attention(ctypes.byref(v), heads, type_, q, qs, out, os, n, e, start, None, kv_len, 1,
                                           0.125, work, size, None, None)
@@ -74,9 +74,15 @@ def test_attention_views_are_checked(bad):
 @pytest.mark.parametrize("bad", [dict(heads=3), dict(heads=0), dict(heads=34), dict(type_=12), dict(q=None),
                                  dict(out=None), dict(start=None), dict(kv_len=None), dict(work=None), dict(qs=255),
                                  dict(os=255), dict(n=-1), dict(e=0), dict(e=4097), dict(q=4097), dict(type_=1, out=4097),
-                                 dict(work=4100), dict(n=1 << 30)])
+                                 dict(work=4100), dict(n=1 << 30), dict(out=4096)])
 def test_attention_arguments_are_checked(bad):
     assert attention(view(), **bad) == lib.ERR_INVALID
+
+
+def test_attention_refuses_more_units_of_work_than_it_counts():
+    wide = view(page_size=256, max_pages=1 << 22)
+    assert attention(wide) == lib.ERR_INVALID and attention(wide, e=4096) == lib.ERR_INVALID
+    assert "too large" in lib.load().ijb_last_error(None).decode()
 
 
 def test_attention_without_tokens_is_no_launch():
