@@ -1246,6 +1246,13 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
     return p;
 }
 
+// The larger, or NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+
 // One row's 128 scores (TMEM columns of ts) become its weights there; m and l
 // are the row's maximum and sum.  MASK: only columns 0..seen count.
 constexpr int kMufuPairs = 6;  // of 8 pairs, on the exponential unit
@@ -1263,10 +1270,12 @@ __device__ __forceinline__ void softmax_block(uint32_t ts, float sc, int seen, u
         for (int j = 0; j < 32; ++j) {
             float v = __uint_as_float(x[k & 1][j]);
             if (MASK) v = 32 * k + j <= seen ? v : -INFINITY;
-            mx4[j & 3] = fmaxf(mx4[j & 3], v);
+            mx4[j & 3] = max_nan(mx4[j & 3], v);
         }
     }
-    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+    float mx = max_nan(max_nan(mx4[0], mx4[1]), max_nan(mx4[2], mx4[3]));
+    // a score of NaN or infinity makes the row NaN by its maximum: ex2_poly gives such a pair no weight
+    if (!(mx < INFINITY)) m = mx = NAN;
     const bool raise = m != -INFINITY && mx * sc > m * sc + kRaise;
     if (__any_sync(0xffffffffu, raise)) {
         const float alpha = raise ? ex2((m - mx) * sc) : 1.f;
@@ -1648,7 +1657,7 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float
         for (int r = s.ti * ROWS + row0; r < min(s.x.rows, min((s.ti + 1) * ROWS, s.ti * ROWS + row0 + RB)); ++r) {
             const int tok = r / a.group, h = s.head * a.group + r % a.group;
             const int n = s.x.kv - s.x.len + tok + 1;  // positions it sees
-            if (n <= 0 || n >= end) continue;
+            if (n >= end) continue;
             const T *q = static_cast<const T *>(a.q) + static_cast<long>(s.x.q0 + tok) * a.q_stride + h * HD;
             T *out = static_cast<T *>(a.out) + static_cast<long>(s.x.q0 + tok) * a.out_stride + h * HD;
             const float now = tid < HD ? static_cast<float>(out[tid]) : 0.f;

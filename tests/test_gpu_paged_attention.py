@@ -212,6 +212,43 @@ def test_values_behind_a_token_do_not_reach_it(cuda, hd, cache, dtype, value):
         assert int(kv.status) == 0
 
 
+@CACHES
+@TYPES
+@pytest.mark.parametrize("entry", [(5, 3), (300, 40)])
+def test_values_that_are_not_finite_and_rows_that_see_nothing(cuda, entry, cache, dtype):
+    """Tokens before position 0 get zeros whatever V holds at the positions there are."""
+    import torch
+    kv, q, clean = check(cuda, [entry], 2, 2, 64, 16, cache, dtype, seed=4)
+    kv.data[int(kv.page_table[0, 0]), 1, :, 0, 3] = float("nan")
+    got = kv.attention(q, torch.tensor([0, entry[0]], dtype=torch.int32, device=cuda),
+                       torch.tensor([entry[1]], dtype=torch.int32, device=cuda))
+    none = entry[0] - entry[1]
+    assert torch.all(got[:none] == 0) and torch.all(got[none:, :, 3].isnan())
+
+
+@TYPES
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_scores_that_are_not_finite(cuda, hd, dtype, value):
+    """A score of NaN or +infinity at any position, in the first block of an entry or a later one, leaves no finite
+    value in the rows that see it."""
+    import torch
+    kv, q, clean = check(cuda, [(200, 500)], 1, 2, hd, 16, "f16", dtype, seed=5)
+    for at in [*range(16), 301, 318, 319, 400, 415]:
+        page, off = int(kv.page_table[0, at // 16]), at % 16
+        kept = kv.data[page, 0, 0, off, 0].clone()
+        kv.data[page, 0, 0, off, 0] = value
+        got = kv.attention(q, torch.tensor([0, 200], dtype=torch.int32, device=cuda),
+                           torch.tensor([500], dtype=torch.int32, device=cuda))
+        kv.data[page, 0, 0, off, 0] = kept
+        hit = torch.arange(300, 500, device=cuda).unsqueeze(1) >= at
+        hit = hit & (q[:, :, 0] > 0) if value > 0 else hit.expand(200, 2)
+        assert not torch.isfinite(got[hit]).any(), at
+        rest = torch.arange(300, 500, device=cuda) < at
+        tol = 4e-5 * 5 if dtype == "float32" else 2.0 ** -9 * 5
+        assert rest.sum() == 0 or float((got[rest].double() - clean[rest].double()).abs().max()) <= tol
+
+
 def test_entries_that_do_not_fit_are_left_and_reported(cuda):
     """Bad starts, sequences and lengths, and an entry longer than max_q: unwritten and reported, the others computed."""
     import torch
