@@ -360,14 +360,16 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * the last of the kv_len_dev[e] positions of sequence seq_dev[e] (NULL: e),
  * whose K and V, the new tokens' included, the cache already holds.  A token
  * sees the positions up to its own, with softmax(scale * q . k), scale > 0; one before
- * position 0 (kv_len shorter than the entry) sees none and gets zeros.  Entries
+ * position 0 (kv_len shorter than the entry) sees none and gets zeros, as does
+ * one whose scores are all -infinity.  n_tokens * heads / kv_heads / 256 + n_entries
+ * may not pass 8192: longer prompts are cut into several calls.  Entries
  * may be empty; rows that belong to no entry are left as they were.  The starts
  * must not fall, and out_dev must not overlap q_dev.  max_q > 0
  * promises that no entry has more new tokens (0: unknown): a longer one may be
  * left unwritten and is reported.
  *
  * fp32 queries and probabilities enter the products as two fp16 parts each
- * (22 bits); fp16 queries as they are, their probabilities rounded to fp16.
+ * (22 bits; queries up to 65504); fp16 queries as they are, their probabilities rounded to fp16.
  * e4m3 rows enter as fp16, exactly while the largest value of a row is within
  * 2^-7 .. 2^15.  Sums, maxima and the softmax are fp32.  The result is the same
  * every time for the same call, but how an entry's positions are cut into
