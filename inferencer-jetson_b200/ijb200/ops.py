@@ -108,8 +108,8 @@ class PagedKV:
         Rows of entries that are skipped (a negative position) hold no meaning."""
         _need(dtype in _TYPE, "dtype must be float32 or float16")
         n = seq.numel()
-        shape = (n, self.kv_heads, self.head_dim)
-        k, v = (_empty(shape, dtype=dtype, device=self.data.device) for _ in range(2))
+        k = _empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self.data.device)
+        v = torch.empty_like(k)
         _call(self.device, self._lib.ijb_kv_gather, self._ref, _TYPE[dtype], k.data_ptr(), v.data_ptr(), self.row, n,
               _ptr(seq, torch.int32, n, self.device, "seq"), _ptr(pos, torch.int32, n, self.device, "pos"), self._status)
         return k, v
