@@ -67,3 +67,44 @@ def test_steps_of_write_attend_sample(cuda, hd):
         again, again_p = ops.sample(logits, st["u"], t, None, p)
         assert torch.equal(token, again) and torch.equal(prob, again_p)
     assert int(status) == 0
+
+
+def test_calls_on_several_streams_at_once(cuda):
+    """A ragged call of single tokens, a prompt's attention, a write elsewhere and sampling, each on its own stream,
+    give what each gives alone, bit for bit."""
+    import torch
+    from ijb200 import ops
+    g = torch.Generator(device=cuda)
+    g.manual_seed(3)
+    kvh, heads, hd, page, seqs, width = 2, 8, 128, 16, 8, 64
+    rand = lambda *s: torch.randn(s, generator=g, device=cuda)  # noqa: E731
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    data = rand(seqs * width, 2, kvh, page, hd).half()
+    table = torch.randperm(seqs * width, generator=g, device=cuda).view(seqs, width).int()
+    kv = ops.PagedKV(data, table)
+    other = ops.PagedKV(torch.zeros_like(data), table)
+    one, lens = rand(seqs, heads, hd), i32([1, 1000, 17, 512, 1024, 3, 700, 900])
+    ones = i32(list(range(seqs + 1)))
+    prompt, p_start, p_len = rand(800, heads, hd).half(), i32([0, 500, 800]), i32([900, 300])
+    rows, r_pos, r_seq = rand(1024, kvh, hd), i32(list(range(1024))), i32([2] * 1024)
+    logits, u = rand(40, 50000) * 3, torch.rand((40,), generator=g, device=cuda)
+    k40, p90 = torch.full((40,), 40, dtype=torch.int32, device=cuda), torch.full((40,), 0.9, device=cuda)
+
+    def write():
+        other.append(rows, rows, r_seq, r_pos)
+        return other.gather(r_seq, r_pos)[0]
+
+    calls = [lambda: kv.attention(one, ones, lens, max_q=1), lambda: kv.attention(prompt, p_start, p_len), write,
+             lambda: ops.sample(logits, u, None, k40, p90)[0]]
+    alone = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for _ in range(10):
+        for f, s, out in zip(calls, streams, got):
+            with torch.cuda.stream(s):
+                out.append(f())
+    torch.cuda.synchronize()
+    for want, outs in zip(alone, got):
+        for x in outs:
+            assert torch.equal(x, want)
