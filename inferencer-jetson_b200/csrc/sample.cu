@@ -630,6 +630,9 @@ struct Leader {
             } else {  // kEqualDone, kCut
                 if (step == kDraw) return false;
                 kept = s.ctl.cut_mass;
+                // The next cut writes it: over a list already in order that is without another
+                // barrier on the way (no masses to search, nothing to put in order).
+                __syncthreads();
                 ++step;
                 phase = kBegin;
             }

@@ -200,3 +200,32 @@ def test_quotient_is_rounded_to_nearest(cuda):
     for sign in (-1, 1):
         token, _ = ops.sample(x, u, dT, None, None, (torch.exp(t) * (1 + sign * 2.0 ** -21)).float())
         assert int((token != (0 if sign > 0 else 1)).sum()) == 0
+
+
+def test_sample_cuts_one_after_another(cuda):
+    """A short top-k list serves the cuts behind it as it stands in shared memory: each has to be read by all threads
+    before the next one is written, which only a barrier there gives (repeated runs show its absence rarely).  The
+    same batch many times beside other work, each run against the definition."""
+    import torch
+    from ijb200 import ops
+    n, vocab = 48, 9001
+    g = torch.Generator(device=cuda)
+    g.manual_seed(12)
+    x = torch.randn((n, vocab), generator=g, device=cuda) * 2.5
+    u = torch.rand((n,), generator=g, device=cuda)
+    t, p, m = torch.full((n,), 0.7, device=cuda), torch.full((n,), 0.95, device=cuda), torch.zeros((n,), device=cuda)
+    k = torch.tensor([40, 1, 2, 64, 100, 120], dtype=torch.int32, device=cuda).repeat(8)
+    p[1::2] = torch.linspace(0.05, 0.999, n // 2, device=cuda)
+    m[::3] = 0.02
+    want_t, want_p = plain(x, u.tolist(), t.tolist(), k.tolist(), p.tolist(), m.tolist())
+    a = torch.randn((2048, 2048), device=cuda)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(60):
+            a = torch.tanh(a @ a)
+    tokens, probs = zip(*[ops.sample(x, u, t, k, p, m) for _ in range(400)])
+    torch.cuda.synchronize()
+    for token, prob in zip(tokens, probs):
+        np.testing.assert_array_equal(token.cpu().numpy(), want_t)
+        np.testing.assert_allclose(prob.cpu().numpy(), want_p, rtol=2.0 ** -23, atol=0)
