@@ -369,9 +369,11 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * left unwritten and is reported.
  *
  * fp32 queries and probabilities enter the products as two fp16 parts each
- * (22 bits; queries up to 65504); fp16 queries as they are, their probabilities rounded to fp16.
- * e4m3 rows enter as fp16, exactly while the largest value of a row is within
- * 2^-7 .. 2^15.  Sums, maxima and the softmax are fp32.  The result is the same
+ * (22 bits, but no finer than 2^-25; queries up to 65504); fp16 queries as they are, their
+ * probabilities rounded to fp16.  e4m3 values enter as the nearest fp16 number, as an fp16
+ * cache would hold them: those of a row whose largest is within 2^-7 .. 2^15 exactly, smaller ones
+ * off by 2^-25 at most; those of 65520 and more may come out as infinities.  Sums,
+ * maxima and the softmax are fp32.  The result is the same
  * every time for the same call, but how an entry's positions are cut into
  * partial sums depends on the whole call.
  *

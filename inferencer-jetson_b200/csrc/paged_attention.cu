@@ -26,8 +26,10 @@
 // Arithmetic.  Products are fp16 x fp16 with fp32 sums.  fp32 queries enter as
 // two fp16 parts (hi + lo, 22 bits), and so do their probabilities; fp16
 // queries enter as they are, their probabilities rounded to fp16 once (the
-// output is fp16 too).  Cached rows enter as fp16: fp16 rows exactly, e4m3 rows as
-// code * 2^e, exact while a row's largest value is in [2^-7, 2^15].
+// output is fp16 too).  Cached rows enter as fp16: fp16 rows exactly, e4m3 values as the
+// fp16 number nearest to code * 2^e, as an fp16 cache would hold them: exactly from 2^-14 on (and
+// every value of a row whose largest is in [2^-7, 2^15]), else off by 2^-25 at most, infinite from
+// 65520 on.  (The decode kernel scales its scores in fp32, so K has no such ends there.)
 #include <mutex>
 #include <type_traits>
 
@@ -391,8 +393,17 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-// 2^(s - 127) as fp16, at most 2^15 (a code of 0 must stay 0).
-__device__ __forceinline__ __half scale_half(uint32_t s) { return __float2half_rn(fminf(kv_scale(s), 32768.f)); }
+// A row's scale 2^(s - 127) as factors for its codes.  2^-24 .. 2^15 are fp16 numbers, so that
+// one product is code * scale, rounded once.  Beyond that (no row of a model at work) there are
+// two: 2^-15 or 2^15, whose product with a code is exact or infinite, and the rest, kept to what
+// leaves 0 or infinity as it is: past 2^-39 all is 0, and past 2^30 all but 0 infinite.
+__device__ __forceinline__ bool scale_fits(uint32_t s) { return s - 103u <= 39u; }
+__device__ __forceinline__ __half scale_half(uint32_t s) {
+    return __float2half_rn(kv_scale(s < 103u ? 112u : min(s, 142u)));
+}
+__device__ __forceinline__ float scale_rest(uint32_t s) {
+    return kv_scale(scale_fits(s) ? 127u : s < 103u ? max(s, 88u) + 15u : min(s, 157u) - 15u);
+}
 // Page id of a position, in bounds whatever the table holds; a bad one is reported.
 __device__ __forceinline__ long page_of(const AttnArgs &a, int seq, int pos) {
     const int page = a.kv.page_table[static_cast<long>(seq) * a.kv.max_pages + (pos >> a.kv.page_shift)];
@@ -659,13 +670,17 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
             const int p0 = b * kChunk;
             float kscale[8];         // of positions t4 + 4 i
             uint32_t vscale[4];      // fp16, of positions t4 + 8 i and t4 + 8 i + 4
+            bool far = false;        // some need a second factor
             if constexpr (E4M3) {
                 // lane r turns position r's scale bytes into numbers, kept so that a lane reads
                 // its eight positions' side by side; those behind the last mean nothing
                 const bool in = p0 + lane < s.x.kv;
                 const int at = (lane & 3) * 8 + (lane >> 2);
                 const float ks = in ? kv_scale(lds8(sc + lane)) : 0.f;
-                const __half vs = in ? scale_half(lds8(sc + 32 + lane)) : __half(0.f);
+                const uint32_t vbyte = lds8(sc + 32 + lane);
+                __half vs = in ? __float2half_rn(kv_scale(vbyte)) : __half(0.f);
+                far = __any_sync(0xffffffffu, in && !scale_fits(vbyte));
+                if (far) vs = scale_half(vbyte);
                 const uint32_t nums = kt + 2 * D::kTile + 64;
                 asm volatile("st.shared.f32 [%0], %1;" ::"r"(nums + at * 4), "f"(ks * a.scale_log2) : "memory");
                 asm volatile("st.shared.u16 [%0], %1;" ::"r"(nums + 128 + at * 2), "h"(__half_as_ushort(vs)) : "memory");
@@ -744,6 +759,12 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
                 for (int i = 0; i < NTILE; ++i)
 #pragma unroll
                     for (int k = 0; k < C; ++k) o[i][k] *= alpha[PAIR ? 0 : k >> 1];
+            }
+            if (E4M3 && far) {  // second factors go to the weights, which have been summed
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2 * H; ++i) p[nt][i] *= scale_rest(lds8(sc + 32 + 8 * nt + t4 + 4 * (i & 1)));
             }
             // ---- values: k slots 2t, 2t+1, 2t+8, 2t+9 are positions 16 st + t, + 4, + 8, + 12
 #pragma unroll
@@ -1112,28 +1133,42 @@ __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, 
                 const long r = rows.row[j] + off;
                 w[k] = in ? *reinterpret_cast<const uint4 *>(a.kv.data + r * RB + (pc + h * R::LANES) * 16)
                           : make_uint4(0, 0, 0, 0);
-                if (h == 0) sc[j] = in ? a.kv.scale[r] : 0u;
+                if (h == 0) sc[j] = in ? a.kv.scale[r] : 127u;
             }
         };
         auto store = [&](const uint4(&w)[STEPS], const uint32_t(&sc)[R::N]) {
             wait_empty(i);
             const uint32_t dst = bufs + (i % BUFS) * part;
+            auto scaled = [&](auto twice) {
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-                const int j = k / R::HALVES, c2 = 2 * (pc + (k % R::HALVES) * R::LANES);
-                const __half2 s2 = __half2half2(scale_half(sc[j]));
-                const uint32_t sb = *reinterpret_cast<const uint32_t *>(&s2);
-                const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-                uint32_t h[8];
+                for (int k = 0; k < STEPS; ++k) {
+                    const int j = k / R::HALVES, c2 = 2 * (pc + (k % R::HALVES) * R::LANES);
+                    const __half2 s2 = __half2half2(twice.value ? scale_half(sc[j]) : __float2half_rn(kv_scale(sc[j])));
+                    const uint32_t sb = *reinterpret_cast<const uint32_t *>(&s2);
+                    const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+                    uint32_t h[8];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    h[2 * n] = hmul2(e4m3x2_half2(u[n] & 0xffffu), sb);
-                    h[2 * n + 1] = hmul2(e4m3x2_half2(u[n] >> 16), sb);
+                    for (int n = 0; n < 4; ++n) {
+                        h[2 * n] = hmul2(e4m3x2_half2(u[n] & 0xffffu), sb);
+                        h[2 * n + 1] = hmul2(e4m3x2_half2(u[n] >> 16), sb);
+                    }
+                    if constexpr (twice.value) {
+                        const __half2 rest = __float2half2_rn(scale_rest(sc[j]));
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) h[n] = hmul2(h[n], *reinterpret_cast<const uint32_t *>(&rest));
+                    }
+                    const int r = j * R::RS + pr;
+                    sts128(dst + tile_off(r, c2), h[0], h[1], h[2], h[3]);
+                    sts128(dst + tile_off(r, c2 + 1), h[4], h[5], h[6], h[7]);
                 }
-                const int r = j * R::RS + pr;
-                sts128(dst + tile_off(r, c2), h[0], h[1], h[2], h[3]);
-                sts128(dst + tile_off(r, c2 + 1), h[4], h[5], h[6], h[7]);
-            }
+            };
+            // a loop of its own for the second factor: 512 tokens behind 32011 take 345 us so, 340 without
+            // it, 404 with a branch a row or with both factors always
+            bool far = false;
+#pragma unroll
+            for (int j = 0; j < R::N; ++j) far |= !scale_fits(sc[j]);
+            if (far) scaled(std::true_type{});
+            else scaled(std::false_type{});
             proxy_fence();
             mbar_arrive(&ctl->full[i % BUFS]);
             ++i;
@@ -1681,8 +1716,7 @@ template <int HD, bool E4M3>
 __device__ __forceinline__ float cached(const AttnArgs &a, long row, int d) {
     if constexpr (E4M3) {
         const uint32_t h = e4m3x2_half2(a.kv.data[row * HD + d]);
-        const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&h), __half2half2(scale_half(a.kv.scale[row])));
-        return __low2float(v);
+        return __half2float(__float2half_rn(__low2float(*reinterpret_cast<const __half2 *>(&h)) * kv_scale(a.kv.scale[row])));
     } else {
         return __half2float(reinterpret_cast<const __half *>(a.kv.data)[row * HD + d]);
     }
