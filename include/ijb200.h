@@ -363,7 +363,8 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * position 0 (kv_len shorter than the entry) sees none and gets zeros, as does
  * one whose scores are all -infinity.  n_tokens * heads / kv_heads / 256 + n_entries
  * may not pass 8192: longer prompts are cut into several calls.  Entries
- * may be empty; rows that belong to no entry are left as they were.  The starts
+ * may be empty; rows that belong to no entry are left as they were.  Positions whose
+ * page id names no page have no weight, as if the sequence did not have them.  The starts
  * must not fall, and out_dev must not overlap q_dev.  max_q > 0
  * promises that no entry has more new tokens (0: unknown): a longer one may be
  * left unwritten and is reported.

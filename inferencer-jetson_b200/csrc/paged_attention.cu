@@ -52,7 +52,7 @@ struct Cursor {
 // What a worker leaves to the merge: the tile that its last run begins and does
 // not end, as rows row0 .. row0 + rows of the entry whose tokens start at q0, and
 // the number of its states (0: there is none); whether any value it computed is
-// not finite; where its runs began.
+// not finite (1) and any page of its runs names nothing (2); where its runs began.
 struct __align__(16) Left {
     int states, q0, row0, rows, head, bad, pad[2];
     Cursor runs;
@@ -404,12 +404,12 @@ __device__ __forceinline__ __half scale_half(uint32_t s) {
 __device__ __forceinline__ float scale_rest(uint32_t s) {
     return kv_scale(scale_fits(s) ? 127u : s < 103u ? max(s, 88u) + 15u : min(s, 157u) - 15u);
 }
-// Page id of a position, in bounds whatever the table holds; a bad one is reported.
+// Page id of a position; -1 for one that names no page, which is reported.
 __device__ __forceinline__ long page_of(const AttnArgs &a, int seq, int pos) {
     const int page = a.kv.page_table[static_cast<long>(seq) * a.kv.max_pages + (pos >> a.kv.page_shift)];
     if (page >= 0 && page < a.kv.num_pages) return page;
     if (a.status) atomicOr(a.status, kDevErrBadIndex);
-    return 0;
+    return -1;
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
@@ -576,14 +576,18 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
     // ---- the loading side: one chunk after another, across runs
     Segment ls;
     int lb = 0, stage_in = 0;
-    long next_row = 0;  // lane r: cache row (K) of position r of the next chunk
+    long next_row = 0;  // lane r: cache row (K) of position r of the next chunk, -1 if there is none
+    bool gone = false;  // a page was none: the merge computes these runs' rows again, without its positions
     bool more = cursor_next(a, load_c, ls);
     if (more) lb = ls.b0;
     auto find_row = [&]() {
         const int pos = lb * kChunk + lane;
-        next_row = pos < ls.x.kv ? kv_row(a.kv, page_of(a, ls.x.seq, pos), 0, ls.head,
-                                          pos & ((1 << a.kv.page_shift) - 1))
-                                 : -1;
+        next_row = -1;
+        if (pos < ls.x.kv) {
+            const long page = page_of(a, ls.x.seq, pos);
+            if (page >= 0) next_row = kv_row(a.kv, page, 0, ls.head, pos & ((1 << a.kv.page_shift) - 1));
+            else gone = true;
+        }
     };
     if (more) find_row();
     auto issue = [&]() {
@@ -595,7 +599,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
                 const int r = (i * 32 + lane) / (RB / 16), c = lane % (RB / 16);
                 // eight rows of a page lie together: their first row's address serves all
                 const long row8 = __shfl_sync(0xffffffffu, next_row, r & ~7);
-                const bool live = r < left;
+                const bool live = r < left && row8 >= 0;
                 const long row = live ? row8 + (r & 7) : 0;
                 const uint8_t *src = a.kv.data + row * RB + c * 16;
                 const uint32_t off = dec_off<RB>(r, c);
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
             if constexpr (E4M3) {  // 4 scale bytes a copy: lanes 0..7 K, 8..15 V
                 const int r = (lane & 7) * 4;
                 const long row8 = __shfl_sync(0xffffffffu, next_row, r & ~7);
-                if (lane < 16 && r < left)
+                if (lane < 16 && r < left && row8 >= 0)
                     cp_async4(st + 2 * D::kTile + lane * 4, a.kv.scale + row8 + (r & 7) + (lane < 8 ? 0 : v_off));
             }
             if (++lb == ls.b1) {
@@ -884,8 +888,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
         }
     }
     cp_async_wait<0>();
-    bad = __any_sync(0xffffffffu, bad);
-    left.bad = bad ? 1 : 0;
+    left.bad = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, gone) ? 2 : 0);
     left.runs = runs;
     if (lane == 0) a.left[worker] = left;
 }
@@ -948,7 +951,8 @@ struct TileCtl {
     uint64_t full[8], empty[8], q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
     uint32_t tmem;
     uint32_t abort;
-    uint32_t bad;  // a value of the output is not finite
+    uint32_t bad;   // a value of the output is not finite
+    uint32_t gone;  // a page was none (see the decode kernel)
 };
 
 __device__ __forceinline__ bool try_bar(uint64_t *bar, uint32_t parity) {
@@ -1071,7 +1075,7 @@ struct Rows {
     static constexpr int RB = HD * (E4M3 ? 1 : 2);
     int next[N];   // page ids of the block after this one
     long row[N];   // cache rows (K)
-    int live;      // bit k: row k's position exists
+    int live;      // bit k: row k's position exists, and its page
     Segment s;
     int b;
     bool more;
@@ -1089,16 +1093,19 @@ struct Rows {
         peek(a, pr);
     }
     // Makes the peeked block the current one and peeks the next; false at the end.
-    __device__ __forceinline__ bool step(const AttnArgs &a, Cursor &c, int pr) {
+    __device__ __forceinline__ bool step(const AttnArgs &a, Cursor &c, int pr, TileCtl *ctl) {
         if (!more) return false;
         live = 0;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int pos = b * kBlock + k * RS + pr;
             const bool in = pos < s.x.kv, ok = next[k] >= 0 && next[k] < a.kv.num_pages;
-            if (in && !ok && a.status) atomicOr(a.status, kDevErrBadIndex);
-            live |= in ? 1 << k : 0;
-            row[k] = in ? kv_row(a.kv, ok ? next[k] : 0, 0, s.head, pos & ((1 << a.kv.page_shift) - 1)) : 0;
+            if (in && !ok) {
+                ctl->gone = 1u;
+                if (a.status) atomicOr(a.status, kDevErrBadIndex);
+            }
+            live |= in && ok ? 1 << k : 0;
+            row[k] = in && ok ? kv_row(a.kv, next[k], 0, s.head, pos & ((1 << a.kv.page_shift) - 1)) : 0;
         }
         if (++b == s.b1) {
             more = cursor_next(a, c, s);
@@ -1173,12 +1180,12 @@ __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, 
             mbar_arrive(&ctl->full[i % BUFS]);
             ++i;
         };
-        bool more = rows.step(a, c, pr);
+        bool more = rows.step(a, c, pr, ctl);
         if (more) load(wk, sk, 0);
         while (more) {
             load(wv, sv, v_off);
             store(wk, sk);
-            more = rows.step(a, c, pr);
+            more = rows.step(a, c, pr, ctl);
             if (more) load(wk, sk, 0);
             store(wv, sv);
         }
@@ -1187,7 +1194,7 @@ __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, 
         // warp frees a V buffer only when the K buffer behind it is full too, so
         // at most BUFS - 2 may be unannounced.
         constexpr int LAG = BUFS >= 6 ? 3 : (BUFS >= 4 ? 2 : 1);
-        while (rows.step(a, c, pr)) {
+        while (rows.step(a, c, pr, ctl)) {
 #pragma unroll 1
             for (int which = 0; which < 2; ++which, ++i) {
                 wait_empty(i);
@@ -1659,7 +1666,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
         while (cursor_next(a, w, s)) left = left_of(a, s, blockIdx.x, po.per);
         left.runs = c;
         a.left[blockIdx.x] = left;
-        ctl.bad = 0u;
+        ctl.bad = ctl.gone = 0u;
     }
     if (c.at >= c.end) return;
     if (threadIdx.x == 0) {
@@ -1700,7 +1707,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
     tc_before();
     __syncthreads();
     tc_after();
-    if (threadIdx.x == 0 && ctl.bad) a.left[blockIdx.x].bad = 1;
+    if (threadIdx.x == 0) a.left[blockIdx.x].bad = ctl.bad + 2 * ctl.gone;
     if (warp == kMmaWarpId)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
@@ -1711,7 +1718,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
 // a later token's V reaches the earlier tokens that share its block.  The kernels
 // say when a value came out that way, and the merge then computes the rows of those
 // tiles again that do not see all of the positions read, one position at a
-// time: RB rows a block, for the tiles that worker w begins.
+// time: RB rows a block, for the tiles that worker w begins.  Where a page id named no
+// page (nothing was read for it, and its positions counted as zeros), `all` rows of
+// the tiles are computed again, without those positions: a mask for them in the kernels' own
+// loops would cost every call.
 template <int HD, bool E4M3>
 __device__ __forceinline__ float cached(const AttnArgs &a, long row, int d) {
     if constexpr (E4M3) {
@@ -1722,7 +1732,7 @@ __device__ __forceinline__ float cached(const AttnArgs &a, long row, int d) {
     }
 }
 template <int ROWS, int HD, int NT, int RB, bool E4M3, typename T>
-__device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float4 *shared) {
+__device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool all, float4 *shared) {
     float *weight = reinterpret_cast<float *>(shared), *red = weight + NT;  // 4 * NT floats are there
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Cursor c = a.left[w].runs;
@@ -1733,20 +1743,21 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float
         for (int r = s.ti * ROWS + row0; r < min(s.x.rows, min((s.ti + 1) * ROWS, s.ti * ROWS + row0 + RB)); ++r) {
             const int tok = r / a.group, h = s.head * a.group + r % a.group;
             const int n = s.x.kv - s.x.len + tok + 1;  // positions it sees
-            if (n >= end) continue;
+            if (n >= end && !all) continue;
             const T *q = static_cast<const T *>(a.q) + static_cast<long>(s.x.q0 + tok) * a.q_stride + h * HD;
             T *out = static_cast<T *>(a.out) + static_cast<long>(s.x.q0 + tok) * a.out_stride + h * HD;
             const float now = tid < HD ? static_cast<float>(out[tid]) : 0.f;
-            if (__syncthreads_and(now * 0.f == 0.f)) continue;
+            if (__syncthreads_and(now * 0.f == 0.f) && !all) continue;
             auto slot = [&](int t) {
-                return kv_row(a.kv, page_of(a, s.x.seq, t), 0, s.head, t & ((1 << a.kv.page_shift) - 1));
+                const long page = page_of(a, s.x.seq, t);
+                return page < 0 ? -1L : kv_row(a.kv, page, 0, s.head, t & ((1 << a.kv.page_shift) - 1));
             };
             const long v_off = static_cast<long>(a.kv.kv_heads) << a.kv.page_shift;
             float m = -INFINITY, l = 0.f, o = 0.f;  // o: dim tid
             for (int t0 = 0; t0 < n; t0 += NT) {
                 float x = -INFINITY;
-                if (t0 + tid < n) {
-                    const long row = slot(t0 + tid);
+                const long row = t0 + tid < n ? slot(t0 + tid) : -1;
+                if (row >= 0) {
                     x = 0.f;
                     for (int d = 0; d < HD; ++d) x = fmaf(static_cast<float>(q[d]), cached<HD, E4M3>(a, row, d), x);
                     x *= a.scale_log2;
@@ -1759,7 +1770,7 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float
                 for (int i = 0; i < NT / 32; ++i) to = fmaxf(to, red[i]);
                 const float mu = to == -INFINITY ? 0.f : to, alpha = ex2(m - mu), p = ex2(x - mu);
                 m = to;
-                weight[tid] = t0 + tid < n ? p : 0.f;
+                weight[tid] = row >= 0 ? p : 0.f;
                 const float add = warp_sum(weight[tid]);
                 __syncthreads();
                 if (lane == 0) red[warp] = add;
@@ -1768,8 +1779,10 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, float
                 for (int i = 0; i < NT / 32; ++i) l += red[i];
                 o *= alpha;
                 if (tid < HD)
-                    for (int i = 0; i < min(NT, n - t0); ++i)
-                        o = fmaf(weight[i], cached<HD, E4M3>(a, slot(t0 + i) + v_off, tid), o);
+                    for (int i = 0; i < min(NT, n - t0); ++i) {
+                        const long v = slot(t0 + i);
+                        if (v >= 0) o = fmaf(weight[i], cached<HD, E4M3>(a, v + v_off, tid), o);
+                    }
             }
             if (tid < HD) out[tid] = static_cast<T>(o * (l > 0.f || l != l ? 1.f / l : 0.f));
             __syncthreads();
@@ -1791,14 +1804,16 @@ __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_consta
     __shared__ float4 sum[NT];
     const int row0 = blockIdx.y * RB;
     pdl_wait();
-    uint32_t some, again;  // bit j: worker j of this block's left a tile; has rows to look at again
+    uint32_t some, again, all;  // bit j: worker j of this block's left a tile; has rows to look at again; all of them
     {
         static_assert(EACH <= 32, "a lane a worker");
         const int j = threadIdx.x & 31, w = blockIdx.x * EACH + j;
         const bool in = j < EACH && w < a.workers;
         const int4 x = in ? *reinterpret_cast<const int4 *>(&a.left[w].states) : make_int4(0, 0, 0, 0);
         some = __ballot_sync(0xffffffffu, x.x > 0 && x.w > row0);
-        again = __ballot_sync(0xffffffffu, in && a.left[w].bad != 0);
+        const int bad = in ? a.left[w].bad : 0;
+        again = __ballot_sync(0xffffffffu, bad != 0);
+        all = __ballot_sync(0xffffffffu, (bad & 2) != 0);
     }
     for (; some; some &= some - 1) {
         const int w0 = blockIdx.x * EACH + __ffs(some) - 1;
@@ -1807,6 +1822,8 @@ __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_consta
         if (rows <= 0) continue;
         constexpr long PF = part_floats<ROWS, HD>();
         auto part = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0 ? 1 : 0)) * PF; };
+        int theirs = 0;  // `bad` of the workers that go on with the tile
+        for (int i = threadIdx.x; i < n; i += NT) theirs |= a.left[w0 + i].bad;
         constexpr int Q = HD / 4;  // float4 of a row
         const int outs = rows * Q, groups = outs < NT ? NT / outs : 1;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1880,9 +1897,15 @@ __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_consta
             }
         }
         // (also: the shared sums have been read)
-        if (__syncthreads_or(!fine)) again |= 1u << (w0 - blockIdx.x * EACH);
+        if (__syncthreads_or(!fine || (theirs & 2))) {
+            again |= 1u << (w0 - blockIdx.x * EACH);
+            if (__syncthreads_or(theirs & 2)) all |= 1u << (w0 - blockIdx.x * EACH);
+        }
     }
-    for (; again; again &= again - 1) mend_rows<ROWS, HD, NT, RB, E4M3, T>(a, blockIdx.x * EACH + __ffs(again) - 1, row0, sum);
+    for (; again; again &= again - 1) {
+        const int j = __ffs(again) - 1;
+        mend_rows<ROWS, HD, NT, RB, E4M3, T>(a, blockIdx.x * EACH + j, row0, (all >> j) & 1, sum);
+    }
 }
 
 // ---------------------------------------------------------------- launch --
