@@ -668,8 +668,14 @@ void run_step(ijb_engine *e, int n, bool need_logits, bool traced = false, StepS
     g_launches += it->second.launches;
     ck(cudaEventRecord(e->ev_start, e->stream), "step timer start");
     ck(cudaGraphLaunch(it->second.exec, e->stream), "graph launch");
-    ck(cudaEventRecord(e->ev_end, e->stream), "step timer end");
-    if (then) then(e->stream);
+    try {
+        ck(cudaEventRecord(e->ev_end, e->stream), "step timer end");
+        if (then) then(e->stream);
+    } catch (...) {
+        // the step reads pinned memory that the next one writes
+        cudaStreamSynchronize(e->stream);
+        throw;
+    }
     ck(cudaStreamSynchronize(e->stream), "step synchronize");
     ck(cudaEventElapsedTime(&e->last_step_ms, e->ev_start, e->ev_end), "step timer");
     check_status_word(e, static_cast<uint32_t>(e->next_host[e->d.max_batch]));

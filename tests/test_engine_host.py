@@ -1,0 +1,68 @@
+"""Host code of engines on a CUDA runtime of host memory (fake_cudart.c, preloaded into a child
+process): what they do when a call fails, without a GPU."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+PRELUDE = """
+import ctypes, sys, types
+sys.path.insert(0, {pkg!r})
+class Array:  # what Engine needs of a torch tensor
+    def __init__(self, a): self.a = a
+    def to(self, where): return self
+    def data_ptr(self): return self.a.ctypes.data
+sys.modules['torch'] = types.SimpleNamespace(from_numpy=Array)
+from ijb200 import lib, synth
+from ijb200.engine import Engine
+F = ctypes.CDLL({fake!r})
+F.fake_call.restype = ctypes.c_char_p
+F.fake_value.restype = ctypes.c_size_t
+def log(start=0):
+    return [(F.fake_call(i).decode(), F.fake_value(i)) for i in range(start, F.fake_calls())]
+cfg = synth.TINY
+weights = synth.make_model(cfg, seed=1)
+"""
+
+
+@pytest.fixture(scope="module")
+def child(tmp_path_factory):
+    """Runs Python code in a process whose CUDA runtime is the fake."""
+    fake = str(tmp_path_factory.mktemp("fake") / "fake_cudart.so")
+    cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-O1", f"-I{cuda_home}/include", os.path.join(HERE, "fake_cudart.c"), "-o",
+                    fake], check=True)
+    prelude = PRELUDE.format(pkg=os.path.join(os.path.dirname(HERE), "inferencer-jetson_b200"), fake=fake)
+
+    def run(code):
+        r = subprocess.run([sys.executable, "-c", prelude + code], env=dict(os.environ, LD_PRELOAD=fake),
+                           capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stdout + r.stderr
+    return run
+
+
+@pytest.mark.parametrize("kv_type", [None, "f16", "e4m3"])
+@pytest.mark.parametrize("fail", ["cudaEventRecord", "cudaMemcpyAsync", "cudaLaunchKernelExC"])
+def test_a_sampled_step_that_fails_waits_for_what_it_started(child, fail, kv_type):
+    """The step's graph reads pinned memory that the next step writes: every way out of the call waits for it."""
+    child(f"""
+e = Engine(cfg, weights, context=64, max_batch=4, max_seqs=2, kv_type={kv_type!r})
+s = e.seq_open()
+e.decode_sample([s], [3], [0.5])
+start = F.fake_calls()
+F.fake_fail(b"{fail}", b"cudaGraphLaunch")
+try:
+    e.decode_sample([s], [4], [0.5])
+    raise SystemExit("no error")
+except lib.IjbError as err:
+    assert "made by the test" in str(err), err
+calls = [n for n, _ in log(start)]
+assert "cudaGraphLaunch" in calls
+behind = calls[len(calls) - calls[::-1].index("cudaGraphLaunch"):]
+assert "{fail}" in behind and "cudaStreamSynchronize" in behind[behind.index("{fail}"):], behind
+assert e.seq_length(s) == 1
+e.decode_sample([s], [4], [0.5])
+assert e.seq_length(s) == 2
+""")
