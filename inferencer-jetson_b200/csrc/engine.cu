@@ -1057,12 +1057,14 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
             e->paged_work = dev_alloc<uint8_t>(e->paged_work_bytes, "paged attention workspace");
             ck(paged_attention_prepare(e->head_dim, e->paged == IJB_KV_E4M3), "paged attention attributes");
         }
-        // attention: partial softmax records per (token, head) at work-item granularity
-        e->attn_split_len = attention_split_len();
-        e->attn_max_splits = (d.context + attention_item_len() - 1) / attention_item_len();
-        e->attn_partial = dev_alloc<float>(B * d.heads * e->attn_max_splits * (e->head_dim + 2), "attention partials");
-        e->attn_counters = dev_alloc<int>(B * d.kv_heads + 2, "attention counters");
-        ck(cudaMemset(e->attn_counters, 0, (B * d.kv_heads + 2) * sizeof(int)), "counters clear");
+        if (e->paged < 0) {
+            // attention: partial softmax records per (token, head) at work-item granularity
+            e->attn_split_len = attention_split_len();
+            e->attn_max_splits = (d.context + attention_item_len() - 1) / attention_item_len();
+            e->attn_partial = dev_alloc<float>(B * d.heads * e->attn_max_splits * (e->head_dim + 2), "attention partials");
+            e->attn_counters = dev_alloc<int>(B * d.kv_heads + 2, "attention counters");
+            ck(cudaMemset(e->attn_counters, 0, (B * d.kv_heads + 2) * sizeof(int)), "counters clear");
+        }
         e->status = reinterpret_cast<uint32_t *>(e->next_dev + B);
         ck(cudaMemset(e->status, 0, sizeof(uint32_t)), "status clear");
         e->scratch_key = dev_alloc<unsigned long long>(1, "argmax scratch");
@@ -1322,7 +1324,7 @@ int ijb_time_layer_attention(ijb_engine *e, int n, const int *seq_ids, int reps,
         if (e->paged >= 0)
             ck(cudaMemcpyAsync(e->meta_dev, e->meta_host, e->meta_ints * sizeof(int), cudaMemcpyHostToDevice, e->stream),
                "meta H2D");
-        const AttnParams a = attn_params(e, 0, n);
+        const AttnParams a = e->paged >= 0 ? AttnParams{} : attn_params(e, 0, n);
         const uint64_t before = g_launches.load();
         const bool pdl = e->pdl || (n >= e->mma_min_batch ? e->attn_pdl : e->small_attn_pdl);
         cudaGraph_t graph;

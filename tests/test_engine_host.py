@@ -66,3 +66,20 @@ assert e.seq_length(s) == 1
 e.decode_sample([s], [4], [0.5])
 assert e.seq_length(s) == 2
 """)
+
+
+@pytest.mark.parametrize("kv_type", ["f16", "e4m3"])
+def test_paged_engines_take_no_memory_of_the_other_attention(child, kv_type):
+    """Its partial records grow with max_batch times context; an engine whose attention is the paged one has none."""
+    child(f"""
+kw = dict(context=5000, max_batch=8, max_seqs=2)
+records = 8 * cfg.heads * -(-5000 // 128) * (cfg.head_dim + 2) * 4 + 16  # an allocation's slack
+e = Engine(cfg, weights, **kw)
+assert ("cudaMalloc", records) in log()
+start = F.fake_calls()
+e = Engine(cfg, weights, kv_type={kv_type!r}, **kw)
+assert ("cudaMalloc", records) not in log(start)
+s = e.seq_open()
+e.decode_step([s], [1])
+assert e.time_layer_attention([s], reps=2)[1] == cfg.kv_heads * 2 * {{"f16": 2 * cfg.head_dim, "e4m3": cfg.head_dim + 1}}[{kv_type!r}]
+""")
