@@ -769,19 +769,22 @@ cudaError_t sample_launch(const float *x, long stride, int n, int vocab, const f
                           const int *top_k, const float *top_p, const float *min_p, int *token, float *prob,
                           cudaStream_t stream) {
     SampleParams p{x, stride, vocab, 0, u, temperature, top_k, top_p, min_p, token, prob};
-    // parts of at most 2048 logits, in clusters of up to 8 CTAs; 16 for few rows, where the row's
-    // time counts (a size that the device has to allow: all of a B200's GPCs hold one)
-    const int most = n <= 8 ? kMaxCluster : 8;
-    int c = 1;
-    while (c < most && (vocab + c - 1) / c > 2048) c *= 2;
-    p.chunk = ((vocab + c - 1) / c + 3) / 4 * 4;
-    const int smem = static_cast<int>(sizeof(Smem)) + p.chunk * 4;
-    static bool ready[64];
+    static bool ready[64], wide[64];
     static std::mutex mu;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kMaxCluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kThreads);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    bool most;
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[dev]) {
@@ -790,24 +793,26 @@ cudaError_t sample_launch(const float *x, long stride, int n, int vocab, const f
             if (e == cudaSuccess)
                 e = cudaFuncSetAttribute(ijb_sample_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                                          cudaSharedmemCarveoutMaxShared);
-            if (e == cudaSuccess)
-                e = cudaFuncSetAttribute(ijb_sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return e;
+            // clusters of 16 only where the device can place one
+            cfg.gridDim = dim3(kMaxCluster);
+            cfg.dynamicSmemBytes = sizeof(Smem) + kMaxVocab / kMaxCluster * 4;
+            int clusters = 0;
+            wide[dev] = cudaFuncSetAttribute(ijb_sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&clusters, ijb_sample_kernel, &cfg) == cudaSuccess && clusters > 0;
+            if (!wide[dev]) cudaGetLastError();
             ready[dev] = true;
         }
+        most = n <= 8 && wide[dev];
     }
-    cudaLaunchConfig_t cfg = {};
+    // parts of at most 2048 logits, in clusters of up to 8 CTAs; 16 for few rows, where the row's time counts
+    int c = 1;
+    while (c < (most ? kMaxCluster : 8) && (vocab + c - 1) / c > 2048) c *= 2;
+    p.chunk = ((vocab + c - 1) / c + 3) / 4 * 4;
     cfg.gridDim = dim3(static_cast<unsigned>(n) * c);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = sizeof(Smem) + static_cast<size_t>(p.chunk) * 4;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = c;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, ijb_sample_kernel, p);
 }
 

@@ -1,5 +1,5 @@
-"""Host code of engines on a CUDA runtime of host memory (fake_cudart.c, preloaded into a child
-process): what they do when a call fails, without a GPU."""
+"""Host code of engines and operators on a CUDA runtime of host memory (fake_cudart.c, preloaded
+into a child process): what they do when a call fails, without a GPU."""
 import os
 import subprocess
 import sys
@@ -82,4 +82,17 @@ assert ("cudaMalloc", records) not in log(start)
 s = e.seq_open()
 e.decode_step([s], [1])
 assert e.time_layer_attention([s], reps=2)[1] == cfg.kv_heads * 2 * {{"f16": 2 * cfg.head_dim, "e4m3": cfg.head_dim + 1}}[{kv_type!r}]
+""")
+
+
+@pytest.mark.parametrize("largest", [16, 8])
+def test_sampling_without_clusters_of_16(child, largest):
+    """Few rows take clusters of 16, a size that a device (or a part of one) need not place: then 8, as many rows do."""
+    child(f"""
+L = lib.load()
+F.fake_largest_cluster({largest})
+for n, want in ((1, {largest}), (8, {largest}), (9, 8)):
+    start = F.fake_calls()
+    assert L.ijb_sample(4096, 128256, n, 128256, 4096, None, None, None, None, 4096, None, None) == 0
+    assert [v for name, v in log(start) if name == "cudaLaunchKernelExC"] == [want]
 """)
