@@ -359,7 +359,7 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * [heads][head_dim], type IJB_TYPE_F32 or IJB_TYPE_F16, strides in elements):
  * the last of the kv_len_dev[e] positions of sequence seq_dev[e] (NULL: e),
  * whose K and V, the new tokens' included, the cache already holds.  A token
- * sees the positions up to its own, with softmax(scale * q . k), scale > 0; one before
+ * sees the positions up to its own, with softmax(scale * q . k), 0 < scale <= 2e38; one before
  * position 0 (kv_len shorter than the entry) sees none and gets zeros, as does
  * one whose scores are all -infinity.  n_tokens * heads / kv_heads / 256 + n_entries
  * may not pass 8192: longer prompts are cut into several calls.  Entries

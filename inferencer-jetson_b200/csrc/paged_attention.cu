@@ -2087,7 +2087,8 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         if (n_entries < 1 || n_entries > kMaxEntries) return kv_fail(IJB_ERR_INVALID, fn, "n_entries must be 1..4096");
         if (n_tokens < 0) return kv_fail(IJB_ERR_INVALID, fn, "negative token count");
         if (n_tokens == 0) return IJB_OK;
-        if (!(scale > 0.f && scale <= 3.402823466e38f)) return kv_fail(IJB_ERR_INVALID, fn, "scale must be positive and finite");
+        // (times log2(e) it has to be finite, too)
+        if (!(scale > 0.f && scale <= 2e38f)) return kv_fail(IJB_ERR_INVALID, fn, "scale must be positive and at most 2e38");
         if (!q_dev || !out_dev || !q_start_dev || !kv_len_dev || !workspace_dev)
             return kv_fail(IJB_ERR_INVALID, fn, "null argument");
         if (q_dev == out_dev) return kv_fail(IJB_ERR_INVALID, fn, "the output must not lie over the queries");

@@ -96,3 +96,18 @@ for n, want in ((1, {largest}), (8, {largest}), (9, 8)):
     assert L.ijb_sample(4096, 128256, n, 128256, 4096, None, None, None, None, 4096, None, None) == 0
     assert [v for name, v in log(start) if name == "cudaLaunchKernelExC"] == [want]
 """)
+
+
+def test_attention_refuses_a_scale_beyond_its_base_2_logarithm(child):
+    """Scores are scaled by scale * log2(e), which has to be a number too: an infinity makes NaN of a score of 0."""
+    child("""
+L = lib.load()
+v = lib.KvView(type=2, kv_heads=2, head_dim=64, page_size=16, num_pages=4, data_dev=4096, scale_dev=8192,
+               page_table_dev=256, n_seqs=1, max_pages=4)
+def attention(scale):
+    return L.ijb_paged_attention(ctypes.byref(v), 4, 0, 4096, 256, 8192, 256, 2, 1, 256, None, 256, 1, scale, 4096, 1 << 40,
+                                 None, None)
+assert attention(0.125) == lib.OK and attention(2e38) == lib.OK
+for scale in (2.4e38, 3.4e38, float("inf"), 0.0, -1.0, float("nan")):
+    assert attention(scale) == lib.ERR_INVALID and "scale" in L.ijb_last_error(None).decode()
+""")
