@@ -444,13 +444,15 @@ constexpr int kDecRows = 16;
 
 // WIDE: more than 8 rows.  Up to 8 leave the upper half of the products' 16 rows
 // unused, and with half the registers an SM holds more warps: 64 ragged
-// sequences of 4 rows took 25 us with the wide kernel's 8 warps.
-template <int HD, bool E4M3, bool WIDE>
+// sequences of 4 rows took 25 us with the wide kernel's 8 warps.  Of the e4m3 kernels at
+// head_dim 64, fp32 queries' does not fit 16 warps' registers: one token at position 4100, 8 KV heads, took
+// 18.0 us with 16 and 14.9 with 12, 16 contexts of 9,001 to 32,768 positions 103 and 98.
+template <int HD, bool E4M3, bool WIDE, typename T>
 struct Dec {
     static constexpr int kRowBytes = HD * (E4M3 ? 1 : 2);
     static constexpr int kTile = kChunk * kRowBytes;
     static constexpr int kStage = 2 * kTile + (E4M3 ? 256 : 0);  // K, V, their scale bytes and what they stand for
-    static constexpr int kWarps = kRowBytes == 256 ? 6 : (WIDE || HD == 128 ? 8 : (E4M3 ? 16 : 12));
+    static constexpr int kWarps = kRowBytes == 256 ? 6 : (WIDE || HD == 128 ? 8 : (E4M3 && sizeof(T) == 2 ? 16 : 12));
     static constexpr int kStages = kRowBytes == 256 ? 2 : (kRowBytes == 128 ? (kWarps == 8 ? 3 : 2) : (WIDE ? 4 : 3));
     static constexpr int kSmem = kWarps * kStages * kStage;
     static_assert(kSmem <= 226 * 1024, "stages");
@@ -534,9 +536,9 @@ __device__ __forceinline__ void add_values(float (&o0)[4], float (&o1)[4], const
 }
 
 template <int HD, bool E4M3, bool WIDE, typename T>
-__global__ void __launch_bounds__(Dec<HD, E4M3, WIDE>::kWarps * 32, 1)
+__global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
     ijb_paged_decode_kernel(const __grid_constant__ AttnArgs a) {
-    using D = Dec<HD, E4M3, WIDE>;
+    using D = Dec<HD, E4M3, WIDE, T>;
     constexpr int H = WIDE ? 2 : 1;  // halves of the 16 rows in use
     // up to 8 fp32 rows: their hi parts are rows 0..7 of the products, their lo
     // parts rows 8..15, for the products of one
@@ -1822,8 +1824,9 @@ __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_consta
         if (rows <= 0) continue;
         constexpr long PF = part_floats<ROWS, HD>();
         auto part = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0 ? 1 : 0)) * PF; };
-        int theirs = 0;  // `bad` of the workers that go on with the tile
-        for (int i = threadIdx.x; i < n; i += NT) theirs |= a.left[w0 + i].bad;
+        // `bad` of the workers that go on with the tile (the first load is not waited for here)
+        int theirs = threadIdx.x < n ? a.left[w0 + threadIdx.x].bad : 0;
+        for (int i = threadIdx.x + NT; i < n; i += NT) theirs |= a.left[w0 + i].bad;
         constexpr int Q = HD / 4;  // float4 of a row
         const int outs = rows * Q, groups = outs < NT ? NT / outs : 1;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1959,14 +1962,14 @@ cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     return e;
 }
 
-template <int HD, bool E4M3, bool WIDE>
+template <int HD, bool E4M3, bool WIDE, typename T>
 constexpr int decode_smem() {
-    return Dec<HD, E4M3, WIDE>::kSmem > kDecPlanBytes ? Dec<HD, E4M3, WIDE>::kSmem : kDecPlanBytes;
+    return Dec<HD, E4M3, WIDE, T>::kSmem > kDecPlanBytes ? Dec<HD, E4M3, WIDE, T>::kSmem : kDecPlanBytes;
 }
 template <int HD, bool E4M3, bool WIDE, typename T>
 cudaError_t decode_allow() {
     auto kernel = ijb_paged_decode_kernel<HD, E4M3, WIDE, T>;
-    return allow_smem<decltype(kernel), Dec<HD, E4M3, WIDE>, T>(kernel, decode_smem<HD, E4M3, WIDE>());
+    return allow_smem<decltype(kernel), Dec<HD, E4M3, WIDE, T>, T>(kernel, decode_smem<HD, E4M3, WIDE, T>());
 }
 template <int HD, bool E4M3, typename T>
 cudaError_t tile_allow() {
@@ -1976,7 +1979,7 @@ cudaError_t tile_allow() {
 
 template <int HD, bool E4M3, bool WIDE, typename T>
 cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
-    using D = Dec<HD, E4M3, WIDE>;
+    using D = Dec<HD, E4M3, WIDE, T>;
     const cudaError_t e = decode_allow<HD, E4M3, WIDE, T>();
     if (e != cudaSuccess) return e;
     a.min_rows = 1;
@@ -1988,7 +1991,7 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.min_units = 2;
     a.over = 1;
     a.least = 1;
-    ijb_paged_decode_kernel<HD, E4M3, WIDE, T><<<sms, D::kWarps * 32, decode_smem<HD, E4M3, WIDE>(), s>>>(a);
+    ijb_paged_decode_kernel<HD, E4M3, WIDE, T><<<sms, D::kWarps * 32, decode_smem<HD, E4M3, WIDE, T>(), s>>>(a);
     return merge_launch<kDecRows, HD, E4M3, T>(a, s);
 }
 
