@@ -359,24 +359,24 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * [heads][head_dim], type IJB_TYPE_F32 or IJB_TYPE_F16, strides in elements):
  * the last of the kv_len_dev[e] positions of sequence seq_dev[e] (NULL: e),
  * whose K and V, the new tokens' included, the cache already holds.  A token
- * sees the positions up to its own, with softmax(scale * q . k), 0 < scale <= 2e38; one before
- * position 0 (kv_len shorter than the entry) sees none and gets zeros, as does
- * one whose scores are all -infinity.  n_tokens * heads / kv_heads / 256 + n_entries
- * may not pass 8192: longer prompts are cut into several calls.  Entries
- * may be empty; rows that belong to no entry are left as they were.  Positions whose
- * page id names no page have no weight, as if the sequence did not have them.  The starts
- * must not fall, and out_dev must not overlap q_dev.  max_q > 0
- * promises that no entry has more new tokens (0: unknown): a longer one may be
- * left unwritten and is reported.
+ * sees the positions up to its own, with softmax(scale * q . k), 0 < scale <=
+ * 2e38; one before position 0 (kv_len shorter than the entry) sees none and gets
+ * zeros, as does one whose scores are all -infinity.  Positions whose page id
+ * names no page have no weight, as if the sequence did not have them.  n_tokens *
+ * heads / kv_heads / 256 + n_entries may not pass 8192: longer prompts are cut into
+ * several calls.  Entries may be empty; rows that belong to no entry are left as
+ * they were.  The starts must not fall, and out_dev must not overlap q_dev.
+ * max_q > 0 promises that no entry has more new tokens (0: unknown): a longer one
+ * may be left unwritten and is reported.  scale_dev has to be 4-byte aligned.
  *
- * fp32 queries and probabilities enter the products as two fp16 parts each
- * (22 bits, but no finer than 2^-25; queries up to 65504); fp16 queries as they are, their
- * probabilities rounded to fp16.  e4m3 values enter as the nearest fp16 number, as an fp16
- * cache would hold them: those of a row whose largest is within 2^-7 .. 2^15 exactly, smaller ones
- * off by 2^-25 at most; those of 65520 and more may come out as infinities.  Sums,
- * maxima and the softmax are fp32.  The result is the same
- * every time for the same call, but how an entry's positions are cut into
- * partial sums depends on the whole call.
+ * fp32 queries and probabilities enter the products as two fp16 parts each (22
+ * bits, but no finer than 2^-25; queries up to 65504); fp16 queries as they are,
+ * their probabilities rounded to fp16.  e4m3 values enter as the nearest fp16
+ * number, as an fp16 cache would hold them: those of a row whose largest is within
+ * 2^-7 .. 2^15 exactly, smaller ones off by 2^-25 at most; those of 65520 and more
+ * may come out as infinities.  Sums, maxima and the softmax are fp32.  The result
+ * is the same every time for the same call, but how an entry's positions are cut
+ * into partial sums depends on the whole call.
  *
  * workspace_dev: ijb_paged_attention_workspace(kv) bytes (the same for every call
  * on caches of that head_dim; 0 for a bad view) of 16-byte aligned device

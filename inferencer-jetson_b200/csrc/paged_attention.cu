@@ -26,7 +26,8 @@
 // Arithmetic.  Products are fp16 x fp16 with fp32 sums.  fp32 queries enter as
 // two fp16 parts (hi + lo, 22 bits), and so do their probabilities; fp16
 // queries enter as they are, their probabilities rounded to fp16 once (the
-// output is fp16 too).  Cached rows enter as fp16: fp16 rows exactly, e4m3 values as the
+// output is fp16 too: 2.6e-4 to 2.9e-4 rel-L2 against 64 bits, of which the output's
+// rounding alone is 2.1e-4).  Cached rows enter as fp16: fp16 rows exactly, e4m3 values as the
 // fp16 number nearest to code * 2^e, as an fp16 cache would hold them: exactly from 2^-14 on (and
 // every value of a row whose largest is in [2^-7, 2^15]), else off by 2^-25 at most, infinite from
 // 65520 on.  (The decode kernel scales its scores in fp32, so K has no such ends there.)
@@ -436,7 +437,7 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 // that both read patterns are free of bank conflicts.
 //
 // Measured: 16 contexts of 9,001 to 32,768 positions, 8 KV heads of 128 in e4m3, fp16
-// queries of 32 heads: 758 MB in 147 us (5.2 TB/s), with the tensor pipe 29 % busy;
+// queries of 32 heads: 757 MB in 148 us (5.1 TB/s), with the tensor pipe 29 % busy;
 // what is left is the loads' latency at the ends of the workers' runs.
 
 constexpr int kChunk = 32;  // positions
@@ -504,8 +505,8 @@ __device__ __forceinline__ void mma(float (&d)[2], const uint32_t (&a)[2], uint3
 // are summed by the tensor core, whose additions drop bits towards zero, and added to O
 // rounded to nearest: left in the product's accumulators, the outputs of 300 entries of 20000
 // positions (runs of some thousand a warp) were off by 5e-6 to 2.6e-5 (rel-L2), so they are by
-// 8e-7 at most, as a plain fp32 sum's.  16 contexts of 9,001 to 32,768 positions took 158 us before
-// and after, 64 ragged single tokens 2 us more.  (volatile: in this order, for the registers.)
+// 8e-7 at most, as a plain fp32 sum's.  16 contexts of 9,001 to 32,768 positions keep their time,
+// 64 ragged single tokens take 1 us more.  (volatile: in this order, for the registers.)
 __device__ __forceinline__ void add2_in_order(float &x, float &y, float a, float b) {
     float2 o = make_float2(x, y), d = make_float2(a, b);
     asm volatile("add.rn.f32x2 %0, %0, %1;" : "+l"(reinterpret_cast<uint64_t &>(o)) : "l"(reinterpret_cast<uint64_t &>(d)));
@@ -920,12 +921,13 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
 // what it held is added, rounded to nearest, to sums kept in TMEM (head_dim 64,
 // where half of O's columns are free) or in the workspace (128).
 //
-// What bounds it: the exponentials (16 a clock and SM: 1024 clocks a tile and
-// block) beside the products (256 clocks at head_dim 64, 512 at 128, for each
-// of S and O; twice that for fp32 queries), which overlap but in part: a block of
-// both tiles takes 3300 to 3600 clocks where 2048 would do.  Measured, 32 heads of 128
-// over 8 KV heads, fp16 queries: 512 tokens behind 32011 in an e4m3 cache 321 us (840
-// TFLOP/s, tensor pipe 40 % busy), a prompt of 8192 633 us (870 TFLOP/s).
+// What bounds it: the waits between a tile's products and its softmax.  A block of both
+// tiles has 2048 clocks of products at head_dim 128 (1024 at 64; twice that for fp32 queries)
+// and 1536 of exponentials (16 a clock and SM, a quarter of them on the FMA pipes; 2048 for fp32
+// queries, which leave none to those); the one tile's fill the other's waits but in part, and a
+// block takes 3300 to 3600.  Measured in a graph, 32 heads of 128 over 8 KV heads: 512 tokens behind
+// 32011 in an e4m3 cache 322 us with fp16 queries (840 TFLOP/s; tensor pipe 40 % and exponential
+// unit 32 % busy) and 635 with fp32 ones, a prompt of 8192 641 and 1298.
 
 constexpr int kTileRows = 256, kBlock = 128;
 constexpr int kTileThreads = 16 * 32, kMmaWarpId = 12, kLoadWarp0 = 8;
@@ -1171,8 +1173,8 @@ __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, 
                     sts128(dst + tile_off(r, c2 + 1), h[4], h[5], h[6], h[7]);
                 }
             };
-            // a loop of its own for the second factor: 512 tokens behind 32011 take 345 us so, 340 without
-            // it, 404 with a branch a row or with both factors always
+            // a loop of its own for the second factor: with a branch a row, or with both factors always,
+            // 512 tokens behind 32011 took 404 us in place of 340
             bool far = false;
 #pragma unroll
             for (int j = 0; j < R::N; ++j) far |= !scale_fits(sc[j]);
@@ -1310,7 +1312,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// 2^x of a pair on the FMA pipes, for x <= 2^8 (below -126: 2^-126 or so): with
+// 2^x of a pair on the FMA pipes, for x <= 8 (see kRaise; below -126: 2^-126 or so): with
 // n = round(x) and f = x - n in [-1/2, 1/2], 2^f by a polynomial of degree 4, fitted by least
 // squares of the relative error over Chebyshev nodes (off by 1e-5 at most), n added to the
 // exponent.  Adding 1.5 * 2^23 rounds x and leaves n in the low bits.
@@ -2015,7 +2017,9 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
 
 // Which kernels serve a call.  Entries of up to 16 rows go to the decode kernel,
 // longer ones to the tile kernel; a call that may hold longer ones and has few
-// entries leaves them all to the tile kernel, for the launches.
+// entries leaves them all to the tile kernel, for the launches: entries of 1 to 40 tokens
+// behind 100 to 2000 take 49 us so and 55 with both kernels for 2 of them, 51 and 56 for 7, 55 and 59 for 8, 77 and
+// 89 for 16 (so the border could lie higher); one of 200 tokens among single ones 54 and 68 for 4, 98 and 83 for 32.
 template <int HD, bool E4M3, typename T>
 cudaError_t attention_call(const AttnArgs &a, int max_q, int sms, cudaStream_t s) {
     const long most = static_cast<long>(max_q > 0 ? min(max_q, a.n_tokens) : a.n_tokens) * a.group;

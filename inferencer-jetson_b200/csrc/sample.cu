@@ -805,7 +805,9 @@ cudaError_t sample_launch(const float *x, long stride, int n, int vocab, const f
         }
         most = n <= 8 && wide[dev];
     }
-    // parts of at most 2048 logits, in clusters of up to 8 CTAs; 16 for few rows, where the row's time counts
+    // parts of at most 2048 logits, in clusters of up to 8 CTAs; 16 for few rows, where the row's time
+    // counts: 128256 logits, in a graph, 24.5 us with 16 and 28.5 with 8 for one row, 26.4 and 28.6 for 4, 28.7
+    // each for 8, 47.5 and 30.7 for 16
     int c = 1;
     while (c < (most ? kMaxCluster : 8) && (vocab + c - 1) / c > 2048) c *= 2;
     p.chunk = ((vocab + c - 1) / c + 3) / 4 * 4;
