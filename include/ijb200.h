@@ -374,9 +374,11 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
  * their probabilities rounded to fp16.  e4m3 values enter as the nearest fp16
  * number, as an fp16 cache would hold them: those of a row whose largest is within
  * 2^-7 .. 2^15 exactly, smaller ones off by 2^-25 at most; those of 65520 and more
- * may come out as infinities.  Sums, maxima and the softmax are fp32.  The result
- * is the same every time for the same call, but how an entry's positions are cut
- * into partial sums depends on the whole call.
+ * may come out as infinities.  Sums, maxima and the softmax are fp32; fp16 queries'
+ * values are summed by the tensor core alone, which loses some of the last bits:
+ * 1.4e-4 of an output over 2^20 positions.  The result is the same every time for
+ * the same call, but how an entry's positions are cut into partial sums depends on
+ * the whole call.
  *
  * workspace_dev: ijb_paged_attention_workspace(kv) bytes (the same for every call
  * on caches of that head_dim; 0 for a bad view) of 16-byte aligned device
