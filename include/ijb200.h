@@ -322,6 +322,8 @@ int ijb_keys_to_tokens(const unsigned long long *keys_dev, int n, int *tokens_de
  * found on the device names nothing: such an entry is skipped. */
 #define IJB_KV_F16 0   /* fp16 rows */
 #define IJB_KV_E4M3 2  /* e4m3 rows, each with a power-of-two scale 2^(s - 127) kept as the byte s (0..254) */
+#define IJB_KV_E2M1 3  /* e2m1 codes, two a byte (the even dim in the low half); 32 dims of a row share a scale, the
+                          fp16 number of the bits s << 7, kept as the byte s (0..226) */
 
 typedef struct {
     int type;                   /* IJB_KV_F16 or IJB_KV_E4M3 */
@@ -352,6 +354,15 @@ int ijb_kv_append(const ijb_kv_view *kv, int src_type, const void *k_dev, const 
  * Rows of skipped entries are left as they were. */
 int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev, long stride, int n,
                   const int *tok_seq_dev, const int *tok_pos_dev, uint32_t *status_dev, void *stream);
+
+/* Copies n whole pages, all rows of K and V with their scales as they are: page
+ * src_page_dev[i] of `from` to page dst_page_dev[i] of `to` (NULL: of `from`
+ * itself; else a cache of the same type, heads and page size on the same device).
+ * Entries with a negative destination are padding and are skipped.  A page
+ * may be the source of several entries, but a destination must not be named
+ * twice, nor as a source of the same call. */
+int ijb_kv_copy_pages(const ijb_kv_view *from, const ijb_kv_view *to, int n, const int *src_page_dev,
+                      const int *dst_page_dev, uint32_t *status_dev, void *stream);
 
 /* Attention of new tokens over the cache, causal, with heads / kv_heads (1..16)
  * query heads to a KV head.  Entry e (of n_entries <= 4096) is the rows

@@ -1055,7 +1055,7 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
             const ijb_kv_view v = layer_view(e.get(), 0);
             e->paged_work_bytes = ijb_paged_attention_workspace(&v);
             e->paged_work = dev_alloc<uint8_t>(e->paged_work_bytes, "paged attention workspace");
-            ck(paged_attention_prepare(e->head_dim, e->paged == IJB_KV_E4M3), "paged attention attributes");
+            ck(paged_attention_prepare(e->head_dim, e->paged), "paged attention attributes");
         }
         if (e->paged < 0) {
             // attention: partial softmax records per (token, head) at work-item granularity

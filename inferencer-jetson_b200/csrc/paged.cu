@@ -24,7 +24,8 @@ constexpr int kRowThreads = 256;
 
 std::string kv_view_check(const ijb_kv_view *v, KvDev *out) {
     if (!v) return "null cache view";
-    if (v->type != IJB_KV_F16 && v->type != IJB_KV_E4M3) return "cache type must be IJB_KV_F16 or IJB_KV_E4M3";
+    if (v->type != IJB_KV_F16 && v->type != IJB_KV_E4M3 && v->type != IJB_KV_E2M1)
+        return "cache type must be IJB_KV_F16, IJB_KV_E4M3 or IJB_KV_E2M1";
     if (v->head_dim != 64 && v->head_dim != 128) return "head_dim must be 64 or 128";
     if (v->kv_heads < 1 || v->kv_heads > 1024) return "kv_heads must be 1..1024";
     if (v->page_size < 8 || v->page_size > 256 || (v->page_size & (v->page_size - 1)) != 0)
@@ -34,7 +35,7 @@ std::string kv_view_check(const ijb_kv_view *v, KvDev *out) {
         return "n_seqs and max_pages must be positive, and max_pages * page_size at most 2^30";
     if (!v->data_dev || !v->page_table_dev) return "null cache data or page table";
     if (reinterpret_cast<uintptr_t>(v->data_dev) % 16 != 0) return "cache data must be 16-byte aligned";
-    if (v->type == IJB_KV_E4M3 && !v->scale_dev) return "an e4m3 cache needs its scale bytes";
+    if (v->type != IJB_KV_F16 && !v->scale_dev) return "an e4m3 or e2m1 cache needs its scale bytes";
     out->data = static_cast<uint8_t *>(v->data_dev);
     out->scale = v->scale_dev;
     out->page_table = v->page_table_dev;
@@ -141,7 +142,39 @@ struct Place {
     }
 };
 
-template <typename T, bool E4M3, bool VEC, int HD, int U>
+// Thread c's 8 of a row's values as e2m1 codes; the row's 4 threads of a block of 32 agree on the scale.
+__device__ __forceinline__ uint32_t e2m1_codes(const float (&f)[8], uint32_t &byte) {
+    float a = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a = fmaxf(a, fabsf(f[i]) <= 3.402823466e38f ? fabsf(f[i]) : 0.f);
+        nan |= f[i] != f[i];
+    }
+    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+    const uint32_t any = __ballot_sync(0xffffffffu, nan), mine = 0xfu << (threadIdx.x & 28);
+    // the nearest scale to a / 6, ties to even: from 2^-14 on the upper bits of the number with 3 of its mantissa,
+    // below in steps of 2^-17
+    const float r = __fdiv_rn(a, 6.f);
+    const uint32_t bits = __float_as_uint(r);
+    byte = r >= 6.103515625e-5f ? ((bits + 0x7ffffu + ((bits >> 20) & 1u)) >> 20) - ((127u - 15u) << 3)
+                                : __float2uint_rn(r * 131072.f);
+    byte = min(byte, kKvTopScale);
+    const float scale = half_bits_to_float(static_cast<uint16_t>(byte << 7));
+    const float inv = byte ? __frcp_rn(scale) : 0.f;
+    uint32_t q = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // an infinity is the largest value, and a block without a scale zeros
+        const float x = byte ? f[2 * i] * inv : 0.f, y = byte ? f[2 * i + 1] * inv : 0.f;
+        q |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(x, y), __NV_E2M1, cudaRoundNearest)) << (8 * i);
+    }
+    if (any & mine) byte = kKvNanScale;  // a NaN is its block's
+    return q;
+}
+
+template <typename T, int KV, bool VEC, int HD, int U>
 __global__ void __launch_bounds__(kRowThreads) ijb_kv_append_kernel(const __grid_constant__ RowsParams p) {
     const Place<HD, U> w(p);
     const long src = w.n ? w.t * p.stride + static_cast<long>(w.head) * HD + w.c * 8 : 0;
@@ -162,7 +195,14 @@ __global__ void __launch_bounds__(kRowThreads) ijb_kv_append_kernel(const __grid
     for (int j = 0; j < U; ++j) {
         const long to = to0 + (static_cast<long>(j) << p.kv.page_shift);
         const bool live = slot >= 0 && j < w.n;
-        if constexpr (E4M3) {
+        if constexpr (KV == IJB_KV_E2M1) {
+            uint32_t byte;
+            const uint32_t q = e2m1_codes(f[j], byte);
+            if (live) {
+                *reinterpret_cast<uint32_t *>(p.kv.data + to * (HD / 2) + w.c * 4) = q;
+                if (w.c % 4 == 0) p.kv.scale[to * (HD / kKvBlock) + w.c / 4] = static_cast<uint8_t>(byte);
+            }
+        } else if constexpr (KV == IJB_KV_E4M3) {
             float a = 0.f;  // over the finite values: an infinity saturates, a NaN stays one
 #pragma unroll
             for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[j][i]) <= 3.402823466e38f ? fabsf(f[j][i]) : 0.f);
@@ -195,7 +235,7 @@ __global__ void __launch_bounds__(kRowThreads) ijb_kv_append_kernel(const __grid
 
 // Reads back: code * 2^e (exact in fp32), or the fp16 row; rows of padding
 // entries and of entries that name no slot are left as they were.
-template <typename T, bool E4M3, bool VEC, int HD, int U>
+template <typename T, int KV, bool VEC, int HD, int U>
 __global__ void __launch_bounds__(kRowThreads) ijb_kv_gather_kernel(const __grid_constant__ RowsParams p) {
     const Place<HD, U> w(p);
     if (w.n == 0) return;
@@ -209,7 +249,10 @@ __global__ void __launch_bounds__(kRowThreads) ijb_kv_gather_kernel(const __grid
     for (int j = 0; j < U; ++j) {
         if (j >= w.n) continue;
         const long from = from0 + (static_cast<long>(j) << p.kv.page_shift);
-        if constexpr (E4M3) {
+        if constexpr (KV == IJB_KV_E2M1) {
+            raw[j].x = *reinterpret_cast<const uint32_t *>(p.kv.data + from * (HD / 2) + w.c * 4);
+            sc[j] = p.kv.scale[from * (HD / kKvBlock) + w.c / 4];
+        } else if constexpr (KV == IJB_KV_E4M3) {
             const uint2 u = *reinterpret_cast<const uint2 *>(p.kv.data + from * HD + w.c * 8);
             raw[j].x = u.x;
             raw[j].y = u.y;
@@ -222,7 +265,17 @@ __global__ void __launch_bounds__(kRowThreads) ijb_kv_gather_kernel(const __grid
     for (int j = 0; j < U; ++j) {
         if (j >= w.n) continue;
         float f[8];
-        if constexpr (E4M3) {
+        if constexpr (KV == IJB_KV_E2M1) {
+            const float s = half_bits_to_float(static_cast<uint16_t>(sc[j] << 7));
+            uint32_t h[4];
+            e2m1x8_half2(raw[j].x, h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+                f[2 * i] = v.x * s;
+                f[2 * i + 1] = v.y * s;
+            }
+        } else if constexpr (KV == IJB_KV_E4M3) {
             const float s = kv_scale(sc[j]);
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
@@ -248,24 +301,31 @@ constexpr int kHeads = 4;              // heads a thread takes of many rows
 // 10.2 each; 16383 written 50.7 and 47.5, read 50.2 and 43.2.
 constexpr long kManyThreads = 1 << 18;
 
-template <bool APPEND, typename T, bool E4M3, bool VEC, int HD, int U>
+template <bool APPEND, typename T, int KV, bool VEC, int HD, int U>
 void rows_launch(const RowsParams &p, cudaStream_t s) {
     const long threads = static_cast<long>(p.n) * 2 * ((p.kv.kv_heads + U - 1) / U) * (HD / 8);
     const unsigned blocks = static_cast<unsigned>((threads + kRowThreads - 1) / kRowThreads);
-    if constexpr (APPEND) ijb_kv_append_kernel<T, E4M3, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
-    else ijb_kv_gather_kernel<T, E4M3, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
+    if constexpr (APPEND) ijb_kv_append_kernel<T, KV, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
+    else ijb_kv_gather_kernel<T, KV, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
 }
-template <bool APPEND, typename T, bool E4M3, int HD>
+template <bool APPEND, typename T, int KV, int HD>
 void rows_launch(const RowsParams &p, bool vec, cudaStream_t s) {
     const bool many = static_cast<long>(p.n) * 2 * p.kv.kv_heads * (HD / 8) > kManyThreads && p.kv.kv_heads >= kHeads;
-    if (!vec) rows_launch<APPEND, T, E4M3, false, HD, 1>(p, s);
-    else if (many) rows_launch<APPEND, T, E4M3, true, HD, kHeads>(p, s);
-    else rows_launch<APPEND, T, E4M3, true, HD, 1>(p, s);
+    if (!vec) rows_launch<APPEND, T, KV, false, HD, 1>(p, s);
+    else if (many) rows_launch<APPEND, T, KV, true, HD, kHeads>(p, s);
+    else rows_launch<APPEND, T, KV, true, HD, 1>(p, s);
 }
-template <bool APPEND, typename T, bool E4M3>
+template <bool APPEND, typename T, int KV>
 void rows_launch(const RowsParams &p, bool vec, cudaStream_t s) {
-    if (p.kv.head_dim == 64) rows_launch<APPEND, T, E4M3, 64>(p, vec, s);
-    else rows_launch<APPEND, T, E4M3, 128>(p, vec, s);
+    if (p.kv.head_dim == 64) rows_launch<APPEND, T, KV, 64>(p, vec, s);
+    else rows_launch<APPEND, T, KV, 128>(p, vec, s);
+}
+
+template <bool APPEND, typename T>
+void rows_launch(const RowsParams &p, int type, bool vec, cudaStream_t s) {
+    if (type == IJB_KV_E2M1) rows_launch<APPEND, T, IJB_KV_E2M1>(p, vec, s);
+    else if (type == IJB_KV_E4M3) rows_launch<APPEND, T, IJB_KV_E4M3>(p, vec, s);
+    else rows_launch<APPEND, T, IJB_KV_F16>(p, vec, s);
 }
 
 template <bool APPEND>
@@ -298,11 +358,82 @@ int rows_call(const char *fn, const ijb_kv_view *view, int type, void *k, void *
         const bool vec = reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 &&
                          stride * elem % 16 == 0;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const bool e4m3 = view->type == IJB_KV_E4M3;
-        if (type == IJB_TYPE_F32)
-            e4m3 ? rows_launch<APPEND, float, true>(p, vec, s) : rows_launch<APPEND, float, false>(p, vec, s);
-        else
-            e4m3 ? rows_launch<APPEND, __half, true>(p, vec, s) : rows_launch<APPEND, __half, false>(p, vec, s);
+        if (type == IJB_TYPE_F32) rows_launch<APPEND, float>(p, view->type, vec, s);
+        else rows_launch<APPEND, __half>(p, view->type, vec, s);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return kv_fail(IJB_ERR_CUDA, fn, cudaGetErrorString(e));
+        count_launches(1);
+        return IJB_OK;
+    } catch (...) {
+        return IJB_ERR_NOMEM;
+    }
+}
+
+// Copies whole pages, one block a piece of kCopyPiece bytes (or less) of a page.
+struct CopyParams {
+    const uint8_t *from, *from_scale;
+    uint8_t *to, *to_scale;
+    long from_pages, to_pages;
+    long data_bytes, scale_bytes;  // of a page
+    int n, pieces;                 // pieces a page's data
+    const int *src, *dst;
+    uint32_t *status;
+};
+constexpr int kCopyThreads = 128, kCopyEach = 4, kCopyPiece = kCopyThreads * kCopyEach * 16;
+
+__global__ void __launch_bounds__(kCopyThreads) ijb_kv_copy_kernel(const __grid_constant__ CopyParams p) {
+    const int i = blockIdx.x / p.pieces, piece = blockIdx.x % p.pieces;
+    const int src = p.src[i], dst = p.dst[i];
+    if (dst < 0) return;
+    if (src < 0 || src >= p.from_pages || dst >= p.to_pages) {
+        if (p.status && threadIdx.x == 0) atomicOr(p.status, kDevErrBadIndex);
+        return;
+    }
+    const uint4 *s = reinterpret_cast<const uint4 *>(p.from + src * p.data_bytes);
+    uint4 *d = reinterpret_cast<uint4 *>(p.to + dst * p.data_bytes);
+    const long at = static_cast<long>(piece) * (kCopyPiece / 16) + threadIdx.x, end = p.data_bytes / 16;
+    uint4 x[kCopyEach];
+#pragma unroll
+    for (int k = 0; k < kCopyEach; ++k)
+        if (at + k * kCopyThreads < end) x[k] = s[at + k * kCopyThreads];
+#pragma unroll
+    for (int k = 0; k < kCopyEach; ++k)
+        if (at + k * kCopyThreads < end) d[at + k * kCopyThreads] = x[k];
+    if (piece == 0)
+        for (long b = threadIdx.x; b < p.scale_bytes; b += kCopyThreads)
+            p.to_scale[dst * p.scale_bytes + b] = p.from_scale[src * p.scale_bytes + b];
+}
+
+int copy_call(const char *fn, const ijb_kv_view *from, const ijb_kv_view *to, int n, const int *src, const int *dst,
+              uint32_t *status, void *stream) {
+    try {
+        KvDev a, b;
+        std::string bad = kv_view_check(from, &a);
+        if (bad.empty()) bad = kv_view_check(to, &b);
+        if (!bad.empty()) return kv_fail(IJB_ERR_INVALID, fn, bad);
+        if (from->type != to->type || from->kv_heads != to->kv_heads || from->head_dim != to->head_dim ||
+            from->page_size != to->page_size)
+            return kv_fail(IJB_ERR_INVALID, fn, "the two caches' pages differ");
+        if (n < 0) return kv_fail(IJB_ERR_INVALID, fn, "negative page count");
+        if (n == 0) return IJB_OK;
+        if (!src || !dst) return kv_fail(IJB_ERR_INVALID, fn, "null argument");
+        CopyParams p;
+        const long rows = 2L * from->kv_heads * from->page_size;
+        p.from = a.data;
+        p.from_scale = a.scale;
+        p.to = b.data;
+        p.to_scale = b.scale;
+        p.from_pages = from->num_pages;
+        p.to_pages = to->num_pages;
+        p.data_bytes = rows * kv_row_bytes(from->type, from->head_dim);
+        p.scale_bytes = from->type == IJB_KV_F16 ? 0 : from->type == IJB_KV_E4M3 ? rows : rows * (from->head_dim / kKvBlock);
+        p.pieces = static_cast<int>((p.data_bytes + kCopyPiece - 1) / kCopyPiece);
+        p.n = n;
+        p.src = src;
+        p.dst = dst;
+        p.status = status;
+        if (static_cast<long>(n) * p.pieces > 0x7fffffffL) return kv_fail(IJB_ERR_INVALID, fn, "too many pages for one call");
+        ijb_kv_copy_kernel<<<static_cast<unsigned>(n) * p.pieces, kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return kv_fail(IJB_ERR_CUDA, fn, cudaGetErrorString(e));
         count_launches(1);
@@ -327,6 +458,11 @@ int ijb_kv_gather(const ijb_kv_view *kv, int dst_type, void *k_dev, void *v_dev,
                   const int *tok_seq_dev, const int *tok_pos_dev, uint32_t *status_dev, void *stream) {
     return ijb::rows_call<false>("ijb_kv_gather", kv, dst_type, k_dev, v_dev, stride, n, tok_seq_dev, tok_pos_dev,
                                  status_dev, stream);
+}
+
+int ijb_kv_copy_pages(const ijb_kv_view *from, const ijb_kv_view *to, int n, const int *src_page_dev,
+                      const int *dst_page_dev, uint32_t *status_dev, void *stream) {
+    return ijb::copy_call("ijb_kv_copy_pages", from, to ? to : from, n, src_page_dev, dst_page_dev, status_dev, stream);
 }
 
 }  // extern "C"

@@ -3,6 +3,7 @@
 // paged_attention.cu).
 #pragma once
 #include <cuda_fp16.h>
+#include <cuda_fp4.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -16,8 +17,8 @@
 namespace ijb {
 
 // A row is one token's K or V of one KV head.  Rows of a page are laid out
-// [K, V][kv head][position in page][head_dim]; the scale byte of an e4m3 row
-// has the row's own index in the same order.
+// [K, V][kv head][position in page][head_dim]; the scale byte of an e4m3 row, or
+// the head_dim / 32 of an e2m1 row, have the row's own index in the same order.
 struct KvDev {
     uint8_t *data;
     uint8_t *scale;
@@ -31,6 +32,32 @@ struct KvDev {
 // 2^(s - 127) of a scale byte (0..254).
 __device__ __forceinline__ float kv_scale(uint32_t s) {
     return __uint_as_float(s ? s << 23 : 0x00400000u);
+}
+
+// e2m1 rows: two codes a byte, the even dim's in the low half; kKvBlock dims share a
+// scale, the fp16 number of the bits byte << 7 (an unsigned number of 5 exponent and 3
+// mantissa bits).  A code has 2 significant bits and a scale 4, so code * scale is an
+// fp16 number as long as it is no larger than one: scales up to 10240 (byte kKvTopScale).
+constexpr int kKvBlock = 32;
+constexpr uint32_t kKvTopScale = 226u, kKvNanScale = 255u;
+
+__host__ __device__ constexpr int kv_row_bytes(int type, int head_dim) {
+    return type == IJB_KV_E2M1 ? head_dim / 2 : (type == IJB_KV_E4M3 ? head_dim : 2 * head_dim);
+}
+
+// Codes of one byte (or the low one) as two fp16 numbers, of four bytes as eight: one
+// instruction a byte.
+__device__ __forceinline__ uint32_t e2m1x2_half2(uint32_t u) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(u));
+    return h;
+}
+__device__ __forceinline__ void e2m1x8_half2(uint32_t u, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(u));
 }
 
 // Row index of (page, which, head, offset); 64 bits: a pool may pass 2^31 rows.
@@ -47,6 +74,6 @@ inline int kv_fail(int code, const char *fn, const std::string &msg) {
 std::string kv_view_check(const ijb_kv_view *v, KvDev *out);
 // Sets the attributes of ijb_paged_attention's fp32 kernels on the current device
 // (done by the first call otherwise; an engine does it before it captures one).
-cudaError_t paged_attention_prepare(int head_dim, bool e4m3);
+cudaError_t paged_attention_prepare(int head_dim, int type);
 
 }  // namespace ijb

@@ -1,4 +1,4 @@
-// Attention of new tokens over the paged K/V cache (fp16 or e4m3 rows).
+// Attention of new tokens over the paged K/V cache (fp16, e4m3 or e2m1 rows).
 //
 // An entry is L new tokens, the last of a sequence's T cached positions.  With
 // G query heads to a KV head, its rows for one KV head are the L * G pairs
@@ -450,11 +450,13 @@ constexpr int kDecRows = 16;
 // sequences of 4 rows took 25 us with the wide kernel's 8 warps.  Of the e4m3 kernels at
 // head_dim 64, fp32 queries' does not fit 16 warps' registers: one token at position 4100, 8 KV heads, took
 // 18.0 us with 16 and 14.9 with 12, 16 contexts of 9,001 to 32,768 positions 103 and 98.
-template <int HD, bool E4M3, bool WIDE, typename T>
+template <int HD, int KV, bool WIDE, typename T>
 struct Dec {
-    static constexpr int kRowBytes = HD * (E4M3 ? 1 : 2);
+    static constexpr bool E4M3 = KV == IJB_KV_E4M3, E2M1 = KV == IJB_KV_E2M1;
+    static constexpr int kRowBytes = kv_row_bytes(KV, HD);
     static constexpr int kTile = kChunk * kRowBytes;
-    static constexpr int kStage = 2 * kTile + (E4M3 ? 256 : 0);  // K, V, their scale bytes and what they stand for
+    static constexpr int kScales = E2M1 ? kChunk * (HD / kKvBlock) : 0;  // K's or V's bytes (e2m1)
+    static constexpr int kStage = 2 * kTile + (E4M3 ? 256 : 2 * kScales);  // K, V, their scale bytes and (e4m3) what they stand for
     static constexpr int kWarps = kRowBytes == 256 ? 6 : (WIDE || HD == 128 ? 8 : (E4M3 && sizeof(T) == 2 ? 16 : 12));
     static constexpr int kStages = kRowBytes == 256 ? 2 : (kRowBytes == 128 ? (kWarps == 8 ? 3 : 2) : (WIDE ? 4 : 3));
     static constexpr int kSmem = kWarps * kStages * kStage;
@@ -465,7 +467,9 @@ constexpr int kDecPlanBytes = (kMaxEntries + 1) * 4;  // entries' first units
 // Byte offset of 16-byte piece c of row r in a chunk tile.
 template <int RB>
 __device__ __forceinline__ uint32_t dec_off(int r, int c) {
-    if constexpr (RB == 64)
+    if constexpr (RB == 32)
+        return static_cast<uint32_t>((r >> 2) * 128 + (((r & 3) ^ ((r >> 1) & 2)) << 5) + (c << 4));
+    else if constexpr (RB == 64)
         return static_cast<uint32_t>((((r >> 3) << 2) | (r & 3)) * 128 + ((((r >> 2) ^ (r >> 1)) & 1) << 6) +
                                      ((c ^ ((r & 1) << 1)) << 4));
     else
@@ -480,6 +484,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ uint32_t lds8(uint32_t addr) {
@@ -538,16 +547,17 @@ __device__ __forceinline__ void add_values(float (&o0)[4], float (&o1)[4], const
     add2_in_order(o1[2], o1[3], d1[2], d1[3]);
 }
 
-template <int HD, bool E4M3, bool WIDE, typename T>
-__global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
+template <int HD, int KV, bool WIDE, typename T>
+__global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
     ijb_paged_decode_kernel(const __grid_constant__ AttnArgs a) {
-    using D = Dec<HD, E4M3, WIDE, T>;
+    using D = Dec<HD, KV, WIDE, T>;
     constexpr int H = WIDE ? 2 : 1;  // halves of the 16 rows in use
     // up to 8 fp32 rows: their hi parts are rows 0..7 of the products, their lo
     // parts rows 8..15, for the products of one
     constexpr bool PAIR = sizeof(T) == 4 && !WIDE;
     constexpr int C = WIDE || PAIR ? 4 : 2;  // accumulators a lane
     constexpr bool SPLIT = sizeof(T) == 4;  // fp32 queries: hi + lo
+    constexpr bool E4M3 = D::E4M3, E2M1 = D::E2M1;
     constexpr int NT = D::kWarps * 32, RB = D::kRowBytes, KS = HD / 16, NTILE = HD / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PlanOut block_po;
@@ -617,6 +627,13 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
                 if (lane < 16 && r < left && row8 >= 0)
                     cp_async4(st + 2 * D::kTile + lane * 4, a.kv.scale + row8 + (r & 7) + (lane < 8 ? 0 : v_off));
             }
+            if constexpr (E2M1) {  // 16 scale bytes a copy, K's and then V's
+                constexpr int NB = HD / kKvBlock, N = D::kScales / 16, R = 16 / NB;  // copies, rows a copy
+                const int r = (lane & (N - 1)) * R;
+                const long row8 = __shfl_sync(0xffffffffu, next_row, r & ~7);
+                if (lane < 2 * N && r < left && row8 >= 0)
+                    cp_async16(st + 2 * D::kTile + lane * 16, a.kv.scale + (row8 + (r & 7) + (lane < N ? 0 : v_off)) * NB, true);
+            }
             if (++lb == ls.b1) {
                 more = cursor_next(a, load_c, ls);
                 lb = ls.b0;
@@ -646,7 +663,8 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
             const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const int d = E4M3 ? (t4 + 4 * (ks >> 2)) * 16 + 4 * (ks & 3) : (t4 + 4 * (ks >> 1)) * 8 + 4 * (ks & 1);
+                const int d = E2M1 ? t4 * (HD / 4) + 4 * ks
+                              : E4M3 ? (t4 + 4 * (ks >> 2)) * 16 + 4 * (ks & 3) : (t4 + 4 * (ks >> 1)) * 8 + 4 * (ks & 1);
                 const float4 v = r < rows ? load4(src + d, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
                 const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
                 qf[ks][hf] = *reinterpret_cast<const uint32_t *>(&h0);
@@ -700,6 +718,24 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
                 for (int i = 0; i < 8; ++i) kscale[i] = __uint_as_float(ku[i]);
                 vscale[0] = vv.x; vscale[1] = vv.y; vscale[2] = vv.z; vscale[3] = vv.w;
             }
+            // e2m1: scales as pairs of fp16 numbers, of position r(nt)'s block of K and of pairs of positions' of V;
+            // those behind the last position mean nothing
+            [[maybe_unused]] uint32_t kpair[4], vpair[4];
+            if constexpr (E2M1) {
+                constexpr int NB = HD / kKvBlock;
+                const int left = s.x.kv - p0;
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt) {
+                    const int r = 8 * nt + (gid >> 1) + 4 * (gid & 1);
+                    kpair[nt] = lds8(sc + r * NB + t4 * NB / 4) * 0x00800080u;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 8 * i + t4, at = sc + D::kScales + gid * NB / 8;
+                    const uint32_t lo = r < left ? lds8(at + r * NB) : 0u, hi = r + 4 < left ? lds8(at + (r + 4) * NB) : 0u;
+                    vpair[i] = (lo | hi << 16) << 7;
+                }
+            }
             // ---- scores: tile nt, column n is position 16 (nt / 2) + 8 (nt % 2) + n / 2 + 4 (n % 2)
             float p[4][C];
 #pragma unroll
@@ -707,6 +743,28 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
 #pragma unroll
                 for (int k = 0; k < C; ++k) p[nt][k] = 0.f;
                 const int r = 8 * nt + (gid >> 1) + 4 * (gid & 1);
+                if constexpr (E2M1) {
+                    uint32_t u[HD / 32];
+                    if constexpr (HD == 128) {
+                        const uint4 w = lds128(kt + dec_off<RB>(r, t4));
+                        u[0] = w.x; u[1] = w.y; u[2] = w.z; u[3] = w.w;
+                    } else {
+                        const uint2 w = lds64(kt + dec_off<RB>(r, t4 >> 1) + 8 * (t4 & 1));
+                        u[0] = w.x; u[1] = w.y;
+                    }
+#pragma unroll
+                    for (int e = 0; e < HD / 32; ++e) {
+                        uint32_t h[4];
+                        e2m1x8_half2(u[e], h);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) h[i] = hmul2(h[i], kpair[nt]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            mma(p[nt], qf[2 * e + i], h[2 * i], h[2 * i + 1]);
+                            if constexpr (SPLIT && WIDE) mma(p[nt], ql[2 * e + i], h[2 * i], h[2 * i + 1]);
+                        }
+                    }
+                } else
 #pragma unroll
                 for (int j = 0; j < RB / 64; ++j) {
                     const uint4 w = lds128(kt + dec_off<RB>(r, t4 + 4 * j));
@@ -800,7 +858,35 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
                     }
                 };
                 const int r0 = 16 * st + t4;
-                if constexpr (E4M3) {
+                if constexpr (E2M1) {
+                    const uint32_t sa = vpair[2 * st], sb = vpair[2 * st + 1];
+                    uint32_t w[4][HD / 64];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = r0 + 4 * i;
+                        if constexpr (HD == 128) {
+                            const uint2 x = lds64(vt + dec_off<RB>(r, gid >> 1) + 8 * (gid & 1));
+                            w[i][0] = x.x; w[i][1] = x.y;
+                        } else {
+                            w[i][0] = lds32(vt + dec_off<RB>(r, gid >> 2) + 4 * (gid & 3));
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < HD / 64; ++k) {
+                        // bytes of two positions' codes of one dim: even dims, odd dims
+                        uint32_t a0[4], a1[4], b0[4], b1[4];
+                        constexpr uint32_t LO = 0x0f0f0f0fu;
+                        e2m1x8_half2((w[0][k] & LO) | ((w[1][k] << 4) & ~LO), a0);
+                        e2m1x8_half2(((w[0][k] >> 4) & LO) | (w[1][k] & ~LO), a1);
+                        e2m1x8_half2((w[2][k] & LO) | ((w[3][k] << 4) & ~LO), b0);
+                        e2m1x8_half2(((w[2][k] >> 4) & LO) | (w[3][k] & ~LO), b1);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t vb[4] = {hmul2(a0[j], sa), hmul2(b0[j], sb), hmul2(a1[j], sa), hmul2(b1[j], sb)};
+                            values(o[8 * k + 2 * j], o[8 * k + 2 * j + 1], vb);
+                        }
+                    }
+                } else if constexpr (E4M3) {
                     const uint32_t sa = vscale[2 * st], sb = vscale[2 * st + 1];
                     uint32_t w[4][HD / 32];
 #pragma unroll
@@ -878,7 +964,7 @@ __global__ void __launch_bounds__(Dec<HD, E4M3, WIDE, T>::kWarps * 32, 1)
                 part[kDecRows * HD + kDecRows + r] = l[hf];
             }
             // lane t4's columns n = 2 t4, 2 t4 + 1 of tile i: dim n * W + i (W dims a piece), pieces of 64 dims apart
-            constexpr int W = E4M3 && HD == 128 ? 16 : 8;
+            constexpr int W = (E4M3 || E2M1) && HD == 128 ? 16 : 8;
 #pragma unroll
             for (int h = 0; h < NTILE / W; ++h)
 #pragma unroll
@@ -1074,11 +1160,12 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c) {
 // copies: LANES 16-byte pieces of a row side by side (an e4m3 row's four then
 // fall on different banks than the next row's once they are fp16), HALVES times.
 // Page ids are read a block ahead, for their latency.
-template <int HD, bool E4M3>
+template <int HD, int KV>
 struct Rows {
-    static constexpr int LANES = E4M3 ? 4 : 8, HALVES = HD / 64;
+    static constexpr bool E4M3 = KV == IJB_KV_E4M3, E2M1 = KV == IJB_KV_E2M1;
+    static constexpr int LANES = E2M1 ? HD / 32 : (E4M3 ? 4 : 8), HALVES = E2M1 ? 1 : HD / 64;
     static constexpr int RS = 128 / LANES, N = 128 / RS;  // rows a step, rows of a thread
-    static constexpr int RB = HD * (E4M3 ? 1 : 2);
+    static constexpr int RB = kv_row_bytes(KV, HD);
     int next[N];   // page ids of the block after this one
     long row[N];   // cache rows (K)
     int live;      // bit k: row k's position exists, and its page
@@ -1123,9 +1210,9 @@ struct Rows {
 };
 
 // Loads the K and V blocks of a worker's runs (128 threads, p of them).
-template <int HD, bool E4M3, int BUFS>
+template <int HD, int KV, int BUFS>
 __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, TileCtl *ctl, int p) {
-    using R = Rows<HD, E4M3>;
+    using R = Rows<HD, KV>;
     constexpr int STEPS = R::N * R::HALVES, RB = R::RB;
     const int pc = p % R::LANES, pr = p / R::LANES;
     const long v_off = static_cast<long>(a.kv.kv_heads) << a.kv.page_shift;
@@ -1135,7 +1222,7 @@ __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, 
         if (i >= BUFS) wait_bar(a, ctl, &ctl->empty[i % BUFS], (i / BUFS - 1) & 1);
     };
     int i = 0;  // buffers filled so far
-    if constexpr (E4M3) {
+    if constexpr (R::E4M3 || R::E2M1) {
         uint4 wk[STEPS], wv[STEPS];
         uint32_t sk[R::N], sv[R::N];
         auto load = [&](uint4(&w)[STEPS], uint32_t(&sc)[R::N], long off) {
@@ -1146,13 +1233,31 @@ __device__ void tile_load(const AttnArgs &a, Cursor c, uint32_t bufs, int part, 
                 const long r = rows.row[j] + off;
                 w[k] = in ? *reinterpret_cast<const uint4 *>(a.kv.data + r * RB + (pc + h * R::LANES) * 16)
                           : make_uint4(0, 0, 0, 0);
-                if (h == 0) sc[j] = in ? a.kv.scale[r] : 127u;
+                if constexpr (R::E2M1) sc[j] = in ? a.kv.scale[r * R::LANES + pc] : 0u;  // a piece is a block of 32
+                else if (h == 0) sc[j] = in ? a.kv.scale[r] : 127u;
             }
         };
         auto store = [&](const uint4(&w)[STEPS], const uint32_t(&sc)[R::N]) {
             wait_empty(i);
             const uint32_t dst = bufs + (i % BUFS) * part;
-            auto scaled = [&](auto twice) {
+            if constexpr (R::E2M1) {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                    const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w}, sb = sc[k] * 0x00800080u;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        uint32_t h[4];
+                        e2m1x8_half2(u[n], h);
+                        sts128(dst + tile_off(k * R::RS + pr, 4 * pc + n), hmul2(h[0], sb), hmul2(h[1], sb), hmul2(h[2], sb),
+                               hmul2(h[3], sb));
+                    }
+                }
+                proxy_fence();
+                mbar_arrive(&ctl->full[i % BUFS]);
+                ++i;
+                return;
+            }
+            [[maybe_unused]] auto scaled = [&](auto twice) {
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
                     const int j = k / R::HALVES, c2 = 2 * (pc + (k % R::HALVES) * R::LANES);
@@ -1651,7 +1756,7 @@ __device__ void tile_softmax(const AttnArgs &a, Cursor c, int worker, uint32_t q
     }
 }
 
-template <int HD, bool E4M3, typename T>
+template <int HD, int KV, typename T>
 __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const __grid_constant__ AttnArgs a) {
     using L = Tile<HD, T>;
     extern __shared__ uint8_t raw[];
@@ -1705,7 +1810,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
             tile_mma<HD, L::kSplit, L::kBufs, L::kFlush>(a, c, q, bufs, L::kPart, &ctl, tmem, warp - kMmaWarpId);
     } else if (warp >= kLoadWarp0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
-        tile_load<HD, E4M3, L::kBufs>(a, c, bufs, L::kPart, &ctl, threadIdx.x - kLoadWarp0 * 32);
+        tile_load<HD, KV, L::kBufs>(a, c, bufs, L::kPart, &ctl, threadIdx.x - kLoadWarp0 * 32);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         tile_softmax<HD, T>(a, c, blockIdx.x, q, L::kPart, &ctl, tmem, warp >> 2, threadIdx.x & 127);
@@ -1728,16 +1833,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) ijb_paged_tile_kernel(const _
 // page (nothing was read for it, and its positions counted as zeros), `all` rows of
 // the tiles are computed again, without those positions: a mask for them in the kernels' own
 // loops would cost every call.
-template <int HD, bool E4M3>
+template <int HD, int KV>
 __device__ __forceinline__ float cached(const AttnArgs &a, long row, int d) {
-    if constexpr (E4M3) {
+    if constexpr (KV == IJB_KV_E2M1) {
+        const uint32_t code = a.kv.data[row * (HD / 2) + (d >> 1)] >> (4 * (d & 1));
+        const uint32_t h = e2m1x2_half2(code & 15u), s = a.kv.scale[row * (HD / kKvBlock) + d / kKvBlock] << 7;
+        return __low2float(__hmul2(*reinterpret_cast<const __half2 *>(&h), *reinterpret_cast<const __half2 *>(&s)));
+    } else if constexpr (KV == IJB_KV_E4M3) {
         const uint32_t h = e4m3x2_half2(a.kv.data[row * HD + d]);
         return __half2float(__float2half_rn(__low2float(*reinterpret_cast<const __half2 *>(&h)) * kv_scale(a.kv.scale[row])));
     } else {
         return __half2float(reinterpret_cast<const __half *>(a.kv.data)[row * HD + d]);
     }
 }
-template <int ROWS, int HD, int NT, int RB, bool E4M3, typename T>
+template <int ROWS, int HD, int NT, int RB, int KV, typename T>
 __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool all, float4 *shared) {
     float *weight = reinterpret_cast<float *>(shared), *red = weight + NT;  // 4 * NT floats are there
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1765,7 +1874,7 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool 
                 const long row = t0 + tid < n ? slot(t0 + tid) : -1;
                 if (row >= 0) {
                     x = 0.f;
-                    for (int d = 0; d < HD; ++d) x = fmaf(static_cast<float>(q[d]), cached<HD, E4M3>(a, row, d), x);
+                    for (int d = 0; d < HD; ++d) x = fmaf(static_cast<float>(q[d]), cached<HD, KV>(a, row, d), x);
                     x *= a.scale_log2;
                 }
                 const float mx = warp_max(x);  // a NaN is left to its weight
@@ -1787,7 +1896,7 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool 
                 if (tid < HD)
                     for (int i = 0; i < min(NT, n - t0); ++i) {
                         const long v = slot(t0 + i);
-                        if (v >= 0) o = fmaf(weight[i], cached<HD, E4M3>(a, v + v_off, tid), o);
+                        if (v >= 0) o = fmaf(weight[i], cached<HD, KV>(a, v + v_off, tid), o);
                     }
             }
             if (tid < HD) out[tid] = static_cast<T>(o * (l > 0.f || l != l ? 1.f / l : 0.f));
@@ -1804,7 +1913,7 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool 
 // positions, 12 rows of 128 each, took 25, 30, 39 and 80 us in all with 1, 2, 4 and 16
 // rows a block, and 64 ragged sequences 27, 25, 25 and 27 us.
 constexpr int kMergeBatch = 4;
-template <int ROWS, int HD, int NT, int EACH, int RB, bool E4M3, typename T>
+template <int ROWS, int HD, int NT, int EACH, int RB, int KV, typename T>
 __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_constant__ AttnArgs a) {
     __shared__ float top[RB], total[RB];
     __shared__ float4 sum[NT];
@@ -1911,7 +2020,7 @@ __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_consta
     }
     for (; again; again &= again - 1) {
         const int j = __ffs(again) - 1;
-        mend_rows<ROWS, HD, NT, RB, E4M3, T>(a, blockIdx.x * EACH + j, row0, (all >> j) & 1, sum);
+        mend_rows<ROWS, HD, NT, RB, KV, T>(a, blockIdx.x * EACH + j, row0, (all >> j) & 1, sum);
     }
 }
 
@@ -1946,7 +2055,7 @@ cudaError_t allow_smem(K kernel, int bytes) {
 
 // The merge behind the kernel just launched, on the GPU early (programmatic
 // dependent launch): it waits there for the states.
-template <int ROWS, int HD, bool E4M3, typename T>
+template <int ROWS, int HD, int KV, typename T>
 cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
@@ -1961,30 +2070,30 @@ cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, ijb_paged_merge_kernel<ROWS, HD, NT, EACH, RB, E4M3, T>, a);
+    e = cudaLaunchKernelEx(&cfg, ijb_paged_merge_kernel<ROWS, HD, NT, EACH, RB, KV, T>, a);
     count_launches(2);
     return e;
 }
 
-template <int HD, bool E4M3, bool WIDE, typename T>
+template <int HD, int KV, bool WIDE, typename T>
 constexpr int decode_smem() {
-    return Dec<HD, E4M3, WIDE, T>::kSmem > kDecPlanBytes ? Dec<HD, E4M3, WIDE, T>::kSmem : kDecPlanBytes;
+    return Dec<HD, KV, WIDE, T>::kSmem > kDecPlanBytes ? Dec<HD, KV, WIDE, T>::kSmem : kDecPlanBytes;
 }
-template <int HD, bool E4M3, bool WIDE, typename T>
+template <int HD, int KV, bool WIDE, typename T>
 cudaError_t decode_allow() {
-    auto kernel = ijb_paged_decode_kernel<HD, E4M3, WIDE, T>;
-    return allow_smem<decltype(kernel), Dec<HD, E4M3, WIDE, T>, T>(kernel, decode_smem<HD, E4M3, WIDE, T>());
+    auto kernel = ijb_paged_decode_kernel<HD, KV, WIDE, T>;
+    return allow_smem<decltype(kernel), Dec<HD, KV, WIDE, T>, T>(kernel, decode_smem<HD, KV, WIDE, T>());
 }
-template <int HD, bool E4M3, typename T>
+template <int HD, int KV, typename T>
 cudaError_t tile_allow() {
-    auto kernel = ijb_paged_tile_kernel<HD, E4M3, T>;
-    return allow_smem<decltype(kernel), Tile<HD, T>, std::bool_constant<E4M3>>(kernel, Tile<HD, T>::kSmem);
+    auto kernel = ijb_paged_tile_kernel<HD, KV, T>;
+    return allow_smem<decltype(kernel), Tile<HD, T>, std::integral_constant<int, KV>>(kernel, Tile<HD, T>::kSmem);
 }
 
-template <int HD, bool E4M3, bool WIDE, typename T>
+template <int HD, int KV, bool WIDE, typename T>
 cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
-    using D = Dec<HD, E4M3, WIDE, T>;
-    const cudaError_t e = decode_allow<HD, E4M3, WIDE, T>();
+    using D = Dec<HD, KV, WIDE, T>;
+    const cudaError_t e = decode_allow<HD, KV, WIDE, T>();
     if (e != cudaSuccess) return e;
     a.min_rows = 1;
     a.max_rows = WIDE ? kDecRows : 8;
@@ -1995,14 +2104,14 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.min_units = 2;
     a.over = 1;
     a.least = 1;
-    ijb_paged_decode_kernel<HD, E4M3, WIDE, T><<<sms, D::kWarps * 32, decode_smem<HD, E4M3, WIDE, T>(), s>>>(a);
-    return merge_launch<kDecRows, HD, E4M3, T>(a, s);
+    ijb_paged_decode_kernel<HD, KV, WIDE, T><<<sms, D::kWarps * 32, decode_smem<HD, KV, WIDE, T>(), s>>>(a);
+    return merge_launch<kDecRows, HD, KV, T>(a, s);
 }
 
-template <int HD, bool E4M3, typename T>
+template <int HD, int KV, typename T>
 cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     using L = Tile<HD, T>;
-    const cudaError_t e = tile_allow<HD, E4M3, T>();
+    const cudaError_t e = tile_allow<HD, KV, T>();
     if (e != cudaSuccess) return e;
     a.min_rows = min_rows;
     a.max_rows = 0x7fffffff;
@@ -2013,8 +2122,8 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     a.min_units = 2;
     a.over = 4;
     a.least = 2;
-    ijb_paged_tile_kernel<HD, E4M3, T><<<sms, kTileThreads, L::kSmem, s>>>(a);
-    return merge_launch<kTileRows, HD, E4M3, T>(a, s);
+    ijb_paged_tile_kernel<HD, KV, T><<<sms, kTileThreads, L::kSmem, s>>>(a);
+    return merge_launch<kTileRows, HD, KV, T>(a, s);
 }
 
 // Which kernels serve a call.  Entries of up to 16 rows go to the decode kernel,
@@ -2022,20 +2131,23 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
 // entries leaves them all to the tile kernel, for the launches: entries of 1 to 40 tokens
 // behind 100 to 2000 take 49 us so and 55 with both kernels for 2 of them, 51 and 56 for 7, 55 and 59 for 8, 77 and
 // 89 for 16 (so the border could lie higher); one of 200 tokens among single ones 54 and 68 for 4, 98 and 83 for 32.
-template <int HD, bool E4M3, typename T>
+template <int HD, int KV, typename T>
 cudaError_t attention_call(const AttnArgs &a, int max_q, int sms, cudaStream_t s) {
     const long most = static_cast<long>(max_q > 0 ? min(max_q, a.n_tokens) : a.n_tokens) * a.group;
-    if (most <= 8) return decode_launch<HD, E4M3, false, T>(a, sms, true, s);
-    if (most <= kDecRows) return decode_launch<HD, E4M3, true, T>(a, sms, true, s);
-    if (a.n_entries < 8) return tile_launch<HD, E4M3, T>(a, sms, 1, s);
-    const cudaError_t e = decode_launch<HD, E4M3, true, T>(a, sms, false, s);
-    return e != cudaSuccess ? e : tile_launch<HD, E4M3, T>(a, sms, kDecRows + 1, s);
+    if (most <= 8) return decode_launch<HD, KV, false, T>(a, sms, true, s);
+    if (most <= kDecRows) return decode_launch<HD, KV, true, T>(a, sms, true, s);
+    if (a.n_entries < 8) return tile_launch<HD, KV, T>(a, sms, 1, s);
+    const cudaError_t e = decode_launch<HD, KV, true, T>(a, sms, false, s);
+    return e != cudaSuccess ? e : tile_launch<HD, KV, T>(a, sms, kDecRows + 1, s);
+}
+template <int KV, typename T>
+cudaError_t attention_call(const AttnArgs &a, int max_q, int sms, cudaStream_t s) {
+    return a.kv.head_dim == 64 ? attention_call<64, KV, T>(a, max_q, sms, s) : attention_call<128, KV, T>(a, max_q, sms, s);
 }
 template <typename T>
-cudaError_t attention_call(const AttnArgs &a, bool e4m3, int max_q, int sms, cudaStream_t s) {
-    if (a.kv.head_dim == 64)
-        return e4m3 ? attention_call<64, true, T>(a, max_q, sms, s) : attention_call<64, false, T>(a, max_q, sms, s);
-    return e4m3 ? attention_call<128, true, T>(a, max_q, sms, s) : attention_call<128, false, T>(a, max_q, sms, s);
+cudaError_t attention_call(const AttnArgs &a, int type, int max_q, int sms, cudaStream_t s) {
+    if (type == IJB_KV_E2M1) return attention_call<IJB_KV_E2M1, T>(a, max_q, sms, s);
+    return type == IJB_KV_E4M3 ? attention_call<IJB_KV_E4M3, T>(a, max_q, sms, s) : attention_call<IJB_KV_F16, T>(a, max_q, sms, s);
 }
 
 constexpr int kMaxWorkers = 16;  // per SM: the decode kernel's warps
@@ -2048,19 +2160,21 @@ size_t workspace_bytes(int sms, int head_dim) {
     return static_cast<size_t>(sms) * kMaxWorkers * sizeof(Left) + held + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
 }
 
-template <int HD, bool E4M3>
+template <int HD, int KV>
 cudaError_t prepare() {
-    cudaError_t e = decode_allow<HD, E4M3, false, float>();
-    if (e == cudaSuccess) e = decode_allow<HD, E4M3, true, float>();
-    if (e == cudaSuccess) e = tile_allow<HD, E4M3, float>();
+    cudaError_t e = decode_allow<HD, KV, false, float>();
+    if (e == cudaSuccess) e = decode_allow<HD, KV, true, float>();
+    if (e == cudaSuccess) e = tile_allow<HD, KV, float>();
     return e;
 }
 
 }  // namespace
 
-cudaError_t paged_attention_prepare(int head_dim, bool e4m3) {
-    if (head_dim == 64) return e4m3 ? prepare<64, true>() : prepare<64, false>();
-    return e4m3 ? prepare<128, true>() : prepare<128, false>();
+cudaError_t paged_attention_prepare(int head_dim, int type) {
+    const bool small = head_dim == 64;
+    if (type == IJB_KV_E2M1) return small ? prepare<64, IJB_KV_E2M1>() : prepare<128, IJB_KV_E2M1>();
+    if (type == IJB_KV_E4M3) return small ? prepare<64, IJB_KV_E4M3>() : prepare<128, IJB_KV_E4M3>();
+    return small ? prepare<64, IJB_KV_F16>() : prepare<128, IJB_KV_F16>();
 }
 
 }  // namespace ijb
@@ -2089,6 +2203,8 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         if (!bad.empty()) return kv_fail(IJB_ERR_INVALID, fn, bad);
         if (reinterpret_cast<uintptr_t>(kv->scale_dev) % 4 && kv->type == IJB_KV_E4M3)
             return kv_fail(IJB_ERR_INVALID, fn, "scale bytes must be 4-byte aligned");
+        if (reinterpret_cast<uintptr_t>(kv->scale_dev) % 16 && kv->type == IJB_KV_E2M1)
+            return kv_fail(IJB_ERR_INVALID, fn, "an e2m1 cache's scale bytes must be 16-byte aligned");
         if (type != IJB_TYPE_F32 && type != IJB_TYPE_F16)
             return kv_fail(IJB_ERR_INVALID, fn, "query type must be IJB_TYPE_F32 or IJB_TYPE_F16");
         if (heads < 1 || heads % kv->kv_heads != 0 || heads / kv->kv_heads > 16)
@@ -2136,9 +2252,8 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
         a.held = a.part + static_cast<size_t>(sms) * 2 * kTileRows * (kv->head_dim + 2);
         a.status = status_dev;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const bool e4m3 = kv->type == IJB_KV_E4M3;
-        const cudaError_t e = type == IJB_TYPE_F32 ? attention_call<float>(a, e4m3, max_q, sms, s)
-                                                   : attention_call<__half>(a, e4m3, max_q, sms, s);
+        const cudaError_t e = type == IJB_TYPE_F32 ? attention_call<float>(a, kv->type, max_q, sms, s)
+                                                   : attention_call<__half>(a, kv->type, max_q, sms, s);
         if (e != cudaSuccess) return kv_fail(IJB_ERR_CUDA, fn, cudaGetErrorString(e));
         return IJB_OK;
     } catch (...) {

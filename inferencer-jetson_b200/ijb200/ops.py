@@ -17,8 +17,9 @@ from . import lib as _L
 from .lib import IjbError  # noqa: F401  (what the calls raise)
 
 F32, F16 = 0, 1  # IJB_TYPE_F32, IJB_TYPE_F16
-KV_F16, KV_E4M3 = 0, 2
+KV_F16, KV_E4M3, KV_E2M1 = 0, 2, 3
 _TYPE = {torch.float32: F32, torch.float16: F16}
+_KV = {torch.float16: KV_F16, torch.float8_e4m3fn: KV_E4M3, torch.float4_e2m1fn_x2: KV_E2M1}
 _stream = torch._C._cuda_getCurrentRawStream
 _current = torch._C._cuda_getDevice
 _empty = torch.empty
@@ -63,29 +64,33 @@ class PagedKV:
     """One paged K/V cache over the caller's tensors: ``data`` [pages, 2, kv_heads,
     page_size, head_dim] float16 or float8_e4m3fn, ``page_table`` [seqs, max_pages]
     int32, and for e4m3 ``scale`` [pages, 2, kv_heads, page_size] uint8 (a row's
-    values are data * 2^(scale - 127)).  ``status``, if given, is one int32 or
+    values are data * 2^(scale - 127)).  A cache in 4 bits has ``data`` [.., head_dim / 2]
+    float4_e2m1fn_x2 (two codes a byte, the even dim in the low half) and ``scale``
+    [.., page_size, head_dim / 32] uint8: 32 dims' values are their codes times the fp16
+    number of the bits scale << 7.  ``status``, if given, is one int32 or
     uint32 that collects the kernels' reports of indexes that name nothing."""
 
     def __init__(self, data, page_table, scale=None, status=None):
         _need(data.is_cuda and data.dim() == 5 and data.shape[1] == 2 and data.is_contiguous(),
               "data: expected a contiguous [pages, 2, kv_heads, page_size, head_dim] CUDA tensor")
-        _need(data.dtype in (torch.float16, torch.float8_e4m3fn), "data: expected float16 or float8_e4m3fn")
-        dev = data.get_device()
+        _need(data.dtype in _KV, "data: expected float16, float8_e4m3fn or float4_e2m1fn_x2")
+        kv, dev = _KV[data.dtype], data.get_device()
         _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_contiguous() and
               page_table.get_device() == dev, "page_table: expected a contiguous [seqs, max_pages] int32 tensor beside data")
-        e4m3 = data.dtype == torch.float8_e4m3fn
-        _need(not e4m3 or scale is not None and scale.dtype == torch.uint8 and scale.shape == data.shape[:4] and
+        self.head_dim = data.shape[4] * (2 if kv == KV_E2M1 else 1)
+        shape = data.shape[:4] + ((self.head_dim // 32,) if kv == KV_E2M1 else ())
+        _need(kv == KV_F16 or scale is not None and scale.dtype == torch.uint8 and scale.shape == shape and
               scale.is_contiguous() and scale.get_device() == dev,
-              "scale: an e4m3 cache needs contiguous uint8 [pages, 2, kv_heads, page_size] beside data")
+              f"scale: this cache needs contiguous uint8 {list(shape)} beside data")
         _need(status is None or status.dtype in (torch.int32, torch.uint32) and status.numel() == 1 and status.get_device() == dev,
               "status: expected one 32-bit word beside data")
-        self.data, self.page_table, self.scale, self.status = data, page_table, scale if e4m3 else None, status
-        self.device, self.kv_heads, self.head_dim = dev, data.shape[2], data.shape[4]
+        self.data, self.page_table, self.scale, self.status = data, page_table, None if kv == KV_F16 else scale, status
+        self.device, self.kv_heads = dev, data.shape[2]
         self.row = self.kv_heads * self.head_dim
         self._lib = _L.load()
-        self._view = _L.KvView(type=KV_E4M3 if e4m3 else KV_F16, kv_heads=self.kv_heads, head_dim=self.head_dim,
+        self._view = _L.KvView(type=kv, kv_heads=self.kv_heads, head_dim=self.head_dim,
                                page_size=data.shape[3], num_pages=data.shape[0], data_dev=data.data_ptr(),
-                               scale_dev=scale.data_ptr() if e4m3 else None, page_table_dev=page_table.data_ptr(),
+                               scale_dev=None if kv == KV_F16 else scale.data_ptr(), page_table_dev=page_table.data_ptr(),
                                n_seqs=page_table.shape[0], max_pages=page_table.shape[1])
         self._ref = ctypes.byref(self._view)
         self._status = status.data_ptr() if status is not None else None
@@ -113,6 +118,15 @@ class PagedKV:
         _call(self.device, self._lib.ijb_kv_gather, self._ref, _TYPE[dtype], k.data_ptr(), v.data_ptr(), self.row, n,
               _ptr(seq, torch.int32, n, self.device, "seq"), _ptr(pos, torch.int32, n, self.device, "pos"), self._status)
         return k, v
+
+    def copy_pages(self, src, dst, to=None) -> None:
+        """Copies pages src [n] of this cache to pages dst [n] of it (or of ``to``, another cache of the same kind beside
+        it), as they are.  No page may be a destination twice, nor both source and destination."""
+        n, dev = src.numel(), self.device
+        if to is not None and to.device != dev:
+            raise ValueError("to: expected a cache on the same device")
+        _call(dev, self._lib.ijb_kv_copy_pages, self._ref, None if to is None else to._ref, n,
+              _ptr(src, torch.int32, n, dev, "src"), _ptr(dst, torch.int32, n, dev, "dst"), self._status)
 
     def attention(self, q, q_start, kv_len, seq=None, max_q: int = 0, scale: float | None = None, out=None):
         """Attention of new tokens: q [tokens, heads, head_dim] fp32 or fp16, entry e's tokens being rows

@@ -1,0 +1,36 @@
+"""Refusals of a cache in 4 bits: bad arguments come back as errors before any CUDA call."""
+import ctypes
+
+import pytest
+
+from ijb200 import lib
+
+
+def view(**kw):
+    base = dict(type=3, kv_heads=2, head_dim=64, page_size=16, num_pages=4, data_dev=4096, scale_dev=8192,
+                page_table_dev=256, n_seqs=1, max_pages=4)
+    base.update(kw)
+    return lib.KvView(**base)
+
+
+BAD_VIEWS = [dict(type=4), dict(kv_heads=0), dict(head_dim=96), dict(head_dim=32), dict(page_size=4), dict(num_pages=0),
+             dict(n_seqs=0), dict(max_pages=0), dict(data_dev=None), dict(data_dev=4104), dict(scale_dev=None),
+             dict(page_table_dev=None)]
+
+
+@pytest.mark.parametrize("bad", BAD_VIEWS)
+@pytest.mark.parametrize("fn", ["ijb_kv_append", "ijb_kv_gather"])
+def test_views_are_checked(fn, bad):
+    L = lib.load()
+    v = view(**bad)
+    assert getattr(L, fn)(ctypes.byref(v), 0, 4096, 4096, 128, 1, 256, 256, None, None) == lib.ERR_INVALID
+    assert fn in L.ijb_last_error(None).decode()
+
+
+@pytest.mark.parametrize("bad", BAD_VIEWS + [dict(scale_dev=8196), dict(scale_dev=8200)])
+def test_attention_views_are_checked(bad):
+    L = lib.load()
+    v = view(**bad)
+    assert L.ijb_paged_attention(ctypes.byref(v), 4, 0, 4096, 256, 8192, 256, 2, 1, 256, None, 256, 1, 0.125, 4096,
+                                 1 << 40, None, None) == lib.ERR_INVALID
+    assert "ijb_paged_attention" in L.ijb_last_error(None).decode()
