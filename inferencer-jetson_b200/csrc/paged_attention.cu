@@ -452,11 +452,10 @@ constexpr int kDecRows = 16;
 // 18.0 us with 16 and 14.9 with 12, 16 contexts of 9,001 to 32,768 positions 103 and 98.
 template <int HD, int KV, bool WIDE, typename T>
 struct Dec {
-    static constexpr bool E4M3 = KV == IJB_KV_E4M3, E2M1 = KV == IJB_KV_E2M1;
+    static constexpr bool E4M3 = KV == IJB_KV_E4M3;
     static constexpr int kRowBytes = kv_row_bytes(KV, HD);
     static constexpr int kTile = kChunk * kRowBytes;
-    static constexpr int kScales = E2M1 ? kChunk * (HD / kKvBlock) : 0;  // K's or V's bytes (e2m1)
-    static constexpr int kStage = 2 * kTile + (E4M3 ? 256 : 2 * kScales);  // K, V, their scale bytes and (e4m3) what they stand for
+    static constexpr int kStage = 2 * kTile + (E4M3 ? 256 : 0);  // K, V, their scale bytes and what they stand for
     static constexpr int kWarps = kRowBytes == 256 ? 6 : (WIDE || HD == 128 ? 8 : (E4M3 && sizeof(T) == 2 ? 16 : 12));
     static constexpr int kStages = kRowBytes == 256 ? 2 : (kRowBytes == 128 ? (kWarps == 8 ? 3 : 2) : (WIDE ? 4 : 3));
     static constexpr int kSmem = kWarps * kStages * kStage;
@@ -467,9 +466,7 @@ constexpr int kDecPlanBytes = (kMaxEntries + 1) * 4;  // entries' first units
 // Byte offset of 16-byte piece c of row r in a chunk tile.
 template <int RB>
 __device__ __forceinline__ uint32_t dec_off(int r, int c) {
-    if constexpr (RB == 32)
-        return static_cast<uint32_t>((r >> 2) * 128 + (((r & 3) ^ ((r >> 1) & 2)) << 5) + (c << 4));
-    else if constexpr (RB == 64)
+    if constexpr (RB == 64)
         return static_cast<uint32_t>((((r >> 3) << 2) | (r & 3)) * 128 + ((((r >> 2) ^ (r >> 1)) & 1) << 6) +
                                      ((c ^ ((r & 1) << 1)) << 4));
     else
@@ -557,7 +554,7 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
     constexpr bool PAIR = sizeof(T) == 4 && !WIDE;
     constexpr int C = WIDE || PAIR ? 4 : 2;  // accumulators a lane
     constexpr bool SPLIT = sizeof(T) == 4;  // fp32 queries: hi + lo
-    constexpr bool E4M3 = D::E4M3, E2M1 = D::E2M1;
+    constexpr bool E4M3 = D::E4M3;
     constexpr int NT = D::kWarps * 32, RB = D::kRowBytes, KS = HD / 16, NTILE = HD / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PlanOut block_po;
@@ -627,13 +624,6 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
                 if (lane < 16 && r < left && row8 >= 0)
                     cp_async4(st + 2 * D::kTile + lane * 4, a.kv.scale + row8 + (r & 7) + (lane < 8 ? 0 : v_off));
             }
-            if constexpr (E2M1) {  // 16 scale bytes a copy, K's and then V's
-                constexpr int NB = HD / kKvBlock, N = D::kScales / 16, R = 16 / NB;  // copies, rows a copy
-                const int r = (lane & (N - 1)) * R;
-                const long row8 = __shfl_sync(0xffffffffu, next_row, r & ~7);
-                if (lane < 2 * N && r < left && row8 >= 0)
-                    cp_async16(st + 2 * D::kTile + lane * 16, a.kv.scale + (row8 + (r & 7) + (lane < N ? 0 : v_off)) * NB, true);
-            }
             if (++lb == ls.b1) {
                 more = cursor_next(a, load_c, ls);
                 lb = ls.b0;
@@ -663,8 +653,7 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
             const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const int d = E2M1 ? t4 * (HD / 4) + 4 * ks
-                              : E4M3 ? (t4 + 4 * (ks >> 2)) * 16 + 4 * (ks & 3) : (t4 + 4 * (ks >> 1)) * 8 + 4 * (ks & 1);
+                const int d = E4M3 ? (t4 + 4 * (ks >> 2)) * 16 + 4 * (ks & 3) : (t4 + 4 * (ks >> 1)) * 8 + 4 * (ks & 1);
                 const float4 v = r < rows ? load4(src + d, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
                 const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
                 qf[ks][hf] = *reinterpret_cast<const uint32_t *>(&h0);
@@ -718,24 +707,6 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
                 for (int i = 0; i < 8; ++i) kscale[i] = __uint_as_float(ku[i]);
                 vscale[0] = vv.x; vscale[1] = vv.y; vscale[2] = vv.z; vscale[3] = vv.w;
             }
-            // e2m1: scales as pairs of fp16 numbers, of position r(nt)'s block of K and of pairs of positions' of V;
-            // those behind the last position mean nothing
-            [[maybe_unused]] uint32_t kpair[4], vpair[4];
-            if constexpr (E2M1) {
-                constexpr int NB = HD / kKvBlock;
-                const int left = s.x.kv - p0;
-#pragma unroll
-                for (int nt = 0; nt < 4; ++nt) {
-                    const int r = 8 * nt + (gid >> 1) + 4 * (gid & 1);
-                    kpair[nt] = lds8(sc + r * NB + t4 * NB / 4) * 0x00800080u;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 8 * i + t4, at = sc + D::kScales + gid * NB / 8;
-                    const uint32_t lo = r < left ? lds8(at + r * NB) : 0u, hi = r + 4 < left ? lds8(at + (r + 4) * NB) : 0u;
-                    vpair[i] = (lo | hi << 16) << 7;
-                }
-            }
             // ---- scores: tile nt, column n is position 16 (nt / 2) + 8 (nt % 2) + n / 2 + 4 (n % 2)
             float p[4][C];
 #pragma unroll
@@ -743,28 +714,6 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
 #pragma unroll
                 for (int k = 0; k < C; ++k) p[nt][k] = 0.f;
                 const int r = 8 * nt + (gid >> 1) + 4 * (gid & 1);
-                if constexpr (E2M1) {
-                    uint32_t u[HD / 32];
-                    if constexpr (HD == 128) {
-                        const uint4 w = lds128(kt + dec_off<RB>(r, t4));
-                        u[0] = w.x; u[1] = w.y; u[2] = w.z; u[3] = w.w;
-                    } else {
-                        const uint2 w = lds64(kt + dec_off<RB>(r, t4 >> 1) + 8 * (t4 & 1));
-                        u[0] = w.x; u[1] = w.y;
-                    }
-#pragma unroll
-                    for (int e = 0; e < HD / 32; ++e) {
-                        uint32_t h[4];
-                        e2m1x8_half2(u[e], h);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) h[i] = hmul2(h[i], kpair[nt]);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            mma(p[nt], qf[2 * e + i], h[2 * i], h[2 * i + 1]);
-                            if constexpr (SPLIT && WIDE) mma(p[nt], ql[2 * e + i], h[2 * i], h[2 * i + 1]);
-                        }
-                    }
-                } else
 #pragma unroll
                 for (int j = 0; j < RB / 64; ++j) {
                     const uint4 w = lds128(kt + dec_off<RB>(r, t4 + 4 * j));
@@ -858,35 +807,7 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
                     }
                 };
                 const int r0 = 16 * st + t4;
-                if constexpr (E2M1) {
-                    const uint32_t sa = vpair[2 * st], sb = vpair[2 * st + 1];
-                    uint32_t w[4][HD / 64];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = r0 + 4 * i;
-                        if constexpr (HD == 128) {
-                            const uint2 x = lds64(vt + dec_off<RB>(r, gid >> 1) + 8 * (gid & 1));
-                            w[i][0] = x.x; w[i][1] = x.y;
-                        } else {
-                            w[i][0] = lds32(vt + dec_off<RB>(r, gid >> 2) + 4 * (gid & 3));
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < HD / 64; ++k) {
-                        // bytes of two positions' codes of one dim: even dims, odd dims
-                        uint32_t a0[4], a1[4], b0[4], b1[4];
-                        constexpr uint32_t LO = 0x0f0f0f0fu;
-                        e2m1x8_half2((w[0][k] & LO) | ((w[1][k] << 4) & ~LO), a0);
-                        e2m1x8_half2(((w[0][k] >> 4) & LO) | (w[1][k] & ~LO), a1);
-                        e2m1x8_half2((w[2][k] & LO) | ((w[3][k] << 4) & ~LO), b0);
-                        e2m1x8_half2(((w[2][k] >> 4) & LO) | (w[3][k] & ~LO), b1);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t vb[4] = {hmul2(a0[j], sa), hmul2(b0[j], sb), hmul2(a1[j], sa), hmul2(b1[j], sb)};
-                            values(o[8 * k + 2 * j], o[8 * k + 2 * j + 1], vb);
-                        }
-                    }
-                } else if constexpr (E4M3) {
+                if constexpr (E4M3) {
                     const uint32_t sa = vscale[2 * st], sb = vscale[2 * st + 1];
                     uint32_t w[4][HD / 32];
 #pragma unroll
@@ -964,7 +885,7 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
                 part[kDecRows * HD + kDecRows + r] = l[hf];
             }
             // lane t4's columns n = 2 t4, 2 t4 + 1 of tile i: dim n * W + i (W dims a piece), pieces of 64 dims apart
-            constexpr int W = (E4M3 || E2M1) && HD == 128 ? 16 : 8;
+            constexpr int W = E4M3 && HD == 128 ? 16 : 8;
 #pragma unroll
             for (int h = 0; h < NTILE / W; ++h)
 #pragma unroll
@@ -977,6 +898,429 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
                         else store4(pd + d, o[j][k], o[j + 1][k], o[j + 2][k], o[j + 3][k]);
                     }
         }
+    }
+    cp_async_wait<0>();
+    left.bad = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, gone) ? 2 : 0);
+    left.runs = runs;
+    if (lane == 0) a.left[worker] = left;
+}
+
+// ------------------------------------------------------- decode, 4 bits --
+//
+// e2m1 rows have a kernel of their own: with a quarter of an fp16 cache's bytes the
+// instructions bound it, not the reading.  Positions are the M side of mma.m16n8k16, the
+// (up to 8, WIDE: 16) rows its 8 columns, so no product is of empty rows:
+//   S^T[pos][row] = K . Q^T: a lane's K fragments are 16 or 8 bytes of one position's
+//   row, one scale's block or half of one; the 16 k slots stand for whichever dims those
+//   hold (Q's fragments are loaded in the same order);
+//   O^T[dim][row] += V^T . P^T: a lane's V fragments are 8 or 4 bytes of each of the four
+//   positions of its k slots, whose codes of one dim are put side by side in a byte
+//   (two bit selections for 8 dims) before they become a pair of fp16 numbers.  P^T
+//   comes from the score accumulators by movmatrix.
+// A byte becomes two fp16 numbers in one instruction, and a second one scales them.
+// Rows' maxima are raised only when a score passes them by more than 2^8 (see the tile
+// kernel), so that a chunk has no shuffles for them.  Page ids are read for 8 chunks at
+// once, a lane for each 8 rows that lie together, and a lane copies 16 bytes at a place
+// that is one multiplication away from their number.
+
+template <int HD, bool WIDE, typename T>
+struct Dec4 {
+    static constexpr int kRowBytes = HD / 2, kBlocks = HD / kKvBlock;  // of a row: bytes, scales
+    static constexpr int kTile = kChunk * kRowBytes, kScales = kChunk * kBlocks;
+    static constexpr int kStage = 2 * (kTile + kScales);  // K, V, their scale bytes
+    static constexpr int kWarps = WIDE ? 8 : (HD == 128 && sizeof(T) == 4 ? 12 : 16);
+    static constexpr int kStages = HD == 128 ? (kWarps == 16 ? 3 : 4) : 4;
+    static constexpr int kSmem = kWarps * kStages * kStage;
+    static_assert(kSmem <= 226 * 1024, "stages");
+};
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// (a & m) | (b & ~m)
+__device__ __forceinline__ uint32_t select_bits(uint32_t a, uint32_t b, uint32_t m) { return (a & m) | (b & ~m); }
+
+template <int HD, bool WIDE, typename T>
+__global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
+    ijb_paged_decode4_kernel(const __grid_constant__ AttnArgs a) {
+    using D = Dec4<HD, WIDE, T>;
+    constexpr int N = WIDE ? 2 : 1;         // tiles of 8 rows
+    constexpr bool SPLIT = sizeof(T) == 4;  // fp32 queries: hi + lo
+    constexpr int NT = D::kWarps * 32, RB = D::kRowBytes, NB = D::kBlocks, KS = HD / 16, W = HD / 64;  // W: words of V
+    constexpr int GROUP = 8 * RB;  // bytes of 8 rows, which lie together
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ PlanOut block_po;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t4 = lane & 3;
+    pdl_trigger();
+    const int worker = blockIdx.x * D::kWarps + warp;
+    Cursor load_c;
+    int per;
+    if (a.n_entries < 32) {
+        int *sums = reinterpret_cast<int *>(smem + warp * D::kStages * D::kStage);
+        PlanOut po;
+        plan_warp(a, sums, &po, worker == 0);
+        load_c = cursor_start<true>(a, nullptr, sums, po, worker);
+        per = po.per;
+        __syncwarp();  // the plan's shared memory becomes the stages
+    } else {
+        int *sums = reinterpret_cast<int *>(smem);
+        plan_build<NT, true>(a, nullptr, sums, &block_po);
+        load_c = cursor_start<true>(a, nullptr, sums, block_po, worker);
+        per = block_po.per;
+        __syncthreads();
+    }
+    Cursor use_c = load_c;
+
+    const uint32_t base = smem_u32(smem) + warp * D::kStages * D::kStage;
+    const T *qp = static_cast<const T *>(a.q);
+    T *op = static_cast<T *>(a.out);
+    const bool qvec = aligned4<T>(a.q, a.q_stride), ovec = aligned4<T>(a.out, a.out_stride);
+
+    // ---- the loading side: one chunk after another, across runs
+    Segment ls;
+    int lb = 0, stage_in = 0, window = 0;  // window: the first of the 8 chunks whose groups the lanes have
+    int page_next = -1;     // lane g: page id of group g (8 positions) of the next window
+    uint32_t group = 0;     // lane g: number of group g's first row of K / 8 (the cache's memory has fewer than 2^32)
+    bool fresh = true;      // the next window becomes the current one
+    bool gone = false;      // a page was none: the merge computes these runs' rows again, without its positions
+    bool more = cursor_next(a, load_c, ls);
+    if (more) lb = ls.b0;
+    auto peek = [&]() {
+        window = lb;
+        const int pos = (lb * 4 + lane) * 8;
+        page_next = 0;
+        if (pos < min(ls.x.kv, ls.b1 * kChunk))
+            page_next = a.kv.page_table[static_cast<long>(ls.x.seq) * a.kv.max_pages + (pos >> a.kv.page_shift)];
+        fresh = true;
+    };
+    if (more) peek();
+    // 16-byte pieces: of K or V `lane` of 512 bytes side by side, of the scales one for K or V each
+    constexpr int C = D::kScales / 16, R = 16 / NB;  // copies of K's scales in a chunk, rows a copy
+    const long v_rows = static_cast<long>(a.kv.kv_heads) << a.kv.page_shift;  // from K to V within a page
+    const uint8_t *from_k = a.kv.data + (HD == 128 ? lane : lane & 15) * 16, *from_v = from_k + v_rows * RB;
+    const uint8_t *from_s = a.kv.scale + ((lane & (C - 1)) * R & 7) * NB + (lane & C ? v_rows * NB : 0);
+    const uint32_t to = HD == 128 ? (lane >> 3) * 128 + ((((lane >> 2 & 1) << 2 | (lane & 3)) ^ (lane >> 2 & 6)) << 4)
+                                  : (lane >> 3) * 128 + (((lane >> 1 & 3) ^ (lane >> 3 & 1)) << 5) + ((lane & 1) << 4);
+    auto issue = [&]() {
+        if (more) {
+            if (fresh) {
+                const int pos = (window * 4 + lane) * 8;
+                const bool ok = page_next >= 0 && page_next < a.kv.num_pages;
+                if (!ok) {
+                    gone = true;
+                    if (a.status) atomicOr(a.status, kDevErrBadIndex);
+                }
+                const uint32_t off = static_cast<uint32_t>(pos & ((1 << a.kv.page_shift) - 1)) >> 3;
+                group = ok ? ((static_cast<uint32_t>(page_next) * 2 * a.kv.kv_heads + ls.head) << (a.kv.page_shift - 3)) + off : 0u;
+                fresh = false;
+            }
+            const uint32_t st = base + stage_in * D::kStage;
+            const int g0 = (lb - window) * 4;
+#pragma unroll
+            for (int i = 0; i < kChunk * RB / 512; ++i) {
+                const uint32_t g = __shfl_sync(0xffffffffu, group, g0 + (HD == 128 ? i : 2 * i + (lane >> 4)));
+                const uint64_t at = static_cast<uint64_t>(g) * GROUP;
+                cp_async16(st + to + i * 512, from_k + at, true);
+                cp_async16(st + D::kTile + to + i * 512, from_v + at, true);
+            }
+            const uint32_t g = __shfl_sync(0xffffffffu, group, g0 + (lane & (C - 1)) * R / 8);
+            if (lane < 2 * C) cp_async16(st + 2 * D::kTile + lane * 16, from_s + static_cast<uint64_t>(g) * (8 * NB), true);
+            if (++lb == ls.b1) {
+                more = cursor_next(a, load_c, ls);
+                lb = ls.b0;
+                if (more) peek();
+            } else if (lb == window + 8) {
+                peek();
+            }
+        }
+        cp_async_commit();
+        stage_in = stage_in + 1 == D::kStages ? 0 : stage_in + 1;
+    };
+    for (int i = 0; i < D::kStages - 1; ++i) issue();
+
+    // ---- the computing side
+    // a lane's places in a stage: K rows gid (+ 8), V rows 2 t4 + j (+ 8), their scale bytes
+    const uint32_t k_at = HD == 128 ? (gid >> 1) * 128 + ((((gid & 1) << 2 | t4) ^ (gid & 6)) << 4)
+                                    : (gid >> 2) * 128 + (((gid & 3) ^ (gid >> 2)) << 5) + t4 * 8;
+    uint32_t v_at[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        v_at[j] = D::kTile + (HD == 128 ? t4 * 128 + (((j << 2 | gid >> 1) ^ 2 * t4) << 4) + (gid & 1) * 8
+                                        : (t4 >> 1) * 128 + (((2 * (t4 & 1) + j) ^ (t4 >> 1)) << 5) + gid * 4);
+    constexpr int ROW8 = 8 * RB;  // bytes of 8 rows in a stage too
+    const uint32_t ks_at = 2 * D::kTile + gid * NB + t4 * NB / 4, vs_at = 2 * D::kTile + D::kScales + 2 * t4 * NB + gid * NB / 8;
+    const float sc = a.scale_log2, raise = fminf(8.f / sc, 3e38f);
+    int stage = 0;
+    Left left = {};
+    bool bad = false;
+    const Cursor runs = use_c;
+    Segment s;
+    while (cursor_next(a, use_c, s)) {
+        const int row0 = s.ti * kDecRows, rows = min(kDecRows, s.x.rows - row0);
+        uint32_t qh[KS][N][2], ql[SPLIT ? KS : 1][N][2];
+        int limit[N][2];  // last position that rows 8 n + 2 t4 + c see
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int r = gid + 8 * n;
+            const int tok = r < rows ? (row0 + r) / a.group : 0, in = r < rows ? (row0 + r) % a.group : 0;
+            const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD + t4 * (HD / 4);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const float4 v = r < rows ? load4(src + 4 * ks, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
+                qh[ks][n][0] = *reinterpret_cast<const uint32_t *>(&h0);
+                qh[ks][n][1] = *reinterpret_cast<const uint32_t *>(&h1);
+                if constexpr (SPLIT) {
+                    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                    ql[ks][n][0] = half2_bits(v.x - f0.x, v.y - f0.y);
+                    ql[ks][n][1] = half2_bits(v.z - f1.x, v.w - f1.y);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int q = 8 * n + 2 * t4 + c;
+                limit[n][c] = q < rows ? s.x.kv - s.x.len + (row0 + q) / a.group : -1;
+            }
+        }
+        // m: the maximum (of raw scores) that weights are relative to, mu the same times sc; l: this lane's positions' sum
+        float m[N][2], mu[N][2], l[N][2], o[4 * W][N][4];
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                m[n][c] = -INFINITY;
+                mu[n][c] = l[n][c] = 0.f;
+            }
+#pragma unroll
+        for (int i = 0; i < 4 * W; ++i)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[i][n][k] = 0.f;
+        const int all_see = s.x.kv - s.x.len + row0 / a.group;  // positions up to here are seen by every row
+
+        for (int b = s.b0; b < s.b1; ++b) {
+            issue();  // into the stage used last
+            cp_async_wait<D::kStages - 1>();
+            __syncwarp();
+            const uint32_t st = base + stage * D::kStage;
+            const int p0 = b * kChunk;
+            if (p0 + kChunk > s.x.kv) {  // what V's scales behind the last position hold means nothing: zeros
+                if (p0 + lane >= s.x.kv) {
+#pragma unroll
+                    for (int i = 0; i < NB / 2; ++i)
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(st + 2 * D::kTile + D::kScales + lane * NB + 2 * i), "h"(static_cast<uint16_t>(0))
+                                     : "memory");
+                }
+                __syncwarp();
+            }
+            // ---- scores: tile t, row gid (+ 8) is position 16 t + gid (+ 8)
+            float p[2][N][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) p[t][n][k] = 0.f;
+                uint32_t u[2][HD / 32], ks2[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t at = st + k_at + (2 * t + h) * ROW8;
+                    if constexpr (HD == 128) {
+                        const uint4 w = lds128(at);
+                        u[h][0] = w.x; u[h][1] = w.y; u[h][2] = w.z; u[h][3] = w.w;
+                    } else {
+                        const uint2 w = lds64(at);
+                        u[h][0] = w.x; u[h][1] = w.y;
+                    }
+                    ks2[h] = lds8(st + ks_at + (16 * t + 8 * h) * NB) * 0x00800080u;
+                }
+#pragma unroll
+                for (int e = 0; e < HD / 32; ++e) {
+                    uint32_t x[4], y[4];
+                    e2m1x8_half2(u[0][e], x);
+                    e2m1x8_half2(u[1][e], y);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t f[4] = {hmul2(x[2 * i], ks2[0]), hmul2(y[2 * i], ks2[1]), hmul2(x[2 * i + 1], ks2[0]),
+                                               hmul2(y[2 * i + 1], ks2[1])};
+                        const int ks = 2 * e + i;
+#pragma unroll
+                        for (int n = 0; n < N; ++n) {
+                            if constexpr (SPLIT) mma(p[t][n], f, ql[ks][n][0], ql[ks][n][1]);
+                            mma(p[t][n], f, qh[ks][n][0], qh[ks][n][1]);
+                        }
+                    }
+                }
+            }
+            // ---- online softmax (base 2)
+            if (p0 + kChunk - 1 > all_see) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (p0 + 16 * t + gid + 4 * (k & 2) > limit[n][k & 1]) p[t][n][k] = -INFINITY;
+            }
+            float mx[N][2];
+            bool need = false;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    mx[n][c] = fmaxf(fmaxf(p[0][n][c], p[0][n][c + 2]), fmaxf(p[1][n][c], p[1][n][c + 2]));
+                    need = need || mx[n][c] > m[n][c] + raise;
+                }
+            if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float x = fmaxf(m[n][c], mx[n][c]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        const float f = x == -INFINITY ? 1.f : ex2((m[n][c] - x) * sc);
+                        m[n][c] = x;
+                        mu[n][c] = x == -INFINITY ? 0.f : x * sc;
+                        l[n][c] *= f;
+#pragma unroll
+                        for (int i = 0; i < 4 * W; ++i) {
+                            o[i][n][c] *= f;
+                            o[i][n][c + 2] *= f;
+                        }
+                    }
+            }
+            // weights as the second product's B: k slots 2 t4, 2 t4 + 1 (+ 8) of tile t, column gid
+            uint32_t ph[2][N][2], pl[SPLIT ? 2 : 1][N][2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float e[2];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            e[c] = ex2(fmaf(p[t][n][2 * h + c], sc, -mu[n][c]));
+                            l[n][c] += e[c];
+                        }
+                        const __half2 w = __floats2half2_rn(e[0], e[1]);
+                        ph[t][n][h] = transpose8x8(*reinterpret_cast<const uint32_t *>(&w));
+                        if constexpr (SPLIT) {
+                            const float2 f = __half22float2(w);
+                            pl[t][n][h] = transpose8x8(half2_bits(e[0] - f.x, e[1] - f.y));
+                        }
+                    }
+            // ---- values: tile 4 k + j, rows gid and gid + 8, are the lane's dims 8 k + 2 j and 8 k + 2 j + 1
+            uint32_t w[2][2][2][W], vs2[2][2];  // [tile][+ 8][j]
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t at = st + v_at[j] + (2 * t + h) * ROW8;
+                        if constexpr (HD == 128) {
+                            const uint2 x = lds64(at);
+                            w[t][h][j][0] = x.x; w[t][h][j][1] = x.y;
+                        } else {
+                            w[t][h][j][0] = lds32(at);
+                        }
+                    }
+                    const uint32_t at = st + vs_at + (16 * t + 8 * h) * NB;
+                    vs2[t][h] = lds8(at) * 0x80u + lds8(at + NB) * 0x800000u;
+                }
+            constexpr uint32_t LOW = 0x0f0f0f0fu;
+#pragma unroll
+            for (int k = 0; k < W; ++k) {
+                uint32_t x[2][2][2][4];  // [tile][+ 8][odd dims][j]: pairs of positions 2 t4, 2 t4 + 1
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        e2m1x8_half2(select_bits(w[t][h][0][k], w[t][h][1][k] << 4, LOW), x[t][h][0]);
+                        e2m1x8_half2(select_bits(w[t][h][0][k] >> 4, w[t][h][1][k], LOW), x[t][h][1]);
+                    }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t f[2][4];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        f[t][0] = hmul2(x[t][0][0][j], vs2[t][0]);
+                        f[t][1] = hmul2(x[t][0][1][j], vs2[t][0]);
+                        f[t][2] = hmul2(x[t][1][0][j], vs2[t][1]);
+                        f[t][3] = hmul2(x[t][1][1][j], vs2[t][1]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        float(&to_o)[4] = o[4 * k + j][n];
+                        if constexpr (SPLIT) {
+                            float d[4];
+                            mma_new(d, f[0], pl[0][n][0], pl[0][n][1]);
+                            mma(d, f[1], pl[1][n][0], pl[1][n][1]);
+                            mma(d, f[0], ph[0][n][0], ph[0][n][1]);
+                            mma(d, f[1], ph[1][n][0], ph[1][n][1]);
+                            add2_in_order(to_o[0], to_o[1], d[0], d[1]);
+                            add2_in_order(to_o[2], to_o[3], d[2], d[3]);
+                        } else {
+                            mma(to_o, f[0], ph[0][n][0], ph[0][n][1]);
+                            mma(to_o, f[1], ph[1][n][0], ph[1][n][1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();  // every lane is done with this stage
+            stage = stage + 1 == D::kStages ? 0 : stage + 1;
+        }
+
+        float zero = 0.f;  // NaN once a value is not finite
+#pragma unroll
+        for (int i = 0; i < 4 * W; ++i)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) zero = fmaf(o[i][n][k], 0.f, zero);
+        bad |= !(zero == 0.f);
+        // ---- the run's end: the output, or its state
+        left = left_of(a, s, worker, per);
+        const bool whole = s.b0 == 0 && s.b1 == s.units;
+        float *part = a.part + part_slot(s, worker) * part_floats<kDecRows, HD>();
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float sum = l[n][c];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int r = 8 * n + 2 * t4 + c;
+                if (r >= rows) continue;
+                const float inv = whole ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
+                T *dst = op + static_cast<long>(s.x.q0 + (row0 + r) / a.group) * a.out_stride +
+                         (s.head * a.group + (row0 + r) % a.group) * HD + gid * (HD / 8);
+                float *pd = part + r * HD + gid * (HD / 8);
+                if (!whole && gid == 0) {
+                    part[kDecRows * HD + r] = m[n][c] == -INFINITY ? m[n][c] : mu[n][c];
+                    part[kDecRows * HD + kDecRows + r] = sum;
+                }
+#pragma unroll
+                for (int i = 0; i < 4 * W; i += 2) {
+                    const float x[4] = {o[i][n][c], o[i][n][c + 2], o[i + 1][n][c], o[i + 1][n][c + 2]};
+                    if (whole) store4(dst + 2 * i, ovec, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                    else store4(pd + 2 * i, x[0], x[1], x[2], x[3]);
+                }
+            }
     }
     cp_async_wait<0>();
     left.bad = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, gone) ? 2 : 0);
@@ -2075,14 +2419,23 @@ cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     return e;
 }
 
+// The decode kernel of a cache type, its launch shape and its shared memory (the plan's at least).
+template <int HD, int KV, bool WIDE, typename T>
+using DecOf = std::conditional_t<KV == IJB_KV_E2M1, Dec4<HD, WIDE, T>, Dec<HD, KV, WIDE, T>>;
+template <int HD, int KV, bool WIDE, typename T>
+constexpr auto decode_kernel() {
+    if constexpr (KV == IJB_KV_E2M1) return ijb_paged_decode4_kernel<HD, WIDE, T>;
+    else return ijb_paged_decode_kernel<HD, KV, WIDE, T>;
+}
 template <int HD, int KV, bool WIDE, typename T>
 constexpr int decode_smem() {
-    return Dec<HD, KV, WIDE, T>::kSmem > kDecPlanBytes ? Dec<HD, KV, WIDE, T>::kSmem : kDecPlanBytes;
+    using D = DecOf<HD, KV, WIDE, T>;
+    return D::kSmem > kDecPlanBytes ? D::kSmem : kDecPlanBytes;
 }
 template <int HD, int KV, bool WIDE, typename T>
 cudaError_t decode_allow() {
-    auto kernel = ijb_paged_decode_kernel<HD, KV, WIDE, T>;
-    return allow_smem<decltype(kernel), Dec<HD, KV, WIDE, T>, T>(kernel, decode_smem<HD, KV, WIDE, T>());
+    const auto kernel = decode_kernel<HD, KV, WIDE, T>();
+    return allow_smem<decltype(kernel), DecOf<HD, KV, WIDE, T>, T>(kernel, decode_smem<HD, KV, WIDE, T>());
 }
 template <int HD, int KV, typename T>
 cudaError_t tile_allow() {
@@ -2092,7 +2445,7 @@ cudaError_t tile_allow() {
 
 template <int HD, int KV, bool WIDE, typename T>
 cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
-    using D = Dec<HD, KV, WIDE, T>;
+    using D = DecOf<HD, KV, WIDE, T>;
     const cudaError_t e = decode_allow<HD, KV, WIDE, T>();
     if (e != cudaSuccess) return e;
     a.min_rows = 1;
@@ -2104,7 +2457,7 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.min_units = 2;
     a.over = 1;
     a.least = 1;
-    ijb_paged_decode_kernel<HD, KV, WIDE, T><<<sms, D::kWarps * 32, decode_smem<HD, KV, WIDE, T>(), s>>>(a);
+    decode_kernel<HD, KV, WIDE, T>()<<<sms, D::kWarps * 32, decode_smem<HD, KV, WIDE, T>(), s>>>(a);
     return merge_launch<kDecRows, HD, KV, T>(a, s);
 }
 
@@ -2205,6 +2558,8 @@ int ijb_paged_attention(const ijb_kv_view *kv, int heads, int type, const void *
             return kv_fail(IJB_ERR_INVALID, fn, "scale bytes must be 4-byte aligned");
         if (reinterpret_cast<uintptr_t>(kv->scale_dev) % 16 && kv->type == IJB_KV_E2M1)
             return kv_fail(IJB_ERR_INVALID, fn, "an e2m1 cache's scale bytes must be 16-byte aligned");
+        if (kv->type == IJB_KV_E2M1 && kv->num_pages * 2 * kv->kv_heads > 0xffffffffL / (kv->page_size / 8))
+            return kv_fail(IJB_ERR_INVALID, fn, "more than 2^32 groups of 8 rows");
         if (type != IJB_TYPE_F32 && type != IJB_TYPE_F16)
             return kv_fail(IJB_ERR_INVALID, fn, "query type must be IJB_TYPE_F32 or IJB_TYPE_F16");
         if (heads < 1 || heads % kv->kv_heads != 0 || heads / kv->kv_heads > 16)
