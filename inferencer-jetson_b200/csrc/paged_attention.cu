@@ -453,6 +453,7 @@ constexpr int kDecRows = 16;
 template <int HD, int KV, bool WIDE, typename T>
 struct Dec {
     static constexpr bool E4M3 = KV == IJB_KV_E4M3;
+    static constexpr int kPos = kChunk;
     static constexpr int kRowBytes = kv_row_bytes(KV, HD);
     static constexpr int kTile = kChunk * kRowBytes;
     static constexpr int kStage = 2 * kTile + (E4M3 ? 256 : 0);  // K, V, their scale bytes and what they stand for
@@ -919,17 +920,18 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
 //   comes from the score accumulators by movmatrix.
 // A byte becomes two fp16 numbers in one instruction, and a second one scales them.
 // Rows' maxima are raised only when a score passes them by more than 2^8 (see the tile
-// kernel), so that a chunk has no shuffles for them.  Page ids are read for 8 chunks at
-// once, a lane for each 8 rows that lie together, and a lane copies 16 bytes at a place
+// kernel), so that a chunk has no shuffles for them.  Page ids are read 256 positions
+// at once, a lane for each 8 rows that lie together, and a lane copies 16 bytes at a place
 // that is one multiplication away from their number.
 
 template <int HD, bool WIDE, typename T>
 struct Dec4 {
     static constexpr int kRowBytes = HD / 2, kBlocks = HD / kKvBlock;  // of a row: bytes, scales
-    static constexpr int kTile = kChunk * kRowBytes, kScales = kChunk * kBlocks;
+    static constexpr int kPos = WIDE ? 32 : 64;                        // positions of a chunk
+    static constexpr int kTile = kPos * kRowBytes, kScales = kPos * kBlocks;
     static constexpr int kStage = 2 * (kTile + kScales);  // K, V, their scale bytes
-    static constexpr int kWarps = WIDE ? 8 : (HD == 128 && sizeof(T) == 4 ? 12 : 16);
-    static constexpr int kStages = HD == 128 ? (kWarps == 16 ? 3 : 4) : 4;
+    static constexpr int kWarps = WIDE || (HD == 128 && sizeof(T) == 4) ? 8 : 12;
+    static constexpr int kStages = WIDE || HD == 64 ? 4 : (kWarps == 12 ? 2 : 3);
     static constexpr int kSmem = kWarps * kStages * kStage;
     static_assert(kSmem <= 226 * 1024, "stages");
 };
@@ -956,7 +958,8 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     constexpr int N = WIDE ? 2 : 1;         // tiles of 8 rows
     constexpr bool SPLIT = sizeof(T) == 4;  // fp32 queries: hi + lo
     constexpr int NT = D::kWarps * 32, RB = D::kRowBytes, NB = D::kBlocks, KS = HD / 16, W = HD / 64;  // W: words of V
-    constexpr int GROUP = 8 * RB;  // bytes of 8 rows, which lie together
+    constexpr int GROUP = 8 * RB;         // bytes of 8 rows, which lie together
+    constexpr int PC = D::kPos, TT = PC / 16, G = PC / 8;  // positions, tiles and groups of a chunk
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PlanOut block_po;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t4 = lane & 3;
@@ -987,7 +990,7 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
 
     // ---- the loading side: one chunk after another, across runs
     Segment ls;
-    int lb = 0, stage_in = 0, window = 0;  // window: the first of the 8 chunks whose groups the lanes have
+    int lb = 0, stage_in = 0, window = 0;  // window: the first of the 32 / G chunks whose groups the lanes have
     int page_next = -1;     // lane g: page id of group g (8 positions) of the next window
     uint32_t group = 0;     // lane g: number of group g's first row of K / 8 (the cache's memory has fewer than 2^32)
     bool fresh = true;      // the next window becomes the current one
@@ -996,9 +999,9 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     if (more) lb = ls.b0;
     auto peek = [&]() {
         window = lb;
-        const int pos = (lb * 4 + lane) * 8;
+        const int pos = (lb * G + lane) * 8;
         page_next = 0;
-        if (pos < min(ls.x.kv, ls.b1 * kChunk))
+        if (pos < min(ls.x.kv, ls.b1 * PC))
             page_next = a.kv.page_table[static_cast<long>(ls.x.seq) * a.kv.max_pages + (pos >> a.kv.page_shift)];
         fresh = true;
     };
@@ -1013,7 +1016,7 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     auto issue = [&]() {
         if (more) {
             if (fresh) {
-                const int pos = (window * 4 + lane) * 8;
+                const int pos = (window * G + lane) * 8;
                 const bool ok = page_next >= 0 && page_next < a.kv.num_pages;
                 if (!ok) {
                     gone = true;
@@ -1024,9 +1027,9 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 fresh = false;
             }
             const uint32_t st = base + stage_in * D::kStage;
-            const int g0 = (lb - window) * 4;
+            const int g0 = (lb - window) * G;
 #pragma unroll
-            for (int i = 0; i < kChunk * RB / 512; ++i) {
+            for (int i = 0; i < PC * RB / 512; ++i) {
                 const uint32_t g = __shfl_sync(0xffffffffu, group, g0 + (HD == 128 ? i : 2 * i + (lane >> 4)));
                 const uint64_t at = static_cast<uint64_t>(g) * GROUP;
                 cp_async16(st + to + i * 512, from_k + at, true);
@@ -1038,7 +1041,7 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 more = cursor_next(a, load_c, ls);
                 lb = ls.b0;
                 if (more) peek();
-            } else if (lb == window + 8) {
+            } else if (lb == window + 32 / G) {
                 peek();
             }
         }
@@ -1113,20 +1116,21 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
             cp_async_wait<D::kStages - 1>();
             __syncwarp();
             const uint32_t st = base + stage * D::kStage;
-            const int p0 = b * kChunk;
-            if (p0 + kChunk > s.x.kv) {  // what V's scales behind the last position hold means nothing: zeros
-                if (p0 + lane >= s.x.kv) {
+            const int p0 = b * PC;
+            if (p0 + PC > s.x.kv) {  // what V's scales behind the last position hold means nothing: zeros
+                for (int r = lane; r < PC; r += 32)
+                    if (p0 + r >= s.x.kv)
 #pragma unroll
-                    for (int i = 0; i < NB / 2; ++i)
-                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(st + 2 * D::kTile + D::kScales + lane * NB + 2 * i), "h"(static_cast<uint16_t>(0))
-                                     : "memory");
-                }
+                        for (int i = 0; i < NB / 2; ++i)
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(st + 2 * D::kTile + D::kScales + r * NB + 2 * i),
+                                         "h"(static_cast<uint16_t>(0))
+                                         : "memory");
                 __syncwarp();
             }
             // ---- scores: tile t, row gid (+ 8) is position 16 t + gid (+ 8)
-            float p[2][N][4];
+            float p[TT][N][4];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < TT; ++t) {
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -1163,9 +1167,9 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 }
             }
             // ---- online softmax (base 2)
-            if (p0 + kChunk - 1 > all_see) {
+            if (p0 + PC - 1 > all_see) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < TT; ++t)
 #pragma unroll
                     for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -1178,7 +1182,9 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
             for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    mx[n][c] = fmaxf(fmaxf(p[0][n][c], p[0][n][c + 2]), fmaxf(p[1][n][c], p[1][n][c + 2]));
+                    mx[n][c] = fmaxf(p[0][n][c], p[0][n][c + 2]);
+#pragma unroll
+                    for (int t = 1; t < TT; ++t) mx[n][c] = fmaxf(mx[n][c], fmaxf(p[t][n][c], p[t][n][c + 2]));
                     need = need || mx[n][c] > m[n][c] + raise;
                 }
             if (__any_sync(0xffffffffu, need)) {
@@ -1202,9 +1208,9 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                     }
             }
             // weights as the second product's B: k slots 2 t4, 2 t4 + 1 (+ 8) of tile t, column gid
-            uint32_t ph[2][N][2], pl[SPLIT ? 2 : 1][N][2];
+            uint32_t ph[TT][N][2], pl[SPLIT ? TT : 1][N][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < TT; ++t)
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -1222,60 +1228,63 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                             pl[t][n][h] = transpose8x8(half2_bits(e[0] - f.x, e[1] - f.y));
                         }
                     }
-            // ---- values: tile 4 k + j, rows gid and gid + 8, are the lane's dims 8 k + 2 j and 8 k + 2 j + 1
-            uint32_t w[2][2][2][W], vs2[2][2];  // [tile][+ 8][j]
+            // ---- values, 32 positions at a time: tile 4 k + j, rows gid and gid + 8, are the lane's dims 8 k + 2 j and 8 k + 2 j + 1
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint32_t at = st + v_at[j] + (2 * t + h) * ROW8;
-                        if constexpr (HD == 128) {
-                            const uint2 x = lds64(at);
-                            w[t][h][j][0] = x.x; w[t][h][j][1] = x.y;
-                        } else {
-                            w[t][h][j][0] = lds32(at);
-                        }
-                    }
-                    const uint32_t at = st + vs_at + (16 * t + 8 * h) * NB;
-                    vs2[t][h] = lds8(at) * 0x80u + lds8(at + NB) * 0x800000u;
-                }
-            constexpr uint32_t LOW = 0x0f0f0f0fu;
-#pragma unroll
-            for (int k = 0; k < W; ++k) {
-                uint32_t x[2][2][2][4];  // [tile][+ 8][odd dims][j]: pairs of positions 2 t4, 2 t4 + 1
+            for (int t0 = 0; t0 < TT; t0 += 2) {
+                uint32_t w[2][2][2][W], vs2[2][2];  // [tile][+ 8][j]
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        e2m1x8_half2(select_bits(w[t][h][0][k], w[t][h][1][k] << 4, LOW), x[t][h][0]);
-                        e2m1x8_half2(select_bits(w[t][h][0][k] >> 4, w[t][h][1][k], LOW), x[t][h][1]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t at = st + v_at[j] + (2 * (t0 + t) + h) * ROW8;
+                            if constexpr (HD == 128) {
+                                const uint2 x = lds64(at);
+                                w[t][h][j][0] = x.x; w[t][h][j][1] = x.y;
+                            } else {
+                                w[t][h][j][0] = lds32(at);
+                            }
+                        }
+                        const uint32_t at = st + vs_at + (16 * (t0 + t) + 8 * h) * NB;
+                        vs2[t][h] = lds8(at) * 0x80u + lds8(at + NB) * 0x800000u;
                     }
+                constexpr uint32_t LOW = 0x0f0f0f0fu;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t f[2][4];
+                for (int k = 0; k < W; ++k) {
+                    uint32_t x[2][2][2][4];  // [tile][+ 8][odd dims][j]: pairs of positions 2 t4, 2 t4 + 1
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        f[t][0] = hmul2(x[t][0][0][j], vs2[t][0]);
-                        f[t][1] = hmul2(x[t][0][1][j], vs2[t][0]);
-                        f[t][2] = hmul2(x[t][1][0][j], vs2[t][1]);
-                        f[t][3] = hmul2(x[t][1][1][j], vs2[t][1]);
-                    }
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int n = 0; n < N; ++n) {
-                        float(&to_o)[4] = o[4 * k + j][n];
-                        if constexpr (SPLIT) {
-                            float d[4];
-                            mma_new(d, f[0], pl[0][n][0], pl[0][n][1]);
-                            mma(d, f[1], pl[1][n][0], pl[1][n][1]);
-                            mma(d, f[0], ph[0][n][0], ph[0][n][1]);
-                            mma(d, f[1], ph[1][n][0], ph[1][n][1]);
-                            add2_in_order(to_o[0], to_o[1], d[0], d[1]);
-                            add2_in_order(to_o[2], to_o[3], d[2], d[3]);
-                        } else {
-                            mma(to_o, f[0], ph[0][n][0], ph[0][n][1]);
-                            mma(to_o, f[1], ph[1][n][0], ph[1][n][1]);
+                        for (int h = 0; h < 2; ++h) {
+                            e2m1x8_half2(select_bits(w[t][h][0][k], w[t][h][1][k] << 4, LOW), x[t][h][0]);
+                            e2m1x8_half2(select_bits(w[t][h][0][k] >> 4, w[t][h][1][k], LOW), x[t][h][1]);
+                        }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t f[2][4];
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            f[t][0] = hmul2(x[t][0][0][j], vs2[t][0]);
+                            f[t][1] = hmul2(x[t][0][1][j], vs2[t][0]);
+                            f[t][2] = hmul2(x[t][1][0][j], vs2[t][1]);
+                            f[t][3] = hmul2(x[t][1][1][j], vs2[t][1]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < N; ++n) {
+                            float(&to_o)[4] = o[4 * k + j][n];
+                            if constexpr (SPLIT) {
+                                float d[4];
+                                mma_new(d, f[0], pl[t0][n][0], pl[t0][n][1]);
+                                mma(d, f[1], pl[t0 + 1][n][0], pl[t0 + 1][n][1]);
+                                mma(d, f[0], ph[t0][n][0], ph[t0][n][1]);
+                                mma(d, f[1], ph[t0 + 1][n][0], ph[t0 + 1][n][1]);
+                                add2_in_order(to_o[0], to_o[1], d[0], d[1]);
+                                add2_in_order(to_o[2], to_o[3], d[2], d[3]);
+                            } else {
+                                mma(to_o, f[0], ph[t0][n][0], ph[t0][n][1]);
+                                mma(to_o, f[1], ph[t0 + 1][n][0], ph[t0 + 1][n][1]);
+                            }
                         }
                     }
                 }
@@ -2452,7 +2461,7 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.max_rows = WIDE ? kDecRows : 8;
     a.report_long = all;
     a.tile_rows = kDecRows;
-    a.unit = kChunk;
+    a.unit = D::kPos;
     a.workers = sms * D::kWarps;
     a.min_units = 2;
     a.over = 1;
