@@ -45,19 +45,22 @@ __host__ __device__ constexpr int kv_row_bytes(int type, int head_dim) {
     return type == IJB_KV_E2M1 ? head_dim / 2 : (type == IJB_KV_E4M3 ? head_dim : 2 * head_dim);
 }
 
-// Codes of one byte (or the low one) as two fp16 numbers, of four bytes as eight: one
-// instruction a byte.
-__device__ __forceinline__ uint32_t e2m1x2_half2(uint32_t u) {
+// The codes of one byte of u as two fp16 numbers, one instruction (`byte` is a constant); of all four as eight.
+__device__ __forceinline__ uint32_t e2m1x2_half2(uint32_t u, int byte = 0) {
     uint32_t h;
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(u));
+    if (byte == 0)
+        asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(u));
+    else if (byte == 1)
+        asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(h) : "r"(u));
+    else if (byte == 2)
+        asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, c;\n\t}" : "=r"(h) : "r"(u));
+    else
+        asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, d;\n\t}" : "=r"(h) : "r"(u));
     return h;
 }
 __device__ __forceinline__ void e2m1x8_half2(uint32_t u, uint32_t (&h)[4]) {
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-        : "r"(u));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = e2m1x2_half2(u, i);
 }
 
 // Row index of (page, which, head, offset); 64 bits: a pool may pass 2^31 rows.

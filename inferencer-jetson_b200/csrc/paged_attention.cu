@@ -927,13 +927,14 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
 template <int HD, bool WIDE, typename T>
 struct Dec4 {
     static constexpr int kRowBytes = HD / 2, kBlocks = HD / kKvBlock;  // of a row: bytes, scales
-    static constexpr int kPos = WIDE ? 32 : 64;                        // positions of a chunk
+    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr int kPos = WIDE && kSplit ? 32 : 64;  // positions of a chunk
     static constexpr int kTile = kPos * kRowBytes, kScales = kPos * kBlocks;
     static constexpr int kStage = 2 * (kTile + kScales);  // K, V, their scale bytes
-    static constexpr int kWarps = WIDE || (HD == 128 && sizeof(T) == 4) ? 8 : 12;
-    static constexpr int kStages = WIDE || HD == 64 ? 4 : (kWarps == 12 ? 2 : 3);
+    static constexpr int kWarps = HD == 128 ? (WIDE || kSplit ? 8 : 12) : (WIDE || kSplit ? 12 : 16);
+    static constexpr int kFit = 224 * 1024 / (kWarps * kStage), kStages = kFit > 4 ? 4 : kFit;
     static constexpr int kSmem = kWarps * kStages * kStage;
-    static_assert(kSmem <= 226 * 1024, "stages");
+    static_assert(kStages >= 2, "stages");
 };
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -962,26 +963,44 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     constexpr int PC = D::kPos, TT = PC / 16, G = PC / 8;  // positions, tiles and groups of a chunk
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PlanOut block_po;
+    // what a warp needs between its runs only: its places in the line (loading, computing), the run it computes
+    __shared__ struct { Cursor load, use; Segment run; } state[D::kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t4 = lane & 3;
     pdl_trigger();
     const int worker = blockIdx.x * D::kWarps + warp;
-    Cursor load_c;
+    auto &my = state[warp];
+    Cursor first;
     int per;
     if (a.n_entries < 32) {
         int *sums = reinterpret_cast<int *>(smem + warp * D::kStages * D::kStage);
         PlanOut po;
         plan_warp(a, sums, &po, worker == 0);
-        load_c = cursor_start<true>(a, nullptr, sums, po, worker);
+        first = cursor_start<true>(a, nullptr, sums, po, worker);
         per = po.per;
         __syncwarp();  // the plan's shared memory becomes the stages
     } else {
         int *sums = reinterpret_cast<int *>(smem);
         plan_build<NT, true>(a, nullptr, sums, &block_po);
-        load_c = cursor_start<true>(a, nullptr, sums, block_po, worker);
+        first = cursor_start<true>(a, nullptr, sums, block_po, worker);
         per = block_po.per;
         __syncthreads();
     }
-    Cursor use_c = load_c;
+    if (lane == 0) {
+        my.load = my.use = first;
+        Left none = {};
+        none.runs = first;
+        a.left[worker] = none;
+    }
+    __syncwarp();
+    // the next run of one of the two sides; false at the end
+    auto next_run = [&](Cursor &at, Segment &s) {
+        Cursor c = at;
+        const bool ok = cursor_next(a, c, s);
+        __syncwarp();
+        if (lane == 0) at = c;
+        __syncwarp();
+        return ok;
+    };
 
     const uint32_t base = smem_u32(smem) + warp * D::kStages * D::kStage;
     const T *qp = static_cast<const T *>(a.q);
@@ -989,22 +1008,31 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     const bool qvec = aligned4<T>(a.q, a.q_stride), ovec = aligned4<T>(a.out, a.out_stride);
 
     // ---- the loading side: one chunk after another, across runs
-    Segment ls;
+    int l_kv = 0, l_seq = 0, l_head = 0, l_end = 0;  // of the run being loaded
     int lb = 0, stage_in = 0, window = 0;  // window: the first of the 32 / G chunks whose groups the lanes have
     int page_next = -1;     // lane g: page id of group g (8 positions) of the next window
     uint32_t group = 0;     // lane g: number of group g's first row of K / 8 (the cache's memory has fewer than 2^32)
     bool fresh = true;      // the next window becomes the current one
     bool gone = false;      // a page was none: the merge computes these runs' rows again, without its positions
-    bool more = cursor_next(a, load_c, ls);
-    if (more) lb = ls.b0;
+    bool more = false;
+    auto load_run = [&]() {
+        Segment s;
+        more = next_run(my.load, s);
+        l_kv = s.x.kv;
+        l_seq = s.x.seq;
+        l_head = s.head;
+        lb = s.b0;
+        l_end = s.b1;
+    };
     auto peek = [&]() {
         window = lb;
         const int pos = (lb * G + lane) * 8;
         page_next = 0;
-        if (pos < min(ls.x.kv, ls.b1 * PC))
-            page_next = a.kv.page_table[static_cast<long>(ls.x.seq) * a.kv.max_pages + (pos >> a.kv.page_shift)];
+        if (pos < min(l_kv, l_end * PC))
+            page_next = a.kv.page_table[static_cast<long>(l_seq) * a.kv.max_pages + (pos >> a.kv.page_shift)];
         fresh = true;
     };
+    load_run();
     if (more) peek();
     // 16-byte pieces: of K or V `lane` of 512 bytes side by side, of the scales one for K or V each
     constexpr int C = D::kScales / 16, R = 16 / NB;  // copies of K's scales in a chunk, rows a copy
@@ -1023,7 +1051,7 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                     if (a.status) atomicOr(a.status, kDevErrBadIndex);
                 }
                 const uint32_t off = static_cast<uint32_t>(pos & ((1 << a.kv.page_shift) - 1)) >> 3;
-                group = ok ? ((static_cast<uint32_t>(page_next) * 2 * a.kv.kv_heads + ls.head) << (a.kv.page_shift - 3)) + off : 0u;
+                group = ok ? ((static_cast<uint32_t>(page_next) * 2 * a.kv.kv_heads + l_head) << (a.kv.page_shift - 3)) + off : 0u;
                 fresh = false;
             }
             const uint32_t st = base + stage_in * D::kStage;
@@ -1037,9 +1065,8 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
             }
             const uint32_t g = __shfl_sync(0xffffffffu, group, g0 + (lane & (C - 1)) * R / 8);
             if (lane < 2 * C) cp_async16(st + 2 * D::kTile + lane * 16, from_s + static_cast<uint64_t>(g) * (8 * NB), true);
-            if (++lb == ls.b1) {
-                more = cursor_next(a, load_c, ls);
-                lb = ls.b0;
+            if (++lb == l_end) {
+                load_run();
                 if (more) peek();
             } else if (lb == window + 32 / G) {
                 peek();
@@ -1063,11 +1090,12 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     const uint32_t ks_at = 2 * D::kTile + gid * NB + t4 * NB / 4, vs_at = 2 * D::kTile + D::kScales + 2 * t4 * NB + gid * NB / 8;
     const float sc = a.scale_log2, raise = fminf(8.f / sc, 3e38f);
     int stage = 0;
-    Left left = {};
     bool bad = false;
-    const Cursor runs = use_c;
-    Segment s;
-    while (cursor_next(a, use_c, s)) {
+    while (true) {
+        Segment s;
+        if (!next_run(my.use, s)) break;
+        if (lane == 0) my.run = s;  // (read behind the run, not held)
+        const int kv = s.x.kv, b1 = s.b1;
         const int row0 = s.ti * kDecRows, rows = min(kDecRows, s.x.rows - row0);
         uint32_t qh[KS][N][2], ql[SPLIT ? KS : 1][N][2];
         int limit[N][2];  // last position that rows 8 n + 2 t4 + c see
@@ -1111,15 +1139,15 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 for (int k = 0; k < 4; ++k) o[i][n][k] = 0.f;
         const int all_see = s.x.kv - s.x.len + row0 / a.group;  // positions up to here are seen by every row
 
-        for (int b = s.b0; b < s.b1; ++b) {
+        for (int b = s.b0; b < b1; ++b) {
             issue();  // into the stage used last
             cp_async_wait<D::kStages - 1>();
             __syncwarp();
             const uint32_t st = base + stage * D::kStage;
             const int p0 = b * PC;
-            if (p0 + PC > s.x.kv) {  // what V's scales behind the last position hold means nothing: zeros
+            if (p0 + PC > kv) {  // what V's scales behind the last position hold means nothing: zeros
                 for (int r = lane; r < PC; r += 32)
-                    if (p0 + r >= s.x.kv)
+                    if (p0 + r >= kv)
 #pragma unroll
                         for (int i = 0; i < NB / 2; ++i)
                             asm volatile("st.shared.u16 [%0], %1;" ::"r"(st + 2 * D::kTile + D::kScales + r * NB + 2 * i),
@@ -1150,13 +1178,11 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 }
 #pragma unroll
                 for (int e = 0; e < HD / 32; ++e) {
-                    uint32_t x[4], y[4];
-                    e2m1x8_half2(u[0][e], x);
-                    e2m1x8_half2(u[1][e], y);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t f[4] = {hmul2(x[2 * i], ks2[0]), hmul2(y[2 * i], ks2[1]), hmul2(x[2 * i + 1], ks2[0]),
-                                               hmul2(y[2 * i + 1], ks2[1])};
+                        uint32_t f[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) f[j] = hmul2(e2m1x2_half2(u[j & 1][e], 2 * i + (j >> 1)), ks2[j & 1]);
                         const int ks = 2 * e + i;
 #pragma unroll
                         for (int n = 0; n < N; ++n) {
@@ -1252,24 +1278,21 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 constexpr uint32_t LOW = 0x0f0f0f0fu;
 #pragma unroll
                 for (int k = 0; k < W; ++k) {
-                    uint32_t x[2][2][2][4];  // [tile][+ 8][odd dims][j]: pairs of positions 2 t4, 2 t4 + 1
+                    uint32_t x[2][2][2];  // [tile][+ 8][odd dims]: bytes of codes of positions 2 t4, 2 t4 + 1
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            e2m1x8_half2(select_bits(w[t][h][0][k], w[t][h][1][k] << 4, LOW), x[t][h][0]);
-                            e2m1x8_half2(select_bits(w[t][h][0][k] >> 4, w[t][h][1][k], LOW), x[t][h][1]);
+                            x[t][h][0] = select_bits(w[t][h][0][k], w[t][h][1][k] << 4, LOW);
+                            x[t][h][1] = select_bits(w[t][h][0][k] >> 4, w[t][h][1][k], LOW);
                         }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t f[2][4];
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            f[t][0] = hmul2(x[t][0][0][j], vs2[t][0]);
-                            f[t][1] = hmul2(x[t][0][1][j], vs2[t][0]);
-                            f[t][2] = hmul2(x[t][1][0][j], vs2[t][1]);
-                            f[t][3] = hmul2(x[t][1][1][j], vs2[t][1]);
-                        }
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) f[t][i] = hmul2(e2m1x2_half2(x[t][i >> 1][i & 1], j), vs2[t][i >> 1]);
 #pragma unroll
                         for (int n = 0; n < N; ++n) {
                             float(&to_o)[4] = o[4 * k + j][n];
@@ -1302,7 +1325,14 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 for (int k = 0; k < 4; ++k) zero = fmaf(o[i][n][k], 0.f, zero);
         bad |= !(zero == 0.f);
         // ---- the run's end: the output, or its state
-        left = left_of(a, s, worker, per);
+        s = my.run;
+        const int end_row0 = s.ti * kDecRows, end_rows = min(kDecRows, s.x.rows - end_row0);
+        if (lane == 0) {
+            const Left left = left_of(a, s, worker, per);
+            int *to_left = &a.left[worker].states;
+            *reinterpret_cast<int4 *>(to_left) = make_int4(left.states, left.q0, left.row0, left.rows);
+            to_left[4] = left.head;
+        }
         const bool whole = s.b0 == 0 && s.b1 == s.units;
         float *part = a.part + part_slot(s, worker) * part_floats<kDecRows, HD>();
 #pragma unroll
@@ -1314,10 +1344,10 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                 const int r = 8 * n + 2 * t4 + c;
-                if (r >= rows) continue;
+                if (r >= end_rows) continue;
                 const float inv = whole ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
-                T *dst = op + static_cast<long>(s.x.q0 + (row0 + r) / a.group) * a.out_stride +
-                         (s.head * a.group + (row0 + r) % a.group) * HD + gid * (HD / 8);
+                T *dst = op + static_cast<long>(s.x.q0 + (end_row0 + r) / a.group) * a.out_stride +
+                         (s.head * a.group + (end_row0 + r) % a.group) * HD + gid * (HD / 8);
                 float *pd = part + r * HD + gid * (HD / 8);
                 if (!whole && gid == 0) {
                     part[kDecRows * HD + r] = m[n][c] == -INFINITY ? m[n][c] : mu[n][c];
@@ -1332,9 +1362,8 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
             }
     }
     cp_async_wait<0>();
-    left.bad = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, gone) ? 2 : 0);
-    left.runs = runs;
-    if (lane == 0) a.left[worker] = left;
+    const int how = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, gone) ? 2 : 0);
+    if (lane == 0) a.left[worker].bad = how;
 }
 
 // ------------------------------------------------------------------ tile --
