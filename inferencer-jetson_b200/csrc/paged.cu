@@ -142,39 +142,7 @@ struct Place {
     }
 };
 
-// Thread c's 8 of a row's values as e2m1 codes; the row's 4 threads of a block of 32 agree on the scale.
-__device__ __forceinline__ uint32_t e2m1_codes(const float (&f)[8], uint32_t &byte) {
-    float a = 0.f;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        a = fmaxf(a, fabsf(f[i]) <= 3.402823466e38f ? fabsf(f[i]) : 0.f);
-        nan |= f[i] != f[i];
-    }
-    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-    const uint32_t any = __ballot_sync(0xffffffffu, nan), mine = 0xfu << (threadIdx.x & 28);
-    // the nearest scale to a / 6, ties to even: from 2^-14 on the upper bits of the number with 3 of its mantissa,
-    // below in steps of 2^-17
-    const float r = __fdiv_rn(a, 6.f);
-    const uint32_t bits = __float_as_uint(r);
-    byte = r >= 6.103515625e-5f ? ((bits + 0x7ffffu + ((bits >> 20) & 1u)) >> 20) - ((127u - 15u) << 3)
-                                : __float2uint_rn(r * 131072.f);
-    byte = min(byte, kKvTopScale);
-    const float scale = half_bits_to_float(static_cast<uint16_t>(byte << 7));
-    const float inv = byte ? __frcp_rn(scale) : 0.f;
-    uint32_t q = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        // an infinity is the largest value, and a block without a scale zeros
-        const float x = byte ? f[2 * i] * inv : 0.f, y = byte ? f[2 * i + 1] * inv : 0.f;
-        q |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(x, y), __NV_E2M1, cudaRoundNearest)) << (8 * i);
-    }
-    if (any & mine) byte = kKvNanScale;  // a NaN is its block's
-    return q;
-}
-
-template <typename T, int KV, bool VEC, int HD, int U>
+template <typename T, bool E4M3, bool VEC, int HD, int U>
 __global__ void __launch_bounds__(kRowThreads) ijb_kv_append_kernel(const __grid_constant__ RowsParams p) {
     const Place<HD, U> w(p);
     const long src = w.n ? w.t * p.stride + static_cast<long>(w.head) * HD + w.c * 8 : 0;
@@ -195,14 +163,7 @@ __global__ void __launch_bounds__(kRowThreads) ijb_kv_append_kernel(const __grid
     for (int j = 0; j < U; ++j) {
         const long to = to0 + (static_cast<long>(j) << p.kv.page_shift);
         const bool live = slot >= 0 && j < w.n;
-        if constexpr (KV == IJB_KV_E2M1) {
-            uint32_t byte;
-            const uint32_t q = e2m1_codes(f[j], byte);
-            if (live) {
-                *reinterpret_cast<uint32_t *>(p.kv.data + to * (HD / 2) + w.c * 4) = q;
-                if (w.c % 4 == 0) p.kv.scale[to * (HD / kKvBlock) + w.c / 4] = static_cast<uint8_t>(byte);
-            }
-        } else if constexpr (KV == IJB_KV_E4M3) {
+        if constexpr (E4M3) {
             float a = 0.f;  // over the finite values: an infinity saturates, a NaN stays one
 #pragma unroll
             for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(f[j][i]) <= 3.402823466e38f ? fabsf(f[j][i]) : 0.f);
@@ -235,7 +196,7 @@ __global__ void __launch_bounds__(kRowThreads) ijb_kv_append_kernel(const __grid
 
 // Reads back: code * 2^e (exact in fp32), or the fp16 row; rows of padding
 // entries and of entries that name no slot are left as they were.
-template <typename T, int KV, bool VEC, int HD, int U>
+template <typename T, bool E4M3, bool VEC, int HD, int U>
 __global__ void __launch_bounds__(kRowThreads) ijb_kv_gather_kernel(const __grid_constant__ RowsParams p) {
     const Place<HD, U> w(p);
     if (w.n == 0) return;
@@ -249,10 +210,7 @@ __global__ void __launch_bounds__(kRowThreads) ijb_kv_gather_kernel(const __grid
     for (int j = 0; j < U; ++j) {
         if (j >= w.n) continue;
         const long from = from0 + (static_cast<long>(j) << p.kv.page_shift);
-        if constexpr (KV == IJB_KV_E2M1) {
-            raw[j].x = *reinterpret_cast<const uint32_t *>(p.kv.data + from * (HD / 2) + w.c * 4);
-            sc[j] = p.kv.scale[from * (HD / kKvBlock) + w.c / 4];
-        } else if constexpr (KV == IJB_KV_E4M3) {
+        if constexpr (E4M3) {
             const uint2 u = *reinterpret_cast<const uint2 *>(p.kv.data + from * HD + w.c * 8);
             raw[j].x = u.x;
             raw[j].y = u.y;
@@ -265,17 +223,7 @@ __global__ void __launch_bounds__(kRowThreads) ijb_kv_gather_kernel(const __grid
     for (int j = 0; j < U; ++j) {
         if (j >= w.n) continue;
         float f[8];
-        if constexpr (KV == IJB_KV_E2M1) {
-            const float s = half_bits_to_float(static_cast<uint16_t>(sc[j] << 7));
-            uint32_t h[4];
-            e2m1x8_half2(raw[j].x, h);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
-                f[2 * i] = v.x * s;
-                f[2 * i + 1] = v.y * s;
-            }
-        } else if constexpr (KV == IJB_KV_E4M3) {
+        if constexpr (E4M3) {
             const float s = kv_scale(sc[j]);
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
@@ -301,31 +249,267 @@ constexpr int kHeads = 4;              // heads a thread takes of many rows
 // 10.2 each; 16383 written 50.7 and 47.5, read 50.2 and 43.2.
 constexpr long kManyThreads = 1 << 18;
 
-template <bool APPEND, typename T, int KV, bool VEC, int HD, int U>
+template <bool APPEND, typename T, bool E4M3, bool VEC, int HD, int U>
 void rows_launch(const RowsParams &p, cudaStream_t s) {
     const long threads = static_cast<long>(p.n) * 2 * ((p.kv.kv_heads + U - 1) / U) * (HD / 8);
     const unsigned blocks = static_cast<unsigned>((threads + kRowThreads - 1) / kRowThreads);
-    if constexpr (APPEND) ijb_kv_append_kernel<T, KV, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
-    else ijb_kv_gather_kernel<T, KV, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
+    if constexpr (APPEND) ijb_kv_append_kernel<T, E4M3, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
+    else ijb_kv_gather_kernel<T, E4M3, VEC, HD, U><<<blocks, kRowThreads, 0, s>>>(p);
 }
-template <bool APPEND, typename T, int KV, int HD>
+template <bool APPEND, typename T, bool E4M3, int HD>
 void rows_launch(const RowsParams &p, bool vec, cudaStream_t s) {
     const bool many = static_cast<long>(p.n) * 2 * p.kv.kv_heads * (HD / 8) > kManyThreads && p.kv.kv_heads >= kHeads;
-    if (!vec) rows_launch<APPEND, T, KV, false, HD, 1>(p, s);
-    else if (many) rows_launch<APPEND, T, KV, true, HD, kHeads>(p, s);
-    else rows_launch<APPEND, T, KV, true, HD, 1>(p, s);
+    if (!vec) rows_launch<APPEND, T, E4M3, false, HD, 1>(p, s);
+    else if (many) rows_launch<APPEND, T, E4M3, true, HD, kHeads>(p, s);
+    else rows_launch<APPEND, T, E4M3, true, HD, 1>(p, s);
 }
-template <bool APPEND, typename T, int KV>
+template <bool APPEND, typename T, bool E4M3>
 void rows_launch(const RowsParams &p, bool vec, cudaStream_t s) {
-    if (p.kv.head_dim == 64) rows_launch<APPEND, T, KV, 64>(p, vec, s);
-    else rows_launch<APPEND, T, KV, 128>(p, vec, s);
+    if (p.kv.head_dim == 64) rows_launch<APPEND, T, E4M3, 64>(p, vec, s);
+    else rows_launch<APPEND, T, E4M3, 128>(p, vec, s);
+}
+
+// ---- e2m1 rows
+//
+// A block takes whole tokens (part of one when it has many heads), a thread E values of
+// each of U heads side by side.
+// Threads a block: with few rows (a head a thread) as many as take a token's at once, for the latency.
+__host__ __device__ constexpr int append4_threads(int u) { return u == 1 ? 256 : 128; }
+__host__ __device__ constexpr int gather4_threads(int u) { return u == 1 ? 256 : 64; }
+template <int HD, int U, int E, int NT>
+struct Place4 {
+    static constexpr int L = HD / E, ROWS = NT / L;  // threads a row, rows a block at a time
+    static __host__ __device__ int groups(const KvDev &kv) { return (kv.kv_heads + U - 1) / U; }
+    // tokens a block takes
+    static __host__ __device__ int tokens(const KvDev &kv) {
+        const int n = ROWS / (2 * groups(kv));
+        return n > 1 ? n : 1;
+    }
+    int c, t, which, head, n;  // n: heads of this thread, 0 past the end
+    // row: of the block's
+    __device__ __forceinline__ Place4(const RowsParams &p, int row) {
+        const unsigned g = groups(p.kv), per = 2 * g;
+        c = threadIdx.x % L;
+        const unsigned in = static_cast<unsigned>(row) / per, r = static_cast<unsigned>(row) % per;
+        const long tok = blockIdx.x * static_cast<long>(tokens(p.kv)) + in;
+        t = static_cast<int>(tok);
+        which = r >= g;
+        head = (which ? r - g : r) * U;
+        n = tok < p.n && in < tokens(p.kv) ? min(U, p.kv.kv_heads - head) : 0;
+    }
+};
+
+// The scale byte of 32 dims whose largest finite magnitude is a: the nearest scale to a / 6, ties to even (from
+// 2^-14 on the upper bits of the number with 3 of its mantissa, below in steps of 2^-17).
+__device__ __forceinline__ uint32_t e2m1_scale_byte(float a) {
+    const float r = __fdiv_rn(a, 6.f);
+    const uint32_t bits = __float_as_uint(r);
+    const uint32_t byte = r >= 6.103515625e-5f ? ((bits + 0x7ffffu + ((bits >> 20) & 1u)) >> 20) - ((127u - 15u) << 3)
+                                               : __float2uint_rn(r * 131072.f);
+    return min(byte, kKvTopScale);
+}
+// What a value is multiplied by before it becomes a code; 0 where the scale is 0.
+__device__ __forceinline__ float e2m1_inverse(uint32_t byte) {
+    return byte ? __frcp_rn(half_bits_to_float(static_cast<uint16_t>(byte << 7))) : 0.f;
+}
+__device__ __forceinline__ float max_abs_nan(float a, float b) {  // the larger magnitude, or NaN if either is
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(fabsf(b)));
+    return c;
+}
+// 8 codes, rounded to nearest, ties to even, larger values to the largest.
+__device__ __forceinline__ uint32_t e2m1_codes(const float (&f)[8], float inv) {
+    uint32_t q;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(q)
+        : "f"(f[0] * inv), "f"(f[1] * inv), "f"(f[2] * inv), "f"(f[3] * inv), "f"(f[4] * inv), "f"(f[5] * inv),
+          "f"(f[6] * inv), "f"(f[7] * inv));
+    return q;
+}
+
+// A thread has 8 values of U heads' rows; 4 threads share a block of 32 dims, and each works out the scale of one
+// head in 4 for all of them.  Measured: 12289 tokens of 8 heads x 128 from fp32 27 us (4.2
+// TB/s), from fp16 22, in blocks of 256 threads, 4 on an SM, 28 and 24 us.
+template <typename T, bool VEC, int HD, int U>
+__global__ void __launch_bounds__(append4_threads(U), U == 1 ? 4 : (sizeof(T) == 4 ? 9 : 10)) ijb_kv_append4_kernel(const __grid_constant__ RowsParams p) {
+    using P = Place4<HD, U, 8, append4_threads(U)>;
+    const int rows = P::tokens(p.kv) * 2 * P::groups(p.kv);
+    const int lane = threadIdx.x & 31, quad = lane & 28;
+    for (int row = threadIdx.x / P::L; row / P::ROWS * P::ROWS < rows; row += P::ROWS) {  // (all threads as often)
+        const P w(p, row);
+        const T *from = static_cast<const T *>(w.which ? p.v : p.k) + (w.n ? w.t * p.stride + static_cast<long>(w.head) * HD + w.c * 8 : 0);
+        float f[U][8], a[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (j < w.n) {
+                load_row8<VEC>(from + j * HD, f[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[j][i] = 0.f;
+            }
+        }
+        const long slot = w.n ? slot_row(p, w.t, w.which) : -1;
+        bool wild = false;  // an infinity or a NaN
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            a[j] = fabsf(f[j][0]);
+#pragma unroll
+            for (int i = 1; i < 8; ++i) a[j] = max_abs_nan(a[j], f[j][i]);
+            wild |= !(a[j] <= 3.402823466e38f);
+        }
+        uint32_t nan = 0;  // bit j: a NaN in this thread's part of head j's block
+        if (__any_sync(0xffffffffu, wild)) {
+            // infinities count as the largest value of their block, and are left to the conversion; zeros take their
+            // place in a block without a scale, and that of a NaN, whose block's scale is NaN
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                a[j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    a[j] = fmaxf(a[j], fabsf(f[j][i]) <= 3.402823466e38f ? fabsf(f[j][i]) : 0.f);
+                    nan |= f[j][i] != f[j][i] ? 1u << j : 0u;
+                }
+            }
+            nan |= __shfl_xor_sync(0xffffffffu, nan, 1);
+            nan |= __shfl_xor_sync(0xffffffffu, nan, 2);
+        }
+        uint32_t byte[(U + 3) / 4];  // of head 4 g + lane % 4 (U 1: of the head)
+        float inv[U];
+#pragma unroll
+        for (int g = 0; g < (U + 3) / 4; ++g) {
+            float mine;
+            if constexpr (U >= 4) {
+                // lane % 4 ends with the maximum of head 4 g + lane % 4
+                const bool odd = lane & 1, high = lane & 2;
+                float x = odd ? a[4 * g + 1] : a[4 * g], y = odd ? a[4 * g + 3] : a[4 * g + 2];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, odd ? a[4 * g] : a[4 * g + 1], 1));
+                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, odd ? a[4 * g + 2] : a[4 * g + 3], 1));
+                mine = fmaxf(high ? y : x, __shfl_xor_sync(0xffffffffu, high ? x : y, 2));
+            } else {
+                mine = fmaxf(a[0], __shfl_xor_sync(0xffffffffu, a[0], 1));
+                mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+            }
+            byte[g] = e2m1_scale_byte(mine);
+            const float x = e2m1_inverse(byte[g]);
+            if constexpr (U >= 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) inv[4 * g + j] = __shfl_sync(0xffffffffu, x, quad + j);
+            } else {
+                inv[0] = x;
+            }
+        }
+        if (slot < 0) continue;
+        const long to0 = slot + (static_cast<long>(w.head) << p.kv.page_shift);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const long to = to0 + (static_cast<long>(j) << p.kv.page_shift);
+            const uint32_t q = inv[j] > 0.f ? e2m1_codes(f[j], inv[j]) : 0u;
+            if (j < w.n) *reinterpret_cast<uint32_t *>(p.kv.data + to * (HD / 2) + w.c * 4) = q;
+        }
+#pragma unroll
+        for (int g = 0; g < (U + 3) / 4; ++g) {
+            const int j = U >= 4 ? 4 * g + (lane & 3) : 0;
+            const long to = to0 + (static_cast<long>(j) << p.kv.page_shift);
+            if (j < w.n && (U >= 4 || w.c % 4 == 0))
+                p.kv.scale[to * (HD / kKvBlock) + w.c / 4] = static_cast<uint8_t>((nan >> j) & 1u ? kKvNanScale : byte[g]);
+        }
+    }
+}
+
+// Code * scale, exact in fp32, and in fp16 for the scales that ijb_kv_append writes (others rounded once).  A thread
+// stores 16 bytes of each of U heads' rows, next to its neighbour's.  Bound by the latency of its three loads in a
+// row (the slot, its page, the codes), so what counts is how many threads are on an SM, and that a block of few
+// has more than one row each: 32749 tokens of 8 heads x 128 to fp16 take 34.7 us (4.9 TB/s) and to fp32 53 (5.7), in
+// blocks of 256 threads, 4 on an SM, 49 and 89.
+template <typename T, bool VEC, int HD, int U>
+__global__ void __launch_bounds__(gather4_threads(U), U == 1 ? 4 : 32) ijb_kv_gather4_kernel(const __grid_constant__ RowsParams p) {
+    constexpr int E = 16 / sizeof(T);
+    using P = Place4<HD, U, E, gather4_threads(U)>;
+    const int rows = P::tokens(p.kv) * 2 * P::groups(p.kv);
+    for (int row = threadIdx.x / P::L; row < rows; row += P::ROWS) {
+        const P w(p, row);
+        if (w.n == 0) continue;
+        const long slot = slot_row(p, w.t, w.which);
+        if (slot < 0) continue;
+        const long from0 = slot + (static_cast<long>(w.head) << p.kv.page_shift);
+        const uint8_t *from = p.kv.data + from0 * (HD / 2) + w.c * E / 8 * 4;  // (two threads' codes when E is 4)
+        const uint8_t *scale = p.kv.scale + from0 * (HD / kKvBlock) + w.c * E / kKvBlock;
+        T *dst = static_cast<T *>(w.which ? p.v : p.k) + w.t * p.stride + static_cast<long>(w.head) * HD + w.c * E;
+        uint32_t raw[U], sc[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (j >= w.n) continue;
+            raw[j] = *reinterpret_cast<const uint32_t *>(from + (static_cast<long>(j * (HD / 2)) << p.kv.page_shift));
+            sc[j] = scale[static_cast<long>(j * (HD / kKvBlock)) << p.kv.page_shift];
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (j >= w.n) continue;
+            if constexpr (E == 8) {
+                const __half2 s = __half2half2(__ushort_as_half(static_cast<uint16_t>(sc[j] << 7)));
+                __half2 h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t x = e2m1x2_half2(raw[j], i);
+                    h[i] = __hmul2(*reinterpret_cast<const __half2 *>(&x), s);
+                }
+                if constexpr (VEC) {
+                    *reinterpret_cast<uint4 *>(dst + j * HD) = *reinterpret_cast<const uint4 *>(h);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        dst[j * HD + 2 * i] = __low2half(h[i]);
+                        dst[j * HD + 2 * i + 1] = __high2half(h[i]);
+                    }
+                }
+            } else {
+                const float s = half_bits_to_float(static_cast<uint16_t>(sc[j] << 7));
+                const uint32_t mine = raw[j] >> (w.c % 2 * 16), x = e2m1x2_half2(mine, 0), y = e2m1x2_half2(mine, 1);
+                const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(&x)),
+                             v = __half22float2(*reinterpret_cast<const __half2 *>(&y));
+                if constexpr (VEC) {
+                    *reinterpret_cast<float4 *>(dst + j * HD) = make_float4(u.x * s, u.y * s, v.x * s, v.y * s);
+                } else {
+                    dst[j * HD] = u.x * s;
+                    dst[j * HD + 1] = u.y * s;
+                    dst[j * HD + 2] = v.x * s;
+                    dst[j * HD + 3] = v.y * s;
+                }
+            }
+        }
+    }
+}
+
+template <bool APPEND, typename T, bool VEC, int HD, int U>
+void rows4_launch(const RowsParams &p, cudaStream_t s) {
+    constexpr int NT = APPEND ? append4_threads(U) : gather4_threads(U);
+    using P = Place4<HD, U, APPEND ? 8 : 16 / static_cast<int>(sizeof(T)), NT>;
+    const int each = P::tokens(p.kv);
+    const unsigned blocks = static_cast<unsigned>((static_cast<long>(p.n) + each - 1) / each);
+    if constexpr (APPEND) ijb_kv_append4_kernel<T, VEC, HD, U><<<blocks, NT, 0, s>>>(p);
+    else ijb_kv_gather4_kernel<T, VEC, HD, U><<<blocks, NT, 0, s>>>(p);
+}
+// Four heads a thread from here on (threads of 8 values of a head).  In a graph, 8 heads, fp32, a head and four a thread:
+// head_dim 64, 512 rows (2^16) written 3.1 and 3.3 us, read 3.1 and 3.0; 1024 (2^17) 3.5 and 3.6, 4.1 and 3.6;
+// head_dim 128, 512 (2^17) 3.6 and 3.5, 4.0 and 3.8; 1024 (2^18) 4.9 and 4.1, 5.4 and 4.5; 4096 12.7 and 7.8, 13.6
+// and 7.9.
+constexpr long kMany4Threads = 1 << 17;
+template <bool APPEND, typename T, int HD>
+void rows4_launch(const RowsParams &p, bool vec, cudaStream_t s) {
+    const bool many = static_cast<long>(p.n) * 2 * p.kv.kv_heads * (HD / 8) >= kMany4Threads && p.kv.kv_heads >= kHeads;
+    if (!vec) rows4_launch<APPEND, T, false, HD, 1>(p, s);
+    else if (many) rows4_launch<APPEND, T, true, HD, kHeads>(p, s);
+    else rows4_launch<APPEND, T, true, HD, 1>(p, s);
 }
 
 template <bool APPEND, typename T>
 void rows_launch(const RowsParams &p, int type, bool vec, cudaStream_t s) {
-    if (type == IJB_KV_E2M1) rows_launch<APPEND, T, IJB_KV_E2M1>(p, vec, s);
-    else if (type == IJB_KV_E4M3) rows_launch<APPEND, T, IJB_KV_E4M3>(p, vec, s);
-    else rows_launch<APPEND, T, IJB_KV_F16>(p, vec, s);
+    if (type == IJB_KV_E2M1) p.kv.head_dim == 64 ? rows4_launch<APPEND, T, 64>(p, vec, s) : rows4_launch<APPEND, T, 128>(p, vec, s);
+    else if (type == IJB_KV_E4M3) rows_launch<APPEND, T, true>(p, vec, s);
+    else rows_launch<APPEND, T, false>(p, vec, s);
 }
 
 template <bool APPEND>
