@@ -326,7 +326,8 @@ __device__ __forceinline__ Left left_of(const AttnArgs &a, const Segment &s, int
     if (s.b0 > 0 || s.b1 == s.units) return x;
     // workers w' > worker begin in the tile up to the last w' * per that leaves `least` units of it
     const long last = s.start + a.over + s.units - a.least;
-    x.states = 1 + static_cast<int>(last / per) - worker;
+    x.states = 1 + ((last >> 32) ? static_cast<int>(last / per)
+                                 : static_cast<int>(static_cast<uint32_t>(last) / static_cast<uint32_t>(per))) - worker;
     x.q0 = s.x.q0;
     x.row0 = s.ti * a.tile_rows;
     x.rows = min(a.tile_rows, s.x.rows - x.row0);
@@ -932,7 +933,7 @@ struct Dec4 {
     static constexpr int kTile = kPos * kRowBytes, kScales = kPos * kBlocks;
     static constexpr int kStage = 2 * (kTile + kScales);  // K, V, their scale bytes
     static constexpr int kWarps = HD == 128 ? (WIDE || kSplit ? 8 : 12) : (WIDE || kSplit ? 12 : 16);
-    static constexpr int kFit = 224 * 1024 / (kWarps * kStage), kStages = kFit > 4 ? 4 : kFit;
+    static constexpr int kFit = 216 * 1024 / (kWarps * kStage), kStages = kFit > 4 ? 4 : kFit;
     static constexpr int kSmem = kWarps * kStages * kStage;
     static_assert(kStages >= 2, "stages");
 };
@@ -963,8 +964,10 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     constexpr int PC = D::kPos, TT = PC / 16, G = PC / 8;  // positions, tiles and groups of a chunk
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PlanOut block_po;
-    // what a warp needs between its runs only: its places in the line (loading, computing), the run it computes
-    __shared__ struct { Cursor load, use; Segment run; } state[D::kWarps];
+    // what a warp needs between its runs only: the loading side's place in the line, and the runs from the one
+    // being computed to the one being loaded (each chunk that is loaded ahead may end one)
+    constexpr int QUEUE = D::kStages + 1;
+    __shared__ struct { Cursor load; Segment run[QUEUE]; } state[D::kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t4 = lane & 3;
     pdl_trigger();
     const int worker = blockIdx.x * D::kWarps + warp;
@@ -986,22 +989,12 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
         __syncthreads();
     }
     if (lane == 0) {
-        my.load = my.use = first;
+        my.load = first;
         Left none = {};
         none.runs = first;
         a.left[worker] = none;
     }
     __syncwarp();
-    // the next run of one of the two sides; false at the end
-    auto next_run = [&](Cursor &at, Segment &s) {
-        Cursor c = at;
-        const bool ok = cursor_next(a, c, s);
-        __syncwarp();
-        if (lane == 0) at = c;
-        __syncwarp();
-        return ok;
-    };
-
     const uint32_t base = smem_u32(smem) + warp * D::kStages * D::kStage;
     const T *qp = static_cast<const T *>(a.q);
     T *op = static_cast<T *>(a.out);
@@ -1015,14 +1008,25 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     bool fresh = true;      // the next window becomes the current one
     bool gone = false;      // a page was none: the merge computes these runs' rows again, without its positions
     bool more = false;
+    int queued = 0, queue_in = 0;
     auto load_run = [&]() {
+        Cursor c = my.load;
         Segment s;
-        more = next_run(my.load, s);
+        more = cursor_next(a, c, s);
+        if (!more) return;
         l_kv = s.x.kv;
         l_seq = s.x.seq;
         l_head = s.head;
         lb = s.b0;
         l_end = s.b1;
+        __syncwarp();
+        if (lane == 0) {
+            my.load = c;
+            my.run[queue_in] = s;
+        }
+        __syncwarp();
+        ++queued;
+        queue_in = queue_in + 1 == QUEUE ? 0 : queue_in + 1;
     };
     auto peek = [&]() {
         window = lb;
@@ -1091,10 +1095,9 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
     const float sc = a.scale_log2, raise = fminf(8.f / sc, 3e38f);
     int stage = 0;
     bool bad = false;
-    while (true) {
-        Segment s;
-        if (!next_run(my.use, s)) break;
-        if (lane == 0) my.run = s;  // (read behind the run, not held)
+    // (the last chunk of a run has been loaded, and the next run been queued, before it is computed)
+    for (int run = 0, queue_out = 0; run < queued; ++run, queue_out = queue_out + 1 == QUEUE ? 0 : queue_out + 1) {
+        Segment s = my.run[queue_out];  // (read again behind the run, not held)
         const int kv = s.x.kv, b1 = s.b1;
         const int row0 = s.ti * kDecRows, rows = min(kDecRows, s.x.rows - row0);
         uint32_t qh[KS][N][2], ql[SPLIT ? KS : 1][N][2];
@@ -1325,7 +1328,7 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 for (int k = 0; k < 4; ++k) zero = fmaf(o[i][n][k], 0.f, zero);
         bad |= !(zero == 0.f);
         // ---- the run's end: the output, or its state
-        s = my.run;
+        s = my.run[queue_out];
         const int end_row0 = s.ti * kDecRows, end_rows = min(kDecRows, s.x.rows - end_row0);
         if (lane == 0) {
             const Left left = left_of(a, s, worker, per);
@@ -2295,6 +2298,67 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool 
 // positions, 12 rows of 128 each, took 25, 30, 39 and 80 us in all with 1, 2, 4 and 16
 // rows a block, and 64 ragged sequences 27, 25, 25 and 27 us.
 constexpr int kMergeBatch = 4;
+
+// One tile's rows row0 .. row0 + RB (of `left`'s, which worker w0 began) by a warp, where they have up to kFewStates
+// states: a lane has a state's maximum and sum, then HD / 32 dims over all of them.  Bit 0: a value is not finite;
+// bit 1: a page was none.
+constexpr int kFewStates = 8;
+template <int ROWS, int HD, int RB, typename T>
+__device__ __forceinline__ int merge_few(const AttnArgs &a, const Left &left, int w0, int row0) {
+    constexpr int E = HD / 32;
+    constexpr long PF = part_floats<ROWS, HD>();
+    const int lane = threadIdx.x & 31, n = left.states, rows = min(RB, left.rows - row0);
+    const float *mine = a.part + (2L * (w0 + lane) + (lane == 0 ? 1 : 0)) * PF;  // lane's state, for lane < n
+    const int theirs = lane < n ? a.left[w0 + lane].bad : 0;
+    T *op = static_cast<T *>(a.out);
+    const bool vec = reinterpret_cast<uintptr_t>(op) % (E * sizeof(T)) == 0 && a.out_stride % E == 0;
+    bool fine = true;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+        if (r >= rows) break;
+        float v[kFewStates][E];
+#pragma unroll
+        for (int i = 0; i < kFewStates; ++i) {
+            const float *p = a.part + (2L * (w0 + i) + (i == 0 ? 1 : 0)) * PF + (row0 + r) * HD + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 x = i < n ? *reinterpret_cast<const float2 *>(p + e) : make_float2(0.f, 0.f);
+                v[i][e] = x.x;
+                v[i][e + 1] = x.y;
+            }
+        }
+        const float m = lane < n ? mine[ROWS * HD + row0 + r] : -INFINITY, l = lane < n ? mine[ROWS * HD + ROWS + row0 + r] : 0.f;
+        const float top = warp_max(m), f = ex2(m - (top == -INFINITY ? 0.f : top));
+        const float sum = warp_sum(f != 0.f ? l * f : 0.f), inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        float acc[E] = {};
+#pragma unroll
+        for (int i = 0; i < kFewStates; ++i) {
+            const float w = __shfl_sync(0xffffffffu, f, i);
+            if (w != 0.f) {  // a state without positions may hold no values
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[i][e], acc[e]);
+            }
+        }
+        const int rr = left.row0 + row0 + r;
+        T *dst = op + static_cast<long>(left.q0 + rr / a.group) * a.out_stride + (left.head * a.group + rr % a.group) * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            fine = fine && acc[e] * 0.f * inv == 0.f;
+            acc[e] *= inv;
+        }
+        if constexpr (E == 4) {
+            store4(dst, vec, acc[0], acc[1], acc[2], acc[3]);
+        } else {
+            if (vec && sizeof(T) == 4) *reinterpret_cast<float2 *>(dst) = make_float2(acc[0], acc[1]);
+            else if (vec) *reinterpret_cast<uint32_t *>(dst) = half2_bits(acc[0], acc[1]);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e) dst[e] = static_cast<T>(acc[e]);
+        }
+    }
+    return (__all_sync(0xffffffffu, fine) ? 0 : 1) | (__any_sync(0xffffffffu, (theirs & 2) != 0) ? 2 : 0);
+}
+
 template <int ROWS, int HD, int NT, int EACH, int RB, int KV, typename T>
 __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_constant__ AttnArgs a) {
     __shared__ float top[RB], total[RB];
@@ -2311,6 +2375,29 @@ __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_consta
         const int bad = in ? a.left[w].bad : 0;
         again = __ballot_sync(0xffffffffu, bad != 0);
         all = __ballot_sync(0xffffffffu, (bad & 2) != 0);
+    }
+    static_assert(KV != IJB_KV_E2M1 || ROWS != kDecRows || EACH == NT / 32, "a warp a worker");
+    if (KV == IJB_KV_E2M1 && ROWS == kDecRows && (some & (some - 1))) {  // several tiles
+        // those of few states are merged at once, a warp each, not one after another: 64 ragged sequences 23.7 -> 19.9 us
+        __shared__ uint32_t done, look, whole;
+        if (threadIdx.x == 0) done = look = whole = 0u;
+        __syncthreads();
+        const int j = threadIdx.x >> 5;
+        if ((some >> j) & 1u) {
+            const Left left = a.left[blockIdx.x * EACH + j];
+            if (left.states <= kFewStates) {
+                const int how = merge_few<ROWS, HD, RB, T>(a, left, blockIdx.x * EACH + j, row0);
+                if ((threadIdx.x & 31) == 0) {
+                    atomicOr(&done, 1u << j);
+                    if (how) atomicOr(&look, 1u << j);
+                    if (how & 2) atomicOr(&whole, 1u << j);
+                }
+            }
+        }
+        __syncthreads();
+        some &= ~done;
+        again |= look;
+        all |= whole;
     }
     for (; some; some &= some - 1) {
         const int w0 = blockIdx.x * EACH + __ffs(some) - 1;
@@ -2492,7 +2579,7 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.tile_rows = kDecRows;
     a.unit = D::kPos;
     a.workers = sms * D::kWarps;
-    a.min_units = 2;
+    a.min_units = 64 / D::kPos;  // 64 positions
     a.over = 1;
     a.least = 1;
     decode_kernel<HD, KV, WIDE, T>()<<<sms, D::kWarps * 32, decode_smem<HD, KV, WIDE, T>(), s>>>(a);
