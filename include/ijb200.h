@@ -85,11 +85,12 @@ typedef struct {
  * inferencer.cu:1218-1230).  Replaces FastGPU::FastGPU + FastRunner::FastRunner. */
 int ijb_create(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, ijb_engine **out);
 
-/* The same engine with its K/V pool of cache type kv_type (IJB_KV_F16 or
- * IJB_KV_E4M3, below; desc->kv_f32 is ignored) and ijb_paged_attention in every
- * step: prompts run their chunks' attention on the tensor cores a tile at a time
- * where an engine of ijb_create reads the cache once for each new token, and an
- * e4m3 pool holds twice the positions.  max_batch <= 4096.  The rounding of a
+/* The same engine with its K/V pool of cache type kv_type (IJB_KV_F16,
+ * IJB_KV_E4M3 or IJB_KV_E2M1, below; desc->kv_f32 is ignored) and
+ * ijb_paged_attention in every step: prompts run their chunks' attention on the
+ * tensor cores a tile at a time where an engine of ijb_create reads the cache once
+ * for each new token, and an e4m3 pool holds twice the positions, an e2m1 pool 3.76
+ * times.  max_batch <= 4096.  The rounding of a
  * token's attention depends on the step it runs in (ijb_paged_attention). */
 int ijb_create_kv(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, int kv_type,
                   ijb_engine **out);
@@ -160,6 +161,18 @@ const float *ijb_residual_dev(const ijb_engine *engine);
 int ijb_seq_open(ijb_engine *engine, int *seq_id);
 int ijb_seq_close(ijb_engine *engine, int seq_id);
 int ijb_seq_length(const ijb_engine *engine, int seq_id);
+
+/* A new sequence that holds the first `length` (0 to its length) positions of
+ * seq_id, as if they had been prefilled: beams, several answers to one prompt, a
+ * system prompt that many sequences begin with.  The two share the pages that
+ * those positions fill; the page that they end within is copied
+ * (ijb_kv_copy_pages, one launch for all layers).  Both go on by themselves: a
+ * shared page is given back when the last of its sequences is closed, and one
+ * that a sequence writes to again (sequence 0, which ijb_forward, ijb_prefill and
+ * ijb_reset set back) is replaced by a page of its own first.  IJB_ERR_CAPACITY
+ * when there is no sequence or page left, in which case nothing has changed.
+ * Returns after the copy completed. */
+int ijb_seq_fork(ijb_engine *engine, int seq_id, int length, int *new_seq);
 
 /* One packed step over n entries: entry i appends tokens[i] to sequence
  * seq_ids[i] at that sequence's next position.  Entries may repeat a

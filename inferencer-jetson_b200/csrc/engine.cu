@@ -98,13 +98,14 @@ struct ijb_engine {
     int kv_elem = 2;
     long page_stride = 0;
     // engines made by ijb_create_kv: attention is ijb_paged_attention over the pool
-    // (IJB_KV_F16 / IJB_KV_E4M3; -1: the engine's own attention).  An e4m3 pool is
+    // (an IJB_KV_* type; -1: the engine's own attention).  An e4m3 or e2m1 pool is
     // written by ijb_kv_append from the fp32 rows that the QKV projection leaves,
     // [max_batch][K, V][kv_dim]: to the projection a cache of one-token pages,
     // entry i in slot i.
     int paged = -1;
-    int pool_elem = 2;            // bytes of a pool element
-    uint8_t *kv_scale = nullptr;  // e4m3: a scale byte per row, like the pool
+    int pool_bits = 16;           // of a pool element
+    uint8_t *kv_scale = nullptr;  // e4m3, e2m1: the rows' scale bytes, like the pool
+    int row_scales = 0;           // scale bytes of a row
     float *kv_rows = nullptr;
     int *row_slot = nullptr;      // 0, 1, 2, ...
     int out_page_size = 0;        // the pages the projection writes
@@ -113,6 +114,11 @@ struct ijb_engine {
     size_t paged_work_bytes = 0;
     long num_pages = 0;
     std::vector<int> free_pages;
+    std::vector<int> page_refs;  // sequences that hold a page: forks share their full pages (ijb_seq_fork)
+    // pages to be copied, in every layer, before the next step's kernels: (from, to)
+    std::vector<std::pair<int, int>> page_copies;
+    int *copy_host = nullptr, *copy_dev = nullptr;  // their ids, pinned and on the device, [2][copy_room]
+    size_t copy_room = 0;
     int max_pages_per_seq = 0;
     int *page_table_dev = nullptr;
     std::vector<CUtensorMap> kv_maps;  // per layer, for the streaming attention (fp16 cache, head_dim 64)
@@ -422,8 +428,8 @@ ijb_kv_view layer_view(const ijb_engine *e, int l) {
     v.head_dim = e->head_dim;
     v.page_size = e->d.page_size;
     v.num_pages = e->num_pages;
-    v.data_dev = static_cast<char *>(e->kv) + l * pool * e->pool_elem;
-    v.scale_dev = e->kv_scale ? e->kv_scale + l * (pool / e->head_dim) : nullptr;
+    v.data_dev = static_cast<char *>(e->kv) + l * (pool * e->pool_bits / 8);
+    v.scale_dev = e->kv_scale ? e->kv_scale + l * (pool / e->head_dim * e->row_scales) : nullptr;
     v.page_table_dev = e->page_table_dev;
     v.n_seqs = e->d.max_seqs;
     v.max_pages = e->max_pages_per_seq;
@@ -682,17 +688,77 @@ void run_step(ijb_engine *e, int n, bool need_logits, bool traced = false, StepS
     e->last_n = n;
 }
 
+int take_page(ijb_engine *e) {
+    require(!e->free_pages.empty(), "KV page pool exhausted", IJB_ERR_CAPACITY);
+    const int p = e->free_pages.back();
+    e->free_pages.pop_back();
+    e->page_refs[p] = 1;
+    return p;
+}
+void release_page(ijb_engine *e, int p) {
+    if (--e->page_refs[p] == 0) e->free_pages.push_back(p);  // (room for all pages is reserved)
+}
+void release_pages(ijb_engine *e, int seq) {
+    for (int p : e->seq_pages[seq]) release_page(e, p);
+    e->seq_pages[seq].clear();
+}
+
+// Queues the copies of page_copies, all layers' in one launch: to the copy a pool of
+// layers * num_pages pages.  The ids' staging is free: every call that queues waits for
+// its stream before it returns.
+void copy_pages(ijb_engine *e) {
+    const std::vector<std::pair<int, int>> todo = std::move(e->page_copies);
+    e->page_copies.clear();
+    if (todo.empty()) return;
+    const int layers = e->d.layers;
+    const size_t n = todo.size() * layers;
+    if (n > e->copy_room) {
+        cudaFree(e->copy_dev);
+        if (e->copy_host) cudaFreeHost(e->copy_host);
+        e->copy_dev = nullptr;
+        e->copy_host = nullptr;
+        e->copy_room = 0;
+        e->copy_dev = dev_alloc<int>(2 * n, "page copies");
+        ck(cudaMallocHost(&e->copy_host, 2 * n * sizeof(int)), "page copy staging");
+        e->copy_room = n;
+    }
+    for (int l = 0; l < layers; ++l)
+        for (size_t i = 0; i < todo.size(); ++i) {
+            e->copy_host[l * todo.size() + i] = static_cast<int>(l * e->num_pages + todo[i].first);
+            e->copy_host[n + l * todo.size() + i] = static_cast<int>(l * e->num_pages + todo[i].second);
+        }
+    ijb_kv_view v = layer_view(e, 0);
+    v.num_pages = layers * e->num_pages;
+    if (e->paged < 0) {  // fp32 pages are fp16 ones of twice the heads
+        v.type = IJB_KV_F16;
+        v.kv_heads *= e->kv_f32 ? 2 : 1;
+    }
+    ck(cudaMemcpyAsync(e->copy_dev, e->copy_host, 2 * n * sizeof(int), cudaMemcpyHostToDevice, e->stream), "page copies H2D");
+    if (ijb_kv_copy_pages(&v, nullptr, static_cast<int>(n), e->copy_dev, e->copy_dev + n, e->status, e->stream) != IJB_OK)
+        throw Error(IJB_ERR_CUDA, t_create_err);
+}
+
 // Makes sure `seq` owns pages for positions [0, upto]; returns the slot of `pos`.
-int slot_for(ijb_engine *e, int seq, int pos) {
+// `write`: the position is to be written, so a page that another sequence shares is
+// replaced by one of this sequence's own (with the positions before pos: copy_pages).
+int slot_for(ijb_engine *e, int seq, int pos, bool write = true) {
     const int ps = e->d.page_size;
     auto &pages = e->seq_pages[seq];
     bool changed = false;
     while (static_cast<int>(pages.size()) * ps <= pos) {
-        require(!e->free_pages.empty(), "KV page pool exhausted", IJB_ERR_CAPACITY);
         require(static_cast<int>(pages.size()) < e->max_pages_per_seq, "sequence exceeds context", IJB_ERR_CAPACITY);
-        pages.push_back(e->free_pages.back());
-        e->free_pages.pop_back();
+        pages.push_back(take_page(e));
         e->page_table_host[static_cast<long>(seq) * e->max_pages_per_seq + pages.size() - 1] = pages.back();
+        changed = true;
+    }
+    int &page = pages[pos / ps];
+    if (write && e->page_refs[page] > 1) {
+        if (pos % ps) e->page_copies.reserve(e->page_copies.size() + 1);
+        const int own = take_page(e);
+        if (pos % ps) e->page_copies.emplace_back(page, own);
+        release_page(e, page);
+        page = own;
+        e->page_table_host[static_cast<long>(seq) * e->max_pages_per_seq + pos / ps] = own;
         changed = true;
     }
     if (changed)
@@ -700,7 +766,7 @@ int slot_for(ijb_engine *e, int seq, int pos) {
                            e->page_table_host + static_cast<long>(seq) * e->max_pages_per_seq,
                            pages.size() * sizeof(int), cudaMemcpyHostToDevice, e->stream),
            "page table H2D");
-    return pages[pos / ps] * ps + pos % ps;
+    return page * ps + pos % ps;
 }
 
 // Fills meta for entries (seq, token) at explicit positions and runs a step.
@@ -719,6 +785,7 @@ void packed_step(ijb_engine *e, int n, const int *seqs, const int *tokens, const
         mt[2 * d.max_batch + i] = pos;
         mt[3 * d.max_batch + i] = slot_for(e, sq, pos);
     }
+    copy_pages(e);
     for (int i = n; i < d.max_batch; ++i) mt[i] = mt[d.max_batch + i] = mt[2 * d.max_batch + i] = mt[3 * d.max_batch + i] = 0;
     run_step(e, n, need_logits, traced, fill_entries(e, n), then);
 }
@@ -775,8 +842,8 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
     std::unique_ptr<ijb_engine> e(new ijb_engine());
     try {
         require(desc && out && tensors, "null argument");
-        require(kv_type == -1 || kv_type == IJB_KV_F16 || kv_type == IJB_KV_E4M3,
-                "cache type must be IJB_KV_F16 or IJB_KV_E4M3");
+        require(kv_type == -1 || kv_type == IJB_KV_F16 || kv_type == IJB_KV_E4M3 || kv_type == IJB_KV_E2M1,
+                "cache type must be IJB_KV_F16, IJB_KV_E4M3 or IJB_KV_E2M1");
         e->paged = kv_type;
         e->d = *desc;
         ijb_model_desc &d = e->d;
@@ -994,14 +1061,16 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
             require(bad.empty(), "paged attention: " + bad);
             require(d.heads / d.kv_heads <= 16, "paged attention: heads must be 1 to 16 times kv_heads");
             require(d.max_batch <= 4096, "max_batch must be <= 4096 with a paged attention cache type");
-            d.kv_f32 = e->paged == IJB_KV_E4M3;  // what the projection writes
+            d.kv_f32 = e->paged != IJB_KV_F16;  // what the projection writes
         }
         e->kv_f32 = d.kv_f32 ? 1 : 0;
         e->kv_elem = e->kv_f32 ? 4 : 2;
-        e->pool_elem = e->paged == IJB_KV_E4M3 ? 1 : e->kv_elem;
+        const bool quantised = e->paged == IJB_KV_E4M3 || e->paged == IJB_KV_E2M1;
+        e->pool_bits = e->paged == IJB_KV_E2M1 ? 4 : (e->paged == IJB_KV_E4M3 ? 8 : 8 * e->kv_elem);
+        e->row_scales = e->paged == IJB_KV_E2M1 ? e->head_dim / kKvBlock : (e->paged == IJB_KV_E4M3 ? 1 : 0);
         e->out_page_size = d.page_size;
         e->out_page_stride = e->page_stride;
-        if (e->paged == IJB_KV_E4M3) {
+        if (quantised) {
             e->out_page_size = 1;
             e->out_page_stride = 2L * e->kv_dim;
             e->kv_rows = dev_alloc<float>(static_cast<size_t>(d.max_batch) * 2 * e->kv_dim, "K/V rows");
@@ -1009,11 +1078,11 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
             for (int i = 0; i < d.max_batch; ++i) slot[i] = i;
             e->row_slot = dev_alloc<int>(d.max_batch, "K/V row slots");
             ck(cudaMemcpy(e->row_slot, slot.data(), d.max_batch * sizeof(int), cudaMemcpyHostToDevice), "K/V row slots");
-            const size_t scales = static_cast<size_t>(d.layers) * e->num_pages * (e->page_stride / e->head_dim);
+            const size_t scales = static_cast<size_t>(d.layers) * e->num_pages * (e->page_stride / e->head_dim) * e->row_scales;
             e->kv_scale = dev_alloc<uint8_t>(scales, "KV scales");
             ck(cudaMemset(e->kv_scale, 0, scales), "KV scales clear");
         }
-        const size_t kv_bytes = static_cast<size_t>(d.layers) * e->num_pages * e->page_stride * e->pool_elem;
+        const size_t kv_bytes = static_cast<size_t>(d.layers) * e->num_pages * (e->page_stride * e->pool_bits / 8);
         e->kv = dev_alloc<char>(kv_bytes, "KV pool");
         ck(cudaMemset(e->kv, 0, kv_bytes), "KV clear");
         if (!e->kv_f32 && e->paged < 0 && (e->head_dim == 64 || e->head_dim == 128)) {
@@ -1025,6 +1094,7 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
                     e->kv_maps.clear();  // the CUDA-core attention serves every layer then
         }
         for (long p = e->num_pages - 1; p >= 0; --p) e->free_pages.push_back(static_cast<int>(p));
+        e->page_refs.assign(e->num_pages, 0);
         const size_t pt = static_cast<size_t>(d.max_seqs) * e->max_pages_per_seq;
         e->page_table_dev = dev_alloc<int>(pt, "page table");
         ck(cudaMemset(e->page_table_dev, 0, pt * sizeof(int)), "page table clear");
@@ -1085,7 +1155,7 @@ int ijb_create(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n
 int ijb_create_kv(const ijb_model_desc *desc, const ijb_tensor_view *tensors, int n_tensors, int kv_type,
                   ijb_engine **out) {
     if (kv_type < 0) {
-        set_thread_error("ijb_create_kv: cache type must be IJB_KV_F16 or IJB_KV_E4M3");
+        set_thread_error("ijb_create_kv: cache type must be IJB_KV_F16, IJB_KV_E4M3 or IJB_KV_E2M1");
         return IJB_ERR_INVALID;
     }
     return create_engine(desc, tensors, n_tensors, kv_type, out);
@@ -1107,6 +1177,8 @@ void ijb_destroy(ijb_engine *e) {
     }
     cudaFree(e->kv);
     cudaFree(e->kv_scale);
+    cudaFree(e->copy_dev);
+    if (e->copy_host) cudaFreeHost(e->copy_host);
     cudaFree(e->kv_rows);
     cudaFree(e->row_slot);
     cudaFree(e->paged_work);
@@ -1286,8 +1358,7 @@ int ijb_time_layer_projections(ijb_engine *e, int n, int reps, float *ms_per_lay
         g_launches += launches;  // the second replay (the capture counted the first)
         check_device_status(e);
         // the timed K/V writes leave sequence 0 holding n positions of no meaning
-        for (int p : e->seq_pages[0]) e->free_pages.push_back(p);
-        e->seq_pages[0].clear();
+        release_pages(e, 0);
         *ms_per_layer = ms / reps;
         return IJB_OK;
     } catch (const std::exception &ex) {
@@ -1315,7 +1386,7 @@ int ijb_time_layer_attention(ijb_engine *e, int n, const int *seq_ids, int reps,
             mt[i] = 0;
             mt[d.max_batch + i] = sq;
             mt[2 * d.max_batch + i] = len - 1;
-            mt[3 * d.max_batch + i] = slot_for(e, sq, len - 1);  // an existing slot: no page is taken
+            mt[3 * d.max_batch + i] = slot_for(e, sq, len - 1, false);  // an existing slot: no page is taken
             positions += len;
         }
         ck(cudaMemcpyAsync(e->meta_dev, e->meta_host, 4 * d.max_batch * sizeof(int), cudaMemcpyHostToDevice, e->stream),
@@ -1364,7 +1435,7 @@ int ijb_time_layer_attention(ijb_engine *e, int n, const int *seq_ids, int reps,
         g_launches += launches;  // the second replay (the capture counted the first)
         check_device_status(e);
         *ms_per_layer = ms / reps;
-        *kv_bytes = positions * d.kv_heads * 2LL * (e->head_dim * e->pool_elem + (e->kv_scale ? 1 : 0));
+        *kv_bytes = positions * d.kv_heads * 2LL * (e->head_dim * e->pool_bits / 8 + e->row_scales);
         return IJB_OK;
     } catch (const std::exception &ex) {
         return fail(e, ex);
@@ -1426,10 +1497,58 @@ int ijb_seq_open(ijb_engine *e, int *seq_id) {
 int ijb_seq_close(ijb_engine *e, int seq) {
     try {
         require(e != nullptr && seq > 0 && seq < e->d.max_seqs && e->seq_used[seq], "unknown sequence id");
-        for (int p : e->seq_pages[seq]) e->free_pages.push_back(p);
-        e->seq_pages[seq].clear();
+        release_pages(e, seq);
         e->seq_len[seq] = 0;
         e->seq_used[seq] = 0;
+        return IJB_OK;
+    } catch (const std::exception &ex) {
+        return fail(e, ex);
+    }
+}
+
+int ijb_seq_fork(ijb_engine *e, int seq, int length, int *new_seq) {
+    try {
+        require(e != nullptr && new_seq != nullptr, "bad arguments");
+        require(seq >= 0 && seq < e->d.max_seqs && e->seq_used[seq], "unknown sequence id");
+        require(length >= 0 && length <= e->seq_len[seq], "length must be 0 to the sequence's length");
+        int to = 1;
+        while (to < e->d.max_seqs && e->seq_used[to]) ++to;
+        require(to < e->d.max_seqs, "sequence table full", IJB_ERR_CAPACITY);
+        ck(cudaSetDevice(e->d.device), "cudaSetDevice");
+        const int full = length / e->d.page_size;
+        const bool tail = length % e->d.page_size != 0;
+        const std::vector<int> &from = e->seq_pages[seq];
+        std::vector<int> &pages = e->seq_pages[to];
+        pages.reserve(full + 1);
+        e->page_copies.reserve(e->page_copies.size() + 1);
+        const int own = tail ? take_page(e) : -1;  // (nothing has changed if there is none)
+        for (int i = 0; i < full; ++i) {
+            pages.push_back(from[i]);
+            ++e->page_refs[from[i]];
+        }
+        if (tail) {
+            pages.push_back(own);
+            e->page_copies.emplace_back(from[full], own);
+        }
+        try {
+            int *row = e->page_table_host + static_cast<long>(to) * e->max_pages_per_seq;
+            for (size_t i = 0; i < pages.size(); ++i) row[i] = pages[i];
+            if (!pages.empty())
+                ck(cudaMemcpyAsync(e->page_table_dev + static_cast<long>(to) * e->max_pages_per_seq, row,
+                                   pages.size() * sizeof(int), cudaMemcpyHostToDevice, e->stream),
+                   "page table H2D");
+            copy_pages(e);
+            ck(cudaStreamSynchronize(e->stream), "fork");
+            check_device_status(e);
+        } catch (...) {
+            cudaStreamSynchronize(e->stream);
+            e->page_copies.clear();
+            release_pages(e, to);
+            throw;
+        }
+        e->seq_used[to] = 1;
+        e->seq_len[to] = length;
+        *new_seq = to;
         return IJB_OK;
     } catch (const std::exception &ex) {
         return fail(e, ex);
@@ -1464,6 +1583,7 @@ int ijb_generate(ijb_engine *e, int seq, int first_token, int max_tokens, const 
         int *mt = e->meta_host;
         std::memset(mt, 0, e->meta_ints * sizeof(int));
         for (int k = steps - 1; k >= 0; --k) slot_for(e, seq, pos0 + k);
+        copy_pages(e);
         mt[0] = first_token;
         mt[d.max_batch] = seq;
         mt[2 * d.max_batch] = pos0;
@@ -1539,7 +1659,7 @@ int ijb_generate(ijb_engine *e, int seq, int first_token, int max_tokens, const 
         auto &pages = e->seq_pages[seq];
         const size_t keep = (e->seq_len[seq] + d.page_size - 1) / d.page_size;
         while (pages.size() > keep) {
-            e->free_pages.push_back(pages.back());
+            release_page(e, pages.back());
             pages.pop_back();
         }
         return IJB_OK;

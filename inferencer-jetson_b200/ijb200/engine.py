@@ -67,8 +67,8 @@ class Engine:
         h = ctypes.c_void_p()
         if kv_type is None:
             rc = self.lib.ijb_create(ctypes.byref(d), views, len(weights), ctypes.byref(h))
-        else:  # "f16" or "e4m3": a pool of that type, read by the paged attention
-            rc = self.lib.ijb_create_kv(ctypes.byref(d), views, len(weights), {"f16": 0, "e4m3": 2}[kv_type],
+        else:  # "f16", "e4m3" or "e2m1": a pool of that type, read by the paged attention
+            rc = self.lib.ijb_create_kv(ctypes.byref(d), views, len(weights), {"f16": 0, "e4m3": 2, "e2m1": 3}[kv_type],
                                         ctypes.byref(h))
         _L.check(rc, None)
         self.h = h
@@ -149,6 +149,13 @@ class Engine:
 
     def seq_length(self, seq: int) -> int:
         return self.lib.ijb_seq_length(self.h, int(seq))
+
+    def seq_fork(self, seq: int, length: int | None = None) -> int:
+        """ijb_seq_fork: a new sequence that holds the first ``length`` (default: all) positions of ``seq``."""
+        s = ctypes.c_int(-1)
+        length = self.seq_length(seq) if length is None else length
+        _L.check(self.lib.ijb_seq_fork(self.h, int(seq), int(length), ctypes.byref(s)), self.h)
+        return s.value
 
     def seq_prefill(self, seq: int, tokens) -> int:
         arr = (ctypes.c_int * len(tokens))(*[int(t) for t in tokens])

@@ -77,6 +77,7 @@ def load():
         "ijb_seq_open": ([P, IP], I),
         "ijb_seq_close": ([P, I], I),
         "ijb_seq_length": ([P, I], I),
+        "ijb_seq_fork": ([P, I, I, IP], I),
         "ijb_decode_step": ([P, I, IP, IP, IP], I),
         "ijb_decode_sample": ([P, I, IP, IP, P, P, P, P, P, IP, P], I),
         "ijb_generate": ([P, I, I, I, IP, I, IP, IP], I),

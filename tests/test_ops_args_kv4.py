@@ -34,3 +34,32 @@ def test_attention_views_are_checked(bad):
     assert L.ijb_paged_attention(ctypes.byref(v), 4, 0, 4096, 256, 8192, 256, 2, 1, 256, None, 256, 1, 0.125, 4096,
                                  1 << 40, None, None) == lib.ERR_INVALID
     assert "ijb_paged_attention" in L.ijb_last_error(None).decode()
+
+
+@pytest.mark.parametrize("bad", BAD_VIEWS)
+def test_copied_pages_views_are_checked(bad):
+    L = lib.load()
+    v, w = view(**bad), view()
+    for a, b in ((v, None), (w, v), (v, w)):
+        rc = L.ijb_kv_copy_pages(ctypes.byref(a), None if b is None else ctypes.byref(b), 1, 256, 256, None, None)
+        assert rc == lib.ERR_INVALID and "ijb_kv_copy_pages" in L.ijb_last_error(None).decode()
+
+
+@pytest.mark.parametrize("other", [dict(type=2), dict(kv_heads=1), dict(head_dim=128), dict(page_size=32)])
+def test_copies_between_pages_that_differ_are_refused(other):
+    L = lib.load()
+    v, w = view(), view(**other)
+    assert L.ijb_kv_copy_pages(ctypes.byref(v), ctypes.byref(w), 1, 256, 256, None, None) == lib.ERR_INVALID
+
+
+def test_copied_pages_arguments_are_checked():
+    L = lib.load()
+    v = view()
+    for n, src, dst in ((-1, 256, 256), (1, None, 256), (1, 256, None)):
+        assert L.ijb_kv_copy_pages(ctypes.byref(v), None, n, src, dst, None, None) == lib.ERR_INVALID
+    assert L.ijb_kv_copy_pages(None, None, 1, 256, 256, None, None) == lib.ERR_INVALID
+    before = L.ijb_kernel_launches()
+    assert L.ijb_kv_copy_pages(ctypes.byref(v), None, 0, None, None, None, None) == lib.OK
+    assert L.ijb_kernel_launches() == before
+    wide = view(kv_heads=1024, page_size=256, head_dim=128)
+    assert L.ijb_kv_copy_pages(ctypes.byref(wide), None, 0x7fffffff, 256, 256, None, None) == lib.ERR_INVALID
