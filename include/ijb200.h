@@ -335,7 +335,7 @@ int ijb_keys_to_tokens(const unsigned long long *keys_dev, int n, int *tokens_de
  * found on the device names nothing: such an entry is skipped. */
 #define IJB_KV_F16 0   /* fp16 rows */
 #define IJB_KV_E4M3 2  /* e4m3 rows, each with a power-of-two scale 2^(s - 127) kept as the byte s (0..254) */
-#define IJB_KV_E2M1 3  /* e2m1 codes, two a byte (the even dim in the low half); 32 dims of a row share a scale, the
+#define IJB_KV_E2M1 4  /* e2m1 codes, two a byte (the even dim in the low half); 32 dims of a row share a scale, the
                           fp16 number of the bits s << 7, kept as the byte s (0..226) */
 
 typedef struct {

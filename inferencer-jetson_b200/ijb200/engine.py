@@ -68,7 +68,7 @@ class Engine:
         if kv_type is None:
             rc = self.lib.ijb_create(ctypes.byref(d), views, len(weights), ctypes.byref(h))
         else:  # "f16", "e4m3" or "e2m1": a pool of that type, read by the paged attention
-            rc = self.lib.ijb_create_kv(ctypes.byref(d), views, len(weights), {"f16": 0, "e4m3": 2, "e2m1": 3}[kv_type],
+            rc = self.lib.ijb_create_kv(ctypes.byref(d), views, len(weights), {"f16": 0, "e4m3": 2, "e2m1": 4}[kv_type],
                                         ctypes.byref(h))
         _L.check(rc, None)
         self.h = h

@@ -7,13 +7,13 @@ from ijb200 import lib
 
 
 def view(**kw):
-    base = dict(type=3, kv_heads=2, head_dim=64, page_size=16, num_pages=4, data_dev=4096, scale_dev=8192,
+    base = dict(type=4, kv_heads=2, head_dim=64, page_size=16, num_pages=4, data_dev=4096, scale_dev=8192,
                 page_table_dev=256, n_seqs=1, max_pages=4)
     base.update(kw)
     return lib.KvView(**base)
 
 
-BAD_VIEWS = [dict(type=4), dict(kv_heads=0), dict(head_dim=96), dict(head_dim=32), dict(page_size=4), dict(num_pages=0),
+BAD_VIEWS = [dict(type=3), dict(type=5), dict(kv_heads=0), dict(head_dim=96), dict(head_dim=32), dict(page_size=4), dict(num_pages=0),
              dict(n_seqs=0), dict(max_pages=0), dict(data_dev=None), dict(data_dev=4104), dict(scale_dev=None),
              dict(page_table_dev=None)]
 
