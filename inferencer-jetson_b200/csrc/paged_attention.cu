@@ -925,10 +925,12 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
 // at once, a lane for each 8 rows that lie together, and a lane copies 16 bytes at a place
 // that is one multiplication away from their number.
 
-template <int HD, bool WIDE, typename T>
+template <int HD, int ROWS, typename T>
 struct Dec4 {
+    static constexpr bool WIDE = ROWS == 16;
     static constexpr int kRowBytes = HD / 2, kBlocks = HD / kKvBlock;  // of a row: bytes, scales
-    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr bool kPair = ROWS == 4, kSplit = sizeof(T) == 4 && !kPair;
+    static_assert(!kPair || sizeof(T) == 4, "fp16 rows have one part");
     static constexpr int kPos = WIDE && kSplit ? 32 : 64;  // positions of a chunk
     static constexpr int kTile = kPos * kRowBytes, kScales = kPos * kBlocks;
     static constexpr int kStage = 2 * (kTile + kScales);  // K, V, their scale bytes
@@ -953,12 +955,13 @@ __device__ __forceinline__ void mma_new(float (&d)[4], const uint32_t (&a)[4], u
 // (a & m) | (b & ~m)
 __device__ __forceinline__ uint32_t select_bits(uint32_t a, uint32_t b, uint32_t m) { return (a & m) | (b & ~m); }
 
-template <int HD, bool WIDE, typename T>
-__global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
+template <int HD, int ROWS, typename T>
+__global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
     ijb_paged_decode4_kernel(const __grid_constant__ AttnArgs a) {
-    using D = Dec4<HD, WIDE, T>;
-    constexpr int N = WIDE ? 2 : 1;         // tiles of 8 rows
-    constexpr bool SPLIT = sizeof(T) == 4;  // fp32 queries: hi + lo
+    using D = Dec4<HD, ROWS, T>;
+    constexpr int N = ROWS == 16 ? 2 : 1;  // tiles of 8 rows
+    // fp32 queries are hi + lo: products of their own, or (up to 4 rows) columns 4..7 of the same
+    constexpr bool SPLIT = D::kSplit, PAIR = D::kPair;
     constexpr int NT = D::kWarps * 32, RB = D::kRowBytes, NB = D::kBlocks, KS = HD / 16, W = HD / 64;  // W: words of V
     constexpr int GROUP = 8 * RB;         // bytes of 8 rows, which lie together
     constexpr int PC = D::kPos, TT = PC / 16, G = PC / 8;  // positions, tiles and groups of a chunk
@@ -1104,13 +1107,18 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
         int limit[N][2];  // last position that rows 8 n + 2 t4 + c see
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int r = gid + 8 * n;
+            const int r = PAIR ? gid & 3 : gid + 8 * n;
             const int tok = r < rows ? (row0 + r) / a.group : 0, in = r < rows ? (row0 + r) % a.group : 0;
             const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD + t4 * (HD / 4);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const float4 v = r < rows ? load4(src + 4 * ks, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
-                const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
+                __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
+                if (PAIR && gid >= 4) {
+                    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                    h0 = __floats2half2_rn(v.x - f0.x, v.y - f0.y);
+                    h1 = __floats2half2_rn(v.z - f1.x, v.w - f1.y);
+                }
                 qh[ks][n][0] = *reinterpret_cast<const uint32_t *>(&h0);
                 qh[ks][n][1] = *reinterpret_cast<const uint32_t *>(&h1);
                 if constexpr (SPLIT) {
@@ -1121,7 +1129,7 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int q = 8 * n + 2 * t4 + c;
+                const int q = PAIR ? (2 * t4 + c) & 3 : 8 * n + 2 * t4 + c;
                 limit[n][c] = q < rows ? s.x.kv - s.x.len + (row0 + q) / a.group : -1;
             }
         }
@@ -1195,6 +1203,12 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                     }
                 }
             }
+            if constexpr (PAIR) {
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) p[t][0][k] += __shfl_xor_sync(0xffffffffu, p[t][0][k], 2);
+            }
             // ---- online softmax (base 2)
             if (p0 + PC - 1 > all_see) {
 #pragma unroll
@@ -1250,7 +1264,12 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                             e[c] = ex2(fmaf(p[t][n][2 * h + c], sc, -mu[n][c]));
                             l[n][c] += e[c];
                         }
-                        const __half2 w = __floats2half2_rn(e[0], e[1]);
+                        __half2 w = __floats2half2_rn(e[0], e[1]);
+                        if constexpr (PAIR) {
+                            const float2 f = __half22float2(w);
+                            const __half2 lo = __floats2half2_rn(e[0] - f.x, e[1] - f.y);
+                            w = t4 & 2 ? lo : w;
+                        }
                         ph[t][n][h] = transpose8x8(*reinterpret_cast<const uint32_t *>(&w));
                         if constexpr (SPLIT) {
                             const float2 f = __half22float2(w);
@@ -1299,7 +1318,13 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
 #pragma unroll
                         for (int n = 0; n < N; ++n) {
                             float(&to_o)[4] = o[4 * k + j][n];
-                            if constexpr (SPLIT) {
+                            if constexpr (PAIR) {
+                                float d[4];
+                                mma_new(d, f[0], ph[t0][n][0], ph[t0][n][1]);
+                                mma(d, f[1], ph[t0 + 1][n][0], ph[t0 + 1][n][1]);
+                                add2_in_order(to_o[0], to_o[1], d[0], d[1]);
+                                add2_in_order(to_o[2], to_o[3], d[2], d[3]);
+                            } else if constexpr (SPLIT) {
                                 float d[4];
                                 mma_new(d, f[0], pl[t0][n][0], pl[t0][n][1]);
                                 mma(d, f[1], pl[t0 + 1][n][0], pl[t0 + 1][n][1]);
@@ -1319,6 +1344,12 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
             stage = stage + 1 == D::kStages ? 0 : stage + 1;
         }
 
+        if constexpr (PAIR) {
+#pragma unroll
+            for (int i = 0; i < 4 * W; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[i][0][k] += __shfl_xor_sync(0xffffffffu, o[i][0][k], 2);
+        }
         float zero = 0.f;  // NaN once a value is not finite
 #pragma unroll
         for (int i = 0; i < 4 * W; ++i)
@@ -1347,7 +1378,7 @@ __global__ void __launch_bounds__(Dec4<HD, WIDE, T>::kWarps * 32, 1)
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                 const int r = 8 * n + 2 * t4 + c;
-                if (r >= end_rows) continue;
+                if (r >= end_rows || (PAIR && r >= 4)) continue;
                 const float inv = whole ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : 1.f;
                 T *dst = op + static_cast<long>(s.x.q0 + (end_row0 + r) / a.group) * a.out_stride +
                          (s.head * a.group + (end_row0 + r) % a.group) * HD + gid * (HD / 8);
@@ -2544,23 +2575,23 @@ cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     return e;
 }
 
-// The decode kernel of a cache type, its launch shape and its shared memory (the plan's at least).
-template <int HD, int KV, bool WIDE, typename T>
-using DecOf = std::conditional_t<KV == IJB_KV_E2M1, Dec4<HD, WIDE, T>, Dec<HD, KV, WIDE, T>>;
-template <int HD, int KV, bool WIDE, typename T>
+// The decode kernel of a cache type for entries of up to ROWS (8 or 16; e2m1, fp32: 4 too) rows, its launch shape and its shared memory (the plan's at least).
+template <int HD, int KV, int ROWS, typename T>
+using DecOf = std::conditional_t<KV == IJB_KV_E2M1, Dec4<HD, ROWS, T>, Dec<HD, KV, ROWS == 16, T>>;
+template <int HD, int KV, int ROWS, typename T>
 constexpr auto decode_kernel() {
-    if constexpr (KV == IJB_KV_E2M1) return ijb_paged_decode4_kernel<HD, WIDE, T>;
-    else return ijb_paged_decode_kernel<HD, KV, WIDE, T>;
+    if constexpr (KV == IJB_KV_E2M1) return ijb_paged_decode4_kernel<HD, ROWS, T>;
+    else return ijb_paged_decode_kernel<HD, KV, ROWS == 16, T>;
 }
-template <int HD, int KV, bool WIDE, typename T>
+template <int HD, int KV, int ROWS, typename T>
 constexpr int decode_smem() {
-    using D = DecOf<HD, KV, WIDE, T>;
+    using D = DecOf<HD, KV, ROWS, T>;
     return D::kSmem > kDecPlanBytes ? D::kSmem : kDecPlanBytes;
 }
-template <int HD, int KV, bool WIDE, typename T>
+template <int HD, int KV, int ROWS, typename T>
 cudaError_t decode_allow() {
-    const auto kernel = decode_kernel<HD, KV, WIDE, T>();
-    return allow_smem<decltype(kernel), DecOf<HD, KV, WIDE, T>, T>(kernel, decode_smem<HD, KV, WIDE, T>());
+    const auto kernel = decode_kernel<HD, KV, ROWS, T>();
+    return allow_smem<decltype(kernel), DecOf<HD, KV, ROWS, T>, T>(kernel, decode_smem<HD, KV, ROWS, T>());
 }
 template <int HD, int KV, typename T>
 cudaError_t tile_allow() {
@@ -2568,13 +2599,13 @@ cudaError_t tile_allow() {
     return allow_smem<decltype(kernel), Tile<HD, T>, std::integral_constant<int, KV>>(kernel, Tile<HD, T>::kSmem);
 }
 
-template <int HD, int KV, bool WIDE, typename T>
+template <int HD, int KV, int ROWS, typename T>
 cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
-    using D = DecOf<HD, KV, WIDE, T>;
-    const cudaError_t e = decode_allow<HD, KV, WIDE, T>();
+    using D = DecOf<HD, KV, ROWS, T>;
+    const cudaError_t e = decode_allow<HD, KV, ROWS, T>();
     if (e != cudaSuccess) return e;
     a.min_rows = 1;
-    a.max_rows = WIDE ? kDecRows : 8;
+    a.max_rows = ROWS;
     a.report_long = all;
     a.tile_rows = kDecRows;
     a.unit = D::kPos;
@@ -2582,7 +2613,7 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.min_units = 64 / D::kPos;  // 64 positions
     a.over = 1;
     a.least = 1;
-    decode_kernel<HD, KV, WIDE, T>()<<<sms, D::kWarps * 32, decode_smem<HD, KV, WIDE, T>(), s>>>(a);
+    decode_kernel<HD, KV, ROWS, T>()<<<sms, D::kWarps * 32, decode_smem<HD, KV, ROWS, T>(), s>>>(a);
     return merge_launch<kDecRows, HD, KV, T>(a, s);
 }
 
@@ -2612,10 +2643,12 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
 template <int HD, int KV, typename T>
 cudaError_t attention_call(const AttnArgs &a, int max_q, int sms, cudaStream_t s) {
     const long most = static_cast<long>(max_q > 0 ? min(max_q, a.n_tokens) : a.n_tokens) * a.group;
-    if (most <= 8) return decode_launch<HD, KV, false, T>(a, sms, true, s);
-    if (most <= kDecRows) return decode_launch<HD, KV, true, T>(a, sms, true, s);
+    if constexpr (KV == IJB_KV_E2M1 && sizeof(T) == 4)
+        if (most <= 4) return decode_launch<HD, KV, 4, T>(a, sms, true, s);
+    if (most <= 8) return decode_launch<HD, KV, 8, T>(a, sms, true, s);
+    if (most <= kDecRows) return decode_launch<HD, KV, kDecRows, T>(a, sms, true, s);
     if (a.n_entries < 8) return tile_launch<HD, KV, T>(a, sms, 1, s);
-    const cudaError_t e = decode_launch<HD, KV, true, T>(a, sms, false, s);
+    const cudaError_t e = decode_launch<HD, KV, kDecRows, T>(a, sms, false, s);
     return e != cudaSuccess ? e : tile_launch<HD, KV, T>(a, sms, kDecRows + 1, s);
 }
 template <int KV, typename T>
@@ -2640,8 +2673,10 @@ size_t workspace_bytes(int sms, int head_dim) {
 
 template <int HD, int KV>
 cudaError_t prepare() {
-    cudaError_t e = decode_allow<HD, KV, false, float>();
-    if (e == cudaSuccess) e = decode_allow<HD, KV, true, float>();
+    cudaError_t e = decode_allow<HD, KV, 8, float>();
+    if (e == cudaSuccess) e = decode_allow<HD, KV, kDecRows, float>();
+    if constexpr (KV == IJB_KV_E2M1)
+        if (e == cudaSuccess) e = decode_allow<HD, KV, 4, float>();
     if (e == cudaSuccess) e = tile_allow<HD, KV, float>();
     return e;
 }
