@@ -934,7 +934,7 @@ struct Dec4 {
     static constexpr int kPos = WIDE && kSplit ? 32 : 64;  // positions of a chunk
     static constexpr int kTile = kPos * kRowBytes, kScales = kPos * kBlocks;
     static constexpr int kStage = 2 * (kTile + kScales);  // K, V, their scale bytes
-    static constexpr int kWarps = HD == 128 ? (WIDE || kSplit ? 8 : 12) : (WIDE || kSplit ? 12 : 16);
+    static constexpr int kWarps = HD == 128 && (WIDE || kSplit) ? 8 : 12;
     static constexpr int kFit = 216 * 1024 / (kWarps * kStage), kStages = kFit > 4 ? 4 : kFit;
     static constexpr int kSmem = kWarps * kStages * kStage;
     static_assert(kStages >= 2, "stages");
@@ -975,19 +975,29 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
     pdl_trigger();
     const int worker = blockIdx.x * D::kWarps + warp;
     auto &my = state[warp];
+    // cursor_start, with the next worker's start found by the odd lanes alongside
+    auto cursor_both = [&](const int *sums, const PlanOut &po) {
+        Cursor c = cursor_at<true>(a, nullptr, sums, po, worker + (lane & 1));
+        c.end = __shfl_sync(0xffffffffu, c.at, 1);
+        c.at = __shfl_sync(0xffffffffu, c.at, 0);
+        c.e = __shfl_sync(0xffffffffu, c.e, 0);
+        c.head = __shfl_sync(0xffffffffu, c.head, 0);
+        c.b0 = __shfl_sync(0xffffffffu, c.b0, 0);
+        return c;
+    };
     Cursor first;
     int per;
     if (a.n_entries < 32) {
         int *sums = reinterpret_cast<int *>(smem + warp * D::kStages * D::kStage);
         PlanOut po;
         plan_warp(a, sums, &po, worker == 0);
-        first = cursor_start<true>(a, nullptr, sums, po, worker);
+        first = cursor_both(sums, po);
         per = po.per;
         __syncwarp();  // the plan's shared memory becomes the stages
     } else {
         int *sums = reinterpret_cast<int *>(smem);
         plan_build<NT, true>(a, nullptr, sums, &block_po);
-        first = cursor_start<true>(a, nullptr, sums, block_po, worker);
+        first = cursor_both(sums, block_po);
         per = block_po.per;
         __syncthreads();
     }
