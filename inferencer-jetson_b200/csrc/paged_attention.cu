@@ -224,12 +224,13 @@ __device__ void plan_build(const AttnArgs &a, int *first, int *sums, PlanOut *po
 }
 
 // plan_build<NT, true> for up to 32 entries by each warp on its own, without the
-// block's barriers: sums in the warp's memory, the rest in *po.
-__device__ __forceinline__ void plan_warp(const AttnArgs &a, int *sums, PlanOut *po, bool report) {
+// block's barriers: sums in the warp's memory, lane e's entry in x, the rest in *po.
+__device__ __forceinline__ void plan_warp(const AttnArgs &a, int *sums, PlanOut *po, bool report, Entry &x) {
     const int lane = threadIdx.x & 31;
     int n = 0;
+    x = {};
     if (lane < a.n_entries) {
-        const Entry x = entry_load(a, lane, report);
+        x = entry_load(a, lane, report);
         n = x.tiles ? tile_units(a, x, 0) + a.over : 0;
     }
     int inc = n;
@@ -284,17 +285,8 @@ __device__ __forceinline__ Cursor cursor_start(const AttnArgs &a, const int *fir
     return c;
 }
 
-// The next run, and the cursor behind it; false at the end.
-__device__ __forceinline__ bool cursor_next(const AttnArgs &a, Cursor &c, Segment &s) {
-    if (c.at >= c.end) return false;
-    s.x = entry_load(a, c.e, false);
-    while (s.x.tiles == 0) {  // entries without rows here
-        if (++c.e == a.n_entries) {
-            c.e = 0;
-            ++c.head;
-        }
-        s.x = entry_load(a, c.e, false);
-    }
+// The next run, of entry s.x, and the cursor behind it.
+__device__ __forceinline__ void cursor_take(const AttnArgs &a, Cursor &c, Segment &s) {
     s.e = c.e;
     s.ti = c.ti;
     s.head = c.head;
@@ -312,6 +304,19 @@ __device__ __forceinline__ bool cursor_next(const AttnArgs &a, Cursor &c, Segmen
             ++c.head;
         }
     }
+}
+// The next run, and the cursor behind it; false at the end.
+__device__ __forceinline__ bool cursor_next(const AttnArgs &a, Cursor &c, Segment &s) {
+    if (c.at >= c.end) return false;
+    s.x = entry_load(a, c.e, false);
+    while (s.x.tiles == 0) {  // entries without rows here
+        if (++c.e == a.n_entries) {
+            c.e = 0;
+            ++c.head;
+        }
+        s.x = entry_load(a, c.e, false);
+    }
+    cursor_take(a, c, s);
     return true;
 }
 
@@ -485,6 +490,9 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ void sts64(uint32_t addr, uint32_t a, uint32_t b) {
+    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -568,7 +576,8 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
     if (a.n_entries < 32) {
         int *sums = reinterpret_cast<int *>(smem + warp * D::kStages * D::kStage);
         PlanOut po;
-        plan_warp(a, sums, &po, worker == 0);
+        Entry x;
+        plan_warp(a, sums, &po, worker == 0, x);
         load_c = cursor_start<true>(a, nullptr, sums, po, worker);
         per = po.per;
         __syncwarp();  // the plan's shared memory becomes the stages
@@ -986,18 +995,26 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
         return c;
     };
     Cursor first;
+    Entry entry;  // of the first run; tiles 0: not read yet
     int per;
     if (a.n_entries < 32) {
         int *sums = reinterpret_cast<int *>(smem + warp * D::kStages * D::kStage);
         PlanOut po;
-        plan_warp(a, sums, &po, worker == 0);
+        plan_warp(a, sums, &po, worker == 0, entry);
         first = cursor_both(sums, po);
+        entry.q0 = __shfl_sync(0xffffffffu, entry.q0, first.e);
+        entry.len = __shfl_sync(0xffffffffu, entry.len, first.e);
+        entry.kv = __shfl_sync(0xffffffffu, entry.kv, first.e);
+        entry.seq = __shfl_sync(0xffffffffu, entry.seq, first.e);
+        entry.rows = __shfl_sync(0xffffffffu, entry.rows, first.e);
+        entry.tiles = __shfl_sync(0xffffffffu, entry.tiles, first.e);
         per = po.per;
         __syncwarp();  // the plan's shared memory becomes the stages
     } else {
         int *sums = reinterpret_cast<int *>(smem);
         plan_build<NT, true>(a, nullptr, sums, &block_po);
         first = cursor_both(sums, block_po);
+        entry.tiles = 0;
         per = block_po.per;
         __syncthreads();
     }
@@ -1025,7 +1042,13 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
     auto load_run = [&]() {
         Cursor c = my.load;
         Segment s;
-        more = cursor_next(a, c, s);
+        if (queued == 0 && entry.tiles > 0) {
+            more = c.at < c.end;
+            s.x = entry;
+            if (more) cursor_take(a, c, s);
+        } else {
+            more = cursor_next(a, c, s);
+        }
         if (!more) return;
         l_kv = s.x.kv;
         l_seq = s.x.seq;
@@ -1117,24 +1140,53 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
         int limit[N][2];  // last position that rows 8 n + 2 t4 + c see
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int r = PAIR ? gid & 3 : gid + 8 * n;
-            const int tok = r < rows ? (row0 + r) / a.group : 0, in = r < rows ? (row0 + r) % a.group : 0;
-            const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD + t4 * (HD / 4);
+            if constexpr (PAIR) {
+                // a row at a time (or two), 4 dims a lane, into the stage that is loaded next, and from there as the
+                // products want them: 12 warps that read 16 bytes of each of 32 lines at once took 4800 cycles for
+                // this at head_dim 128, 2100 so (but not so for more rows: the loop came out slower)
+                constexpr int L = HD / 4, STEP = 32 / L, SQ = 2 * HD + 8;  // SQ: bytes of a part of a row
+                const uint32_t qs = base + stage_in * D::kStage;
+                float4 v[4 / STEP];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const float4 v = r < rows ? load4(src + 4 * ks, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
-                __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
-                if (PAIR && gid >= 4) {
-                    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                    h0 = __floats2half2_rn(v.x - f0.x, v.y - f0.y);
-                    h1 = __floats2half2_rn(v.z - f1.x, v.w - f1.y);
+                for (int i = 0; i < 4 / STEP; ++i) {
+                    const int r = i * STEP + lane / L;
+                    const int tok = r < rows ? (row0 + r) / a.group : 0, in = r < rows ? (row0 + r) % a.group : 0;
+                    const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD + lane % L * 4;
+                    v[i] = r < rows ? load4(src, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-                qh[ks][n][0] = *reinterpret_cast<const uint32_t *>(&h0);
-                qh[ks][n][1] = *reinterpret_cast<const uint32_t *>(&h1);
-                if constexpr (SPLIT) {
-                    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                    ql[ks][n][0] = half2_bits(v.x - f0.x, v.y - f0.y);
-                    ql[ks][n][1] = half2_bits(v.z - f1.x, v.w - f1.y);
+#pragma unroll
+                for (int i = 0; i < 4 / STEP; ++i) {
+                    const uint32_t at = qs + (i * STEP + lane / L) * SQ + lane % L * 8, h0 = half2_bits(v[i].x, v[i].y),
+                                   h1 = half2_bits(v[i].z, v[i].w);
+                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0)),
+                                 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
+                    sts64(at, h0, h1);
+                    sts64(at + 4 * SQ, half2_bits(v[i].x - f0.x, v[i].y - f0.y), half2_bits(v[i].z - f1.x, v[i].w - f1.y));
+                }
+                __syncwarp();
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint2 x = lds64(qs + gid * SQ + t4 * (HD / 2) + 8 * ks);  // (rows 4..7: lo parts)
+                    qh[ks][n][0] = x.x;
+                    qh[ks][n][1] = x.y;
+                }
+                __syncwarp();
+                static_assert(8 * SQ <= D::kStage, "the queries fit a stage");
+            } else {
+                const int r = gid + 8 * n;
+                const int tok = r < rows ? (row0 + r) / a.group : 0, in = r < rows ? (row0 + r) % a.group : 0;
+                const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD + t4 * (HD / 4);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const float4 v = r < rows ? load4(src + 4 * ks, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
+                    qh[ks][n][0] = *reinterpret_cast<const uint32_t *>(&h0);
+                    qh[ks][n][1] = *reinterpret_cast<const uint32_t *>(&h1);
+                    if constexpr (SPLIT) {
+                        const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                        ql[ks][n][0] = half2_bits(v.x - f0.x, v.y - f0.y);
+                        ql[ks][n][1] = half2_bits(v.z - f1.x, v.w - f1.y);
+                    }
                 }
             }
 #pragma unroll
