@@ -11,7 +11,8 @@
 // Two kernels, by rows:
 //  * ijb_paged_decode_kernel, up to 16 rows an entry and KV head (single tokens,
 //    a few drafted ones): bound by reading the cache.  Every warp streams
-//    32-position chunks of its own through shared memory.
+//    32-position chunks of its own through shared memory.  For e2m1 rows, whose
+//    reading takes less time than their arithmetic, ijb_paged_decode4_kernel.
 //  * ijb_paged_tile_kernel, more rows (chunks, prompts): bound by the matrix
 //    products and the exponentials.  256 rows at a time on tcgen05.
 // Both cut all the call's work (tiles of rows x units of positions, over all
@@ -32,7 +33,8 @@
 // over 2^20, 5.5e-4 over 2^22.  Cached rows enter as fp16: fp16 rows exactly, e4m3 values as the
 // fp16 number nearest to code * 2^e, as an fp16 cache would hold them: exactly from 2^-14 on (and
 // every value of a row whose largest is in [2^-7, 2^15]), else off by 2^-25 at most, infinite from
-// 65520 on.  (The decode kernel scales its scores in fp32, so K has no such ends there.)
+// 65520 on.  (The decode kernel scales its scores in fp32, so K has no such ends there.)  e2m1 values,
+// code * scale, are fp16 numbers.
 #include <mutex>
 #include <type_traits>
 
@@ -919,28 +921,45 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
 // ------------------------------------------------------- decode, 4 bits --
 //
 // e2m1 rows have a kernel of their own: with a quarter of an fp16 cache's bytes the
-// instructions bound it, not the reading.  Positions are the M side of mma.m16n8k16, the
-// (up to 8, WIDE: 16) rows its 8 columns, so no product is of empty rows:
+// instructions bound it, not the reading (the general kernel, its operands unpacked in
+// place: 170 us for the contexts below).  Positions are the M side of mma.m16n8k16, the
+// entry's rows its 8 columns (16 rows: twice 8), so half the products of the other way
+// round, where up to 8 rows left half of the M side empty:
 //   S^T[pos][row] = K . Q^T: a lane's K fragments are 16 or 8 bytes of one position's
 //   row, one scale's block or half of one; the 16 k slots stand for whichever dims those
 //   hold (Q's fragments are loaded in the same order);
 //   O^T[dim][row] += V^T . P^T: a lane's V fragments are 8 or 4 bytes of each of the four
 //   positions of its k slots, whose codes of one dim are put side by side in a byte
-//   (two bit selections for 8 dims) before they become a pair of fp16 numbers.  P^T
-//   comes from the score accumulators by movmatrix.
-// A byte becomes two fp16 numbers in one instruction, and a second one scales them.
+//   (two shifts and two bit selections for 16 codes) before they become a pair of fp16
+//   numbers.  P^T comes from the score accumulators by movmatrix.
+// A byte becomes two fp16 numbers in one instruction, and a second one scales them: 512
+// of the 1030 instructions that a warp has for 64 positions of 128 dims.  fp32 rows have
+// two parts, hi + lo: up to 4 rows take the 8 columns with both (the parts of a score
+// are added by a shuffle), more need a product for each.
 // Rows' maxima are raised only when a score passes them by more than 2^8 (see the tile
 // kernel), so that a chunk has no shuffles for them.  Page ids are read 256 positions
 // at once, a lane for each 8 rows that lie together, and a lane copies 16 bytes at a place
-// that is one multiplication away from their number.
+// that is one multiplication away from their number.  What a warp needs between its runs
+// only is kept in shared memory, for the registers.
+//
+// Measured in a graph, 8 KV heads: 16 contexts of 11,003 to 40,111 positions, 32 heads of 128: 467 MB in 93 us
+// with fp16 queries (5.0 TB/s; issue slots 63 % and the ALU, which converts, 52 % busy) and 104 with fp32 ones;
+// heads of 64 63 and 69.  64 ragged single tokens behind 23 to 1,499, fp32, heads of 64: 18.3 us (27.7 with the
+// general kernel).  2 to 5 drafted tokens of 24 heads of 128 in 24 sequences behind 700 to 9,001: fp16 55 us, fp32 75,
+// the tensor pipe 46 % busy, for want of more than 2 warps a scheduler beside so many sums.
 
 template <int HD, int ROWS, typename T>
 struct Dec4 {
     static constexpr bool WIDE = ROWS == 16;
+    // Positions of a chunk: 64 halve what a chunk costs beside its values (16 long contexts, heads of 128, fp16 queries:
+    // 93 us, with 32 103); 16 fp32 rows have no registers for them.  Warps: as many as have the registers, the same
+    // number on each scheduler; 12 and not 16 at head_dim 64, whose launch costs more than it gains (64 ragged tokens
+    // 18.3 and 21.3 us, 16 long contexts 69 and 64), and 8 rather than 12 that spill (8 fp32 rows of 128: 125 and 129 us).
+    // Not kept: 10 and 14 warps (uneven), 16 fp32 rows' queries in shared memory for 12 warps (drafts 88 us for 75).
     static constexpr int kRowBytes = HD / 2, kBlocks = HD / kKvBlock;  // of a row: bytes, scales
     static constexpr bool kPair = ROWS == 4, kSplit = sizeof(T) == 4 && !kPair;
     static_assert(!kPair || sizeof(T) == 4, "fp16 rows have one part");
-    static constexpr int kPos = WIDE && kSplit ? 32 : 64;  // positions of a chunk
+    static constexpr int kPos = WIDE && kSplit ? 32 : 64;
     static constexpr int kTile = kPos * kRowBytes, kScales = kPos * kBlocks;
     static constexpr int kStage = 2 * (kTile + kScales);  // K, V, their scale bytes
     static constexpr int kWarps = HD == 128 && (WIDE || kSplit) ? 8 : 12;
@@ -2672,7 +2691,8 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.tile_rows = kDecRows;
     a.unit = D::kPos;
     a.workers = sms * D::kWarps;
-    a.min_units = 64 / D::kPos;  // 64 positions
+    // 64 positions a worker at least: one token at position 2043 of an e2m1 cache took 13.1 us so and 15.0 with 128
+    a.min_units = 64 / D::kPos;
     a.over = 1;
     a.least = 1;
     decode_kernel<HD, KV, ROWS, T>()<<<sms, D::kWarps * 32, decode_smem<HD, KV, ROWS, T>(), s>>>(a);
@@ -2699,7 +2719,8 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
 
 // Which kernels serve a call.  Entries of up to 16 rows go to the decode kernel,
 // longer ones to the tile kernel; a call that may hold longer ones and has few
-// entries leaves them all to the tile kernel, for the launches: entries of 1 to 40 tokens
+// entries leaves them all to the tile kernel, for the launches (up to 4 fp32 rows of an e2m1 cache have a kernel of their
+// own: see Dec4): entries of 1 to 40 tokens
 // behind 100 to 2000 take 49 us so and 55 with both kernels for 2 of them, 51 and 56 for 7, 55 and 59 for 8, 77 and
 // 89 for 16 (so the border could lie higher); one of 200 tokens among single ones 54 and 68 for 4, 98 and 83 for 32.
 template <int HD, int KV, typename T>
