@@ -339,13 +339,14 @@ int ijb_keys_to_tokens(const unsigned long long *keys_dev, int n, int *tokens_de
                           fp16 number of the bits s << 7, kept as the byte s (0..226) */
 
 typedef struct {
-    int type;                   /* IJB_KV_F16 or IJB_KV_E4M3 */
+    int type;                   /* IJB_KV_F16, IJB_KV_E4M3 or IJB_KV_E2M1 */
     int kv_heads;
     int head_dim;               /* 64 or 128 */
     int page_size;              /* positions per page: 8, 16, 32, 64, 128 or 256 */
     long num_pages;
     void *data_dev;             /* [num_pages][K, V][kv_heads][page_size][head_dim], 16-byte aligned */
-    uint8_t *scale_dev;         /* e4m3: [num_pages][K, V][kv_heads][page_size]; else ignored */
+    uint8_t *scale_dev;         /* e4m3: [num_pages][K, V][kv_heads][page_size], e2m1: [..][page_size][head_dim / 32];
+                                   fp16: ignored */
     const int *page_table_dev;  /* [n_seqs][max_pages] page ids; only those of a call's positions are read */
     int n_seqs;
     int max_pages;
@@ -356,9 +357,16 @@ typedef struct {
  * token) at position tok_pos_dev[i] of sequence tok_seq_dev[i].  fp16 rows are
  * rounded to nearest; an e4m3 row gets the least scale 2^e with max|row| <=
  * 448 * 2^e over its finite values (2^-126 at least), its values are rounded
- * to nearest, infinities to the largest finite value, NaN stays NaN.  Entries
- * with a negative position are padding and are skipped.  A (sequence,
- * position) must not be named by two of the call's tokens. */
+ * to nearest, infinities to the largest finite value, NaN stays NaN.  32 dims of
+ * an e2m1 row get the scale nearest to max|x| / 6 over their finite values (an
+ * fp32 quotient; ties to even; 10240 at most, 0 below 2^-18) and the codes nearest
+ * to fp32's products of x and 1 / scale, ties to the even code, infinities and
+ * larger values to the largest; a NaN makes its 32 dims NaN (scale byte 255).
+ * What is read back is code * scale, exact in fp16 too, and off by 0.18 of the
+ * largest of the 32 at most (0.09 for values up to half of it): 10 % rms of
+ * normally distributed values.  Entries with a negative position are padding
+ * and are skipped.  A (sequence, position) must not be named by two of the call's
+ * tokens. */
 int ijb_kv_append(const ijb_kv_view *kv, int src_type, const void *k_dev, const void *v_dev, long stride, int n,
                   const int *tok_seq_dev, const int *tok_pos_dev, uint32_t *status_dev, void *stream);
 
@@ -391,14 +399,15 @@ int ijb_kv_copy_pages(const ijb_kv_view *from, const ijb_kv_view *to, int n, con
  * several calls.  Entries may be empty; rows that belong to no entry are left as
  * they were.  The starts must not fall, and out_dev must not overlap q_dev.
  * max_q > 0 promises that no entry has more new tokens (0: unknown): a longer one
- * may be left unwritten and is reported.  scale_dev has to be 4-byte aligned.
+ * may be left unwritten and is reported.  scale_dev has to be 4-byte aligned, an
+ * e2m1 cache's 16-byte, and that may have 2^32 groups of 8 rows.
  *
  * fp32 queries and probabilities enter the products as two fp16 parts each (22
  * bits, but no finer than 2^-25; queries up to 65504); fp16 queries as they are,
  * their probabilities rounded to fp16.  e4m3 values enter as the nearest fp16
  * number, as an fp16 cache would hold them: those of a row whose largest is within
  * 2^-7 .. 2^15 exactly, smaller ones off by 2^-25 at most; those of 65520 and more
- * may come out as infinities.  Sums, maxima and the softmax are fp32; fp16 queries'
+ * may come out as infinities.  e2m1 values are fp16 numbers.  Sums, maxima and the softmax are fp32; fp16 queries'
  * values are summed by the tensor core alone, which loses some of the last bits:
  * 1.4e-4 of an output over 2^20 positions.  The result is the same every time for
  * the same call, but how an entry's positions are cut into partial sums depends on

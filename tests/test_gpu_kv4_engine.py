@@ -1,7 +1,8 @@
 """Engines whose pool is held in 4 bits, against engines of ijb_create on the same weights.
 
-A 4-bit pool rounds a value by up to a sixth of the largest of its 32 (half the step between 4 and 6, where 6 is the
-largest); logits are held to twice that, as an e4m3 pool's are to twice its own largest rounding (test_gpu_paged_engine.py)."""
+A 4-bit pool rounds a value by about a sixth of the largest of its 32 at most (half the step between 4 and 6, where 6 is
+the largest, give or take a scale's rounding by a sixteenth); logits are held to two sixths, as an e4m3 pool's are to
+twice its own largest rounding (test_gpu_paged_engine.py)."""
 import numpy as np
 import pytest
 
