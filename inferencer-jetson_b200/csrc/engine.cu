@@ -704,8 +704,7 @@ void release_pages(ijb_engine *e, int seq) {
 }
 
 // Queues the copies of page_copies, all layers' in one launch: to the copy a pool of
-// layers * num_pages pages.  The ids' staging is free: every call that queues waits for
-// its stream before it returns.
+// layers * num_pages pages.
 void copy_pages(ijb_engine *e) {
     const std::vector<std::pair<int, int>> todo = std::move(e->page_copies);
     e->page_copies.clear();
@@ -722,6 +721,7 @@ void copy_pages(ijb_engine *e) {
         ck(cudaMallocHost(&e->copy_host, 2 * n * sizeof(int)), "page copy staging");
         e->copy_room = n;
     }
+    ck(cudaStreamSynchronize(e->stream), "page copies");  // the ids of the last copies have left their staging
     for (int l = 0; l < layers; ++l)
         for (size_t i = 0; i < todo.size(); ++i) {
             e->copy_host[l * todo.size() + i] = static_cast<int>(l * e->num_pages + todo[i].first);
