@@ -331,8 +331,8 @@ __device__ __forceinline__ uint32_t e2m1_codes(const float (&f)[8], float inv) {
 }
 
 // A thread has 8 values of U heads' rows; 4 threads share a block of 32 dims, and each works out the scale of one
-// head in 4 for all of them.  Measured: 12289 tokens of 8 heads x 128 from fp32 27 us (4.2
-// TB/s), from fp16 22, in blocks of 256 threads, 4 on an SM, 28 and 24 us.
+// head in 4 for all of them.  Measured: 12289 tokens of 8 heads x 128 from fp32 26 us (4.4
+// TB/s), from fp16 22; before, in blocks of 256 threads, 4 on an SM, 28 and 24 us.
 template <typename T, bool VEC, int HD, int U>
 __global__ void __launch_bounds__(append4_threads(U), U == 1 ? 4 : (sizeof(T) == 4 ? 9 : 10)) ijb_kv_append4_kernel(const __grid_constant__ RowsParams p) {
     using P = Place4<HD, U, 8, append4_threads(U)>;
@@ -403,11 +403,12 @@ __global__ void __launch_bounds__(append4_threads(U), U == 1 ? 4 : (sizeof(T) ==
         }
         if (slot < 0) continue;
         const long to0 = slot + (static_cast<long>(w.head) << p.kv.page_shift);
+        uint8_t *codes = p.kv.data + to0 * (HD / 2) + w.c * 4;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const long to = to0 + (static_cast<long>(j) << p.kv.page_shift);
             const uint32_t q = inv[j] > 0.f ? e2m1_codes(f[j], inv[j]) : 0u;
-            if (j < w.n) *reinterpret_cast<uint32_t *>(p.kv.data + to * (HD / 2) + w.c * 4) = q;
+            if (j < w.n) *reinterpret_cast<uint32_t *>(codes) = q;
+            codes += static_cast<long>(HD / 2) << p.kv.page_shift;
         }
 #pragma unroll
         for (int g = 0; g < (U + 3) / 4; ++g) {
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(append4_threads(U), U == 1 ? 4 : (sizeof(T) ==
 // Code * scale, exact in fp32, and in fp16 for the scales that ijb_kv_append writes (others rounded once).  A thread
 // stores 16 bytes of each of U heads' rows, next to its neighbour's.  Bound by the latency of its three loads in a
 // row (the slot, its page, the codes), so what counts is how many threads are on an SM, and that a block of few
-// has more than one row each: 32749 tokens of 8 heads x 128 to fp16 take 34.7 us (4.9 TB/s) and to fp32 53 (5.7), in
+// has more than one row each: 32749 tokens of 8 heads x 128 to fp16 take 34.3 us (5.0 TB/s) and to fp32 53 (5.8), in
 // blocks of 256 threads, 4 on an SM, 49 and 89.
 template <typename T, bool VEC, int HD, int U>
 __global__ void __launch_bounds__(gather4_threads(U), U == 1 ? 4 : 32) ijb_kv_gather4_kernel(const __grid_constant__ RowsParams p) {
@@ -438,12 +439,16 @@ __global__ void __launch_bounds__(gather4_threads(U), U == 1 ? 4 : 32) ijb_kv_ga
         const uint8_t *from = p.kv.data + from0 * (HD / 2) + w.c * E / 8 * 4;  // (two threads' codes when E is 4)
         const uint8_t *scale = p.kv.scale + from0 * (HD / kKvBlock) + w.c * E / kKvBlock;
         T *dst = static_cast<T *>(w.which ? p.v : p.k) + w.t * p.stride + static_cast<long>(w.head) * HD + w.c * E;
+        const long next = static_cast<long>(HD / 2) << p.kv.page_shift, next_scale = static_cast<long>(HD / kKvBlock) << p.kv.page_shift;
         uint32_t raw[U], sc[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            if (j >= w.n) continue;
-            raw[j] = *reinterpret_cast<const uint32_t *>(from + (static_cast<long>(j * (HD / 2)) << p.kv.page_shift));
-            sc[j] = scale[static_cast<long>(j * (HD / kKvBlock)) << p.kv.page_shift];
+            if (j < w.n) {
+                raw[j] = *reinterpret_cast<const uint32_t *>(from);
+                sc[j] = *scale;
+            }
+            from += next;
+            scale += next_scale;
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) {
