@@ -358,8 +358,8 @@ typedef struct {
  * rounded to nearest; an e4m3 row gets the least scale 2^e with max|row| <=
  * 448 * 2^e over its finite values (2^-126 at least), its values are rounded
  * to nearest, infinities to the largest finite value, NaN stays NaN.  32 dims of
- * an e2m1 row get the scale nearest to max|x| / 6 over their finite values (an
- * fp32 quotient; ties to even; 10240 at most, 0 below 2^-18) and the codes nearest
+ * an e2m1 row get the scale nearest to max|x| / 6 over their finite values (fp32's
+ * product with 1 / 6; ties to even; 10240 at most, 0 below 2^-18) and the codes nearest
  * to fp32's products of x and 1 / scale, ties to the even code, infinities and
  * larger values to the largest; a NaN makes its 32 dims NaN (scale byte 255).
  * What is read back is code * scale, exact in fp16 too, and off by 0.18 of the

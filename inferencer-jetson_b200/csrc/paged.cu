@@ -300,9 +300,10 @@ struct Place4 {
 };
 
 // The scale byte of 32 dims whose largest finite magnitude is a: the nearest scale to a / 6, ties to even (from
-// 2^-14 on the upper bits of the number with 3 of its mantissa, below in steps of 2^-17).
+// 2^-14 on the upper bits of the number with 3 of its mantissa, below in steps of 2^-17).  a / 6 is fp32's product of a
+// and 1 / 6, a unit of the last place off the quotient at most, which is a millionth of the rounding that follows.
 __device__ __forceinline__ uint32_t e2m1_scale_byte(float a) {
-    const float r = __fdiv_rn(a, 6.f);
+    const float r = a * (1.f / 6.f);
     const uint32_t bits = __float_as_uint(r);
     const uint32_t byte = r >= 6.103515625e-5f ? ((bits + 0x7ffffu + ((bits >> 20) & 1u)) >> 20) - ((127u - 15u) << 3)
                                                : __float2uint_rn(r * 131072.f);

@@ -1,7 +1,7 @@
 """A paged cache in 4 bits (e2m1 codes, a scale for 32 dims) on a B200 against its definition in 64 bits.
 
-Write: codes and scale bytes are equal to the definition's, whose only roundings to fp32 are max|x| / 6, 1 / scale and
-their product with x.  Read-back: code * scale has 6 significant bits and is exact in fp32 and fp16.
+Write: codes and scale bytes are equal to the definition's, whose only roundings to fp32 are max|x| times 1 / 6, 1 / scale
+and its product with x.  Read-back: code * scale has 6 significant bits and is exact in fp32 and fp16.
 
 Attention: K and V enter the products as the fp16 numbers that they are, so the bounds are those of the other caches
 (test_gpu_paged_attention.py): fp32 queries 2e-5 * max|v| (sum |q k| scale about 11 in these inputs), fp16 queries
@@ -33,7 +33,7 @@ def quantise(x):
     x = np.asarray(x, np.float32)
     b = x.reshape(x.shape[:-1] + (-1, 32))
     a = np.where(np.isfinite(b), np.abs(b), 0).max(-1)
-    byte = nearest(scale_table()[:227], (a / np.float32(6)).astype(np.float64))
+    byte = nearest(scale_table()[:227], (a * (np.float32(1) / np.float32(6))).astype(np.float64))
     s = scale_table()[byte].astype(np.float32)
     inv = np.where(s > 0, np.float32(1) / np.where(s > 0, s, 1), 0).astype(np.float32)
     with np.errstate(over="ignore", invalid="ignore"):
