@@ -918,6 +918,13 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
     if (lane == 0) a.left[worker] = left;
 }
 
+// (below)
+template <int ROWS, int HD, int NT, int RB, typename T>
+__device__ __forceinline__ int merge_block(const AttnArgs &a, const Left &left, int w0, int row0, float *top, float *total,
+                                           float4 *sum);
+template <int ROWS, int HD, int NT, int RB, int KV, typename T>
+__device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool all, float4 *shared);
+
 // ------------------------------------------------------- decode, 4 bits --
 //
 // e2m1 rows have a kernel of their own: with a quarter of an fp16 cache's bytes the
@@ -940,7 +947,9 @@ __global__ void __launch_bounds__(Dec<HD, KV, WIDE, T>::kWarps * 32, 1)
 // kernel), so that a chunk has no shuffles for them.  Page ids are read 256 positions
 // at once, a lane for each 8 rows that lie together, and a lane copies 16 bytes at a place
 // that is one multiplication away from their number.  What a warp needs between its runs
-// only is kept in shared memory, for the registers.
+// only is kept in shared memory, for the registers.  A call of few tiles has a cluster of
+// CTAs for each (CLUSTER), which cut it without a plan and join their states behind a
+// barrier of the cluster.
 //
 // Measured in a graph, 8 KV heads: 16 contexts of 11,003 to 40,111 positions, 32 heads of 128: 467 MB in 93 us
 // with fp16 queries (5.0 TB/s; issue slots 63 % and the ALU, which converts, 52 % busy) and 104 with fp32 ones;
@@ -983,7 +992,7 @@ __device__ __forceinline__ void mma_new(float (&d)[4], const uint32_t (&a)[4], u
 // (a & m) | (b & ~m)
 __device__ __forceinline__ uint32_t select_bits(uint32_t a, uint32_t b, uint32_t m) { return (a & m) | (b & ~m); }
 
-template <int HD, int ROWS, typename T>
+template <int HD, int ROWS, typename T, bool CLUSTER>
 __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
     ijb_paged_decode4_kernel(const __grid_constant__ AttnArgs a) {
     using D = Dec4<HD, ROWS, T>;
@@ -1013,10 +1022,25 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
         c.b0 = __shfl_sync(0xffffffffu, c.b0, 0);
         return c;
     };
-    Cursor first;
+    Cursor first = {};
     Entry entry;  // of the first run; tiles 0: not read yet
     int per;
-    if (a.n_entries < 32) {
+    // CLUSTER: the tile, its units, and those of this worker
+    [[maybe_unused]] int rank = 0, size = 1, tile = 0, units = 0, b0 = 0, b1 = 0;
+    if constexpr (CLUSTER) {
+        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+        tile = static_cast<int>(blockIdx.x) / size;
+        first.e = tile / a.kv.kv_heads;
+        first.head = tile % a.kv.kv_heads;
+        entry = entry_load(a, first.e, first.head == 0 && rank == 0 && warp == 0);
+        if (entry.tiles == 0) return;  // (and so does the rest of the cluster)
+        units = tile_units(a, entry, 0);
+        per = (units + size * D::kWarps - 1) / (size * D::kWarps);
+        b0 = min(units, (rank * D::kWarps + warp) * per);
+        b1 = min(units, b0 + per);
+        first.end = a.over + units;  // (the whole tile, for mend_rows)
+    } else if (a.n_entries < 32) {
         int *sums = reinterpret_cast<int *>(smem + warp * D::kStages * D::kStage);
         PlanOut po;
         plan_warp(a, sums, &po, worker == 0, entry);
@@ -1061,7 +1085,17 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
     auto load_run = [&]() {
         Cursor c = my.load;
         Segment s;
-        if (queued == 0 && entry.tiles > 0) {
+        if constexpr (CLUSTER) {
+            more = queued == 0 && b0 < b1;
+            s.x = entry;
+            s.e = first.e;
+            s.ti = 0;
+            s.head = first.head;
+            s.b0 = b0;
+            s.b1 = b1;
+            s.units = units;
+            s.start = 0;
+        } else if (queued == 0 && entry.tiles > 0) {
             more = c.at < c.end;
             s.x = entry;
             if (more) cursor_take(a, c, s);
@@ -1442,7 +1476,7 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
         // ---- the run's end: the output, or its state
         s = my.run[queue_out];
         const int end_row0 = s.ti * kDecRows, end_rows = min(kDecRows, s.x.rows - end_row0);
-        if (lane == 0) {
+        if (!CLUSTER && lane == 0) {
             const Left left = left_of(a, s, worker, per);
             int *to_left = &a.left[worker].states;
             *reinterpret_cast<int4 *>(to_left) = make_int4(left.states, left.q0, left.row0, left.rows);
@@ -1479,6 +1513,27 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
     cp_async_wait<0>();
     const int how = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, gone) ? 2 : 0);
     if (lane == 0) a.left[worker].bad = how;
+    if constexpr (CLUSTER) {
+        // the states are in the workspace: the cluster's CTAs join them, a row each
+        __shared__ float top[1], total[1];
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        const int w0 = tile * size * D::kWarps, states = (units + per - 1) / per;
+        Left left = {};
+        left.states = states;
+        left.q0 = entry.q0;
+        left.rows = entry.rows;
+        left.head = first.head;
+        float4 *shared = reinterpret_cast<float4 *>(smem);  // the stages are idle
+        static_assert(NT * sizeof(float4) <= D::kSmem, "a value a thread");
+        for (int row0 = rank; row0 < entry.rows; row0 += size) {
+            const int bad0 = a.left[w0].bad;
+            int again = (bad0 ? 1 : 0) | (bad0 & 2);
+            if (states > 1) again |= merge_block<kDecRows, HD, NT, 1, T>(a, left, w0, row0, top, total, shared);
+            if (again) mend_rows<kDecRows, HD, NT, 1, IJB_KV_E2M1, T>(a, w0, row0, again & 2, shared);
+            __syncthreads();
+        }
+    }
 }
 
 // ------------------------------------------------------------------ tile --
@@ -2411,6 +2466,94 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool 
 // rows a block, and 64 ragged sequences 27, 25, 25 and 27 us.
 constexpr int kMergeBatch = 4;
 
+// Joins the states of one tile (`left`, which worker w0 began): its rows row0 .. row0 + RB. Bit 0: rows to look at again;
+// bit 1: all of them (a page was none).
+template <int ROWS, int HD, int NT, int RB, typename T>
+__device__ __forceinline__ int merge_block(const AttnArgs &a, const Left &left, int w0, int row0, float *top, float *total,
+                                           float4 *sum) {
+    const int n = left.states, rows = min(RB, left.rows - row0);
+    constexpr long PF = part_floats<ROWS, HD>();
+    auto part = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0 ? 1 : 0)) * PF; };
+    // `bad` of the workers that go on with the tile (the first load is not waited for here)
+    int theirs = threadIdx.x < n ? a.left[w0 + threadIdx.x].bad : 0;
+    for (int i = threadIdx.x + NT; i < n; i += NT) theirs |= a.left[w0 + i].bad;
+    constexpr int Q = HD / 4;  // float4 of a row
+    const int outs = rows * Q, groups = outs < NT ? NT / outs : 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    T *op = static_cast<T *>(a.out);
+    const bool vec = aligned4<T>(a.out, a.out_stride);
+    bool fine = true;
+    for (int o0 = 0; o0 < outs; o0 += NT) {
+        const int g = outs < NT ? threadIdx.x / outs : 0, o = outs < NT ? threadIdx.x % outs : o0 + threadIdx.x;
+        const int r = min(o / Q, rows - 1), c = o % Q;
+        const bool mine = g < groups && o < outs;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = g; i0 - g < n; i0 += kMergeBatch * groups) {
+            float4 v[kMergeBatch];
+            float m[kMergeBatch];
+#pragma unroll
+            for (int k = 0; k < kMergeBatch; ++k) {
+                const int i = i0 + k * groups;
+                m[k] = -INFINITY;
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (mine && i < n) {
+                    const float *p = part(i);
+                    m[k] = p[ROWS * HD + row0 + r];
+                    v[k] = *reinterpret_cast<const float4 *>(p + (row0 + r) * HD + 4 * c);
+                }
+            }
+            if (o0 == 0 && i0 == g) {  // the rows' maxima and sums, a warp a row
+                for (int q = warp; q < rows; q += NT / 32) {
+                    float mx = -INFINITY, l = 0.f;
+                    for (int i = lane; i < n; i += 32) {
+                        const float *p = part(i) + ROWS * HD + row0 + q;
+                        const float pm = p[0], pl = p[ROWS], to = fmaxf(mx, pm);
+                        if (to != -INFINITY) l = l * ex2(mx - to) + pl * ex2(pm - to);
+                        mx = to;
+                    }
+                    const float all = warp_max(mx), mu = all == -INFINITY ? 0.f : all;
+                    l = warp_sum(l * ex2(mx - mu));
+                    if (lane == 0) {
+                        top[q] = mu;
+                        total[q] = l;
+                    }
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int k = 0; k < kMergeBatch; ++k) {
+                const float f = ex2(m[k] - top[r]);
+                if (f != 0.f) {  // a state without positions may hold no values
+                    acc.x = fmaf(f, v[k].x, acc.x);
+                    acc.y = fmaf(f, v[k].y, acc.y);
+                    acc.z = fmaf(f, v[k].z, acc.z);
+                    acc.w = fmaf(f, v[k].w, acc.w);
+                }
+            }
+        }
+        __syncthreads();
+        sum[threadIdx.x] = acc;
+        __syncthreads();
+        if (g == 0 && o < outs) {
+            for (int k = 1; k < groups; ++k) {
+                const float4 v = sum[k * outs + o];
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+            }
+            const float l = total[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            fine = fine && (acc.x * 0.f + acc.y * 0.f + acc.z * 0.f + acc.w * 0.f) * inv == 0.f;
+            const int rr = left.row0 + row0 + r;
+            store4(op + static_cast<long>(left.q0 + rr / a.group) * a.out_stride + (left.head * a.group + rr % a.group) * HD + 4 * c,
+                   vec, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        }
+    }
+    // (also: the shared sums have been read)
+    if (!__syncthreads_or(!fine || (theirs & 2))) return 0;
+    return __syncthreads_or(theirs & 2) ? 3 : 1;
+}
+
 // One tile's rows row0 .. row0 + RB (of `left`'s, which worker w0 began) by a warp, where they have up to kFewStates
 // states: a lane has a state's maximum and sum, then HD / 32 dims over all of them.  Bit 0: a value is not finite;
 // bit 1: a page was none.
@@ -2514,90 +2657,10 @@ __global__ void __launch_bounds__(NT) ijb_paged_merge_kernel(const __grid_consta
     for (; some; some &= some - 1) {
         const int w0 = blockIdx.x * EACH + __ffs(some) - 1;
         const Left left = a.left[w0];
-        const int n = left.states, rows = min(RB, left.rows - row0);
-        if (rows <= 0) continue;
-        constexpr long PF = part_floats<ROWS, HD>();
-        auto part = [&](int i) { return a.part + (2L * (w0 + i) + (i == 0 ? 1 : 0)) * PF; };
-        // `bad` of the workers that go on with the tile (the first load is not waited for here)
-        int theirs = threadIdx.x < n ? a.left[w0 + threadIdx.x].bad : 0;
-        for (int i = threadIdx.x + NT; i < n; i += NT) theirs |= a.left[w0 + i].bad;
-        constexpr int Q = HD / 4;  // float4 of a row
-        const int outs = rows * Q, groups = outs < NT ? NT / outs : 1;
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        T *op = static_cast<T *>(a.out);
-        const bool vec = aligned4<T>(a.out, a.out_stride);
-        bool fine = true;
-        for (int o0 = 0; o0 < outs; o0 += NT) {
-            const int g = outs < NT ? threadIdx.x / outs : 0, o = outs < NT ? threadIdx.x % outs : o0 + threadIdx.x;
-            const int r = min(o / Q, rows - 1), c = o % Q;
-            const bool mine = g < groups && o < outs;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int i0 = g; i0 - g < n; i0 += kMergeBatch * groups) {
-                float4 v[kMergeBatch];
-                float m[kMergeBatch];
-    #pragma unroll
-                for (int k = 0; k < kMergeBatch; ++k) {
-                    const int i = i0 + k * groups;
-                    m[k] = -INFINITY;
-                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (mine && i < n) {
-                        const float *p = part(i);
-                        m[k] = p[ROWS * HD + row0 + r];
-                        v[k] = *reinterpret_cast<const float4 *>(p + (row0 + r) * HD + 4 * c);
-                    }
-                }
-                if (o0 == 0 && i0 == g) {  // the rows' maxima and sums, a warp a row
-                    for (int q = warp; q < rows; q += NT / 32) {
-                        float mx = -INFINITY, l = 0.f;
-                        for (int i = lane; i < n; i += 32) {
-                            const float *p = part(i) + ROWS * HD + row0 + q;
-                            const float pm = p[0], pl = p[ROWS], to = fmaxf(mx, pm);
-                            if (to != -INFINITY) l = l * ex2(mx - to) + pl * ex2(pm - to);
-                            mx = to;
-                        }
-                        const float all = warp_max(mx), mu = all == -INFINITY ? 0.f : all;
-                        l = warp_sum(l * ex2(mx - mu));
-                        if (lane == 0) {
-                            top[q] = mu;
-                            total[q] = l;
-                        }
-                    }
-                    __syncthreads();
-                }
-    #pragma unroll
-                for (int k = 0; k < kMergeBatch; ++k) {
-                    const float f = ex2(m[k] - top[r]);
-                    if (f != 0.f) {  // a state without positions may hold no values
-                        acc.x = fmaf(f, v[k].x, acc.x);
-                        acc.y = fmaf(f, v[k].y, acc.y);
-                        acc.z = fmaf(f, v[k].z, acc.z);
-                        acc.w = fmaf(f, v[k].w, acc.w);
-                    }
-                }
-            }
-            __syncthreads();
-            sum[threadIdx.x] = acc;
-            __syncthreads();
-            if (g == 0 && o < outs) {
-                for (int k = 1; k < groups; ++k) {
-                    const float4 v = sum[k * outs + o];
-                    acc.x += v.x;
-                    acc.y += v.y;
-                    acc.z += v.z;
-                    acc.w += v.w;
-                }
-                const float l = total[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
-                fine = fine && (acc.x * 0.f + acc.y * 0.f + acc.z * 0.f + acc.w * 0.f) * inv == 0.f;
-                const int rr = left.row0 + row0 + r;
-                store4(op + static_cast<long>(left.q0 + rr / a.group) * a.out_stride + (left.head * a.group + rr % a.group) * HD + 4 * c,
-                       vec, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            }
-        }
-        // (also: the shared sums have been read)
-        if (__syncthreads_or(!fine || (theirs & 2))) {
-            again |= 1u << (w0 - blockIdx.x * EACH);
-            if (__syncthreads_or(theirs & 2)) all |= 1u << (w0 - blockIdx.x * EACH);
-        }
+        if (left.rows <= row0) continue;
+        const int how = merge_block<ROWS, HD, NT, RB, T>(a, left, w0, row0, top, total, sum);
+        if (how & 1) again |= 1u << (w0 - blockIdx.x * EACH);
+        if (how & 2) all |= 1u << (w0 - blockIdx.x * EACH);
     }
     for (; again; again &= again - 1) {
         const int j = __ffs(again) - 1;
@@ -2661,7 +2724,7 @@ template <int HD, int KV, int ROWS, typename T>
 using DecOf = std::conditional_t<KV == IJB_KV_E2M1, Dec4<HD, ROWS, T>, Dec<HD, KV, ROWS == 16, T>>;
 template <int HD, int KV, int ROWS, typename T>
 constexpr auto decode_kernel() {
-    if constexpr (KV == IJB_KV_E2M1) return ijb_paged_decode4_kernel<HD, ROWS, T>;
+    if constexpr (KV == IJB_KV_E2M1) return ijb_paged_decode4_kernel<HD, ROWS, T, false>;
     else return ijb_paged_decode_kernel<HD, KV, ROWS == 16, T>;
 }
 template <int HD, int KV, int ROWS, typename T>
@@ -2680,6 +2743,48 @@ cudaError_t tile_allow() {
     return allow_smem<decltype(kernel), Tile<HD, T>, std::integral_constant<int, KV>>(kernel, Tile<HD, T>::kSmem);
 }
 
+// A call of few tiles (entries x KV heads) over an e2m1 cache: a cluster of CTAs for each of them, which joins its
+// states itself.  One launch, and no plan.  The lengths are on the device, so the rule goes by the longest there may
+// be: a cluster has its own tile only, and long ones of a few tiles want all SMs.  Measured in a graph, 8 KV heads of 64
+// (128), 4 fp32 rows each, so and with plan and merge: one sequence of 300 positions 8.0 and 11.3 us (9.5 and 15.0), of
+// 2,043 9.4 and 12.3 (11.3 and 16.2), of 30,000 17.2 and 20.3 (23.7 and 25.4), of 40,000 20.7 and 21.8 (29.1 and 28.3);
+// two of 8,000 at most 13.1 and 14.5 (17.1 and 18.7), of 16,000 18.5 and 17.6 (25.1 and 23.2); four of 2,043 9.9 and
+// 13.6 (11.6 and 17.1), of 16,000 at most 18.7 and 21.3 (27.1 and 30.9).  16 clusters of 8 do not fit the GPU's
+// groups of SMs at once (two sequences of 2,043: 15.1).  8 sequences in clusters of 2 gained as much on short ones as
+// they lost on ragged ones.
+constexpr int kManyCtas = 8, kManyTiles = 8, kFewCtas = 4, kFewTiles = 32;  // CTAs a cluster, up to so many tiles
+constexpr long kManyPositions = 32768, kFewPositions = 512;                  // in all; a tile
+int cluster_size(const AttnArgs &a, int sms) {
+    const long tiles = static_cast<long>(a.n_entries) * a.kv.kv_heads, positions = static_cast<long>(a.kv.max_pages) << a.kv.page_shift;
+    if (tiles <= kManyTiles) return positions <= kManyPositions && tiles * kManyCtas <= sms ? kManyCtas : 0;
+    return tiles <= kFewTiles && positions <= kFewPositions * tiles && tiles * kFewCtas <= sms ? kFewCtas : 0;
+}
+template <int HD, int ROWS, typename T>
+cudaError_t cluster_allow() {
+    const auto kernel = ijb_paged_decode4_kernel<HD, ROWS, T, true>;
+    return allow_smem<decltype(kernel), Dec4<HD, ROWS, T>, std::true_type>(kernel, Dec4<HD, ROWS, T>::kSmem);
+}
+template <int HD, int ROWS, typename T>
+cudaError_t cluster_launch(const AttnArgs &a, int size, cudaStream_t s) {
+    using D = Dec4<HD, ROWS, T>;
+    cudaError_t e = cluster_allow<HD, ROWS, T>();
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.n_entries * a.kv.kv_heads * size);
+    cfg.blockDim = dim3(D::kWarps * 32);
+    cfg.dynamicSmemBytes = D::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, ijb_paged_decode4_kernel<HD, ROWS, T, true>, a);
+    count_launches(1);
+    return e;
+}
+
 template <int HD, int KV, int ROWS, typename T>
 cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     using D = DecOf<HD, KV, ROWS, T>;
@@ -2695,6 +2800,10 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.min_units = 64 / D::kPos;
     a.over = 1;
     a.least = 1;
+    if constexpr (KV == IJB_KV_E2M1) {
+        const int size = all ? cluster_size(a, sms) : 0;
+        if (size) return cluster_launch<HD, ROWS, T>(a, size, s);
+    }
     decode_kernel<HD, KV, ROWS, T>()<<<sms, D::kWarps * 32, decode_smem<HD, KV, ROWS, T>(), s>>>(a);
     return merge_launch<kDecRows, HD, KV, T>(a, s);
 }
@@ -2758,8 +2867,12 @@ template <int HD, int KV>
 cudaError_t prepare() {
     cudaError_t e = decode_allow<HD, KV, 8, float>();
     if (e == cudaSuccess) e = decode_allow<HD, KV, kDecRows, float>();
-    if constexpr (KV == IJB_KV_E2M1)
+    if constexpr (KV == IJB_KV_E2M1) {
         if (e == cudaSuccess) e = decode_allow<HD, KV, 4, float>();
+        if (e == cudaSuccess) e = cluster_allow<HD, 4, float>();
+        if (e == cudaSuccess) e = cluster_allow<HD, 8, float>();
+        if (e == cudaSuccess) e = cluster_allow<HD, kDecRows, float>();
+    }
     if (e == cudaSuccess) e = tile_allow<HD, KV, float>();
     return e;
 }
