@@ -409,3 +409,64 @@ def test_the_largest_values(cuda, dtype):
             # whatever their size
             tol = tol + 2.0 ** -11 * (top + want.abs()) + 2.0 ** -25
         assert bool(((got[0] - want).abs() <= tol).all())
+
+
+@TYPES
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_bad_blocks_and_absent_pages_among_many_entries(cuda, hd, dtype, tokens):
+    """40 sequences (more than get a cluster of CTAs each): a NaN block of V behind a token's position, and pages that
+    name nothing, reach no other entry and no earlier token."""
+    import torch
+    lens = [5 + 37 * i for i in range(40)]
+    kv, q, clean = check(cuda, [(min(tokens, n), n) for n in lens], 2, 2, hd, 16, dtype, seed=13)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    start = list(range(0, 40 * tokens + 1, tokens))
+    tol = 4e-5 * 6 if dtype == "float32" else 2.0 ** -9 * 6
+    for e in (3, 30, 39):
+        at = lens[e] - 1
+        page = int(kv.page_table[e, at // 16])
+        kept = kv.scale[page, 1, 0, at % 16].clone()
+        kv.scale[page, 1, 0, at % 16] = 255
+        got = kv.attention(q, i32(start), i32(lens), max_q=tokens)
+        kv.scale[page, 1, 0, at % 16] = kept
+        hit = torch.zeros(got.shape[:2], dtype=torch.bool, device=cuda)
+        hit[start[e + 1] - 1, :2] = True  # the last token, the first KV head
+        assert got[hit].isnan().all()
+        assert float((got[~hit].double() - clean[~hit].double()).abs().max()) <= tol
+        kept = int(kv.page_table[e, 0])
+        kv.page_table[e, 0] = -1
+        got = kv.attention(q, i32(start), i32(lens), max_q=tokens)
+        assert int(kv.status) != 0
+        kv.status.zero_()
+        kv.page_table[e, 0] = kept
+        other = torch.ones(got.shape[0], dtype=torch.bool, device=cuda)
+        other[start[e]:start[e + 1]] = False
+        assert float((got[other].double() - clean[other].double()).abs().max()) <= tol
+        k, v = kv.gather(i32([e] * (lens[e] - 16)), i32(list(range(16, lens[e]))), torch.float32)
+        for t in range(tokens):
+            n = lens[e] - tokens + t + 1 - 16
+            s = torch.einsum("hgd,thd->hgt", q[start[e] + t].double().view(2, 2, hd), k[:n].double()) * hd ** -0.5
+            want = torch.einsum("hgt,thd->hgd", torch.softmax(s, -1), v[:n].double()).reshape(4, hd)
+            assert float((got[start[e] + t].double() - want).abs().max()) <= tol
+
+
+@TYPES
+@pytest.mark.parametrize("entries,kvh", [([(1, 2000)], 8), ([(1, 70)] * 3 + [(1, 3000)], 8), ([(4, 500), (1, 1)], 2),
+                                         ([(1, 33000)], 1), ([(1, 31000), (2, 5)], 4), ([(0, 7)], 8), ([(3, 0), (1, 9)], 3)])
+def test_calls_of_few_tiles(cuda, entries, kvh, dtype):
+    """One launch (a cluster of CTAs a tile) up to its limits, two behind them."""
+    from ijb200 import lib
+    check(cuda, entries, kvh, 4, 64, 16, dtype, seed=2)
+    check(cuda, entries, kvh, 4, 128, 16, dtype, seed=2)
+    kv, _ = build(cuda, [max(t, 1) for _, t in entries], kvh, 64, 16)
+    import torch
+    n = sum(l for l, _ in entries)
+    q = torch.zeros((max(n, 1), 4 * kvh, 64), device=cuda, dtype=getattr(torch, dtype))
+    start = np.cumsum([0] + [l for l, _ in entries]).astype(np.int32)
+    args = (q, torch.from_numpy(start).to(cuda), torch.tensor([t for _, t in entries], dtype=torch.int32, device=cuda))
+    before = lib.load().ijb_kernel_launches()
+    kv.attention(*args, max_q=max(l for l, _ in entries) or 1)
+    tiles, positions = len(entries) * kvh, kv.page_table.shape[1] * 16
+    few = positions <= 32768 if tiles <= 8 else tiles <= 32 and positions <= 512 * tiles
+    assert lib.load().ijb_kernel_launches() - before == (1 if few else 2)
