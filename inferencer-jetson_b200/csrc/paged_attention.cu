@@ -12,7 +12,8 @@
 //  * ijb_paged_decode_kernel, up to 16 rows an entry and KV head (single tokens,
 //    a few drafted ones): bound by reading the cache.  Every warp streams
 //    32-position chunks of its own through shared memory.  For e2m1 rows, whose
-//    reading takes less time than their arithmetic, ijb_paged_decode4_kernel.
+//    reading takes less time than their arithmetic, ijb_paged_decode4_kernel (calls of
+//    few tiles: in one launch, without what the next paragraph says).
 //  * ijb_paged_tile_kernel, more rows (chunks, prompts): bound by the matrix
 //    products and the exponentials.  256 rows at a time on tcgen05.
 // Both cut all the call's work (tiles of rows x units of positions, over all
@@ -2797,6 +2798,7 @@ cudaError_t decode_launch(AttnArgs a, int sms, bool all, cudaStream_t s) {
     a.unit = D::kPos;
     a.workers = sms * D::kWarps;
     // 64 positions a worker at least: one token at position 2043 of an e2m1 cache took 13.1 us so and 15.0 with 128
+    // (before such calls had clusters)
     a.min_units = 64 / D::kPos;
     a.over = 1;
     a.least = 1;
