@@ -115,10 +115,7 @@ struct ijb_engine {
     long num_pages = 0;
     std::vector<int> free_pages;
     std::vector<int> page_refs;  // sequences that hold a page: forks share their full pages (ijb_seq_fork)
-    // pages to be copied, in every layer, before the next step's kernels: (from, to)
-    std::vector<std::pair<int, int>> page_copies;
-    int *copy_host = nullptr, *copy_dev = nullptr;  // their ids, pinned and on the device, [2][copy_room]
-    size_t copy_room = 0;
+    int *copy_host = nullptr, *copy_dev = nullptr;  // ids of a page copy, pinned and on the device: [from, to][layers]
     int max_pages_per_seq = 0;
     int *page_table_dev = nullptr;
     std::vector<CUtensorMap> kv_maps;  // per layer, for the streaming attention (fp16 cache, head_dim 64)
@@ -703,44 +700,32 @@ void release_pages(ijb_engine *e, int seq) {
     e->seq_pages[seq].clear();
 }
 
-// Queues the copies of page_copies, all layers' in one launch: to the copy a pool of
-// layers * num_pages pages.
-void copy_pages(ijb_engine *e) {
-    const std::vector<std::pair<int, int>> todo = std::move(e->page_copies);
-    e->page_copies.clear();
-    if (todo.empty()) return;
-    const int layers = e->d.layers;
-    const size_t n = todo.size() * layers;
-    if (n > e->copy_room) {
-        cudaFree(e->copy_dev);
-        if (e->copy_host) cudaFreeHost(e->copy_host);
-        e->copy_dev = nullptr;
-        e->copy_host = nullptr;
-        e->copy_room = 0;
-        e->copy_dev = dev_alloc<int>(2 * n, "page copies");
-        ck(cudaMallocHost(&e->copy_host, 2 * n * sizeof(int)), "page copy staging");
-        e->copy_room = n;
+// Queues the copy of a page in every layer, in one launch: to the copy a pool of layers * num_pages pages.
+void copy_page(ijb_engine *e, int from, int to) {
+    const int n = e->d.layers;
+    if (!e->copy_host) ck(cudaMallocHost(&e->copy_host, 2 * n * sizeof(int)), "page copy staging");
+    if (!e->copy_dev) e->copy_dev = dev_alloc<int>(2 * n, "page copies");
+    ck(cudaStreamSynchronize(e->stream), "page copies");  // the last copy's ids have left their staging
+    for (int l = 0; l < n; ++l) {
+        e->copy_host[l] = static_cast<int>(l * e->num_pages + from);
+        e->copy_host[n + l] = static_cast<int>(l * e->num_pages + to);
     }
-    ck(cudaStreamSynchronize(e->stream), "page copies");  // the ids of the last copies have left their staging
-    for (int l = 0; l < layers; ++l)
-        for (size_t i = 0; i < todo.size(); ++i) {
-            e->copy_host[l * todo.size() + i] = static_cast<int>(l * e->num_pages + todo[i].first);
-            e->copy_host[n + l * todo.size() + i] = static_cast<int>(l * e->num_pages + todo[i].second);
-        }
     ijb_kv_view v = layer_view(e, 0);
-    v.num_pages = layers * e->num_pages;
+    v.num_pages = n * e->num_pages;
     if (e->paged < 0) {  // fp32 pages are fp16 ones of twice the heads
         v.type = IJB_KV_F16;
         v.kv_heads *= e->kv_f32 ? 2 : 1;
     }
     ck(cudaMemcpyAsync(e->copy_dev, e->copy_host, 2 * n * sizeof(int), cudaMemcpyHostToDevice, e->stream), "page copies H2D");
-    if (ijb_kv_copy_pages(&v, nullptr, static_cast<int>(n), e->copy_dev, e->copy_dev + n, e->status, e->stream) != IJB_OK)
+    if (ijb_kv_copy_pages(&v, nullptr, n, e->copy_dev, e->copy_dev + n, e->status, e->stream) != IJB_OK)
         throw Error(IJB_ERR_CUDA, t_create_err);
 }
 
 // Makes sure `seq` owns pages for positions [0, upto]; returns the slot of `pos`.
 // `write`: the position is to be written, so a page that another sequence shares is
-// replaced by one of this sequence's own (with the positions before pos: copy_pages).
+// replaced by one of this sequence's own, with the positions before pos:
+// they are copied before the page changes hands, so a call that fails here or
+// later loses none of them.
 int slot_for(ijb_engine *e, int seq, int pos, bool write = true) {
     const int ps = e->d.page_size;
     auto &pages = e->seq_pages[seq];
@@ -753,9 +738,13 @@ int slot_for(ijb_engine *e, int seq, int pos, bool write = true) {
     }
     int &page = pages[pos / ps];
     if (write && e->page_refs[page] > 1) {
-        if (pos % ps) e->page_copies.reserve(e->page_copies.size() + 1);
         const int own = take_page(e);
-        if (pos % ps) e->page_copies.emplace_back(page, own);
+        try {
+            if (pos % ps) copy_page(e, page, own);
+        } catch (...) {
+            release_page(e, own);
+            throw;
+        }
         release_page(e, page);
         page = own;
         e->page_table_host[static_cast<long>(seq) * e->max_pages_per_seq + pos / ps] = own;
@@ -785,7 +774,6 @@ void packed_step(ijb_engine *e, int n, const int *seqs, const int *tokens, const
         mt[2 * d.max_batch + i] = pos;
         mt[3 * d.max_batch + i] = slot_for(e, sq, pos);
     }
-    copy_pages(e);
     for (int i = n; i < d.max_batch; ++i) mt[i] = mt[d.max_batch + i] = mt[2 * d.max_batch + i] = mt[3 * d.max_batch + i] = 0;
     run_step(e, n, need_logits, traced, fill_entries(e, n), then);
 }
@@ -1520,16 +1508,12 @@ int ijb_seq_fork(ijb_engine *e, int seq, int length, int *new_seq) {
         const std::vector<int> &from = e->seq_pages[seq];
         std::vector<int> &pages = e->seq_pages[to];
         pages.reserve(full + 1);
-        e->page_copies.reserve(e->page_copies.size() + 1);
         const int own = tail ? take_page(e) : -1;  // (nothing has changed if there is none)
         for (int i = 0; i < full; ++i) {
             pages.push_back(from[i]);
             ++e->page_refs[from[i]];
         }
-        if (tail) {
-            pages.push_back(own);
-            e->page_copies.emplace_back(from[full], own);
-        }
+        if (tail) pages.push_back(own);
         try {
             int *row = e->page_table_host + static_cast<long>(to) * e->max_pages_per_seq;
             for (size_t i = 0; i < pages.size(); ++i) row[i] = pages[i];
@@ -1537,12 +1521,11 @@ int ijb_seq_fork(ijb_engine *e, int seq, int length, int *new_seq) {
                 ck(cudaMemcpyAsync(e->page_table_dev + static_cast<long>(to) * e->max_pages_per_seq, row,
                                    pages.size() * sizeof(int), cudaMemcpyHostToDevice, e->stream),
                    "page table H2D");
-            copy_pages(e);
+            if (tail) copy_page(e, from[full], own);
             ck(cudaStreamSynchronize(e->stream), "fork");
             check_device_status(e);
         } catch (...) {
             cudaStreamSynchronize(e->stream);
-            e->page_copies.clear();
             release_pages(e, to);
             throw;
         }
@@ -1583,7 +1566,6 @@ int ijb_generate(ijb_engine *e, int seq, int first_token, int max_tokens, const 
         int *mt = e->meta_host;
         std::memset(mt, 0, e->meta_ints * sizeof(int));
         for (int k = steps - 1; k >= 0; --k) slot_for(e, seq, pos0 + k);
-        copy_pages(e);
         mt[0] = first_token;
         mt[d.max_batch] = seq;
         mt[2 * d.max_batch] = pos0;

@@ -1,0 +1,67 @@
+"""Calls that fail over shared pages, on the host, with a CUDA runtime of host memory (see test_engine_host.py): a sequence
+that writes to a page which a fork shares keeps what it held, whichever call fails, and the device's page table follows the
+host's."""
+import pytest
+
+from test_engine_host import child  # noqa: F401  (a fixture)
+
+KW = "context=64, max_batch=4, max_seqs=5, page_size=8"
+TYPES = pytest.mark.parametrize("kv_type", [None, "f16", "e4m3", "e2m1"])
+CODE = """
+ids = ("cudaMemcpyAsync", 2 * cfg.layers * 4)  # source and destination of one page in every layer
+def fails(name, call):
+    '''call() with its first call of name failing'''
+    F.fake_fail(name.encode(), b"cudaSetDevice")
+    F.cudaSetDevice(0)
+    try:
+        call()
+    except lib.IjbError as err:
+        assert "made by the test" in str(err), err
+        return
+    raise SystemExit("no error")
+def copies(call):
+    start = F.fake_calls()
+    call()
+    return log(start).count(ids)
+"""
+
+
+@TYPES
+@pytest.mark.parametrize("fail", ["cudaMalloc", "cudaHostAlloc", "cudaStreamSynchronize", "cudaMemcpyAsync", "cudaGraphLaunch"])
+def test_a_failed_write_to_a_shared_page_is_made_good(child, kv_type, fail):  # noqa: F811
+    """The positions before the one that is written are copied by the failed call, and its copy stays, or by the next one."""
+    child(f"""{CODE}
+e = Engine(cfg, weights, {KW}, kv_type={kv_type!r})
+e.prefill(list(range(24)))
+t = e.seq_fork(0, 24)                         # whole pages: nothing has been copied
+start = F.fake_calls()
+fails({fail!r}, lambda: e.forward(1, 11))
+done = [n for n, (name, size) in enumerate(log(start)) if (name, size) == ids]
+if {fail!r} == "cudaMemcpyAsync":             # (the ids' own upload, which is logged all the same)
+    assert len(done) == 1
+    done = []
+assert e.seq_length(0) == 24
+assert len(done) + copies(lambda: e.forward(1, 11)) == 1
+assert copies(lambda: e.forward(1, 12)) == 0
+""")
+
+
+@TYPES
+def test_a_fork_after_a_failed_step_copies_its_own_page_only(child, kv_type):  # noqa: F811
+    """A copy that was left for later would be in one call with one that reads its destination."""
+    child(f"""{CODE}
+e = Engine(cfg, weights, {KW}, kv_type={kv_type!r}, num_pages=6)
+e.prefill(list(range(24)))                    # 3 pages
+e.seq_fork(0, 24)
+s = e.seq_open()
+e.seq_prefill(s, list(range(16)))             # 2: one is left
+try:
+    e.decode_step([0, s], [1, 2])             # each needs one: sequence 0 goes on behind its shared pages
+    raise SystemExit("no error")
+except lib.IjbError as err:
+    assert err.code == lib.ERR_CAPACITY
+e.seq_close(s)
+fails("cudaStreamSynchronize", lambda: e.forward(1, 11))
+before = e.lib.ijb_kernel_launches()
+assert copies(lambda: e.seq_fork(0, 10)) == 1 and e.lib.ijb_kernel_launches() - before == 1
+""")
