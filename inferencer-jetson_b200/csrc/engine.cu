@@ -114,6 +114,7 @@ struct ijb_engine {
     size_t paged_work_bytes = 0;
     long num_pages = 0;
     std::vector<int> free_pages;
+    std::vector<char> row_stale;  // by sequence: its page table row has changed since its last upload was queued
     std::vector<int> page_refs;  // sequences that hold a page: forks share their full pages (ijb_seq_fork)
     int *copy_host = nullptr, *copy_dev = nullptr;  // ids of a page copy, pinned and on the device: [from, to][layers]
     int max_pages_per_seq = 0;
@@ -721,6 +722,16 @@ void copy_page(ijb_engine *e, int from, int to) {
         throw Error(IJB_ERR_CUDA, t_create_err);
 }
 
+// Queues the upload of the page table's row of `seq`, if the device has not got it as it is.
+void upload_row(ijb_engine *e, int seq) {
+    if (!e->row_stale[seq]) return;
+    const long row = static_cast<long>(seq) * e->max_pages_per_seq;
+    ck(cudaMemcpyAsync(e->page_table_dev + row, e->page_table_host + row, e->seq_pages[seq].size() * sizeof(int),
+                       cudaMemcpyHostToDevice, e->stream),
+       "page table H2D");
+    e->row_stale[seq] = 0;
+}
+
 // Makes sure `seq` owns pages for positions [0, upto]; returns the slot of `pos`.
 // `write`: the position is to be written, so a page that another sequence shares is
 // replaced by one of this sequence's own, with the positions before pos:
@@ -729,12 +740,12 @@ void copy_page(ijb_engine *e, int from, int to) {
 int slot_for(ijb_engine *e, int seq, int pos, bool write = true) {
     const int ps = e->d.page_size;
     auto &pages = e->seq_pages[seq];
-    bool changed = false;
+    int *row = e->page_table_host + static_cast<long>(seq) * e->max_pages_per_seq;
     while (static_cast<int>(pages.size()) * ps <= pos) {
         require(static_cast<int>(pages.size()) < e->max_pages_per_seq, "sequence exceeds context", IJB_ERR_CAPACITY);
         pages.push_back(take_page(e));
-        e->page_table_host[static_cast<long>(seq) * e->max_pages_per_seq + pages.size() - 1] = pages.back();
-        changed = true;
+        row[pages.size() - 1] = pages.back();
+        e->row_stale[seq] = 1;
     }
     int &page = pages[pos / ps];
     if (write && e->page_refs[page] > 1) {
@@ -746,15 +757,10 @@ int slot_for(ijb_engine *e, int seq, int pos, bool write = true) {
             throw;
         }
         release_page(e, page);
-        page = own;
-        e->page_table_host[static_cast<long>(seq) * e->max_pages_per_seq + pos / ps] = own;
-        changed = true;
+        page = row[pos / ps] = own;
+        e->row_stale[seq] = 1;
     }
-    if (changed)
-        ck(cudaMemcpyAsync(e->page_table_dev + static_cast<long>(seq) * e->max_pages_per_seq,
-                           e->page_table_host + static_cast<long>(seq) * e->max_pages_per_seq,
-                           pages.size() * sizeof(int), cudaMemcpyHostToDevice, e->stream),
-           "page table H2D");
+    upload_row(e, seq);
     return page * ps + pos % ps;
 }
 
@@ -1083,6 +1089,7 @@ static int create_engine(const ijb_model_desc *desc, const ijb_tensor_view *tens
         }
         for (long p = e->num_pages - 1; p >= 0; --p) e->free_pages.push_back(static_cast<int>(p));
         e->page_refs.assign(e->num_pages, 0);
+        e->row_stale.assign(d.max_seqs, 0);
         const size_t pt = static_cast<size_t>(d.max_seqs) * e->max_pages_per_seq;
         e->page_table_dev = dev_alloc<int>(pt, "page table");
         ck(cudaMemset(e->page_table_dev, 0, pt * sizeof(int)), "page table clear");
@@ -1517,10 +1524,8 @@ int ijb_seq_fork(ijb_engine *e, int seq, int length, int *new_seq) {
         try {
             int *row = e->page_table_host + static_cast<long>(to) * e->max_pages_per_seq;
             for (size_t i = 0; i < pages.size(); ++i) row[i] = pages[i];
-            if (!pages.empty())
-                ck(cudaMemcpyAsync(e->page_table_dev + static_cast<long>(to) * e->max_pages_per_seq, row,
-                                   pages.size() * sizeof(int), cudaMemcpyHostToDevice, e->stream),
-                   "page table H2D");
+            e->row_stale[to] = !pages.empty();
+            upload_row(e, to);
             if (tail) copy_page(e, from[full], own);
             ck(cudaStreamSynchronize(e->stream), "fork");
             check_device_status(e);

@@ -65,3 +65,41 @@ fails("cudaStreamSynchronize", lambda: e.forward(1, 11))
 before = e.lib.ijb_kernel_launches()
 assert copies(lambda: e.seq_fork(0, 10)) == 1 and e.lib.ijb_kernel_launches() - before == 1
 """)
+
+
+@TYPES
+def test_the_page_table_is_sent_again(child, kv_type):  # noqa: F811
+    """An upload of a sequence's row that failed, or that the call did not come to, is made up for by the next call."""
+    child(f"""{CODE}
+e = Engine(cfg, weights, {KW}, kv_type={kv_type!r}, num_pages=4)
+s = e.seq_open()
+fails("cudaMemcpyAsync", lambda: e.decode_step([s], [1]))
+start = F.fake_calls()
+e.decode_step([s], [1])
+assert ("cudaMemcpyAsync", 4) in log(start)
+try:
+    e.generate(s, 1, 40)                      # 6 pages, of which there are 4
+    raise SystemExit("no error")
+except lib.IjbError as err:
+    assert err.code == lib.ERR_CAPACITY
+start = F.fake_calls()
+e.decode_step([s], [1])                       # its page was there, the 3 others have been taken since
+assert ("cudaMemcpyAsync", 16) in log(start)
+start = F.fake_calls()
+e.decode_step([s], [1])
+assert ("cudaMemcpyAsync", 16) not in log(start)
+""")
+
+
+@TYPES
+def test_the_page_table_is_sent_again_for_a_shared_page(child, kv_type):  # noqa: F811
+    child(f"""{CODE}
+e = Engine(cfg, weights, {KW}, kv_type={kv_type!r})
+e.prefill(list(range(24)))
+e.seq_fork(0, 24)
+e.reset()
+fails("cudaMemcpyAsync", lambda: e.forward(1, 0))  # no copy: the row's upload
+start = F.fake_calls()
+assert copies(lambda: e.forward(1, 0)) == 0
+assert ("cudaMemcpyAsync", 12) in log(start)
+""")
