@@ -734,9 +734,9 @@ void upload_row(ijb_engine *e, int seq) {
 
 // Makes sure `seq` owns pages for positions [0, upto]; returns the slot of `pos`.
 // `write`: the position is to be written, so a page that another sequence shares is
-// replaced by one of this sequence's own, with the positions before pos:
-// they are copied before the page changes hands, so a call that fails here or
-// later loses none of them.
+// replaced by one of this sequence's own.  Positions that the sequence holds are
+// copied before the page changes hands, so a call that fails here or later loses
+// none of them (a step sets a sequence back when it has succeeded).
 int slot_for(ijb_engine *e, int seq, int pos, bool write = true) {
     const int ps = e->d.page_size;
     auto &pages = e->seq_pages[seq];
@@ -751,7 +751,7 @@ int slot_for(ijb_engine *e, int seq, int pos, bool write = true) {
     if (write && e->page_refs[page] > 1) {
         const int own = take_page(e);
         try {
-            if (pos % ps) copy_page(e, page, own);
+            if (pos / ps * ps < e->seq_len[seq]) copy_page(e, page, own);
         } catch (...) {
             release_page(e, own);
             throw;

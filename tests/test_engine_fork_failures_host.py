@@ -103,3 +103,35 @@ start = F.fake_calls()
 assert copies(lambda: e.forward(1, 0)) == 0
 assert ("cudaMemcpyAsync", 12) in log(start)
 """)
+
+
+@TYPES
+@pytest.mark.parametrize("fail", ["cudaMalloc", "cudaMemcpyAsync", "cudaGraphLaunch"])
+def test_a_failed_write_to_a_page_s_start_keeps_what_is_behind_it(child, kv_type, fail):  # noqa: F811
+    """The sequence is set back by a step that succeeds only: until then it may go on at any of its positions."""
+    child(f"""{CODE}
+e = Engine(cfg, weights, {KW}, kv_type={kv_type!r})
+e.prefill(list(range(24)))
+e.seq_fork(0, 24)
+start = F.fake_calls()
+fails({fail!r}, lambda: e.forward(1, 16))
+done = log(start).count(ids) if {fail!r} == "cudaGraphLaunch" else 0
+assert e.seq_length(0) == 24
+assert done + copies(lambda: e.forward(1, 20)) == 1
+""")
+
+
+@TYPES
+def test_generate_copies_no_page_that_it_writes_anew(child, kv_type):  # noqa: F811
+    child(f"""{CODE}
+def launches(fork):
+    e = Engine(cfg, weights, {KW}, kv_type={kv_type!r})
+    e.prefill(list(range(40)))                # 5 pages
+    if fork:
+        e.seq_fork(0, 40)
+    e.forward(1, 11)                          # the second is sequence 0's own
+    before = e.lib.ijb_kernel_launches()
+    e.generate(0, 1, 29)                      # positions 12 to 39
+    return e.lib.ijb_kernel_launches() - before
+assert launches(True) == launches(False)
+""")
