@@ -359,14 +359,17 @@ typedef struct {
  * 448 * 2^e over its finite values (2^-126 at least), its values are rounded
  * to nearest, infinities to the largest finite value, NaN stays NaN.  32 dims of
  * an e2m1 row get the scale nearest to max|x| / 6 over their finite values (fp32's
- * product with 1 / 6; ties to even; 10240 at most, 0 below 2^-18) and the codes nearest
+ * product with 1 / 6; ties to even; 10240 at most, 0 up to 2^-18) and the codes nearest
  * to fp32's products of x and 1 / scale, ties to the even code, infinities and
- * larger values to the largest; a NaN makes its 32 dims NaN (scale byte 255).
- * What is read back is code * scale, exact in fp16 too, and off by 0.18 of the
- * largest of the 32 at most (0.09 for values up to half of it): 10 % rms of
- * normally distributed values.  Entries with a negative position are padding
- * and are skipped.  A (sequence, position) must not be named by two of the call's
- * tokens. */
+ * larger values to the largest (where the scale is 0 all are 0, infinities too); a
+ * NaN makes its 32 dims NaN (scale byte 255).
+ * What is read back is code * scale, exact in fp16 too.  Where the largest finite
+ * magnitude a of the 32 is 6 * 2^-14 (3.7e-4) to 61440, values are off by 0.18 a at
+ * most (0.09 a for those up to a / 2): 10 % rms of normally distributed values.
+ * Below, scales come in steps of 2^-17, and values are off by a / 6 + 2^-18 or
+ * 6 * 2^-18 (2.3e-5), whichever is more; past 61440 values become 61440.  Entries with
+ * a negative position are padding and are skipped.  A (sequence, position) must
+ * not be named by two of the call's tokens. */
 int ijb_kv_append(const ijb_kv_view *kv, int src_type, const void *k_dev, const void *v_dev, long stride, int n,
                   const int *tok_seq_dev, const int *tok_pos_dev, uint32_t *status_dev, void *stream);
 
