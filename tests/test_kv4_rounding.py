@@ -3,7 +3,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_kv4 import LEVELS, quantise, scale_table
+from test_gpu_kv4 import LEVELS, nearest, quantise, scale_table
 
 
 def blocks(largest):
@@ -57,3 +57,44 @@ def test_larger_values_and_infinities_become_the_largest():
     x[:, 5] = np.inf
     assert (values(x)[:, 5] == [3.0, 0.0]).all()
     assert (values(np.full((1, 32), -np.inf, np.float32)) == 0).all()
+
+
+def borders():
+    """Largest magnitudes where max|x| times fp32's 1 / 6 is halfway between two scales, or beside that.  Below 7.125
+    (0x1.c7fffep+2) the product is a tie, and rounds up, where the quotient lies a unit of the last place below it."""
+    m = np.array([1.0625, 1.1875, 1.3125, 1.4375, 1.5625, 1.6875, 1.8125, 1.9375], np.float32) * np.float32(6)
+    near = np.stack([np.nextafter(m, np.float32(0)), m, np.nextafter(m, np.float32(99))])
+    return (near[..., None] * np.float32(2) ** np.arange(-16, 14, dtype=np.float32)).ravel()
+
+
+def test_the_borders_tell_the_product_from_the_quotient():
+    a = borders()
+    scales = scale_table()[:227]
+    by = [nearest(scales, r.astype(np.float64)) for r in (a * (np.float32(1) / np.float32(6)), a / np.float32(6))]
+    assert (by[0] != by[1]).any()
+    low = np.nextafter(np.float32(7.125), np.float32(0))
+    assert quantise(blocks([low]))[1].item() == 122 and scales[121] < low / np.float32(6) < scales[[121, 122]].mean()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kvh,hd", [(1, 64), (2, 64), (8, 64), (1, 128), (8, 128)])
+def test_kernel_at_the_borders(cuda, kvh, hd):
+    """Codes and scale bytes at the borders and all over the range, rows of few heads a thread each and of many."""
+    import torch
+    from test_gpu_kv4 import make
+    a = np.concatenate([borders(), spread(2.0 ** -24, 1e5, 20000 // hd * hd), [0.0] * 16]).astype(np.float32)
+    x = blocks(a)
+    n = len(x) * 32 // (2 * kvh * hd)
+    x = x[:n * 2 * kvh * hd // 32].reshape(2, n, kvh, hd)
+    kv = make(cuda, kvh, hd, 16, pages=-(-n // 16), seqs=1, max_pages=-(-n // 16))
+    seq = torch.zeros((n,), dtype=torch.int32, device=cuda)
+    pos = torch.arange(n, dtype=torch.int32, device=cuda)
+    t = torch.from_numpy(x).to(cuda)
+    kv.append(t[0], t[1], seq, pos)
+    code, s = quantise(x)
+    page = kv.page_table[0, (pos // 16).long()].cpu().numpy()
+    off = pos.cpu().numpy() % 16
+    got, got_s = kv.data.view(torch.uint8).cpu().numpy(), kv.scale.cpu().numpy()
+    for which in range(2):
+        np.testing.assert_array_equal(got_s[page, which, :, off], s[which])
+        np.testing.assert_array_equal(got[page, which, :, off], code[which])
