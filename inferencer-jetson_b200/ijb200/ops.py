@@ -19,7 +19,9 @@ from .lib import IjbError  # noqa: F401  (what the calls raise)
 F32, F16 = 0, 1  # IJB_TYPE_F32, IJB_TYPE_F16
 KV_F16, KV_E4M3, KV_E2M1 = 0, 2, 4
 _TYPE = {torch.float32: F32, torch.float16: F16}
-_KV = {torch.float16: KV_F16, torch.float8_e4m3fn: KV_E4M3, torch.float4_e2m1fn_x2: KV_E2M1}
+_KV = {torch.float16: KV_F16, torch.float8_e4m3fn: KV_E4M3}
+if hasattr(torch, "float4_e2m1fn_x2"):  # (younger than the others)
+    _KV[torch.float4_e2m1fn_x2] = KV_E2M1
 _stream = torch._C._cuda_getCurrentRawStream
 _current = torch._C._cuda_getDevice
 _empty = torch.empty

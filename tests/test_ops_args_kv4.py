@@ -63,3 +63,16 @@ def test_copied_pages_arguments_are_checked():
     assert L.ijb_kernel_launches() == before
     wide = view(kv_heads=1024, page_size=256, head_dim=128)
     assert L.ijb_kv_copy_pages(ctypes.byref(wide), None, 0x7fffffff, 256, 256, None, None) == lib.ERR_INVALID
+
+
+def test_a_torch_without_4_bit_tensors_keeps_the_other_caches():
+    """Only the cache in 4 bits needs torch.float4_e2m1fn_x2."""
+    import os
+    import subprocess
+    import sys
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "inferencer-jetson_b200")
+    code = ("import sys, torch; sys.path.insert(0, sys.argv[1]); del torch.float4_e2m1fn_x2\n"
+            "from ijb200 import ops\n"
+            "assert torch.float16 in ops._KV and torch.float8_e4m3fn in ops._KV and len(ops._KV) == 2")
+    r = subprocess.run([sys.executable, "-c", code, pkg], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
