@@ -3,7 +3,6 @@
 // paged_attention.cu).
 #pragma once
 #include <cuda_fp16.h>
-#include <cuda_fp4.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
