@@ -332,16 +332,20 @@ __device__ __forceinline__ uint32_t e2m1_codes(const float (&f)[8], float inv) {
 }
 
 // A thread has 8 values of U heads' rows; 4 threads share a block of 32 dims, and each works out the scale of one
-// head in 4 for all of them.  Measured: 12289 tokens of 8 heads x 128 from fp32 26 us (4.4
-// TB/s), from fp16 22; before, in blocks of 256 threads, 4 on an SM, 28 and 24 us.
+// head in 4 for all of them.  Measured: 12289 tokens of 8 heads x 128 from fp32 26 us (4.5 TB/s), from fp16 21 (3.1);
+// before, in blocks of 256 threads, 4 on an SM, 28 and 24 us.  No unit is full (DRAM 51 %, issue slots 40 %, the ALU
+// 37 %): of the 20 clocks from one of a warp's instructions to its next 12 go to waiting for its loads, and half the
+// warps that an SM could hold are there.
 template <typename T, bool VEC, int HD, int U>
-__global__ void __launch_bounds__(append4_threads(U), U == 1 ? 4 : (sizeof(T) == 4 ? 9 : 10)) ijb_kv_append4_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(append4_threads(U), U == 1 ? 4 : (sizeof(T) == 4 ? 9 : 10))
+    ijb_kv_append4_kernel(const __grid_constant__ RowsParams p) {
     using P = Place4<HD, U, 8, append4_threads(U)>;
     const int rows = P::tokens(p.kv) * 2 * P::groups(p.kv);
     const int lane = threadIdx.x & 31, quad = lane & 28;
     for (int row = threadIdx.x / P::L; row / P::ROWS * P::ROWS < rows; row += P::ROWS) {  // (all threads as often)
         const P w(p, row);
-        const T *from = static_cast<const T *>(w.which ? p.v : p.k) + (w.n ? w.t * p.stride + static_cast<long>(w.head) * HD + w.c * 8 : 0);
+        const T *from = static_cast<const T *>(w.which ? p.v : p.k) +
+                        (w.n ? w.t * p.stride + static_cast<long>(w.head) * HD + w.c * 8 : 0);
         float f[U][8], a[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
@@ -423,11 +427,12 @@ __global__ void __launch_bounds__(append4_threads(U), U == 1 ? 4 : (sizeof(T) ==
 
 // Code * scale, exact in fp32, and in fp16 for the scales that ijb_kv_append writes (others rounded once).  A thread
 // stores 16 bytes of each of U heads' rows, next to its neighbour's.  Bound by the latency of its three loads in a
-// row (the slot, its page, the codes), so what counts is how many threads are on an SM, and that a block of few
-// has more than one row each: 32749 tokens of 8 heads x 128 to fp16 take 34.3 us (5.0 TB/s) and to fp32 53 (5.8), in
-// blocks of 256 threads, 4 on an SM, 49 and 89.
+// row (the slot, its page, the codes; 18 of 25 clocks an instruction go to waiting for them, issue slots 54 %), so
+// what counts is how many threads are on an SM, and that a block of few has more than one row each: 32749 tokens of 8
+// heads x 128 to fp16 take 34.3 us (5.0 TB/s) and to fp32 53 (5.8), in blocks of 256 threads, 4 on an SM, 49 and 89.
 template <typename T, bool VEC, int HD, int U>
-__global__ void __launch_bounds__(gather4_threads(U), U == 1 ? 4 : 32) ijb_kv_gather4_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(gather4_threads(U), U == 1 ? 4 : 32)
+    ijb_kv_gather4_kernel(const __grid_constant__ RowsParams p) {
     constexpr int E = 16 / sizeof(T);
     using P = Place4<HD, U, E, gather4_threads(U)>;
     const int rows = P::tokens(p.kv) * 2 * P::groups(p.kv);
@@ -440,7 +445,8 @@ __global__ void __launch_bounds__(gather4_threads(U), U == 1 ? 4 : 32) ijb_kv_ga
         const uint8_t *from = p.kv.data + from0 * (HD / 2) + w.c * E / 8 * 4;  // (two threads' codes when E is 4)
         const uint8_t *scale = p.kv.scale + from0 * (HD / kKvBlock) + w.c * E / kKvBlock;
         T *dst = static_cast<T *>(w.which ? p.v : p.k) + w.t * p.stride + static_cast<long>(w.head) * HD + w.c * E;
-        const long next = static_cast<long>(HD / 2) << p.kv.page_shift, next_scale = static_cast<long>(HD / kKvBlock) << p.kv.page_shift;
+        const long next = static_cast<long>(HD / 2) << p.kv.page_shift,
+                   next_scale = static_cast<long>(HD / kKvBlock) << p.kv.page_shift;
         uint32_t raw[U], sc[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
@@ -513,7 +519,8 @@ void rows4_launch(const RowsParams &p, bool vec, cudaStream_t s) {
 
 template <bool APPEND, typename T>
 void rows_launch(const RowsParams &p, int type, bool vec, cudaStream_t s) {
-    if (type == IJB_KV_E2M1) p.kv.head_dim == 64 ? rows4_launch<APPEND, T, 64>(p, vec, s) : rows4_launch<APPEND, T, 128>(p, vec, s);
+    if (type == IJB_KV_E2M1 && p.kv.head_dim == 64) rows4_launch<APPEND, T, 64>(p, vec, s);
+    else if (type == IJB_KV_E2M1) rows4_launch<APPEND, T, 128>(p, vec, s);
     else if (type == IJB_KV_E4M3) rows_launch<APPEND, T, true>(p, vec, s);
     else rows_launch<APPEND, T, false>(p, vec, s);
 }

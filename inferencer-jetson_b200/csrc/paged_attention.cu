@@ -952,11 +952,13 @@ __device__ __noinline__ void mend_rows(const AttnArgs &a, int w, int row0, bool 
 // CTAs for each (CLUSTER), which cut it without a plan and join their states behind a
 // barrier of the cluster.
 //
-// Measured in a graph, 8 KV heads: 16 contexts of 11,003 to 40,111 positions, 32 heads of 128: 467 MB in 93 us
-// with fp16 queries (5.0 TB/s; issue slots 63 % and the ALU, which converts, 52 % busy) and 104 with fp32 ones;
-// heads of 64 63 and 69.  64 ragged single tokens behind 23 to 1,499, fp32, heads of 64: 18.3 us (27.7 with the
-// general kernel).  2 to 5 drafted tokens of 24 heads of 128 in 24 sequences behind 700 to 9,001: fp16 55 us, fp32 75,
-// the tensor pipe 46 % busy, for want of more than 2 warps a scheduler beside so many sums.
+// Measured in a graph, 8 KV heads: 16 contexts of 11,003 to 40,111 positions, 32 heads of 128: 467 MB in 93 us with
+// fp16 queries (5.0 TB/s) and 104 with fp32 ones; heads of 64 63 and 69.  No unit is full (issue slots 63 %, the ALU,
+// which converts, 52 %), but the 3 warps a scheduler has wait for one another's instructions, not for memory: of the
+// 4.6 clocks from one of a warp's to its next 0.8 go to a pipe that is taken, 0.6 to dispatch, 0.9 to another warp's
+// turn, 0.8 to the last result and 0.2 to loads.  64 ragged single tokens behind 23 to 1,499, fp32, heads of 64: 18.3
+// us (27.7 with the general kernel).  2 to 5 drafted tokens of 24 heads of 128 in 24 sequences behind 700 to 9,001:
+// fp16 55 us, fp32 75, the tensor pipe 46 % busy, for want of more than 2 warps a scheduler beside so many sums.
 
 template <int HD, int ROWS, typename T>
 struct Dec4 {
@@ -1145,7 +1147,8 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
                     if (a.status) atomicOr(a.status, kDevErrBadIndex);
                 }
                 const uint32_t off = static_cast<uint32_t>(pos & ((1 << a.kv.page_shift) - 1)) >> 3;
-                group = ok ? ((static_cast<uint32_t>(page_next) * 2 * a.kv.kv_heads + l_head) << (a.kv.page_shift - 3)) + off : 0u;
+                const uint32_t head = static_cast<uint32_t>(page_next) * 2 * a.kv.kv_heads + l_head;
+                group = ok ? (head << (a.kv.page_shift - 3)) + off : 0u;
                 fresh = false;
             }
             const uint32_t st = base + stage_in * D::kStage;
@@ -1205,7 +1208,8 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
                 for (int i = 0; i < 4 / STEP; ++i) {
                     const int r = i * STEP + lane / L;
                     const int tok = r < rows ? (row0 + r) / a.group : 0, in = r < rows ? (row0 + r) % a.group : 0;
-                    const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride + (s.head * a.group + in) * HD + lane % L * 4;
+                    const T *src = qp + static_cast<long>(s.x.q0 + tok) * a.q_stride +
+                                   (s.head * a.group + in) * HD + lane % L * 4;
                     v[i] = r < rows ? load4(src, qvec) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
@@ -1392,7 +1396,8 @@ __global__ void __launch_bounds__(Dec4<HD, ROWS, T>::kWarps * 32, 1)
                             pl[t][n][h] = transpose8x8(half2_bits(e[0] - f.x, e[1] - f.y));
                         }
                     }
-            // ---- values, 32 positions at a time: tile 4 k + j, rows gid and gid + 8, are the lane's dims 8 k + 2 j and 8 k + 2 j + 1
+            // ---- values, 32 positions at a time: tile 4 k + j, rows gid and gid + 8, are the lane's dims 8 k + 2 j and
+            // 8 k + 2 j + 1
 #pragma unroll
             for (int t0 = 0; t0 < TT; t0 += 2) {
                 uint32_t w[2][2][2][W], vs2[2][2];  // [tile][+ 8][j]
@@ -2546,7 +2551,8 @@ __device__ __forceinline__ int merge_block(const AttnArgs &a, const Left &left, 
             const float l = total[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
             fine = fine && (acc.x * 0.f + acc.y * 0.f + acc.z * 0.f + acc.w * 0.f) * inv == 0.f;
             const int rr = left.row0 + row0 + r;
-            store4(op + static_cast<long>(left.q0 + rr / a.group) * a.out_stride + (left.head * a.group + rr % a.group) * HD + 4 * c,
+            store4(op + static_cast<long>(left.q0 + rr / a.group) * a.out_stride +
+                       (left.head * a.group + rr % a.group) * HD + 4 * c,
                    vec, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
         }
     }
@@ -2596,7 +2602,8 @@ __device__ __forceinline__ int merge_few(const AttnArgs &a, const Left &left, in
             }
         }
         const int rr = left.row0 + row0 + r;
-        T *dst = op + static_cast<long>(left.q0 + rr / a.group) * a.out_stride + (left.head * a.group + rr % a.group) * HD + lane * E;
+        T *dst = op + static_cast<long>(left.q0 + rr / a.group) * a.out_stride +
+                 (left.head * a.group + rr % a.group) * HD + lane * E;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             fine = fine && acc[e] * 0.f * inv == 0.f;
@@ -2720,7 +2727,8 @@ cudaError_t merge_launch(const AttnArgs &a, cudaStream_t s) {
     return e;
 }
 
-// The decode kernel of a cache type for entries of up to ROWS (8 or 16; e2m1, fp32: 4 too) rows, its launch shape and its shared memory (the plan's at least).
+// The decode kernel of a cache type for entries of up to ROWS (8 or 16; e2m1, fp32: 4 too) rows, its launch shape and
+// its shared memory (the plan's at least).
 template <int HD, int KV, int ROWS, typename T>
 using DecOf = std::conditional_t<KV == IJB_KV_E2M1, Dec4<HD, ROWS, T>, Dec<HD, KV, ROWS == 16, T>>;
 template <int HD, int KV, int ROWS, typename T>
@@ -2756,7 +2764,8 @@ cudaError_t tile_allow() {
 constexpr int kManyCtas = 8, kManyTiles = 8, kFewCtas = 4, kFewTiles = 32;  // CTAs a cluster, up to so many tiles
 constexpr long kManyPositions = 32768, kFewPositions = 512;                  // in all; a tile
 int cluster_size(const AttnArgs &a, int sms) {
-    const long tiles = static_cast<long>(a.n_entries) * a.kv.kv_heads, positions = static_cast<long>(a.kv.max_pages) << a.kv.page_shift;
+    const long tiles = static_cast<long>(a.n_entries) * a.kv.kv_heads;
+    const long positions = static_cast<long>(a.kv.max_pages) << a.kv.page_shift;
     if (tiles <= kManyTiles) return positions <= kManyPositions && tiles * kManyCtas <= sms ? kManyCtas : 0;
     return tiles <= kFewTiles && positions <= kFewPositions * tiles && tiles * kFewCtas <= sms ? kFewCtas : 0;
 }
@@ -2828,12 +2837,17 @@ cudaError_t tile_launch(AttnArgs a, int sms, int min_rows, cudaStream_t s) {
     return merge_launch<kTileRows, HD, KV, T>(a, s);
 }
 
-// Which kernels serve a call.  Entries of up to 16 rows go to the decode kernel,
-// longer ones to the tile kernel; a call that may hold longer ones and has few
-// entries leaves them all to the tile kernel, for the launches (up to 4 fp32 rows of an e2m1 cache have a kernel of their
-// own: see Dec4): entries of 1 to 40 tokens
-// behind 100 to 2000 take 49 us so and 55 with both kernels for 2 of them, 51 and 56 for 7, 55 and 59 for 8, 77 and
-// 89 for 16 (so the border could lie higher); one of 200 tokens among single ones 54 and 68 for 4, 98 and 83 for 32.
+// Which kernels serve a call.  Entries of up to 16 rows go to the decode kernel, longer ones to the tile kernel; a
+// call that may hold longer ones and has few entries leaves them all to the tile kernel, for the launches (up to 4
+// fp32 rows of an e2m1 cache have a kernel of their own: see Dec4): entries of 1 to 40 tokens behind 100 to 2000 take
+// 49 us so and 55 with both kernels for 2 of them, 51 and 56 for 7, 55 and 59 for 8, 77 and 89 for 16 (so the border
+// could lie higher); one of 200 tokens among single ones 54 and 68 for 4, 98 and 83 for 32. Over e2m1 (heads of 64,
+// fp32): 38 and 44 for 2, 41 and 47 for 7, 43 and 49 for 8, 64 and 76 for 16, 86 and 102 for 32; one of 200 tokens
+// among single ones behind 100 to 2000 35 and 51 for 4, 52 and 60 for 8, 63 and 61 for 16, 93 and 65 for 32, behind
+// 8000 to 9000 103 and 93 for 4, 139 and 100 for 7, 149 and 100 for 8, 231 and 124 for 16: long contexts of single
+// tokens have the border lower, short entries higher.  The border at 16 rows is the decode kernel's tile, which its
+// plan has one of an entry; it is a cliff (24 x 4 and 24 x 5 tokens behind 700 to 9,001, 4 heads to a KV head: 52 and
+// 150 us with heads of 64, 80 and 242 with heads of 128), for want of a tile in between.
 template <int HD, int KV, typename T>
 cudaError_t attention_call(const AttnArgs &a, int max_q, int sms, cudaStream_t s) {
     const long most = static_cast<long>(max_q > 0 ? min(max_q, a.n_tokens) : a.n_tokens) * a.group;
@@ -2852,7 +2866,8 @@ cudaError_t attention_call(const AttnArgs &a, int max_q, int sms, cudaStream_t s
 template <typename T>
 cudaError_t attention_call(const AttnArgs &a, int type, int max_q, int sms, cudaStream_t s) {
     if (type == IJB_KV_E2M1) return attention_call<IJB_KV_E2M1, T>(a, max_q, sms, s);
-    return type == IJB_KV_E4M3 ? attention_call<IJB_KV_E4M3, T>(a, max_q, sms, s) : attention_call<IJB_KV_F16, T>(a, max_q, sms, s);
+    if (type == IJB_KV_E4M3) return attention_call<IJB_KV_E4M3, T>(a, max_q, sms, s);
+    return attention_call<IJB_KV_F16, T>(a, max_q, sms, s);
 }
 
 constexpr int kMaxWorkers = 16;  // per SM: the decode kernel's warps
@@ -2862,7 +2877,8 @@ size_t workspace_bytes(int sms, int head_dim) {
     static_assert(kMaxWorkers * kDecRows <= kTileRows, "the decode kernel's states fit in the tile kernel's");
     // a word per worker, and two states each
     const size_t held = head_dim == 128 ? static_cast<size_t>(sms) * kTileRows * head_dim * sizeof(float) : 0;
-    return static_cast<size_t>(sms) * kMaxWorkers * sizeof(Left) + held + static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
+    return static_cast<size_t>(sms) * kMaxWorkers * sizeof(Left) + held +
+           static_cast<size_t>(sms) * 2 * rows * (head_dim + 2) * sizeof(float);
 }
 
 template <int HD, int KV>
