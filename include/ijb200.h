@@ -169,7 +169,8 @@ int ijb_seq_length(const ijb_engine *engine, int seq_id);
  * (ijb_kv_copy_pages, one launch for all layers).  Both go on by themselves: a
  * shared page is given back when the last of its sequences is closed, and one
  * that a sequence writes to again (sequence 0, which ijb_forward, ijb_prefill and
- * ijb_reset set back) is replaced by a page of its own first.  IJB_ERR_CAPACITY
+ * ijb_reset set back) is replaced by a page of its own first, a copy where it holds
+ * positions of the sequence.  IJB_ERR_CAPACITY
  * when there is no sequence or page left, in which case nothing has changed.
  * Returns after the copy completed. */
 int ijb_seq_fork(ijb_engine *engine, int seq_id, int length, int *new_seq);
